@@ -363,6 +363,101 @@ M5B_API int m5b_projection_qkv_rope(const void* a, const void* b, int64_t m, int
                                     int rope_half, float epsilon, void* q_out, void* k_out,
                                     void* v_out, void* stream);
 
+/* ---- paged key/value cache ------------------------------------------------
+ * A batch of sequences whose keys and values live in fixed-size pages.  The
+ * `tokens` new rows are grouped by sequence: rows query_start[b] up to
+ * query_start[b + 1] (n_b of them, none allowed) belong to sequence b, whose
+ * length seq_lens[b] counts them.  Row t of sequence b stands at position
+ *     pos = seq_lens[b] - n_b + (t - query_start[b]).
+ * Position p of sequence b is slot p % page_size of page
+ * page_table[b * table_stride + p / page_size].  k_cache and v_cache are
+ * [num_pages, kv_heads, page_size, head_dim] views with the strides below (in
+ * elements; the channels are contiguous), so a [page, slot, head, channel]
+ * allocation is described as well.  Both calls read the lengths and the table
+ * on the device.  Positions from max_pages * page_size on have no page: they
+ * are not appended and hold no visible key.  A page number outside
+ * [0, num_pages) is never followed: nothing is appended there, and its keys
+ * and values read as zeros.
+ * The reference has no cache and no attention: these entry points take its
+ * Q/K/V projection (src/m5kernels/qk_rope.py:120-182) on to the next
+ * projection's input. */
+typedef struct m5b_paged_batch {
+  int64_t tokens, batch, q_heads, kv_heads, head_dim;
+  const int32_t* query_start; /* [batch + 1] */
+  const int32_t* seq_lens;    /* [batch] */
+  void* k_cache;
+  void* v_cache;
+  int64_t cache_dtype; /* M5B_BF16, M5B_F16 or M5B_F32 */
+  int64_t num_pages, page_size;
+  int64_t k_page_stride, k_head_stride, k_slot_stride;
+  int64_t v_page_stride, v_head_stride, v_slot_stride;
+  const int32_t* page_table;
+  int64_t max_pages, table_stride; /* columns of the table, elements between its rows */
+} m5b_paged_batch;
+
+/* Appends the new tokens' keys and values, rotating the keys (and, when q is
+ * given, the queries into q_out [tokens, q_heads, head_dim], contiguous, in
+ * the cache's dtype) by their positions on the way:
+ *   interleaved == 0: channels (j, j + rope_half) for j < rope_half
+ *   interleaved == 1: channels (2j, 2j + 1)
+ *   (a, b) -> (a cos[pos, j] - b sin[pos, j], b cos[pos, j] + a sin[pos, j])
+ * in FP32, rounded once to the cache's dtype; channels >= 2 rope_half and the
+ * values are only rounded.  cos, sin: [table_rows, rope_half] fp32 / fp16 /
+ * bf16; rope_half == 0 (no tables) rotates nothing.  q, k, v share x_dtype and
+ * have contiguous channels.  A token whose position is negative or not below
+ * table_rows is not appended and gets q_out = 0, as do rows of q outside
+ * every sequence.  The inputs must not overlap the outputs. */
+typedef struct m5b_paged_append_args {
+  m5b_paged_batch b;
+  const void* q; /* NULL: keys and values only */
+  const void* k;
+  const void* v;
+  int64_t x_dtype;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
+      v_head_stride;
+  const void* cos;
+  const void* sin;
+  int64_t table_dtype, table_rows, rope_half, interleaved;
+  void* q_out;
+} m5b_paged_append_args;
+M5B_API int m5b_paged_append(const m5b_paged_append_args* args, void* stream);
+
+/* Attention of the new tokens over the cache (which holds their keys and
+ * values already): with G = q_heads / kv_heads, query head h reads kv head
+ * h / G, and for key j of the row's sequence
+ *   x = scale * q.k_j;  x = softcap tanh(x / softcap)   (softcap > 0)
+ *   x -= slopes[h] * |pos - j|                          (slopes != NULL)
+ * key j is visible when j < seq_lens[b] and (j < prefix_lens[b], or j <= pos
+ * and (window == 0 or pos - j < window)).  out = softmax over the visible keys
+ * times V, rounded once to the cache's dtype (which q and out share); lse
+ * (optional, fp32 [tokens, q_heads]) = ln of the sum of exponentials of x.  A
+ * row that sees no key gets out = 0 and lse = -inf.  max_query_len is the
+ * largest n_b and chooses the kernel; the result does not depend on it.
+ * Slots behind a sequence's end may hold anything; keys and values of the
+ * sequences themselves are finite.  The workspace
+ * (m5b_paged_attention_workspace_bytes) is scratch, overwritten by every call;
+ * calls that overlap on the GPU need separate ones. */
+typedef struct m5b_paged_attention_args {
+  m5b_paged_batch b;
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  void* out;
+  int64_t out_token_stride, out_head_stride;
+  float* lse;
+  int64_t max_query_len;
+  double scale, softcap;
+  const float* slopes;        /* [q_heads] or NULL */
+  int64_t window;             /* 0: none */
+  const int32_t* prefix_lens; /* [batch] or NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+} m5b_paged_attention_args;
+M5B_API int m5b_paged_attention(const m5b_paged_attention_args* args, void* stream);
+
+/* Workspace bytes of m5b_paged_attention on the current device: depends on
+ * the head dimension and the SM count only. */
+M5B_API int64_t m5b_paged_attention_workspace_bytes(int64_t head_dim);
+
 #ifdef __cplusplus
 }
 #endif

@@ -229,6 +229,8 @@ int norm_setup(RowPrepArgs& a, const void* gamma, int gamma_dtype, const void* s
 
 int m5b::set_last_error(int code, const char* msg) { return fail(code, "%s", msg); }
 
+int m5b::current_device_state(unsigned int** status, int* sms) { return device_state(status, sms); }
+
 extern "C" {
 
 int m5b_version(void) { return 100; }

@@ -96,6 +96,8 @@ struct RowMaps {
 
 // Record `msg` as this thread's m5b_last_error() text and return `code`.
 int set_last_error(int code, const char* msg);
+// Status word and SM count of the current device (an M5B_* code; api.cu).
+int current_device_state(unsigned int** status, int* sms);
 
 int row_prep_warps(int64_t K, int block);
 bool quant_rows_applicable(const RowPrepArgs& a, int x_dtype, int block, int out);

@@ -1,0 +1,146 @@
+// C-ABI entry points of the paged key/value cache (declared in
+// include/m5b200.h): contract checks, kernel choice, launches.  Nothing here
+// allocates or synchronizes, and nothing throws.
+#include <cmath>
+#include <cstdio>
+
+#include "m5b200.h"
+#include "paged.cuh"
+
+using namespace m5b;
+
+namespace {
+
+int einval(const char* msg) { return set_last_error(M5B_EINVAL, msg); }
+int eunsupported(const char* msg) { return set_last_error(M5B_EUNSUPPORTED, msg); }
+
+int launched(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return set_last_error(M5B_OK, "");
+  char msg[256];
+  snprintf(msg, sizeof(msg), "%s: %s", what, cudaGetErrorString(e));
+  return set_last_error(M5B_ECUDA, msg);
+}
+
+bool float_dtype(int64_t dt) { return dt == M5B_F32 || dt == M5B_F16 || dt == M5B_BF16; }
+bool fits_int(int64_t v) { return v >= 0 && v <= INT_MAX; }
+
+int take_batch(const m5b_paged_batch& s, PagedBatch& d) {
+  if (s.tokens < 0 || s.batch < 1 || s.q_heads < 1 || s.kv_heads < 1 || s.head_dim < 1)
+    return einval("tokens, batch, heads and head_dim must be positive");
+  if (s.q_heads % s.kv_heads) return einval("q_heads must be a multiple of kv_heads");
+  if (s.num_pages < 1 || s.page_size < 1 || s.max_pages < 0 || s.table_stride < 0)
+    return einval("the cache needs pages and a page table");
+  if (!float_dtype(s.cache_dtype)) return einval("cache dtype must be float16, bfloat16 or float32");
+  if (!fits_int(s.tokens) || !fits_int(s.batch) || !fits_int(s.num_pages) ||
+      !fits_int(s.page_size) || !fits_int(s.max_pages) || s.q_heads > 65535 || s.head_dim > 65535)
+    return eunsupported("batch or cache dimensions exceed the index range");
+  if (s.tokens * s.q_heads > INT_MAX) return eunsupported("tokens x heads exceed the launch grid limit");
+  if (!s.query_start || !s.seq_lens || !s.k_cache || !s.v_cache || (!s.page_table && s.max_pages > 0))
+    return einval("query_start, seq_lens, the caches and the page table are required");
+  d = PagedBatch{};
+  d.tokens = static_cast<int>(s.tokens);
+  d.batch = static_cast<int>(s.batch);
+  d.q_heads = static_cast<int>(s.q_heads);
+  d.kv_heads = static_cast<int>(s.kv_heads);
+  d.group = d.q_heads / d.kv_heads;
+  d.head_dim = static_cast<int>(s.head_dim);
+  d.query_start = s.query_start;
+  d.seq_lens = s.seq_lens;
+  d.k_cache = s.k_cache;
+  d.v_cache = s.v_cache;
+  d.num_pages = static_cast<int>(s.num_pages);
+  d.page_size = static_cast<int>(s.page_size);
+  d.k_page = s.k_page_stride;
+  d.k_head = s.k_head_stride;
+  d.k_slot = s.k_slot_stride;
+  d.v_page = s.v_page_stride;
+  d.v_head = s.v_head_stride;
+  d.v_slot = s.v_slot_stride;
+  d.page_table = s.page_table;
+  d.max_pages = static_cast<int>(s.max_pages);
+  d.table_stride = s.table_stride;
+  const int64_t capacity = s.max_pages * s.page_size;
+  d.capacity = capacity > INT_MAX ? INT_MAX : static_cast<int>(capacity);
+  return M5B_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int m5b_paged_append(const m5b_paged_append_args* s, void* stream) {
+  if (!s) return einval("arguments are NULL");
+  PagedAppendArgs a{};
+  int rc = take_batch(s->b, a.b);
+  if (rc) return rc;
+  if (!float_dtype(s->x_dtype)) return einval("input dtype must be float16, bfloat16 or float32");
+  if (s->rope_half < 0 || 2 * s->rope_half > s->b.head_dim)
+    return einval("the rotated channels must fit the head");
+  if (s->rope_half > 0) {
+    if (!s->cos || !s->sin || s->table_rows < 1) return einval("cos and sin tables are required");
+    if (!float_dtype(s->table_dtype)) return einval("cos and sin must have floating dtype");
+    if (!fits_int(s->table_rows)) return eunsupported("cos and sin tables exceed the index range");
+  }
+  if (s->b.tokens == 0) return set_last_error(M5B_OK, "");
+  if (!s->k || !s->v) return einval("k and v are required");
+  if (s->q && !s->q_out) return einval("q_out is required with q");
+  a.q = s->q;
+  a.k = s->k;
+  a.v = s->v;
+  a.q_token = s->q_token_stride;
+  a.q_head = s->q_head_stride;
+  a.k_token = s->k_token_stride;
+  a.k_head = s->k_head_stride;
+  a.v_token = s->v_token_stride;
+  a.v_head = s->v_head_stride;
+  a.cos = s->cos;
+  a.sin = s->sin;
+  a.table_dtype = static_cast<int>(s->table_dtype);
+  a.table_rows = static_cast<int>(s->table_rows);
+  a.rope_half = static_cast<int>(s->rope_half);
+  a.interleaved = s->interleaved ? 1 : 0;
+  a.q_out = s->q_out;
+  return launched(launch_paged_append(a, static_cast<int>(s->x_dtype),
+                                      static_cast<int>(s->b.cache_dtype),
+                                      static_cast<cudaStream_t>(stream)),
+                  "paged append launch");
+}
+
+int64_t m5b_paged_attention_workspace_bytes(int64_t head_dim) {
+  (void)head_dim;
+  return 0;
+}
+
+int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
+  if (!s) return einval("arguments are NULL");
+  PagedAttnArgs a{};
+  int rc = take_batch(s->b, a.b);
+  if (rc) return rc;
+  if (s->b.head_dim > 256) return eunsupported("head_dim above 256 is unsupported");
+  if (!(s->scale > 0.0) || !std::isfinite(static_cast<float>(s->scale)))
+    return einval("scale must be a positive finite real scalar");
+  if (!(s->softcap >= 0.0) || !std::isfinite(static_cast<float>(s->softcap)))
+    return einval("softcap must be a positive finite real scalar");
+  if (s->window < 0) return einval("window must be positive");
+  if (s->max_query_len < 0) return einval("max_query_len must not be negative");
+  if (s->b.tokens == 0) return set_last_error(M5B_OK, "");
+  if (!s->q || !s->out) return einval("q and out are required");
+  a.q = s->q;
+  a.q_token = s->q_token_stride;
+  a.q_head = s->q_head_stride;
+  a.out = s->out;
+  a.o_token = s->out_token_stride;
+  a.o_head = s->out_head_stride;
+  a.lse = s->lse;
+  a.max_query_len = s->max_query_len > INT_MAX ? INT_MAX : static_cast<int>(s->max_query_len);
+  a.scale = static_cast<float>(s->scale);
+  a.softcap = static_cast<float>(s->softcap);
+  a.slopes = s->slopes;
+  a.window = s->window == 0 || s->window > INT_MAX ? INT_MAX : static_cast<int>(s->window);
+  a.prefix_lens = s->prefix_lens;
+  return launched(launch_paged_attention_rows(a, static_cast<int>(s->b.cache_dtype),
+                                              static_cast<cudaStream_t>(stream)),
+                  "paged attention launch");
+}
+
+}  // extern "C"

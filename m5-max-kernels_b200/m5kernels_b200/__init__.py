@@ -11,6 +11,8 @@ The `cuda-b200` backend of the m5kernels operator contracts:
     projection_qkv_rope                (grouped Q/K/V layout of the H3 integration)
     rms_quantize                       (twin of m5kernels.rms_quant)
     linear, OnlineProjection           (the online quantize -> gemm stage in one call / bound step)
+    paged_append, paged_attention      (what follows the Q/K/V projection: a paged cache and
+                                        attention of new tokens over it)
 All of them run hand-written CUDA kernels from libm5b200.so through its C ABI
 (include/m5b200.h); there is no CPU fallback.
 """
@@ -20,6 +22,7 @@ from .hadamard import SUPPORTED_BLOCK_SIZES, hadamard_quantize, rotate
 from .linear import OnlineProjection, linear
 from .norm_hadamard import (fused_gated_residual_norm_hadamard_quantize,
                             fused_norm_hadamard_quantize, gated_residual_add, unfused_norm)
+from .paged import paged_append, paged_attention
 from .qk_rope import (grouped_qkv_weights, projection_qk_rope, projection_qkv_rope, qk_norm_rope,
                       rope_tables)
 from .rms_quant import rms_quantize
@@ -29,5 +32,5 @@ __all__ = [
     "fused_norm_hadamard_quantize", "fused_gated_residual_norm_hadamard_quantize",
     "projection_qk_rope", "rope_tables", "linear", "rms_quantize", "gated_residual_add",
     "unfused_norm", "qk_norm_rope", "projection_qkv_rope", "grouped_qkv_weights",
-    "OnlineProjection",
+    "OnlineProjection", "paged_append", "paged_attention",
 ]

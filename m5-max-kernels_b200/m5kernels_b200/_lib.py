@@ -59,6 +59,9 @@ _SIGNATURES = {
     "m5b_linear_ex": ([P, I, I64, I64, I, P, P, P, I64, I, P, I, P, I64, P, I64, P], I),
     "m5b_linear_noalloc": ([P, I, I64, I64, I, P, P, P, I64, I, P, I, P], I),
     "m5b_gemm_set_schedule": ([I, I], I),
+    "m5b_paged_append": ([P, P], I),
+    "m5b_paged_attention": ([P, P], I),
+    "m5b_paged_attention_workspace_bytes": ([I64], I64),
 }
 
 
