@@ -98,6 +98,10 @@ struct RowMaps {
 int set_last_error(int code, const char* msg);
 // Status word and SM count of the current device (an M5B_* code; api.cu).
 int current_device_state(unsigned int** status, int* sms);
+// A tiled map of 16-bit elements with the 128-byte swizzle; false when the
+// driver refuses it (api.cu).
+bool make_swizzled_map16(CUtensorMap* map, bool f16, int rank, const void* ptr,
+                         const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
 
 int row_prep_warps(int64_t K, int block);
 bool quant_rows_applicable(const RowPrepArgs& a, int x_dtype, int block, int out);

@@ -50,11 +50,26 @@ struct PagedAttnArgs {
   const float* slopes;
   int window;  // INT_MAX: none
   const int32_t* prefix_lens;
+  void* workspace;       // the tiled kernels' PagedPartials
+  unsigned int* status;  // device status word (bounded-wait errors)
+};
+
+// Tensor maps of the caches, {channel, slot, head, page}, boxes of 64
+// channels x box_rows slots, 128-byte swizzle.
+struct PagedMaps {
+  CUtensorMap k, v;
+  int box_rows;
 };
 
 cudaError_t launch_paged_append(const PagedAppendArgs& a, int x_dtype, int cache_dtype,
                                 cudaStream_t stream);
 cudaError_t launch_paged_attention_rows(const PagedAttnArgs& a, int dtype, cudaStream_t stream);
+// The tiled kernels: 16-bit types, 64 or 128 channels, pages of 2^k >= 8
+// slots, everything on the 16-byte grid.
+constexpr int kDecodeRows = 32;  // rows per kv head and sequence that the decode kernel is for
+cudaError_t launch_paged_decode(const PagedAttnArgs& a, const PagedMaps& m, int dtype, int sms,
+                                cudaStream_t stream);
+int64_t paged_decode_workspace(int head_dim, int sms);
 
 // Rows of sequence b, clipped to the batch's rows whatever query_start holds.
 __device__ __forceinline__ int2 paged_rows(const PagedBatch& b, int seq) {

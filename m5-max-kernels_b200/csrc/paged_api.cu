@@ -64,6 +64,40 @@ int take_batch(const m5b_paged_batch& s, PagedBatch& d) {
   return M5B_OK;
 }
 
+bool pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
+bool grid16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Whether the tiled kernels can take the call: 16-bit elements, 64 or 128
+// channels, pages of 2^k >= 8 slots (a box of the swizzled copy is whole
+// 8-row groups) and all rows on the 16-byte grid.
+bool tiled(const PagedAttnArgs& a, int64_t dtype) {
+  const PagedBatch& b = a.b;
+  if (dtype == M5B_F32 || (b.head_dim != 64 && b.head_dim != 128)) return false;
+  if (!pow2(b.page_size) || b.page_size < 8) return false;
+  const int64_t strides[] = {b.k_page, b.k_head, b.k_slot, b.v_page, b.v_head, b.v_slot,
+                             a.q_token, a.q_head, a.o_token, a.o_head};
+  for (int64_t s : strides)
+    if (s < 0 || s % 8) return false;
+  return grid16(b.k_cache) && grid16(b.v_cache) && grid16(a.q) && grid16(a.out);
+}
+
+// Boxes of up to `block` slots x 64 channels of one head of one page.
+bool cache_map(CUtensorMap* map, const void* ptr, const PagedBatch& b, bool f16, int64_t page,
+               int64_t head, int64_t slot, int box_rows) {
+  const uint64_t dims[4] = {uint64_t(b.head_dim), uint64_t(b.page_size), uint64_t(b.kv_heads),
+                            uint64_t(b.num_pages)};
+  const uint64_t strides[3] = {uint64_t(slot) * 2, uint64_t(head) * 2, uint64_t(page) * 2};
+  const uint32_t box[4] = {64, uint32_t(box_rows), 1, 1};
+  return make_swizzled_map16(map, f16, 4, ptr, dims, strides, box);
+}
+
+bool cache_maps(PagedMaps& m, const PagedAttnArgs& a, int64_t dtype, int block) {
+  const PagedBatch& b = a.b;
+  m.box_rows = b.page_size < block ? b.page_size : block;
+  return cache_map(&m.k, b.k_cache, b, dtype == M5B_F16, b.k_page, b.k_head, b.k_slot, m.box_rows) &&
+         cache_map(&m.v, b.v_cache, b, dtype == M5B_F16, b.v_page, b.v_head, b.v_slot, m.box_rows);
+}
+
 }  // namespace
 
 extern "C" {
@@ -107,8 +141,9 @@ int m5b_paged_append(const m5b_paged_append_args* s, void* stream) {
 }
 
 int64_t m5b_paged_attention_workspace_bytes(int64_t head_dim) {
-  (void)head_dim;
-  return 0;
+  int sms = 0;
+  if ((head_dim != 64 && head_dim != 128) || current_device_state(nullptr, &sms)) return 0;
+  return paged_decode_workspace(static_cast<int>(head_dim), sms);
 }
 
 int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
@@ -138,8 +173,21 @@ int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
   a.slopes = s->slopes;
   a.window = s->window == 0 || s->window > INT_MAX ? INT_MAX : static_cast<int>(s->window);
   a.prefix_lens = s->prefix_lens;
-  return launched(launch_paged_attention_rows(a, static_cast<int>(s->b.cache_dtype),
-                                              static_cast<cudaStream_t>(stream)),
+  const int dtype = static_cast<int>(s->b.cache_dtype);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (tiled(a, dtype) && int64_t(a.max_query_len) * a.b.group <= kDecodeRows) {
+    int sms = 0;
+    rc = current_device_state(&a.status, &sms);
+    if (rc) return rc;
+    a.workspace = s->workspace;
+    if (!a.workspace || !grid16(a.workspace) ||
+        s->workspace_bytes < m5b_paged_attention_workspace_bytes(a.b.head_dim))
+      return einval("workspace of m5b_paged_attention_workspace_bytes(head_dim) bytes required");
+    PagedMaps m;
+    if (cache_maps(m, a, dtype, 64))
+      return launched(launch_paged_decode(a, m, dtype, sms, st), "paged attention launch");
+  }
+  return launched(launch_paged_attention_rows(a, dtype, st),
                   "paged attention launch");
 }
 

@@ -1,0 +1,332 @@
+// Work distribution of the tiled attention kernels (paged_decode.cu,
+// paged_prompt.cu), and the joining of what it splits.
+//
+// A tile is up to ROWS packed rows of one kv head of one sequence (row r is
+// new token r / G and query head kv * G + r % G, so that a group shares the
+// keys) against the key blocks (BK keys each) that any of its rows sees.  All
+// tiles' blocks, in the order sequence, head, row tile, block, form one line;
+// every CTA takes an equal stretch of it, found from the lengths on the
+// device.  Whole tiles leave finished.  Of a tile that crosses a CTA's border
+// each part goes to the workspace: unnormalized fp32 sums with the row
+// maximum they refer to.  A CTA has at most two such parts, one that continues
+// an earlier CTA's tile (slot 2 c) and one that a later CTA continues (slot
+// 2 c + 1), so the workspace does not grow with the batch; and the parts of a
+// tile are added in the order of the line, whichever is finished first.
+#pragma once
+
+#include "paged.cuh"
+
+namespace m5b {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct PagedSeq {
+  int row0;    // first row of the batch
+  int n;       // new tokens
+  int pos0;    // position of the first
+  int keys;    // keys that pages can hold
+  int prefix;  // keys that every row sees
+};
+
+__device__ __forceinline__ PagedSeq paged_seq(const PagedAttnArgs& a, int seq) {
+  const int2 rows = paged_rows(a.b, seq);
+  const int len = paged_len(a.b, seq);
+  PagedSeq s;
+  s.row0 = rows.x;
+  s.n = rows.y - rows.x;
+  s.pos0 = len - s.n;
+  s.keys = min(len, a.b.capacity);
+  s.prefix = a.prefix_lens ? max(0, min(a.prefix_lens[seq], s.keys)) : 0;
+  return s;
+}
+
+// Key blocks of a row tile: [0, pre) and [from, from + blocks - pre).  A tile
+// whose rows see nothing has one block all the same, hidden entirely.
+struct PagedBlocks {
+  int pre, from, blocks;
+  __device__ __forceinline__ int at(int i) const { return i < pre ? i : from + (i - pre); }
+};
+
+template <int ROWS, int BK>
+__device__ __forceinline__ PagedBlocks paged_blocks(const PagedAttnArgs& a, const PagedSeq& s,
+                                                    int rt) {
+  const int g = a.b.group;
+  const int lo = s.pos0 + (rt * ROWS) / g;
+  const int hi = s.pos0 + min(rt * ROWS + ROWS - 1, s.n * g - 1) / g;
+  const int last = min(hi, s.keys - 1);
+  PagedBlocks r;
+  r.pre = (s.prefix + BK - 1) / BK;
+  r.from = max(r.pre, lo >= a.window ? (lo - a.window + 1) / BK : 0);
+  r.blocks = max(1, r.pre + (last >= 0 ? max(0, last / BK + 1 - r.from) : 0));
+  return r;
+}
+
+__device__ __forceinline__ int paged_tiles(const PagedAttnArgs& a, int n, int rows) {
+  return (n * a.b.group + rows - 1) / rows;
+}
+
+// Blocks of one kv head of a sequence; all lanes of the warp pass their own.
+template <int ROWS, int BK>
+__device__ __forceinline__ long long paged_seq_blocks(const PagedAttnArgs& a, const PagedSeq& s) {
+  constexpr int kAlone = 4;  // longer sums are shared by the warp's lanes
+  const int tiles = paged_tiles(a, s.n, ROWS);
+  long long sum = 0;
+  if (tiles <= kAlone)
+    for (int t = 0; t < tiles; ++t) sum += paged_blocks<ROWS, BK>(a, s, t).blocks;
+  const int lane = threadIdx.x % 32;
+  for (uint32_t left = __ballot_sync(~0u, tiles > kAlone); left; left &= left - 1) {
+    const int src = __ffs(left) - 1;
+    PagedSeq o;
+    o.n = __shfl_sync(~0u, s.n, src);
+    o.pos0 = __shfl_sync(~0u, s.pos0, src);
+    o.keys = __shfl_sync(~0u, s.keys, src);
+    o.prefix = __shfl_sync(~0u, s.prefix, src);
+    const int all = __shfl_sync(~0u, tiles, src);
+    long long part = 0;
+    for (int t = lane; t < all; t += 32) part += paged_blocks<ROWS, BK>(a, o, t).blocks;
+    for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(~0u, part, d);
+    if (lane == src) sum = part;
+  }
+  return sum;
+}
+
+// One stretch of a tile: blocks [begin, end) of its `r.blocks`.
+struct PagedPiece {
+  int seq, head, rt, begin, end;
+  PagedSeq s;
+  PagedBlocks r;
+  __device__ __forceinline__ bool whole() const { return begin == 0 && end == r.blocks; }
+};
+
+// The stretch of this CTA, piece by piece.  Every thread that walks it sees
+// the same pieces.
+template <int ROWS, int BK>
+struct PagedWalk {
+  int seq, head, rt, tiles, blk;
+  long long left, share;
+  PagedSeq s;
+
+  __device__ __forceinline__ void enter(const PagedAttnArgs& a) {  // first tile of a sequence >= seq
+    while (seq < a.b.batch) {
+      s = paged_seq(a, seq);
+      tiles = paged_tiles(a, s.n, ROWS);
+      if (tiles > 0) return;
+      ++seq;
+    }
+    left = 0;
+  }
+
+  __device__ __forceinline__ bool next(const PagedAttnArgs& a, PagedPiece& p) {
+    if (left <= 0) return false;
+    p.seq = seq;
+    p.head = head;
+    p.rt = rt;
+    p.s = s;
+    p.r = paged_blocks<ROWS, BK>(a, s, rt);
+    p.begin = blk;
+    p.end = static_cast<int>(min(static_cast<long long>(p.r.blocks), blk + left));
+    left -= p.end - p.begin;
+    if (p.end == p.r.blocks) {
+      blk = 0;
+      if (++rt == tiles) {
+        rt = 0;
+        if (++head == a.b.kv_heads) {
+          head = 0;
+          ++seq;
+          if (left > 0) enter(a);
+        }
+      }
+    }
+    return true;
+  }
+};
+
+// Called by all threads of the CTA (THREADS of them, whole warps); `scratch`
+// is shared memory for THREADS / 32 + 4 values.
+template <int ROWS, int BK, int THREADS>
+__device__ __forceinline__ PagedWalk<ROWS, BK> paged_walk(const PagedAttnArgs& a,
+                                                          long long* scratch) {
+  constexpr int kWarps = THREADS / 32;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int per = (a.b.batch + THREADS - 1) / THREADS;
+  const int b0 = threadIdx.x * per;
+  long long mine = 0;
+  for (int i = 0; i < per; ++i) {
+    PagedSeq s{};
+    if (b0 + i < a.b.batch) s = paged_seq(a, b0 + i);
+    mine += paged_seq_blocks<ROWS, BK>(a, s) * a.b.kv_heads;
+  }
+  long long upto = mine;
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(~0u, upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 31) scratch[warp] = upto;
+  if (threadIdx.x == 0) scratch[kWarps] = -1;
+  __syncthreads();
+  long long before = upto - mine, total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += scratch[w];
+    total += scratch[w];
+  }
+  PagedWalk<ROWS, BK> walk;
+  walk.share = (total + gridDim.x - 1) / gridDim.x;
+  const long long at = walk.share * blockIdx.x;
+  walk.left = max(0ll, min(walk.share, total - at));
+  // the thread whose sequences hold block `at` looks which one does (all lanes
+  // of its warp take part in the sums)
+  const bool here = walk.left > 0 && before <= at && at < before + mine;
+  if (__any_sync(~0u, here)) {
+    long long base = before;
+    bool found = false;
+    for (int i = 0; i < per; ++i) {
+      PagedSeq s{};
+      if (b0 + i < a.b.batch) s = paged_seq(a, b0 + i);
+      const long long one = paged_seq_blocks<ROWS, BK>(a, s), all = one * a.b.kv_heads;
+      if (here && !found && at < base + all) {
+        found = true;
+        scratch[kWarps] = b0 + i;
+        scratch[kWarps + 1] = (at - base) / one;
+        scratch[kWarps + 2] = (at - base) % one;
+      }
+      base += all;
+    }
+  }
+  __syncthreads();
+  walk.seq = static_cast<int>(scratch[kWarps]);
+  walk.head = 0;
+  walk.rt = 0;
+  walk.blk = 0;
+  walk.tiles = 0;
+  if (walk.seq < 0) walk.left = 0;
+  if (walk.left > 0) {
+    walk.head = static_cast<int>(scratch[kWarps + 1]);
+    long long rest = scratch[kWarps + 2];
+    walk.s = paged_seq(a, walk.seq);
+    walk.tiles = paged_tiles(a, walk.s.n, ROWS);
+    for (int base = 0; base < walk.tiles; base += 32) {  // 32 row tiles at a time
+      const int t = base + lane;
+      const int blocks = t < walk.tiles ? paged_blocks<ROWS, BK>(a, walk.s, t).blocks : 0;
+      long long sum = blocks;
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long o = __shfl_up_sync(~0u, sum, d);
+        if (lane >= d) sum += o;
+      }
+      const uint32_t past = __ballot_sync(~0u, sum > rest);
+      if (past) {
+        const int src = __ffs(past) - 1;
+        walk.rt = base + src;
+        walk.blk = static_cast<int>(rest - __shfl_sync(~0u, sum - blocks, src));
+        break;
+      }
+      rest -= __shfl_sync(~0u, sum, 31);
+    }
+  }
+  return walk;
+}
+
+// Workspace of a launch of `ctas` CTAs.
+struct PagedSplit {  // the tile that CTA c leaves to later ones
+  int parts;         // slots: 2 c + 1, then 2 (c + 1), 2 (c + 2), ...; 0: none
+  int row0, first, rows, head;  // batch row, packed rows [first, first + rows), kv head
+  int pad[3];
+};
+template <int ROWS, int D>
+struct PagedPartials {
+  PagedSplit* split;  // [ctas]
+  float2* ml;         // [2 ctas][ROWS]: maximum (in log2 units) and sum
+  float* o;           // [2 ctas][ROWS][D]
+  __host__ __device__ PagedPartials(void* ws, int ctas) {
+    split = static_cast<PagedSplit*>(ws);
+    ml = reinterpret_cast<float2*>(split + (ctas + 7) / 8 * 8);
+    o = reinterpret_cast<float*>(ml + int64_t(2) * ctas * ROWS);
+  }
+  static int64_t bytes(int ctas) {
+    return (ctas + 7) / 8 * 8 * int64_t(sizeof(PagedSplit)) +
+           int64_t(2) * ctas * ROWS * (sizeof(float2) + D * sizeof(float));
+  }
+};
+
+// Written by one thread of every CTA, after its last piece (or without any).
+__device__ __forceinline__ void paged_write_split(PagedSplit* at, const PagedPiece* last,
+                                                  long long share, int rows_per_tile, int group) {
+  PagedSplit m{};
+  if (last && last->end < last->r.blocks && last->begin == 0) {
+    m.parts = 1 + static_cast<int>((last->r.blocks - last->end + share - 1) / share);
+    m.row0 = last->s.row0;
+    m.first = last->rt * rows_per_tile;
+    m.rows = min(rows_per_tile, last->s.n * group - m.first);
+    m.head = last->head;
+  }
+  *at = m;
+}
+
+// Joins the parts of the tiles that were split: CTA (c, i) takes rows 4 i .. 4 i + 3
+// of the tile that CTA c left to others, one warp a row, the lanes across the
+// channels.
+template <typename T, int ROWS, int D>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnArgs a, int ctas) {
+  constexpr int V = D / 32;
+  grid_dependency_wait();
+  const PagedPartials<ROWS, D> w(a.workspace, ctas);
+  const int c = blockIdx.x;
+  const PagedSplit m = w.split[c];
+  const int row = blockIdx.y * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (row >= m.rows || m.parts == 0) return;
+  float top = -INFINITY;
+  for (int i = lane; i < m.parts; i += 32) {
+    const int slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
+    top = fmaxf(top, w.ml[int64_t(slot) * ROWS + row].x);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+  float sum = 0.0f, o[V] = {};
+#pragma unroll 4
+  for (int i = 0; i < m.parts; ++i) {
+    const int slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
+    const float2 ml = w.ml[int64_t(slot) * ROWS + row];
+    const float* po = w.o + (int64_t(slot) * ROWS + row) * D + lane * V;
+    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+#pragma unroll
+    for (int v = 0; v < V; v += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(po + v);
+      o[v] = fmaf(x.x, f, o[v]);
+      o[v + 1] = fmaf(x.y, f, o[v + 1]);
+    }
+  }
+  const int packed = m.first + row, t = m.row0 + packed / a.b.group;
+  const int h = m.head * a.b.group + packed % a.b.group;
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  T* out = static_cast<T*>(a.out) + t * a.o_token + h * a.o_head + lane * V;
+#pragma unroll
+  for (int v = 0; v < V; ++v) out[v] = from_f32<T>(o[v] * inv);
+  if (a.lse && lane == 0)
+    a.lse[int64_t(t) * a.b.q_heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+}
+
+// Rows outside every sequence leave as zeros; `id` of `count` threads.
+template <typename T, int D>
+__device__ __forceinline__ void paged_zero_outside(const PagedAttnArgs& a, int64_t id, int64_t count) {
+  const int lo = max(0, min(a.b.query_start[0], a.b.tokens));
+  const int hi = max(lo, min(a.b.query_start[a.b.batch], a.b.tokens));
+  const int64_t per = int64_t(a.b.q_heads) * (D / 8);
+  const int64_t all = (int64_t(lo) + a.b.tokens - hi) * per;
+  for (int64_t i = id; i < all; i += count) {
+    int64_t t = i / per;
+    if (t >= lo) t += hi - lo;
+    const int h = static_cast<int>(i % per) / (D / 8), c = static_cast<int>(i % (D / 8));
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + t * a.o_token + h * a.o_head + c * 8) =
+        make_uint4(0u, 0u, 0u, 0u);
+    if (a.lse && c == 0) a.lse[t * a.b.q_heads + h] = -INFINITY;
+  }
+}
+
+}  // namespace m5b

@@ -16,8 +16,10 @@ BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 @pytest.fixture(scope="module")
 def ops():
     import m5kernels_b200 as m
+    from m5kernels_b200 import _lib
 
-    return m
+    yield m
+    assert _lib.device_status() == 0  # no bounded wait gave up
 
 
 def attend(ops, batch, *, hint=None, **kw):
