@@ -70,6 +70,9 @@ constexpr int kDecodeRows = 32;  // rows per kv head and sequence that the decod
 cudaError_t launch_paged_decode(const PagedAttnArgs& a, const PagedMaps& m, int dtype, int sms,
                                 cudaStream_t stream);
 int64_t paged_decode_workspace(int head_dim, int sms);
+cudaError_t launch_paged_prompt(const PagedAttnArgs& a, const PagedMaps& m, int dtype, int sms,
+                                cudaStream_t stream);
+int64_t paged_prompt_workspace(int head_dim, int sms);
 
 // Rows of sequence b, clipped to the batch's rows whatever query_start holds.
 __device__ __forceinline__ int2 paged_rows(const PagedBatch& b, int seq) {

@@ -143,7 +143,9 @@ int m5b_paged_append(const m5b_paged_append_args* s, void* stream) {
 int64_t m5b_paged_attention_workspace_bytes(int64_t head_dim) {
   int sms = 0;
   if ((head_dim != 64 && head_dim != 128) || current_device_state(nullptr, &sms)) return 0;
-  return paged_decode_workspace(static_cast<int>(head_dim), sms);
+  const int64_t few = paged_decode_workspace(static_cast<int>(head_dim), sms);
+  const int64_t many = paged_prompt_workspace(static_cast<int>(head_dim), sms);
+  return few > many ? few : many;
 }
 
 int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
@@ -175,7 +177,7 @@ int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
   a.prefix_lens = s->prefix_lens;
   const int dtype = static_cast<int>(s->b.cache_dtype);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (tiled(a, dtype) && int64_t(a.max_query_len) * a.b.group <= kDecodeRows) {
+  if (tiled(a, dtype)) {
     int sms = 0;
     rc = current_device_state(&a.status, &sms);
     if (rc) return rc;
@@ -183,9 +185,12 @@ int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
     if (!a.workspace || !grid16(a.workspace) ||
         s->workspace_bytes < m5b_paged_attention_workspace_bytes(a.b.head_dim))
       return einval("workspace of m5b_paged_attention_workspace_bytes(head_dim) bytes required");
+    const bool few = int64_t(a.max_query_len) * a.b.group <= kDecodeRows;
     PagedMaps m;
-    if (cache_maps(m, a, dtype, 64))
-      return launched(launch_paged_decode(a, m, dtype, sms, st), "paged attention launch");
+    if (cache_maps(m, a, dtype, few ? 64 : 128))
+      return launched(few ? launch_paged_decode(a, m, dtype, sms, st)
+                          : launch_paged_prompt(a, m, dtype, sms, st),
+                      "paged attention launch");
   }
   return launched(launch_paged_attention_rows(a, dtype, st),
                   "paged attention launch");

@@ -268,9 +268,9 @@ __device__ __forceinline__ void paged_write_split(PagedSplit* at, const PagedPie
   *at = m;
 }
 
-// Joins the parts of the tiles that were split: CTA (c, i) takes rows 4 i .. 4 i + 3
-// of the tile that CTA c left to others, one warp a row, the lanes across the
-// channels.
+// Joins the parts of the tiles that were split: CTA (c, i) takes every
+// gridDim.y-th four rows of the tile that CTA c left to others, one warp a
+// row, the lanes across the channels.
 template <typename T, int ROWS, int D>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnArgs a, int ctas) {
   constexpr int V = D / 32;
@@ -278,38 +278,40 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnArgs a, 
   const PagedPartials<ROWS, D> w(a.workspace, ctas);
   const int c = blockIdx.x;
   const PagedSplit m = w.split[c];
-  const int row = blockIdx.y * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (row >= m.rows || m.parts == 0) return;
-  float top = -INFINITY;
-  for (int i = lane; i < m.parts; i += 32) {
-    const int slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
-    top = fmaxf(top, w.ml[int64_t(slot) * ROWS + row].x);
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-  float sum = 0.0f, o[V] = {};
-#pragma unroll 4
-  for (int i = 0; i < m.parts; ++i) {
-    const int slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
-    const float2 ml = w.ml[int64_t(slot) * ROWS + row];
-    const float* po = w.o + (int64_t(slot) * ROWS + row) * D + lane * V;
-    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-#pragma unroll
-    for (int v = 0; v < V; v += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(po + v);
-      o[v] = fmaf(x.x, f, o[v]);
-      o[v + 1] = fmaf(x.y, f, o[v + 1]);
+  if (m.parts == 0) return;
+  const int lane = threadIdx.x % 32;
+  for (int row = blockIdx.y * 4 + threadIdx.x / 32; row < m.rows; row += gridDim.y * 4) {
+    float top = -INFINITY;
+    for (int i = lane; i < m.parts; i += 32) {
+      const int slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
+      top = fmaxf(top, w.ml[int64_t(slot) * ROWS + row].x);
     }
-  }
-  const int packed = m.first + row, t = m.row0 + packed / a.b.group;
-  const int h = m.head * a.b.group + packed % a.b.group;
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  T* out = static_cast<T*>(a.out) + t * a.o_token + h * a.o_head + lane * V;
 #pragma unroll
-  for (int v = 0; v < V; ++v) out[v] = from_f32<T>(o[v] * inv);
-  if (a.lse && lane == 0)
-    a.lse[int64_t(t) * a.b.q_heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+    float sum = 0.0f, o[V] = {};
+#pragma unroll 4
+    for (int i = 0; i < m.parts; ++i) {
+      const int slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
+      const float2 ml = w.ml[int64_t(slot) * ROWS + row];
+      const float* po = w.o + (int64_t(slot) * ROWS + row) * D + lane * V;
+      const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+      sum = fmaf(ml.y, f, sum);
+#pragma unroll
+      for (int v = 0; v < V; v += 2) {
+        const float2 x = *reinterpret_cast<const float2*>(po + v);
+        o[v] = fmaf(x.x, f, o[v]);
+        o[v + 1] = fmaf(x.y, f, o[v + 1]);
+      }
+    }
+    const int packed = m.first + row, t = m.row0 + packed / a.b.group;
+    const int h = m.head * a.b.group + packed % a.b.group;
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    T* out = static_cast<T*>(a.out) + t * a.o_token + h * a.o_head + lane * V;
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = from_f32<T>(o[v] * inv);
+    if (a.lse && lane == 0)
+      a.lse[int64_t(t) * a.b.q_heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  }
 }
 
 // Rows outside every sequence leave as zeros; `id` of `count` threads.
