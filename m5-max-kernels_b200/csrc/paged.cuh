@@ -36,6 +36,7 @@ struct PagedAppendArgs {
   const void* sin;
   int table_dtype, table_rows, rope_half, interleaved;
   void* q_out;
+  int units;  // whole 16-channel units in 16-byte accesses
 };
 
 struct PagedAttnArgs {

@@ -81,6 +81,21 @@ bool tiled(const PagedAttnArgs& a, int64_t dtype) {
   return grid16(b.k_cache) && grid16(b.v_cache) && grid16(a.q) && grid16(a.out);
 }
 
+// Whether appending can go by 16-channel units: a power of two of them makes a
+// head, the rotated part is whole units, and all rows (8 table entries too)
+// are on the 16-byte grid.  9914 rows of 32 + 8 + 8 heads of 128: 127 us by
+// channel pairs.
+bool whole_units(const PagedAppendArgs& a) {
+  const PagedBatch& b = a.b;
+  if (b.head_dim % 16 || !pow2(b.head_dim / 16) || b.head_dim > 2048 || a.rope_half % 8) return false;
+  const int64_t strides[] = {b.k_page, b.k_head, b.k_slot, b.v_page, b.v_head, b.v_slot,
+                             a.k_token, a.k_head, a.v_token, a.v_head, a.q_token, a.q_head};
+  for (int64_t s : strides)
+    if (s % 8) return false;
+  return grid16(b.k_cache) && grid16(b.v_cache) && grid16(a.q) && grid16(a.k) && grid16(a.v) &&
+         grid16(a.q_out) && (!a.rope_half || (grid16(a.cos) && grid16(a.sin)));
+}
+
 // Boxes of up to `block` slots x 64 channels of one head of one page.
 bool cache_map(CUtensorMap* map, const void* ptr, const PagedBatch& b, bool f16, int64_t page,
                int64_t head, int64_t slot, int box_rows) {
@@ -134,6 +149,7 @@ int m5b_paged_append(const m5b_paged_append_args* s, void* stream) {
   a.rope_half = static_cast<int>(s->rope_half);
   a.interleaved = s->interleaved ? 1 : 0;
   a.q_out = s->q_out;
+  a.units = whole_units(a) ? 1 : 0;
   return launched(launch_paged_append(a, static_cast<int>(s->x_dtype),
                                       static_cast<int>(s->b.cache_dtype),
                                       static_cast<cudaStream_t>(stream)),

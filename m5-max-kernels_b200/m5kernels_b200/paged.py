@@ -29,70 +29,104 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .linear import _key, _workspaces, _ws_lock
+from .linear import _workspaces, _ws_lock
 
-_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+_CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 # m5b_paged_batch, m5b_paged_append_args and m5b_paged_attention_args (include/m5b200.h):
 # every field is 8 bytes
 _PACK_APPEND = struct.Struct("@38q")
 _PACK_ATTEND = struct.Struct("@29q2d5q")
+_Tensor = torch.Tensor
+_CONTIGUOUS = torch.contiguous_format
 
 
 def _ints(t, name):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+    if not isinstance(t, _Tensor) or t.dtype is not torch.int32:
         raise ValueError(f"{name} must be an int32 tensor")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _rows(t, name, heads=None, dim=None):
-    """A [T, heads, dim] operand with contiguous channels (copied if they are not)."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 3:
+def _rows(t, name):
+    """(t, shape, strides) of a [T, heads, dim] operand, its channels made contiguous."""
+    if not isinstance(t, _Tensor) or t.dim() != 3:
         raise ValueError(f"{name} must have shape [tokens, heads, head_dim]")
-    if (heads is not None and t.shape[1] != heads) or (dim is not None and t.shape[2] != dim):
-        raise ValueError(f"{name} does not match the cache's heads and head_dim")
-    return t if t.stride(2) == 1 else t.contiguous()
+    strides = t.stride()
+    if strides[2] != 1:
+        t = t.contiguous()
+        strides = t.stride()
+    return t, t.shape, strides
 
 
 def _batch(tokens, q_heads, k_cache, v_cache, page_table, query_start, seq_lens):
-    """The fields of m5b_paged_batch and the tensors that must outlive the call."""
-    if (not isinstance(k_cache, torch.Tensor) or not isinstance(v_cache, torch.Tensor)
+    """The fields of m5b_paged_batch, the cache's shape and dtype, and the index tensors."""
+    if (not isinstance(k_cache, _Tensor) or not isinstance(v_cache, _Tensor)
             or k_cache.dim() != 4 or k_cache.shape != v_cache.shape
-            or k_cache.dtype != v_cache.dtype):
+            or k_cache.dtype is not v_cache.dtype):
         raise ValueError("k_cache and v_cache must share one [pages, kv_heads, page, head_dim] "
                          "shape and dtype")
-    if k_cache.dtype not in _FLOATS:
+    dtype = k_cache.dtype
+    code = _CODE.get(dtype)
+    if code is None:
         raise ValueError("cache dtype must be float16, bfloat16 or float32")
-    pages, kv_heads, page, dim = k_cache.shape
-    if 0 in (pages, kv_heads, page, dim):
+    shape = k_cache.shape
+    pages, kv_heads, page, dim = shape
+    if not (pages and kv_heads and page and dim):
         raise ValueError("the cache must be nonempty")
-    ks, vs = k_cache.stride(), v_cache.stride()
-    if (ks[3] != 1 or vs[3] != 1) and dim > 1:
+    kp, kh, ks, k1 = k_cache.stride()
+    vp, vh, vs, v1 = v_cache.stride()
+    if (k1 != 1 or v1 != 1) and dim > 1:
         raise ValueError("the cache's channels must be contiguous")
     query_start, seq_lens = _ints(query_start, "query_start"), _ints(seq_lens, "seq_lens")
+    page_table = _ints(page_table, "page_table")
     batch = seq_lens.numel()
     if seq_lens.dim() != 1 or batch == 0 or query_start.shape != (batch + 1,):
         raise ValueError("seq_lens must be a nonempty vector [B] and query_start [B + 1]")
-    page_table = _ints(page_table, "page_table")
     if page_table.dim() != 2 or page_table.shape[0] != batch:
         raise ValueError("page_table must have shape [B, pages per sequence]")
+    width = page_table.shape[1]
     fields = (tokens, batch, q_heads, kv_heads, dim, query_start.data_ptr(), seq_lens.data_ptr(),
-              k_cache.data_ptr(), v_cache.data_ptr(), _lib.DTYPE_CODE[k_cache.dtype], pages, page,
-              ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], page_table.data_ptr(),
-              page_table.shape[1], page_table.shape[1])
-    return fields, (query_start, seq_lens, page_table)
+              k_cache.data_ptr(), v_cache.data_ptr(), code, pages, page, kp, kh, ks, vp, vh, vs,
+              page_table.data_ptr(), width, width)
+    return fields, kv_heads, dim, dtype, [k_cache, v_cache, query_start, seq_lens, page_table]
 
 
-def _scratch(device, nbytes):
+def _call(function, args, index):
+    """Run a C-ABI call on the device `index` and torch's current stream there."""
+    if index == torch._C._cuda_getDevice():
+        check(function(args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(function(args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def _device(tensors):
+    """The CUDA device index that all the tensors share."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0:
+            return _lib.require_cuda(*tensors).index
+    return index
+
+
+_scratch_bytes: dict = {}
+
+
+def _scratch(index, dim):
     """Cached scratch of the attention kernels, one per device and stream."""
-    if nbytes <= 0:
-        return None
-    key = _key(device, "paged")
-    with _ws_lock:
-        buf = _workspaces.get(key)
-        if buf is None or buf.numel() < nbytes:
-            buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    need = _scratch_bytes.get((index, dim))
+    if need is None:
+        with torch.cuda.device(index):
+            need = int(_lib.lib().m5b_paged_attention_workspace_bytes(dim))
+        _scratch_bytes[index, dim] = need
+    if need <= 0:
+        return 0, 0
+    key = ("paged", "cuda", index, torch._C._cuda_getCurrentRawStream(index))
+    buf = _workspaces.get(key)
+    if buf is None or buf.numel() < need:
+        with _ws_lock:
+            buf = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index))
             _workspaces[key] = buf
-        return buf
+    return buf.data_ptr(), need
 
 
 def paged_append(k, v, k_cache, v_cache, page_table, query_start, seq_lens, *, cos=None, sin=None,
@@ -109,57 +143,58 @@ def paged_append(k, v, k_cache, v_cache, page_table, query_start, seq_lens, *, c
     A token at a position without a table row is not appended, and its query
     is zero.
     """
-    k = _rows(k, "k")
-    tokens = k.shape[0]
-    q_heads = k.shape[1]
+    k, (tokens, kv, width), (kt, kh, _) = _rows(k, "k")
+    v, v_shape, (vt, vh, _) = _rows(v, "v")
+    x_dtype, q_heads = k.dtype, kv
+    qt = qh = q_ptr = 0
     if q is not None:
-        q = _rows(q, "q", None, k.shape[2])
-        q_heads = q.shape[1]
-        if q.shape[0] != tokens or q.dtype != k.dtype:
-            raise ValueError("q, k and v must share tokens and dtype")
-    fields, keep = _batch(tokens, q_heads, k_cache, v_cache, page_table, query_start, seq_lens)
-    kv_heads, dim = k_cache.shape[1], k_cache.shape[3]
-    if k.shape[1] != kv_heads or k.shape[2] != dim:
+        q, q_shape, (qt, qh, _) = _rows(q, "q")
+        q_heads = q_shape[1]
+        q_ptr = q.data_ptr()
+    fields, kv_heads, dim, dtype, used = _batch(tokens, q_heads, k_cache, v_cache, page_table,
+                                                query_start, seq_lens)
+    if kv != kv_heads or width != dim:
         raise ValueError("k does not match the cache's heads and head_dim")
-    v = _rows(v, "v", kv_heads, dim)
-    if v.shape[0] != tokens or v.dtype != k.dtype:
-        raise ValueError("q, k and v must share tokens and dtype")
-    if k.dtype not in _FLOATS:
+    x_code = _CODE.get(x_dtype)
+    if x_code is None:
         raise ValueError("input dtype must be float16, bfloat16 or float32")
-    if q_heads < 1 or q_heads % kv_heads:
-        raise ValueError("q_heads must be a multiple of kv_heads")
+    if v_shape != (tokens, kv, dim) or v.dtype is not x_dtype:
+        raise ValueError("q, k and v must share tokens and dtype, v also k's heads and head_dim")
+    used += (k, v)
+    if q is not None:
+        if q_heads < 1 or q_heads % kv_heads:
+            raise ValueError("q_heads must be a multiple of kv_heads")
+        if q_shape != (tokens, q_heads, dim) or q.dtype is not x_dtype:
+            raise ValueError("q, k and v must share tokens and dtype, q also k's head_dim")
+        used.append(q)
     if layout not in ("half", "interleaved"):
         raise ValueError("layout must be 'half' or 'interleaved'")
-    half = rows = table_dtype = 0
+    half = rows = table_dtype = cos_ptr = sin_ptr = 0
     if cos is not None or sin is not None:
-        if (not isinstance(cos, torch.Tensor) or not isinstance(sin, torch.Tensor)
-                or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype
-                or cos.dtype not in _FLOATS or 0 in cos.shape):
+        if (not isinstance(cos, _Tensor) or not isinstance(sin, _Tensor)
+                or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not sin.dtype
+                or cos.dtype not in _CODE or cos.numel() == 0):
             raise ValueError("cos and sin must be matching floating tables [positions, R]")
         rows, half = cos.shape
         if 2 * half > dim:
             raise ValueError("cos and sin rotate 2 R channels, at most head_dim")
-        table_dtype = _lib.DTYPE_CODE[cos.dtype]
+        table_dtype = _CODE[cos.dtype]
         cos, sin = cos.contiguous(), sin.contiguous()
-    dev = _lib.require_cuda(k, v, q, k_cache, v_cache, *keep, cos, sin)
-    out = None
+        cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
+        used += (cos, sin)
+    index = _device(used)
+    out, out_ptr = None, 0
     if q is not None:
-        out = torch.empty((tokens, q_heads, dim), dtype=k_cache.dtype, device=dev)
-    if tokens == 0:
-        return out
-    args = _PACK_APPEND.pack(
-        *fields, 0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(),
-        _lib.DTYPE_CODE[k.dtype], 0 if q is None else q.stride(0),
-        0 if q is None else q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-        0 if cos is None else cos.data_ptr(), 0 if cos is None else sin.data_ptr(), table_dtype,
-        rows, half, layout == "interleaved", 0 if out is None else out.data_ptr())
-    check(_lib.lib().m5b_paged_append(args, _lib.stream_handle(dev)))
+        out = torch.empty_like(q, dtype=dtype, memory_format=_CONTIGUOUS)
+        out_ptr = out.data_ptr()
+    if tokens > 0:
+        _call(_lib.lib().m5b_paged_append, _PACK_APPEND.pack(
+            *fields, q_ptr, k.data_ptr(), v.data_ptr(), x_code, qt, qh, kt, kh, vt, vh, cos_ptr,
+            sin_ptr, table_dtype, rows, half, layout == "interleaved", out_ptr), index)
     return out
 
 
-def _positive(value, name, allow_none=True):
-    if value is None and allow_none:
-        return 0.0
+def _positive(value, name):
     if (isinstance(value, bool) or not isinstance(value, Real) or not math.isfinite(value)
             or value <= 0):
         raise ValueError(f"{name} must be a positive finite real scalar")
@@ -183,47 +218,56 @@ def paged_attention(q, k_cache, v_cache, page_table, query_start, seq_lens, *, m
     exp(x), -inf for a token that sees no key.  `out` may be given, any
     strides with contiguous channels.
     """
-    q = _rows(q, "q")
-    tokens, q_heads, dim = q.shape
-    fields, keep = _batch(tokens, q_heads, k_cache, v_cache, page_table, query_start, seq_lens)
-    if dim != k_cache.shape[3] or q.dtype != k_cache.dtype:
+    q, (tokens, q_heads, width), (qt, qh, _) = _rows(q, "q")
+    fields, kv_heads, dim, dtype, used = _batch(tokens, q_heads, k_cache, v_cache, page_table,
+                                                query_start, seq_lens)
+    if width != dim or q.dtype is not dtype:
         raise ValueError("q must have the cache's head_dim and dtype")
-    if q_heads < 1 or q_heads % k_cache.shape[1]:
+    if q_heads < 1 or q_heads % kv_heads:
         raise ValueError("q_heads must be a multiple of kv_heads")
     if dim > 256:
         raise NotImplementedError("head_dim above 256 is unsupported")
-    if isinstance(max_query_len, bool) or not isinstance(max_query_len, Integral) or max_query_len < 0:
+    if type(max_query_len) is not int and (isinstance(max_query_len, bool)
+                                           or not isinstance(max_query_len, Integral)):
         raise ValueError("max_query_len must be a whole number")
-    scale = dim ** -0.5 if scale is None else _positive(scale, "scale", False)
-    softcap = _positive(softcap, "softcap")
+    if max_query_len < 0:
+        raise ValueError("max_query_len must not be negative")
+    scale = dim ** -0.5 if scale is None else _positive(scale, "scale")
+    softcap = 0.0 if softcap is None else _positive(softcap, "softcap")
     if window is None:
         window = 0
     elif isinstance(window, bool) or not isinstance(window, Integral) or window < 1:
         raise ValueError("window must be a positive whole number")
+    used.append(q)
+    slopes_ptr = prefix_ptr = lse_ptr = 0
     if slopes is not None:
-        if (not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32
+        if (not isinstance(slopes, _Tensor) or slopes.dtype is not torch.float32
                 or slopes.shape != (q_heads,)):
             raise ValueError("slopes must be a float32 vector of length q_heads")
         slopes = slopes.contiguous()
+        slopes_ptr = slopes.data_ptr()
+        used.append(slopes)
     if prefix_lens is not None:
         prefix_lens = _ints(prefix_lens, "prefix_lens")
         if prefix_lens.shape != seq_lens.shape:
             raise ValueError("prefix_lens must be a vector [B]")
-    if out is not None and (not isinstance(out, torch.Tensor) or out.shape != q.shape
-                            or out.dtype != q.dtype or out.stride(2) != 1):
-        raise ValueError("out must match q, with contiguous channels")
-    dev = _lib.require_cuda(q, k_cache, v_cache, *keep, slopes, prefix_lens, out)
+        prefix_ptr = prefix_lens.data_ptr()
+        used.append(prefix_lens)
+    if out is not None:
+        if (not isinstance(out, _Tensor) or out.shape != q.shape or out.dtype is not dtype
+                or out.stride(2) != 1):
+            raise ValueError("out must match q, with contiguous channels")
+        used.append(out)
+    index = _device(used)
     if out is None:
-        out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=dev)
-    lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=dev) if return_lse else None
+        out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    lse = None
+    if return_lse:
+        lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=q.device)
+        lse_ptr = lse.data_ptr()
     if tokens > 0:
-        lib = _lib.lib()
-        ws = _scratch(dev, lib.m5b_paged_attention_workspace_bytes(dim))
-        args = _PACK_ATTEND.pack(
-            *fields, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
-            out.stride(1), 0 if lse is None else lse.data_ptr(), max_query_len, scale, softcap,
-            0 if slopes is None else slopes.data_ptr(), window,
-            0 if prefix_lens is None else prefix_lens.data_ptr(),
-            0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
-        check(lib.m5b_paged_attention(args, _lib.stream_handle(dev)))
+        ot, oh, _ = out.stride()
+        _call(_lib.lib().m5b_paged_attention, _PACK_ATTEND.pack(
+            *fields, q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, lse_ptr, max_query_len, scale,
+            softcap, slopes_ptr, window, prefix_ptr, *_scratch(index, dim)), index)
     return (out, lse) if return_lse else out
