@@ -37,6 +37,7 @@ struct PagedAppendArgs {
   int table_dtype, table_rows, rope_half, interleaved;
   void* q_out;
   int units;  // whole 16-channel units in 16-byte accesses
+  int sms;
 };
 
 struct PagedAttnArgs {

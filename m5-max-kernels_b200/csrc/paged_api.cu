@@ -81,13 +81,13 @@ bool tiled(const PagedAttnArgs& a, int64_t dtype) {
   return grid16(b.k_cache) && grid16(b.v_cache) && grid16(a.q) && grid16(a.out);
 }
 
-// Whether appending can go by 16-channel units: a power of two of them makes a
-// head, the rotated part is whole units, and all rows (8 table entries too)
-// are on the 16-byte grid.  9914 rows of 32 + 8 + 8 heads of 128: 127 us by
+// Whether appending can go by 16-channel units: heads and their rotated part
+// are whole units, and all rows (8 table entries too) are on the 16-byte grid.
+//  9914 rows of 32 + 8 + 8 heads of 128: 127 us by
 // channel pairs.
 bool whole_units(const PagedAppendArgs& a) {
   const PagedBatch& b = a.b;
-  if (b.head_dim % 16 || !pow2(b.head_dim / 16) || b.head_dim > 2048 || a.rope_half % 8) return false;
+  if (b.head_dim % 16 || b.head_dim > 1024 || a.rope_half % 8) return false;
   const int64_t strides[] = {b.k_page, b.k_head, b.k_slot, b.v_page, b.v_head, b.v_slot,
                              a.k_token, a.k_head, a.v_token, a.v_head, a.q_token, a.q_head};
   for (int64_t s : strides)
@@ -150,6 +150,7 @@ int m5b_paged_append(const m5b_paged_append_args* s, void* stream) {
   a.interleaved = s->interleaved ? 1 : 0;
   a.q_out = s->q_out;
   a.units = whole_units(a) ? 1 : 0;
+  if ((rc = current_device_state(nullptr, &a.sms))) return rc;
   return launched(launch_paged_append(a, static_cast<int>(s->x_dtype),
                                       static_cast<int>(s->b.cache_dtype),
                                       static_cast<cudaStream_t>(stream)),
