@@ -58,6 +58,7 @@ struct PagedAttnArgs {
 
 // Tensor maps of the caches, {channel, slot, head, page}, boxes of 64
 // channels x box_rows slots, 128-byte swizzle.
+constexpr int kPagedBlock = 64;  // keys of a block of the tiled kernels
 struct PagedMaps {
   CUtensorMap k, v;
   int box_rows;

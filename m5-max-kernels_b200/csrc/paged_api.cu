@@ -96,7 +96,7 @@ bool whole_units(const PagedAppendArgs& a) {
          grid16(a.q_out) && (!a.rope_half || (grid16(a.cos) && grid16(a.sin)));
 }
 
-// Boxes of up to `block` slots x 64 channels of one head of one page.
+// Boxes of up to kPagedBlock slots x 64 channels of one head of one page.
 bool cache_map(CUtensorMap* map, const void* ptr, const PagedBatch& b, bool f16, int64_t page,
                int64_t head, int64_t slot, int box_rows) {
   const uint64_t dims[4] = {uint64_t(b.head_dim), uint64_t(b.page_size), uint64_t(b.kv_heads),
@@ -106,9 +106,9 @@ bool cache_map(CUtensorMap* map, const void* ptr, const PagedBatch& b, bool f16,
   return make_swizzled_map16(map, f16, 4, ptr, dims, strides, box);
 }
 
-bool cache_maps(PagedMaps& m, const PagedAttnArgs& a, int64_t dtype, int block) {
+bool cache_maps(PagedMaps& m, const PagedAttnArgs& a, int64_t dtype) {
   const PagedBatch& b = a.b;
-  m.box_rows = b.page_size < block ? b.page_size : block;
+  m.box_rows = b.page_size < kPagedBlock ? b.page_size : kPagedBlock;
   return cache_map(&m.k, b.k_cache, b, dtype == M5B_F16, b.k_page, b.k_head, b.k_slot, m.box_rows) &&
          cache_map(&m.v, b.v_cache, b, dtype == M5B_F16, b.v_page, b.v_head, b.v_slot, m.box_rows);
 }
@@ -204,7 +204,7 @@ int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
       return einval("workspace of m5b_paged_attention_workspace_bytes(head_dim) bytes required");
     const bool few = int64_t(a.max_query_len) * a.b.group <= kDecodeRows;
     PagedMaps m;
-    if (cache_maps(m, a, dtype, few ? 64 : 128))
+    if (cache_maps(m, a, dtype))
       return launched(few ? launch_paged_decode(a, m, dtype, sms, st)
                           : launch_paged_prompt(a, m, dtype, sms, st),
                       "paged attention launch");

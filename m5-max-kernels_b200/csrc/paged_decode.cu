@@ -19,7 +19,7 @@
 namespace m5b {
 namespace {
 
-constexpr int kBlock = 64;     // keys per ring stage
+constexpr int kBlock = kPagedBlock;  // keys per ring stage
 constexpr float kGrow = 8.0f;  // log2 of the growth that m may lag behind
 
 template <int D, int MT> struct Cfg {

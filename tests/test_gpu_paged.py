@@ -100,6 +100,17 @@ def test_attention_split_over_a_long_context(ops, dim, new, ctx):
     compare(ops, Batch(new, ctx, q_heads=4, kv_heads=1, dim=dim, page=64, dtype=BF16, seed=4))
 
 
+@pytest.mark.parametrize("dim,dtype,kw", [(128, BF16, {}), (64, F16, {}),
+                                          (128, F16, dict(softcap=9.0, window=50))])
+@pytest.mark.parametrize("hint", [1, 200])
+def test_many_tiles_for_every_sm(ops, hint, dim, dtype, kw):
+    """Short and long tiles, full and half ones, one after another."""
+    new = [(7 * i * i) % 140 + 1 for i in range(40)]
+    ctx = [(11 * i) % 90 if i % 3 else 0 for i in range(40)]
+    compare(ops, Batch(new, ctx, q_heads=24, kv_heads=12, dim=dim, page=16, dtype=dtype, seed=10),
+            hint=hint, **kw)
+
+
 @pytest.mark.parametrize("kw", [{}, dict(softcap=10.0, window=100, prefix=[30, 0, 500, 64, 3, 9])])
 @pytest.mark.parametrize("hint", [0, 1, 16, 100, 5000])
 def test_the_hint_does_not_change_the_result(ops, hint, kw):
