@@ -6,17 +6,22 @@
 //   S = Q K^T          A, B from shared memory, 128 x 64 fp32 in TMEM
 //   t = S scale log2 e, p = 2^(t - m), l += sum p   one thread a row
 //   O += P V           P (the cache's type) from TMEM over S, V from shared memory
-// Roles: two warpgroups, one per half, each thread owning a row of S and O;
-// one thread issuing the MMAs in the order  PV0(s) QK0(s+2) PV1(s) QK1(s+2);
-// one warp filling a ring with K and V blocks by TMA, one box per page.  O
+// Roles: two warpgroups, one per half, each thread owning a row of S and O; one
+// thread per half issuing its MMAs, PV(s) QK(s+2) PV(s+1) ... (a wait on an
+// mbarrier costs an issuing thread some 55 cycles even when there is nothing
+// to wait for, and the tensor cores' queue holds but four to six MMAs: by one
+// thread for both halves a step took 2090 cycles); one warp filling a ring
+// with K and V blocks by TMA, one box per page; one warp finding the CTA's
+// pieces of tiles and loading their rows, one piece ahead.  O
 // takes 2 x 128 columns of TMEM, S 2 x 2 x 64: with two buffers a half, the
 // scores of step s + 1 are there when the softmax of step s ends, and neither
 // the softmax nor the tensor cores wait for a chain through the other.  (One
 // S buffer of 128 keys a half fits as well, but chains softmax -> PV -> QK ->
 // softmax: 1.64 ms against TIME for two prompts of 8192, 32 heads.)  P
-// overwrites its S.  m only follows the maximum when that has grown by more
-// than 2^8; then O is rescaled in place.  The rows of the next tile are loaded
-// during this one, into a second buffer.
+// overwrites its S.  m only follows the row's maximum when that has grown by
+// more than 2^8, which the softmax finds out after the fact: it takes the
+// exponentials with the old m, looks at the largest, and in the rare case
+// takes them again after rescaling O in place.
 //
 // Bound by shared memory's bandwidth in the products: an MMA of 128 x 64 x 16
 // reads 6 KB where its 32 cycles have 4, so that a step takes 8 * 48 + 4 * 64
@@ -29,9 +34,18 @@ namespace {
 
 constexpr int kBlock = kPagedBlock;  // keys per step
 constexpr int kRows = 256;     // packed rows per tile, two halves
-constexpr float kGrow = 8.0f;  // log2 of the growth that m may lag behind
-constexpr int kThreads = 384;  // warps 0-3, 4-7: halves; 8: MMA; 9: TMA
-constexpr int kMmaWarp = 8, kTmaWarp = 9;
+constexpr float kGrow = 8.0f;           // log2 of the growth that m may lag behind
+constexpr int kThreads = 384;  // warps 0-3, 4-7: halves; 8, 9: their MMAs; 10: K, V; 11: rows
+constexpr int kMmaWarp = 8, kTmaWarp = 10, kRowWarp = 11;
+
+// What the CTA's other warps need to know of a piece.
+struct Piece {
+  int begin, end;       // steps; end == 0: there is no piece any more
+  int pre, from;        // PagedBlocks
+  int keys, prefix, pos0;
+  int rows, first;      // packed rows of the sequence's kv head, first of the tile
+  int row0, head, whole, slot;
+};
 
 template <int D> struct Cfg {
   static constexpr int HALVES = D / 64;              // 64-channel halves of a row
@@ -43,9 +57,12 @@ template <int D> struct Cfg {
   static constexpr int SMEM = 4 * Q_BYTES + STAGES * TILE_BYTES + 1024;
   struct Small {
     uint64_t full[STAGES], empty[STAGES];
-    uint64_t q_full[2][2], s_full[2][2], p_full[2][2];  // [half][buffer]
-    uint64_t pv_done[2], o_full[2], drain;  // after every PV, after a piece's last
+    uint64_t q_full[2], q_empty[2];          // [buffer] of rows and pieces
+    uint64_t s_full[2][2], p_full[2][2];     // [half][buffer]
+    uint64_t pv_done[2], o_full[2], drain[2];  // after every PV, after a piece's last
+    uint64_t landed;                            // a V block to be blanked
     long long scratch[kThreads / 32 + 4];
+    Piece piece[2];
     uint32_t tmem;
     volatile int abort_flag;
   };
@@ -98,10 +115,11 @@ __device__ __forceinline__ float modify(float x, float softcap, float slope, int
   return (x - slope * fabsf(static_cast<float>(pos - key))) * kLog2e;
 }
 
-// One step of the MMA thread's stream: first or last of its piece, second half
-// in use.
+// One step of an MMA thread's stream: first or last of its piece, one that its
+// half takes part in, with the rows in buffer buf.
 struct Step {
-  bool valid, first, last, two;
+  bool valid, first, last, mine;
+  int buf;
 };
 
 template <typename T, int D, bool MOD>
@@ -119,18 +137,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], 1);
+      mbar_init(&sm.empty[i], 2);
     }
     for (int h = 0; h < 2; ++h) {
+      mbar_init(&sm.q_full[h], 1);
+      mbar_init(&sm.q_empty[h], 10);  // the softmax warps and the MMA threads
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&sm.q_full[h][i], 4);
         mbar_init(&sm.s_full[h][i], 1);
         mbar_init(&sm.p_full[h][i], 4);
       }
       mbar_init(&sm.pv_done[h], 1);
       mbar_init(&sm.o_full[h], 1);
+      mbar_init(&sm.drain[h], 1);
     }
-    mbar_init(&sm.drain, 1);
+    mbar_init(&sm.landed, 1);
     sm.abort_flag = 0;
     fence_mbarrier_init();
     tma_prefetch_desc(&maps.k);
@@ -152,145 +172,223 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int boxes = kBlock / maps.box_rows * C::HALVES;
     const int row = lane / C::HALVES * maps.box_rows, half = lane % C::HALVES;
     int stage = 0, phase = 0, issued = 0;
+    int blank = -1, blank_from = 0, ph_landed = 0;  // a stage whose last keys are to be blanked
     bool ok = true;
-    auto load = [&](const CUtensorMap* map, int head, int page, int slot) {
-      ok = mbar_wait_bounded(&sm.empty[stage], phase ^ 1, &sm.abort_flag, a.status,
-                             DEV_TIMEOUT_PRODUCER);
+    auto load = [&](const CUtensorMap* map, int head, int page, int slot, int live) {
+      if (ok)
+        ok = mbar_wait_bounded(&sm.empty[stage], phase ^ 1, &sm.abort_flag, a.status,
+                               DEV_TIMEOUT_PRODUCER);
       ok = __all_sync(~0u, ok);
       if (!ok) return;
-      if (lane == 0) mbar_arrive_expect_tx(&sm.full[stage], C::TILE_BYTES);
+      uint64_t* bar = live < kBlock ? &sm.landed : &sm.full[stage];
+      if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE_BYTES);
       __syncwarp();
       if (lane < boxes)
-        tma_load_4d(ring + stage * C::TILE_BYTES + half * C::HALF_BYTES + row * 128, map,
-                    &sm.full[stage], half * 64, slot, head, page);
+        tma_load_4d(ring + stage * C::TILE_BYTES + half * C::HALF_BYTES + row * 128, map, bar,
+                    half * 64, slot, head, page);
+      if (live < kBlock) blank = stage, blank_from = max(live, 0);
       ++issued;
       if (++stage == STAGES) stage = 0, phase ^= 1;
     };
+    // Slots behind the sequence's end may hold NaN, which a zero probability
+    // would not stop: V blocks that reach there land here first and are
+    // blanked, while the K block after them is on its way.
+    auto finish = [&]() {
+      if (blank < 0) return;
+      if (ok)
+        ok = mbar_wait_bounded(&sm.landed, ph_landed, &sm.abort_flag, a.status,
+                               DEV_TIMEOUT_PRODUCER);
+      ok = __all_sync(~0u, ok);
+      if (!ok) return;
+      ph_landed ^= 1;
+      uint8_t* v = ring + blank * C::TILE_BYTES;
+      for (int i = blank_from * C::HALVES * 8 + lane; i < kBlock * C::HALVES * 8; i += 32)
+        *reinterpret_cast<uint4*>(v + (i / 8 % C::HALVES) * C::HALF_BYTES + i / (C::HALVES * 8) * 128 +
+                                  i % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.full[blank]);
+      blank = -1;
+    };
     PagedPiece p;
-    int head = -1, page = 0, slot = 0;  // of the step before
+    int head = -1, page = 0, slot = 0, live = 0;  // of the step before
     while (ok && walk.next(a, p)) {
       for (int i = p.begin; ok && i < p.end; ++i) {
-        const int key = p.r.at(i) * kBlock + row;
+        const int block0 = p.r.at(i) * kBlock, key = block0 + row;
         int page2 = a.b.num_pages, slot2 = 0;  // out of range: zeros
         if (lane < boxes && key < p.s.keys) {
           const int at = paged_page(a.b, p.seq, key);
           if (at >= 0) page2 = at;
           slot2 = key % a.b.page_size;
         }
-        load(&maps.k, p.head, page2, slot2);
-        if (ok && head >= 0) load(&maps.v, head, page, slot);
-        head = p.head, page = page2, slot = slot2;
+        load(&maps.k, p.head, page2, slot2, kBlock);
+        finish();
+        if (head >= 0) load(&maps.v, head, page, slot, live);
+        head = p.head, page = page2, slot = slot2, live = p.s.keys - block0;
       }
     }
-    if (ok && head >= 0) load(&maps.v, head, page, slot);
+    finish();
+    if (head >= 0) load(&maps.v, head, page, slot, live);
+    finish();
     if (!ok) {  // let the copies in flight land before the CTA ends
       for (int i = 0; i < STAGES && i < issued; ++i) {
         if (--stage < 0) stage = STAGES - 1, phase ^= 1;
         const unsigned long long start = globaltimer_ns();
-        while (!mbar_try_wait(&sm.full[stage], phase) && globaltimer_ns() - start < kWaitLimitNs) {
+        while (!(stage == blank ? mbar_try_wait(&sm.landed, ph_landed)
+                                : mbar_try_wait(&sm.full[stage], phase)) &&
+               globaltimer_ns() - start < kWaitLimitNs) {
         }
       }
     }
-  } else if (warp == kMmaWarp) {  // ---- matrix products, all by one thread
+  } else if (warp == kRowWarp) {  // ---- pieces and their rows
+    constexpr int CH = D / 8;  // 16-byte chunks of a row
+    const int chunk = lane % CH;
+    bool ok = true, any = false;
+    PagedPiece p;
+    for (int n = 0; ok; ++n) {
+      const int buf = n & 1;
+      const bool more = walk.next(a, p);
+      any |= more;
+      ok = mbar_wait_bounded(&sm.q_empty[buf], (n >> 1 & 1) ^ 1, &sm.abort_flag, a.status,
+                             DEV_TIMEOUT_PRODUCER);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      const int rows = p.s.n * group, first = p.rt * kRows;
+      if (more) {
+        const int here = min(rows - first, kRows), all = here > 128 ? kRows : 128;
+        int r = lane / CH, tok = (first + r) / group, g = (first + r) % group;
+        for (; r < all; r += 32 / CH) {
+          const bool in = r < here;
+          const T* src = static_cast<const T*>(a.q) + int64_t(p.s.row0 + (in ? tok : 0)) * a.q_token +
+                         (p.head * group + g) * a.q_head + chunk * 8;
+          cp_async16(smem_u32(q_smem + buf * 2 * C::Q_BYTES + (r / 128) * C::Q_BYTES +
+                              (chunk / 8) * C::Q_HALF + (r % 128) * 128 +
+                              (((chunk % 8) ^ (r & 7)) << 4)), src, in);
+          for (g += 32 / CH; g >= group; g -= group) ++tok;
+        }
+      }
+      if (lane == 0) {
+        Piece d{};
+        if (more) {
+          d.begin = p.begin;
+          d.end = p.end;
+          d.pre = p.r.pre;
+          d.from = p.r.from;
+          d.keys = p.s.keys;
+          d.prefix = p.s.prefix;
+          d.pos0 = p.s.pos0;
+          d.rows = rows;
+          d.first = first;
+          d.row0 = p.s.row0;
+          d.head = p.head;
+          d.whole = p.whole();
+          d.slot = 2 * blockIdx.x + (p.begin == 0 ? 1 : 0);
+        }
+        sm.piece[buf] = d;
+      }
+      cp_async_wait_all();
+      fence_proxy_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_full[buf]);
+      if (!more) break;
+    }
+    if (lane == 0)  // (p is the last piece)
+      paged_write_split(&PagedPartials<kRows, D>(a.workspace, gridDim.x).split[blockIdx.x],
+                        any ? &p : nullptr, walk.share, kRows, group);
+  } else if (warp >= kMmaWarp) {  // ---- matrix products of half h, by one thread
+    const int h = warp - kMmaWarp;
     if (elect_one()) {
       constexpr int kind = DTypeOf<T>::value == DT_BF16 ? KIND_BF16 : KIND_F16;
       constexpr uint32_t idesc_s = make_idesc(kind, 128, kBlock);
       constexpr uint32_t idesc_o = make_idesc(kind, 128, D) | (1u << 16);  // B is MN-major
-      const uint64_t q_desc = smem_desc_k128(smem_u32(q_smem));
+      const uint64_t q_desc = smem_desc_k128(smem_u32(q_smem + h * C::Q_BYTES));
       const uint64_t k_desc = smem_desc_k128(smem_u32(ring));
       const uint64_t v_desc = smem_desc_mn128(smem_u32(ring), C::HALF_BYTES);
+      const uint32_t t_s = tmem + kColS + h * 128, t_o = tmem + kColO + h * 128;
       int stage = 0, phase = 0;
-      int qt[2] = {0, 0}, si[2] = {0, 0}, pi[2] = {0, 0};  // pieces, QK and PV steps of the halves
-      bool ok = true;
+      int piece = -1, si = 0, pi = 0;  // QK and PV steps of this half
+      int left = 0;  // steps of the piece
+      bool ok = true, mine = false, ended = false;
       auto wait = [&](uint64_t* bar, int parity) {
         if (ok) ok = mbar_wait_bounded(bar, parity, &sm.abort_flag, a.status, DEV_TIMEOUT_MMA);
-        return ok;
+        tc_fence_after();
       };
-      PagedPiece p{};
-      int at = 0;
-      bool open = false;
       auto advance = [&]() {
         Step s{};
-        if (!open || at == p.end) {
-          open = walk.next(a, p);
-          if (!open) return s;
-          at = p.begin;
+        if (ended) return s;
+        if (left == 0) {
+          ++piece;
+          wait(&sm.q_full[piece & 1], piece >> 1 & 1);
+          if (ok) {
+            const Piece& d = sm.piece[piece & 1];
+            left = d.end - d.begin;
+            mine = h == 0 || d.rows - d.first > 128;
+            mbar_arrive(&sm.q_empty[piece & 1]);
+          }
+          ended = !ok || left == 0;
+          if (ended) return s;
+          s.first = true;
         }
         s.valid = true;
-        s.first = at == p.begin;
-        s.two = p.s.n * group - p.rt * kRows > 128;
-        s.last = ++at == p.end;
+        s.mine = mine;
+        s.buf = piece & 1;
+        s.last = --left == 0;
         return s;
       };
-      auto take = [&](int& st) {  // the next stage of the ring, filled
-        st = stage;
-        wait(&sm.full[stage], phase);
+      // The next stage of the ring, once it is filled, for a step of this half
+      // or of the other alone.
+      auto use = [&](bool mine, auto&& products) {
+        const int st = stage;
+        wait(&sm.full[st], phase);
         if (++stage == STAGES) stage = 0, phase ^= 1;
-        tc_fence_after();
-      };
-      auto qk = [&](int h, int st, const Step& s) {  // S_h = Q_h K^T
-        if (s.first) {
-          wait(&sm.q_full[h][qt[h] & 1], (qt[h] >> 1) & 1);
-          ++qt[h];
-          tc_fence_after();
+        if (mine && ok) {
+          products(st * C::TILE_BYTES >> 4);
+          tc_commit(&sm.empty[st]);
+        } else {
+          mbar_arrive(&sm.empty[st]);
         }
-        if (!ok) return;
-        const int buf = si[h]++ & 1;
-        const uint64_t qd = q_desc + ((((qt[h] - 1) & 1) * 2 + h) * C::Q_BYTES >> 4);
-        const uint64_t kd = k_desc + (st * C::TILE_BYTES >> 4);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          tc_mma<KIND_F16>(tmem + kColS + h * 128 + buf * 64,
-                           qd + (((k / 4) * C::Q_HALF + (k % 4) * 32) >> 4),
-                           kd + (((k / 4) * C::HALF_BYTES + (k % 4) * 32) >> 4), idesc_s, k > 0);
-        tc_commit(&sm.s_full[h][buf]);
       };
-      auto pv = [&](int h, int st, const Step& s) {  // O_h (+)= P_h V
-        const int buf = pi[h] & 1;
-        wait(&sm.p_full[h][buf], (pi[h] >> 1) & 1);
-        ++pi[h];
-        tc_fence_after();
-        if (!ok) return;
-        const uint64_t vd = v_desc + (st * C::TILE_BYTES >> 4);
+      auto qk = [&](const Step& s) {  // S = Q K^T
+        use(s.mine, [&](int off) {
+          const int buf = si++ & 1;
+          const uint64_t qd = q_desc + (s.buf * 2 * C::Q_BYTES >> 4), kd = k_desc + off;
 #pragma unroll
-        for (int k = 0; k < kBlock / 16; ++k)
-          tc_mma_ts(tmem + kColO + h * 128, tmem + kColS + h * 128 + buf * 64 + k * 8,
-                    vd + (k * 2048 >> 4), idesc_o, !s.first || k > 0);
-        tc_commit(&sm.pv_done[h]);
-        if (s.last) tc_commit(&sm.o_full[h]);
+          for (int k = 0; k < D / 16; ++k)
+            tc_mma<KIND_F16>(t_s + buf * 64, qd + (((k / 4) * C::Q_HALF + (k % 4) * 32) >> 4),
+                             kd + (((k / 4) * C::HALF_BYTES + (k % 4) * 32) >> 4), idesc_s, k > 0);
+          tc_commit(&sm.s_full[h][buf]);
+        });
       };
-
-      Step cur = advance(), nx1 = advance();
-      int ks = 0, vs = 0;
-      for (int i = 0; i < 2; ++i) {
-        const Step& s = i ? nx1 : cur;
-        if (!ok || !s.valid) break;
-        take(ks);
-        qk(0, ks, s);
-        if (s.two) qk(1, ks, s);
-        tc_commit(&sm.empty[ks]);
-      }
+      auto pv = [&](const Step& s) {  // O (+)= P V
+        use(s.mine, [&](int off) {
+          const int buf = pi & 1;
+          wait(&sm.p_full[h][buf], (pi >> 1) & 1);
+          ++pi;
+          const uint64_t vd = v_desc + off;
+#pragma unroll
+          for (int k = 0; k < kBlock / 16; ++k)
+            tc_mma_ts(t_o, t_s + buf * 64 + k * 8, vd + (k * 2048 >> 4), idesc_o, !s.first || k > 0);
+          tc_commit(&sm.pv_done[h]);
+          if (s.last) tc_commit(&sm.o_full[h]);
+        });
+      };
+      Step cur = advance();
+      if (cur.valid) qk(cur);
+      Step nx1 = advance();
+      if (nx1.valid) qk(nx1);
       while (ok && cur.valid) {
+        pv(cur);
+        // (a piece's rows may have to wait for the softmax of the piece two
+        // before, which needs this PV)
         const Step nx2 = advance();
-        take(vs);
-        pv(0, vs, cur);
-        if (nx2.valid) {
-          take(ks);
-          qk(0, ks, nx2);
-        }
-        if (cur.two) pv(1, vs, cur);
-        tc_commit(&sm.empty[vs]);
-        if (nx2.valid) {
-          if (nx2.two) qk(1, ks, nx2);
-          tc_commit(&sm.empty[ks]);
-        }
+        if (nx2.valid) qk(nx2);
         cur = nx1;
         nx1 = nx2;
       }
       // every MMA has retired before TMEM is freed
-      tc_commit(&sm.drain);
+      tc_commit(&sm.drain[h]);
       const unsigned long long start = globaltimer_ns();
-      while (!mbar_try_wait(&sm.drain, 0)) {
+      while (!mbar_try_wait(&sm.drain[h], 0)) {
         if (globaltimer_ns() - start > kWaitLimitNs) {
           atomicOr(a.status, DEV_TIMEOUT_DRAIN);
           break;
@@ -298,68 +396,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp < kMmaWarp) {  // ---- softmax: thread `row` of half h
+  } else {  // ---- softmax: thread `row` of half h
     const int h = warp / 4;
     const int row = threadIdx.x % 128;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
     const uint32_t t_s = lanes + kColS + h * 128, t_o = lanes + kColO + h * 128;
-    const PagedPartials<kRows, D> parts(a.workspace, gridDim.x);
-    const float c = a.scale * kLog2e;
-    int step = 0, piece = 0;  // of this half
-    bool ok = true, any = false;
+    const float c = MOD ? 1.0f : a.scale * kLog2e;
+    int step = 0, outs = 0;  // steps and pieces of this half
+    bool ok = true;
     auto wait = [&](uint64_t* bar, int parity) {
       ok = mbar_wait_bounded(bar, parity, &sm.abort_flag, a.status, DEV_TIMEOUT_EPILOGUE);
       ok = __all_sync(~0u, ok);
       tc_fence_after();
       return ok;
     };
-    // Row `row` of a piece into the buffer of the half's piece number n.
-    auto fetch = [&](const PagedPiece& p, int n) {
-      const int packed = p.rt * kRows + h * 128 + row, rows = p.s.n * group;
-      const bool in = packed < rows;
-      const int tok = (in ? packed : rows - 1) / group, qh = p.head * group + packed % group;
-      const T* src = static_cast<const T*>(a.q) + int64_t(p.s.row0 + tok) * a.q_token + qh * a.q_head;
-      const uint32_t dst = smem_u32(q_smem + ((n & 1) * 2 + h) * C::Q_BYTES) + row * 128;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-        cp_async16(dst + (i / 8) * C::Q_HALF + (((i % 8) ^ (row & 7)) << 4), src + i * 8, in);
-    };
-    auto fetched = [&](int n) {
-      cp_async_wait_all();
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.q_full[h][n & 1]);
-    };
-    // The next piece with rows for this half (the first half has some in all).
-    auto next = [&](PagedPiece& p) {
-      while (walk.next(a, p))
-        if (h == 0 || p.s.n * group - p.rt * kRows > 128) return true;
-      return false;
-    };
-    PagedPiece p, pn;
-    bool have = next(p);
-    if (have) {
-      fetch(p, 0);
-      fetched(0);
-    }
-    while (have && ok) {
-      any = true;
-      const int rows = p.s.n * group, packed = p.rt * kRows + h * 128 + row;
-      const int tok = min(packed, rows - 1) / group;
-      const int pos = p.s.pos0 + tok;
-      const float slope = MOD && a.slopes && packed < rows
-                              ? a.slopes[p.head * group + packed % group] : 0.0f;
-      const int pos_lo = p.s.pos0 + (p.rt * kRows + h * 128) / group;
-      const int pos_hi = p.s.pos0 + min(p.rt * kRows + h * 128 + 127, rows - 1) / group;
+    for (int piece = 0;; ++piece) {
+      const int qb = piece & 1;
+      if (!wait(&sm.q_full[qb], piece >> 1 & 1)) break;
+      const Piece& d = sm.piece[qb];
+      const int end = d.end, packed = d.first + h * 128 + row;
+      if (end == 0) break;
+      if (d.rows - d.first <= h * 128) {  // no rows for this half
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_empty[qb]);
+        continue;
+      }
+      const int tok = min(packed, d.rows - 1) / group, head = d.head * group + packed % group;
+      const int pos = d.pos0 + tok;
+      const float slope = MOD && a.slopes && packed < d.rows ? a.slopes[head] : 0.0f;
+      const int pre = d.pre, from = d.from, prefix = d.prefix;
+      // this row sees keys [0, prefix) and [row_lo, row_hi]; all rows see [all_lo, all_hi]
+      const int row_lo = pos >= a.window ? pos - a.window + 1 : 0, row_hi = min(pos, d.keys - 1);
+      const int pos_lo = d.pos0 + (d.first + h * 128) / group;
+      const int pos_hi = d.pos0 + min(d.first + h * 128 + 127, d.rows - 1) / group;
+      const int all_lo = pos_hi >= a.window ? pos_hi - a.window + 1 : 0, all_hi = min(pos_lo, d.keys - 1);
+      const int begin = d.begin;
       float m = -INFINITY, l = 0.0f;
-      bool more = false;
-      for (int i = p.begin; i < p.end; ++i, ++step) {
-        const int block0 = p.r.at(i) * kBlock, buf = step & 1;
+      for (int i = begin; i < end; ++i, ++step) {
+        const int block0 = (i < pre ? i : from + i - pre) * kBlock, buf = step & 1;
         if (!wait(&sm.s_full[h][buf], (step >> 1) & 1)) break;
-        if (i == p.begin) {  // the products with the last piece's rows are done
-          more = next(pn);
-          if (more) fetch(pn, piece + 1);
-        }
         uint32_t s[2][32];
         tmem_ld32(t_s + buf * 64, s[0]);
         tmem_ld32(t_s + buf * 64 + 32, s[1]);
@@ -370,126 +445,141 @@ __global__ void __launch_bounds__(kThreads, 1)
             s[e / 32][e % 32] = __float_as_uint(modify(__uint_as_float(s[e / 32][e % 32]) * a.scale,
                                                        a.softcap, slope, pos, block0 + e));
         }
-        const bool open = block0 + kBlock <= p.s.keys &&
-                          (block0 + kBlock <= p.s.prefix ||
-                           (block0 + kBlock - 1 <= pos_lo && pos_hi - block0 < a.window));
-        if (!open) {
-          const int hi = min(pos, p.s.keys - 1) - block0;
-          const int lo = (pos >= a.window ? pos - a.window + 1 : 0) - block0;
-          const int pre = p.s.prefix - block0;
+        if (!(block0 + kBlock <= prefix || (block0 >= all_lo && block0 + kBlock - 1 <= all_hi))) {
+          const int hi = row_hi - block0, lo = row_lo - block0, pr = prefix - block0;
 #pragma unroll
           for (int e = 0; e < kBlock; ++e)
-            if (!(e < pre || (e <= hi && e >= lo))) s[e / 32][e % 32] = 0xff800000u;
-          if (h == 0 && block0 + kBlock > p.s.keys) {
-            // slots behind the sequence's end may hold NaN, which a zero
-            // probability would not stop: blank them before PV is issued.  (V
-            // of step s is the ring's load 2 s + 2, but for the last step.)
-            const int at = 2 * step + (i + 1 == p.end && !more ? 1 : 2);
-            if (!wait(&sm.full[at % STAGES], (at / STAGES) & 1)) break;
-            const int dead = row / 2;  // two threads a key
-            if (block0 + dead >= p.s.keys)
-              for (int k = row % 2; k < C::HALVES * 8; k += 2)
-                *reinterpret_cast<uint4*>(ring + (at % STAGES) * C::TILE_BYTES +
-                                          (k / 8) * C::HALF_BYTES + dead * 128 + (k % 8) * 16) =
-                    make_uint4(0u, 0u, 0u, 0u);
-            fence_proxy_async_shared();
-          }
+            if (!(e < pr || (e <= hi && e >= lo))) s[e / 32][e % 32] = 0xff800000u;
         }
-        float top[4];
+        uint32_t pk[32];
+        float2 sum[2];
+        float over;  // the largest t - m
+        auto exponentials = [&]() {
+          const float base = m == -INFINITY ? 0.0f : -m;
+          const float2 c2 = make_float2(c, c), b2 = make_float2(base, base);
+          float top[2] = {-INFINITY, -INFINITY};
+          sum[0] = sum[1] = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          top[q] = __uint_as_float(s[q / 2][(q % 2) * 16]);
+          for (int e = 0; e < 32; e += 8) {  // (16 at a time, to have them in flight)
+            float2 x[8];
 #pragma unroll
-          for (int e = 1; e < 16; ++e)
-            top[q] = fmaxf(top[q], __uint_as_float(s[q / 2][(q % 2) * 16 + e]));
-        }
-        float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        if (!MOD) high *= c;
-        const bool grow = high > m + kGrow;
-        if (__any_sync(~0u, grow)) {
-          const float m2 = grow ? high : m;
-          const float f = m == -INFINITY ? 0.0f : ex2(m - m2);
-          m = m2;
-          l *= f;
-          if (i > p.begin) {
-            // O holds the steps before this one, once they are done.  (S of
-            // this step says so of all but the last, so that the parity is
-            // not two phases off.)
-            if (!wait(&sm.pv_done[h], (step - 1) & 1)) break;
-            uint32_t o[32];
+            for (int k = 0; k < 8; ++k) {
+              const int at = 2 * (e + k);
+              x[k] = __ffma2_rn(make_float2(__uint_as_float(s[at / 32][at % 32]),
+                                            __uint_as_float(s[at / 32][at % 32 + 1])), c2, b2);
+            }
 #pragma unroll
-            for (int q = 0; q < D / 32; ++q) {
-              tmem_ld32(t_o + q * 32, o);
-              tmem_wait_ld();
+            for (int k = 0; k < 8; ++k) top[k & 1] = fmaxf(top[k & 1], fmaxf(x[k].x, x[k].y));
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st32(t_o + q * 32, o);
+            for (int k = 0; k < 8; ++k) x[k] = make_float2(ex2(x[k].x), ex2(x[k].y));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              sum[k & 1] = __fadd2_rn(sum[k & 1], x[k]);
+              pk[e + k] = pack2<T>(x[k].x, x[k].y);
             }
           }
-        }
-        const float base = m == -INFINITY ? 0.0f : m;
-        float2 sum[2] = {};
-        const float2 c2 = make_float2(c, c), b2 = make_float2(-base, -base);
-        uint32_t pk[32];
+          over = fmaxf(top[0], top[1]);
+        };
+        auto maximum = [&]() {
+          float top[4];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float2 x = make_float2(__uint_as_float(s[e / 16][(2 * e) % 32]),
-                                 __uint_as_float(s[e / 16][(2 * e) % 32 + 1]));
-          x = MOD ? __fadd2_rn(x, b2) : __ffma2_rn(x, c2, b2);
-          x.x = ex2(x.x);
-          x.y = ex2(x.y);
-          sum[e & 1] = __fadd2_rn(sum[e & 1], x);
-          pk[e] = pack2<T>(x.x, x.y);
+          for (int q = 0; q < 4; ++q) {
+            top[q] = __uint_as_float(s[q / 2][(q % 2) * 16]);
+#pragma unroll
+            for (int e = 1; e < 16; ++e)
+              top[q] = fmaxf(top[q], __uint_as_float(s[q / 2][(q % 2) * 16 + e]));
+          }
+          return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+        };
+        if (i == begin) m = maximum();
+        exponentials();
+        // (a row without any key so far has no m yet)
+        if (__any_sync(~0u, over > (m == -INFINITY ? -INFINITY : kGrow))) {
+          // O holds the steps before this one, once they are done.  (S of this
+          // step says so of all but the last, so that the parity is not two
+          // phases off.)
+          if (!wait(&sm.pv_done[h], (step - 1) & 1)) break;
+          const float m2 = fmaxf(m, maximum()), f = m == -INFINITY ? 0.0f : ex2(m - m2);
+          m = m2;
+          l *= f;
+          uint32_t o[32];
+#pragma unroll
+          for (int q = 0; q < D / 32; ++q) {
+            tmem_ld32(t_o + q * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st32(t_o + q * 32, o);
+          }
+          exponentials();
         }
-        tmem_st32(t_s + buf * 64, pk);
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        tmem_st32(t_s + buf * 64, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.p_full[h][buf]);
-        if (i == p.begin && more) fetched(piece + 1);
       }
       if (!ok) break;
 
-      if (!wait(&sm.o_full[h], piece & 1)) break;
-      const bool whole = p.whole(), in = packed < rows;
-      const float inv = whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
-      const int qh = p.head * group + packed % group;
-      const int64_t t = p.s.row0 + tok;
-      T* out = static_cast<T*>(a.out) + t * a.o_token + qh * a.o_head;
-      const int64_t part = (2 * int64_t(blockIdx.x) + (p.begin == 0 ? 1 : 0)) * kRows + h * 128 + row;
+      if (!wait(&sm.o_full[h], outs++ & 1)) break;
+      const bool in = packed < d.rows;
+      const int64_t t = d.row0 + tok;
+      if (d.whole) {
+        // by way of the rows' buffer, which is done with: a thread has a row,
+        // a row's stores shall be whole lines
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        uint8_t* const stage = q_smem + (qb * 2 + h) * C::Q_BYTES;
 #pragma unroll
-      for (int q = 0; q < D / 32; ++q) {
-        uint32_t o[32];
-        tmem_ld32(t_o + q * 32, o);
-        tmem_wait_ld();
-        if (!in) continue;
-        if (whole) {
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
+          tmem_ld32(t_o + q * 32, o);
+          tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
+          for (int e = 0; e < 4; ++e) {
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              w[k] = pack2<T>(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
-            *reinterpret_cast<uint4*>(out + q * 32 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              w[k] = pack2<T>(__uint_as_float(o[e * 8 + 2 * k]) * inv,
+                              __uint_as_float(o[e * 8 + 2 * k + 1]) * inv);
+            const int chunk = q * 4 + e;
+            *reinterpret_cast<uint4*>(stage + (chunk / 8) * C::Q_HALF + row * 128 +
+                                      (((chunk % 8) ^ (row & 7)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
           }
-        } else {
+        }
+        if (in && a.lse) a.lse[t * a.b.q_heads + head] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        __syncwarp();
+        constexpr int CH = D / 8;
+        const long long at = in ? t * a.o_token + head * a.o_head : -1;
+#pragma unroll 4
+        for (int i = 0; i < CH; ++i) {
+          const int r = i * (32 / CH) + lane / CH, chunk = lane % CH, from_row = (warp % 4) * 32 + r;
+          const long long to = __shfl_sync(~0u, at, r);
+          const uint4 w = *reinterpret_cast<const uint4*>(
+              stage + (chunk / 8) * C::Q_HALF + from_row * 128 + (((chunk % 8) ^ (from_row & 7)) << 4));
+          if (to >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to + chunk * 8) = w;
+        }
+      } else {
+        const PagedPartials<kRows, D> parts(a.workspace, gridDim.x);
+        float* o_part = parts.o + int64_t(d.slot) * kRows * D + (h * 128 + row) * 4;
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
+          tmem_ld32(t_o + q * 32, o);
+          tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(parts.o + part * D + q * 32 + e) =
-                make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            if (in)
+              *reinterpret_cast<uint4*>(o_part + (q * 8 + e / 4) * (kRows * 4)) =
+                  make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
+        if (in) parts.ml[int64_t(d.slot) * kRows + h * 128 + row] = make_float2(m, l);
       }
-      if (in && whole && a.lse)
-        a.lse[t * a.b.q_heads + qh] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
-      if (in && !whole) parts.ml[part] = make_float2(m, l);
       tc_fence_before();
-      if (!more) break;
-      p = pn;
-      ++piece;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_empty[qb]);
     }
-    if (h == 0 && row == 0)  // (p is the CTA's last piece)
-      paged_write_split(&parts.split[blockIdx.x], any ? &p : nullptr, walk.share, kRows, group);
     paged_zero_outside<T, D>(a, int64_t(blockIdx.x) * 256 + threadIdx.x, int64_t(gridDim.x) * 256);
   }
   __syncthreads();
@@ -517,10 +607,10 @@ cudaError_t launch(const PagedAttnArgs& a, const PagedMaps& m, int sms, cudaStre
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kern, a, m);
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3(static_cast<unsigned>(sms), 16);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(static_cast<unsigned>(sms), D / 16);
+  cfg.blockDim = dim3(kRows);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, kRows, D>, a, sms);
+  return cudaLaunchKernelEx(&cfg, paged_join_columns_kernel<T, kRows, D>, a, sms);
 }
 
 template <typename T, int D>

@@ -242,7 +242,7 @@ template <int ROWS, int D>
 struct PagedPartials {
   PagedSplit* split;  // [ctas]
   float2* ml;         // [2 ctas][ROWS]: maximum (in log2 units) and sum
-  float* o;           // [2 ctas][ROWS][D]
+  float* o;           // [2 ctas][ROWS][D], or [2 ctas][D / 4][ROWS][4]
   __host__ __device__ PagedPartials(void* ws, int ctas) {
     split = static_cast<PagedSplit*>(ws);
     ml = reinterpret_cast<float2*>(split + (ctas + 7) / 8 * 8);
@@ -312,6 +312,48 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnArgs a, 
     if (a.lse && lane == 0)
       a.lse[int64_t(t) * a.b.q_heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
   }
+}
+
+// The same for parts stored by columns, [D / 4][ROWS][4]: CTA (c, i) takes
+// channels 16 i .. 16 i + 15, a thread a row.
+template <typename T, int ROWS, int D>
+__global__ void __launch_bounds__(ROWS) paged_join_columns_kernel(const PagedAttnArgs a, int ctas) {
+  grid_dependency_wait();
+  const PagedPartials<ROWS, D> w(a.workspace, ctas);
+  const int c = blockIdx.x, row = threadIdx.x;
+  const PagedSplit m = w.split[c];
+  if (row >= m.rows || m.parts == 0) return;
+  float top = -INFINITY, sum = 0.0f, o[16] = {};
+  for (int i = 0; i < m.parts; ++i)
+    top = fmaxf(top, w.ml[int64_t(i == 0 ? 2 * c + 1 : 2 * (c + i)) * ROWS + row].x);
+#pragma unroll 2
+  for (int i = 0; i < m.parts; ++i) {
+    const int64_t slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
+    const float2 ml = w.ml[slot * ROWS + row];
+    const float4* po = reinterpret_cast<const float4*>(w.o + slot * ROWS * D) + blockIdx.y * 4 * ROWS + row;
+    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 x = po[k * ROWS];
+      o[4 * k] = fmaf(x.x, f, o[4 * k]);
+      o[4 * k + 1] = fmaf(x.y, f, o[4 * k + 1]);
+      o[4 * k + 2] = fmaf(x.z, f, o[4 * k + 2]);
+      o[4 * k + 3] = fmaf(x.w, f, o[4 * k + 3]);
+    }
+  }
+  const int packed = m.first + row, t = m.row0 + packed / a.b.group;
+  const int h = m.head * a.b.group + packed % a.b.group;
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  __align__(16) T y[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) y[k] = from_f32<T>(o[k] * inv);
+  uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + t * a.o_token + h * a.o_head +
+                                        blockIdx.y * 16);
+  out[0] = *reinterpret_cast<const uint4*>(y);
+  out[1] = *reinterpret_cast<const uint4*>(y + 8);
+  if (a.lse && blockIdx.y == 0)
+    a.lse[int64_t(t) * a.b.q_heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
 // Rows outside every sequence leave as zeros; `id` of `count` threads.
