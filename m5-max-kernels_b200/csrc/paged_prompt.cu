@@ -35,6 +35,7 @@ namespace {
 constexpr int kBlock = kPagedBlock;  // keys per step
 constexpr int kRows = 256;     // packed rows per tile, two halves
 constexpr float kGrow = 8.0f;           // log2 of the growth that m may lag behind
+constexpr int kFmaPairs = 3;             // of 8 pairs of exponentials, those by ex2_fma
 constexpr int kThreads = 384;  // warps 0-3, 4-7: halves; 8, 9: their MMAs; 10: K, V; 11: rows
 constexpr int kMmaWarp = 8, kTmaWarp = 10, kRowWarp = 11;
 
@@ -108,6 +109,35 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool i
 __device__ __forceinline__ void cp_async_wait_all() {
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
+// 2^x of a pair on the FMA pipes, for x < 100: x = n + f with n the nearest
+// integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a polynomial,
+// n added to its exponent.  The coefficients are the minimax fit of the
+// relative error on [-1/2, 1/2] (Remez exchange): 7.5e-5 with four, for bf16
+// probabilities (their rounding: up to 3.9e-3), 2.6e-6 with five, for fp16
+// (4.9e-4).  Below -126 the result stays near 2^-126, not zero: a row that saw
+// no key is known by its m.
+template <typename T> __device__ __forceinline__ float2 ex2_fma(float2 x) {
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 big = make_float2(12582912.0f, 12582912.0f);
+  const float2 neg = make_float2(-12582912.0f, -12582912.0f), one = make_float2(-1.0f, -1.0f);
+  const float2 r = __fadd2_rn(x, big);
+  const float2 f = __ffma2_rn(__fadd2_rn(r, neg), one, x);
+  float2 p;
+  if (DTypeOf<T>::value == DT_BF16) {
+    p = __ffma2_rn(make_float2(0x1.c3f76p-5f, 0x1.c3f76p-5f), f, make_float2(0x1.f0de1ap-3f, 0x1.f0de1ap-3f));
+    p = __ffma2_rn(p, f, make_float2(0x1.62f31ap-1f, 0x1.62f31ap-1f));
+    p = __ffma2_rn(p, f, make_float2(0x1.fff692p-1f, 0x1.fff692p-1f));
+  } else {
+    p = __ffma2_rn(make_float2(0x1.3997d6p-7f, 0x1.3997d6p-7f), f, make_float2(0x1.ca144p-5f, 0x1.ca144p-5f));
+    p = __ffma2_rn(p, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+    p = __ffma2_rn(p, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+    p = __ffma2_rn(p, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  }
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
+}
+
 // x of one score: capped and biased, in log2 units.
 __device__ __forceinline__ float modify(float x, float softcap, float slope, int pos, int key) {
   if (softcap > 0.0f)  // tanh(y) = 1 - 2 / (e^2y + 1)
@@ -405,8 +435,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     int step = 0, outs = 0;  // steps and pieces of this half
     bool ok = true;
     auto wait = [&](uint64_t* bar, int parity) {
-      ok = mbar_wait_bounded(bar, parity, &sm.abort_flag, a.status, DEV_TIMEOUT_EPILOGUE);
-      ok = __all_sync(~0u, ok);
+      if (!__all_sync(~0u, mbar_try_wait(bar, parity))) {
+        ok = mbar_wait_bounded(bar, parity, &sm.abort_flag, a.status, DEV_TIMEOUT_EPILOGUE);
+        ok = __all_sync(~0u, ok);
+      }
       tc_fence_after();
       return ok;
     };
@@ -471,7 +503,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 8; ++k) top[k & 1] = fmaxf(top[k & 1], fmaxf(x[k].x, x[k].y));
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = make_float2(ex2(x[k].x), ex2(x[k].y));
+            for (int k = 0; k < 8; ++k)
+              x[k] = k % 8 < kFmaPairs ? ex2_fma<T>(x[k]) : make_float2(ex2(x[k].x), ex2(x[k].y));
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               sum[k & 1] = __fadd2_rn(sum[k & 1], x[k]);
@@ -528,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (d.whole) {
         // by way of the rows' buffer, which is done with: a thread has a row,
         // a row's stores shall be whole lines
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = m > -INFINITY ? 1.0f / l : 0.0f;
         uint8_t* const stage = q_smem + (qb * 2 + h) * C::Q_BYTES;
 #pragma unroll
         for (int q = 0; q < D / 32; ++q) {
@@ -548,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        if (in && a.lse) a.lse[t * a.b.q_heads + head] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        if (in && a.lse) a.lse[t * a.b.q_heads + head] = (m + log2f(l)) * kLn2;
         __syncwarp();
         constexpr int CH = D / 8;
         const long long at = in ? t * a.o_token + head * a.o_head : -1;
