@@ -361,6 +361,27 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// The same for warps that share their scheduler with working ones and need not
+// be quick: between looks the thread sleeps for about `ns`, where
+// mbar_wait_bounded looks again after a few tens of cycles and takes issue
+// slots from the others.
+__device__ __forceinline__ bool mbar_wait_relaxed(uint64_t* bar, uint32_t parity,
+                                                  volatile int* abort, unsigned int* status,
+                                                  unsigned int code, unsigned int ns) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const unsigned long long start = globaltimer_ns();
+  while (!mbar_test_wait(bar, parity)) {
+    __nanosleep(ns);
+    if (*abort) return false;
+    if (globaltimer_ns() - start > kWaitLimitNs) {
+      if (status) atomicOr(status, code);
+      *abort = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
 // ---------------------------------------------------------------------------
 // TMA (non-multicast tiled loads only)
 // ---------------------------------------------------------------------------

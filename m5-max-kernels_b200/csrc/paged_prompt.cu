@@ -7,21 +7,24 @@
 //   t = S scale log2 e, p = 2^(t - m), l += sum p   one thread a row
 //   O += P V           P (the cache's type) from TMEM over S, V from shared memory
 // Roles: two warpgroups, one per half, each thread owning a row of S and O; one
-// thread per half issuing its MMAs, PV(s) QK(s+2) PV(s+1) ... (a wait on an
+// thread issuing QK of both halves in turn and one issuing PV (a wait on an
 // mbarrier costs an issuing thread some 55 cycles even when there is nothing
-// to wait for, and the tensor cores' queue holds but four to six MMAs: by one
-// thread for both halves a step took 2090 cycles); one warp filling a ring
-// with K and V blocks by TMA, one box per page; one warp finding the CTA's
-// pieces of tiles and loading their rows, one piece ahead.  O
-// takes 2 x 128 columns of TMEM, S 2 x 2 x 64: with two buffers a half, the
-// scores of step s + 1 are there when the softmax of step s ends, and neither
-// the softmax nor the tensor cores wait for a chain through the other.  (One
-// S buffer of 128 keys a half fits as well, but chains softmax -> PV -> QK ->
-// softmax: 1.64 ms against TIME for two prompts of 8192, 32 heads.)  P
-// overwrites its S.  m only follows the row's maximum when that has grown by
-// more than 2^8, which the softmax finds out after the fact: it takes the
-// exponentials with the old m, looks at the largest, and in the rare case
-// takes them again after rescaling O in place.
+// to wait for, and the tensor cores' queue holds but four to six MMAs: a step
+// took 2090 cycles when one thread issued all; a thread for each product of
+// each half lets the halves fall into step, so that all wait at once: 1850);
+// one warp filling a ring with K and V blocks by TMA, one box per page; one
+// warp finding the CTA's pieces of tiles and loading their rows, one piece
+// ahead.
+//
+// TMEM's 512 columns hold O (2 x 128), S (2 x 64) and P (2 x 2 x 32): QK of
+// the next step starts when the softmax has read S, and PV of this one when P
+// is there, and neither waits for the other.  (One S buffer of 128 keys a
+// half, with P over it, fits as well and needs fewer bytes of shared memory a
+// flop, but chains softmax, PV, QK, softmax: 4250 cycles for 128 keys.)  m
+// only follows the row's maximum when that has grown by more than 2^8; then O
+// is rescaled in place.  (Taking the exponentials with the old m while looking
+// for the maximum, and again in the rare case, keeps the scores in registers
+// for longer: 2200 cycles a step for TIME.)
 //
 // Bound by shared memory's bandwidth in the products: an MMA of 128 x 64 x 16
 // reads 6 KB where its 32 cycles have 4, so that a step takes 8 * 48 + 4 * 64
@@ -36,7 +39,7 @@ constexpr int kBlock = kPagedBlock;  // keys per step
 constexpr int kRows = 256;     // packed rows per tile, two halves
 constexpr float kGrow = 8.0f;           // log2 of the growth that m may lag behind
 constexpr int kFmaPairs = 3;             // of 8 pairs of exponentials, those by ex2_fma
-constexpr int kThreads = 384;  // warps 0-3, 4-7: halves; 8, 9: their MMAs; 10: K, V; 11: rows
+constexpr int kThreads = 384;  // warps 0-3, 4-7: halves; 8: QK; 9: PV; 10: K, V; 11: rows
 constexpr int kMmaWarp = 8, kTmaWarp = 10, kRowWarp = 11;
 
 // What the CTA's other warps need to know of a piece.
@@ -59,18 +62,20 @@ template <int D> struct Cfg {
   struct Small {
     uint64_t full[STAGES], empty[STAGES];
     uint64_t q_full[2], q_empty[2];          // [buffer] of rows and pieces
-    uint64_t s_full[2][2], p_full[2][2];     // [half][buffer]
-    uint64_t pv_done[2], o_full[2], drain[2];  // after every PV, after a piece's last
+    uint64_t s_full[2], s_free[2];           // [half]
+    uint64_t p_full[2][2];                   // [half][buffer]
+    uint64_t pv_done[2][2];                  // [half][buffer]
+    uint64_t o_full[2], drain[2];            // after a piece's last PV; [MMA thread]
     uint64_t landed;                            // a V block to be blanked
     long long scratch[kThreads / 32 + 4];
     Piece piece[2];
     uint32_t tmem;
     volatile int abort_flag;
   };
-  static_assert(sizeof(Small) <= 1024, "shared memory layout");
+  static_assert(STAGES % 2 == 0 && sizeof(Small) <= 1024, "shared memory layout");
 };
-// TMEM columns: S [half][buffer] of 64, O [half] of 128
-constexpr uint32_t kColS = 0, kColO = 256;
+// TMEM columns: S [half] of 64, P [half][buffer] of 32, O [half] of 128
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
@@ -106,6 +111,12 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool i
                "l"(__cvta_generic_to_global(src)), "r"(in ? 16 : 0)
                : "memory");
 }
+template <int N> __device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N> __device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 __device__ __forceinline__ void cp_async_wait_all() {
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -138,18 +149,66 @@ template <typename T> __device__ __forceinline__ float2 ex2_fma(float2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
 }
 
-// x of one score: capped and biased, in log2 units.
-__device__ __forceinline__ float modify(float x, float softcap, float slope, int pos, int key) {
-  if (softcap > 0.0f)  // tanh(y) = 1 - 2 / (e^2y + 1)
-    x = softcap * (1.0f - __fdividef(2.0f, ex2(x * (2.0f * kLog2e / softcap)) + 1.0f));
-  return (x - slope * fabsf(static_cast<float>(pos - key))) * kLog2e;
+// tanh(y) / y for a pair of y^2 in [0, 1]: the minimax fit of the relative
+// error (Remez exchange), 6e-7.
+__device__ __forceinline__ float2 tanh_ratio(float2 z) {
+  float2 p = make_float2(-0x1.920178p-9f, -0x1.920178p-9f);
+  p = __ffma2_rn(p, z, make_float2(0x1.1251b6p-6f, 0x1.1251b6p-6f));
+  p = __ffma2_rn(p, z, make_float2(-0x1.a6c0f2p-5f, -0x1.a6c0f2p-5f));
+  p = __ffma2_rn(p, z, make_float2(0x1.1000f6p-3f, 0x1.1000f6p-3f));
+  p = __ffma2_rn(p, z, make_float2(-0x1.554a16p-2f, -0x1.554a16p-2f));
+  return __ffma2_rn(p, z, make_float2(0x1.ffffecp-1f, 0x1.ffffecp-1f));
 }
 
-// One step of an MMA thread's stream: first or last of its piece, one that its
-// half takes part in, with the rows in buffer buf.
-struct Step {
-  bool valid, first, last, mine;
-  int buf;
+// A row's 64 scores capped, biased and in log2 units; `ahead` is the row's
+// position minus that of the first key.  Special functions would take as long
+// as the exponentials do three times over, so scores within the cap, the usual
+// case, go by tanh_ratio; a warp with any beyond it takes
+// tanh(y) = 1 - 2 / (e^2y + 1) for all of its own.
+__device__ __forceinline__ void modify(uint32_t (&s)[2][32], float scale, float softcap,
+                                       bool biased, float slope, int ahead) {
+  const float k = scale * kLog2e;
+  if (softcap > 0.0f) {
+    const float r = scale / softcap;
+    float top[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 64; e += 2)
+      top[e / 2 & 1] = fmaxf(top[e / 2 & 1], fmaxf(fabsf(__uint_as_float(s[e / 32][e % 32])),
+                                                   fabsf(__uint_as_float(s[e / 32][e % 32 + 1]))));
+    if (__all_sync(~0u, fmaxf(top[0], top[1]) * r <= 1.0f)) {
+      const float2 r2 = make_float2(r * r, r * r), k2 = make_float2(k, k);
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) {
+        const float2 x = make_float2(__uint_as_float(s[e / 32][e % 32]),
+                                     __uint_as_float(s[e / 32][e % 32 + 1]));
+        const float2 y = __fmul2_rn(__fmul2_rn(x, k2), tanh_ratio(__fmul2_rn(__fmul2_rn(x, x), r2)));
+        s[e / 32][e % 32] = __float_as_uint(y.x);
+        s[e / 32][e % 32 + 1] = __float_as_uint(y.y);
+      }
+    } else {
+      const float cap = softcap * kLog2e, two = 2.0f * r * kLog2e;
+#pragma unroll
+      for (int e = 0; e < 64; ++e) {
+        const float x = __uint_as_float(s[e / 32][e % 32]);
+        s[e / 32][e % 32] = __float_as_uint(cap * (1.0f - __fdividef(2.0f, ex2(x * two) + 1.0f)));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 64; ++e)
+      s[e / 32][e % 32] = __float_as_uint(__uint_as_float(s[e / 32][e % 32]) * k);
+  }
+  if (biased) {
+    const float down = -slope * kLog2e, first = static_cast<float>(ahead);
+#pragma unroll
+    for (int e = 0; e < 64; ++e)
+      s[e / 32][e % 32] = __float_as_uint(
+          fmaf(down, fabsf(first - static_cast<float>(e)), __uint_as_float(s[e / 32][e % 32])));
+  }
+}
+
+template <bool B> struct Flag {
+  static constexpr bool value = B;
 };
 
 template <typename T, int D, bool MOD>
@@ -167,16 +226,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], 2);
+      mbar_init(&sm.empty[i], 1);
     }
     for (int h = 0; h < 2; ++h) {
       mbar_init(&sm.q_full[h], 1);
       mbar_init(&sm.q_empty[h], 10);  // the softmax warps and the MMA threads
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&sm.s_full[h][i], 1);
-        mbar_init(&sm.p_full[h][i], 4);
-      }
-      mbar_init(&sm.pv_done[h], 1);
+      mbar_init(&sm.s_full[h], 1);
+      mbar_init(&sm.s_free[h], 4);
+      mbar_init(&sm.p_full[h][0], 4);
+      mbar_init(&sm.p_full[h][1], 4);
+      mbar_init(&sm.pv_done[h][0], 1);
+      mbar_init(&sm.pv_done[h][1], 1);
       mbar_init(&sm.o_full[h], 1);
       mbar_init(&sm.drain[h], 1);
     }
@@ -198,239 +258,211 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = sm.tmem;
   const int group = a.b.group;
 
-  if (warp == kTmaWarp) {  // ---- K and V blocks, in the order K0 K1 V0 K2 V1 ...
-    const int boxes = kBlock / maps.box_rows * C::HALVES;
-    const int row = lane / C::HALVES * maps.box_rows, half = lane % C::HALVES;
-    int stage = 0, phase = 0, issued = 0;
-    int blank = -1, blank_from = 0, ph_landed = 0;  // a stage whose last keys are to be blanked
-    bool ok = true;
-    auto load = [&](const CUtensorMap* map, int head, int page, int slot, int live) {
-      if (ok)
-        ok = mbar_wait_bounded(&sm.empty[stage], phase ^ 1, &sm.abort_flag, a.status,
-                               DEV_TIMEOUT_PRODUCER);
-      ok = __all_sync(~0u, ok);
-      if (!ok) return;
-      uint64_t* bar = live < kBlock ? &sm.landed : &sm.full[stage];
-      if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE_BYTES);
-      __syncwarp();
-      if (lane < boxes)
-        tma_load_4d(ring + stage * C::TILE_BYTES + half * C::HALF_BYTES + row * 128, map, bar,
-                    half * 64, slot, head, page);
-      if (live < kBlock) blank = stage, blank_from = max(live, 0);
-      ++issued;
-      if (++stage == STAGES) stage = 0, phase ^= 1;
-    };
-    // Slots behind the sequence's end may hold NaN, which a zero probability
-    // would not stop: V blocks that reach there land here first and are
-    // blanked, while the K block after them is on its way.
-    auto finish = [&]() {
-      if (blank < 0) return;
-      if (ok)
-        ok = mbar_wait_bounded(&sm.landed, ph_landed, &sm.abort_flag, a.status,
-                               DEV_TIMEOUT_PRODUCER);
-      ok = __all_sync(~0u, ok);
-      if (!ok) return;
-      ph_landed ^= 1;
-      uint8_t* v = ring + blank * C::TILE_BYTES;
-      for (int i = blank_from * C::HALVES * 8 + lane; i < kBlock * C::HALVES * 8; i += 32)
-        *reinterpret_cast<uint4*>(v + (i / 8 % C::HALVES) * C::HALF_BYTES + i / (C::HALVES * 8) * 128 +
-                                  i % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.full[blank]);
-      blank = -1;
-    };
-    PagedPiece p;
-    int head = -1, page = 0, slot = 0, live = 0;  // of the step before
-    while (ok && walk.next(a, p)) {
-      for (int i = p.begin; ok && i < p.end; ++i) {
-        const int block0 = p.r.at(i) * kBlock, key = block0 + row;
-        int page2 = a.b.num_pages, slot2 = 0;  // out of range: zeros
-        if (lane < boxes && key < p.s.keys) {
-          const int at = paged_page(a.b, p.seq, key);
-          if (at >= 0) page2 = at;
-          slot2 = key % a.b.page_size;
-        }
-        load(&maps.k, p.head, page2, slot2, kBlock);
-        finish();
-        if (head >= 0) load(&maps.v, head, page, slot, live);
-        head = p.head, page = page2, slot = slot2, live = p.s.keys - block0;
-      }
-    }
-    finish();
-    if (head >= 0) load(&maps.v, head, page, slot, live);
-    finish();
-    if (!ok) {  // let the copies in flight land before the CTA ends
-      for (int i = 0; i < STAGES && i < issued; ++i) {
-        if (--stage < 0) stage = STAGES - 1, phase ^= 1;
-        const unsigned long long start = globaltimer_ns();
-        while (!(stage == blank ? mbar_try_wait(&sm.landed, ph_landed)
-                                : mbar_try_wait(&sm.full[stage], phase)) &&
-               globaltimer_ns() - start < kWaitLimitNs) {
-        }
-      }
-    }
-  } else if (warp == kRowWarp) {  // ---- pieces and their rows
-    constexpr int CH = D / 8;  // 16-byte chunks of a row
-    const int chunk = lane % CH;
-    bool ok = true, any = false;
-    PagedPiece p;
-    for (int n = 0; ok; ++n) {
-      const int buf = n & 1;
-      const bool more = walk.next(a, p);
-      any |= more;
-      ok = mbar_wait_bounded(&sm.q_empty[buf], (n >> 1 & 1) ^ 1, &sm.abort_flag, a.status,
-                             DEV_TIMEOUT_PRODUCER);
-      ok = __all_sync(~0u, ok);
-      if (!ok) break;
-      const int rows = p.s.n * group, first = p.rt * kRows;
-      if (more) {
-        const int here = min(rows - first, kRows), all = here > 128 ? kRows : 128;
-        int r = lane / CH, tok = (first + r) / group, g = (first + r) % group;
-        for (; r < all; r += 32 / CH) {
-          const bool in = r < here;
-          const T* src = static_cast<const T*>(a.q) + int64_t(p.s.row0 + (in ? tok : 0)) * a.q_token +
-                         (p.head * group + g) * a.q_head + chunk * 8;
-          cp_async16(smem_u32(q_smem + buf * 2 * C::Q_BYTES + (r / 128) * C::Q_BYTES +
-                              (chunk / 8) * C::Q_HALF + (r % 128) * 128 +
-                              (((chunk % 8) ^ (r & 7)) << 4)), src, in);
-          for (g += 32 / CH; g >= group; g -= group) ++tok;
-        }
-      }
-      if (lane == 0) {
-        Piece d{};
-        if (more) {
-          d.begin = p.begin;
-          d.end = p.end;
-          d.pre = p.r.pre;
-          d.from = p.r.from;
-          d.keys = p.s.keys;
-          d.prefix = p.s.prefix;
-          d.pos0 = p.s.pos0;
-          d.rows = rows;
-          d.first = first;
-          d.row0 = p.s.row0;
-          d.head = p.head;
-          d.whole = p.whole();
-          d.slot = 2 * blockIdx.x + (p.begin == 0 ? 1 : 0);
-        }
-        sm.piece[buf] = d;
-      }
-      cp_async_wait_all();
-      fence_proxy_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.q_full[buf]);
-      if (!more) break;
-    }
-    if (lane == 0)  // (p is the last piece)
-      paged_write_split(&PagedPartials<kRows, D>(a.workspace, gridDim.x).split[blockIdx.x],
-                        any ? &p : nullptr, walk.share, kRows, group);
-  } else if (warp >= kMmaWarp) {  // ---- matrix products of half h, by one thread
-    const int h = warp - kMmaWarp;
-    if (elect_one()) {
-      constexpr int kind = DTypeOf<T>::value == DT_BF16 ? KIND_BF16 : KIND_F16;
-      constexpr uint32_t idesc_s = make_idesc(kind, 128, kBlock);
-      constexpr uint32_t idesc_o = make_idesc(kind, 128, D) | (1u << 16);  // B is MN-major
-      const uint64_t q_desc = smem_desc_k128(smem_u32(q_smem + h * C::Q_BYTES));
-      const uint64_t k_desc = smem_desc_k128(smem_u32(ring));
-      const uint64_t v_desc = smem_desc_mn128(smem_u32(ring), C::HALF_BYTES);
-      const uint32_t t_s = tmem + kColS + h * 128, t_o = tmem + kColO + h * 128;
-      int stage = 0, phase = 0;
-      int piece = -1, si = 0, pi = 0;  // QK and PV steps of this half
-      int left = 0;  // steps of the piece
-      bool ok = true, mine = false, ended = false;
-      auto wait = [&](uint64_t* bar, int parity) {
-        if (ok) ok = mbar_wait_bounded(bar, parity, &sm.abort_flag, a.status, DEV_TIMEOUT_MMA);
-        tc_fence_after();
-      };
-      auto advance = [&]() {
-        Step s{};
-        if (ended) return s;
-        if (left == 0) {
-          ++piece;
-          wait(&sm.q_full[piece & 1], piece >> 1 & 1);
-          if (ok) {
-            const Piece& d = sm.piece[piece & 1];
-            left = d.end - d.begin;
-            mine = h == 0 || d.rows - d.first > 128;
-            mbar_arrive(&sm.q_empty[piece & 1]);
-          }
-          ended = !ok || left == 0;
-          if (ended) return s;
-          s.first = true;
-        }
-        s.valid = true;
-        s.mine = mine;
-        s.buf = piece & 1;
-        s.last = --left == 0;
-        return s;
-      };
-      // The next stage of the ring, once it is filled, for a step of this half
-      // or of the other alone.
-      auto use = [&](bool mine, auto&& products) {
-        const int st = stage;
-        wait(&sm.full[st], phase);
+  // Registers: 256 threads of 208 and 128 of 88 make the 384 x 168 of the launch.
+  if (warp >= kMmaWarp) {
+    regs_dec<88>();
+    if (warp == kTmaWarp) {  // ---- K and V blocks
+      const int boxes = kBlock / maps.box_rows * C::HALVES;
+      const int row = lane / C::HALVES * maps.box_rows, half = lane % C::HALVES;
+      int stage = 0, phase = 0, issued = 0;
+      int blank = -1, blank_from = 0, ph_landed = 0;  // a stage whose last keys are to be blanked
+      bool ok = true;
+      auto load = [&](const CUtensorMap* map, int head, int page, int slot, int live) {
+        if (ok)
+          ok = mbar_wait_relaxed(&sm.empty[stage], phase ^ 1, &sm.abort_flag, a.status,
+                                 DEV_TIMEOUT_PRODUCER, 100);
+        ok = __all_sync(~0u, ok);
+        if (!ok) return;
+        uint64_t* bar = live < kBlock ? &sm.landed : &sm.full[stage];
+        if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE_BYTES);
+        __syncwarp();
+        if (lane < boxes)
+          tma_load_4d(ring + stage * C::TILE_BYTES + half * C::HALF_BYTES + row * 128, map, bar,
+                      half * 64, slot, head, page);
+        if (live < kBlock) blank = stage, blank_from = max(live, 0);
+        ++issued;
         if (++stage == STAGES) stage = 0, phase ^= 1;
-        if (mine && ok) {
-          products(st * C::TILE_BYTES >> 4);
-          tc_commit(&sm.empty[st]);
-        } else {
-          mbar_arrive(&sm.empty[st]);
-        }
       };
-      auto qk = [&](const Step& s) {  // S = Q K^T
-        use(s.mine, [&](int off) {
-          const int buf = si++ & 1;
-          const uint64_t qd = q_desc + (s.buf * 2 * C::Q_BYTES >> 4), kd = k_desc + off;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            tc_mma<KIND_F16>(t_s + buf * 64, qd + (((k / 4) * C::Q_HALF + (k % 4) * 32) >> 4),
-                             kd + (((k / 4) * C::HALF_BYTES + (k % 4) * 32) >> 4), idesc_s, k > 0);
-          tc_commit(&sm.s_full[h][buf]);
-        });
+      // Slots behind the sequence's end may hold NaN, which a zero probability
+      // would not stop: V blocks that reach there land here first and are
+      // blanked, while the K block after them is on its way.
+      auto finish = [&]() {
+        if (blank < 0) return;
+        if (ok)
+          ok = mbar_wait_relaxed(&sm.landed, ph_landed, &sm.abort_flag, a.status,
+                                 DEV_TIMEOUT_PRODUCER, 100);
+        ok = __all_sync(~0u, ok);
+        if (!ok) return;
+        ph_landed ^= 1;
+        uint8_t* v = ring + blank * C::TILE_BYTES;
+        for (int i = blank_from * C::HALVES * 8 + lane; i < kBlock * C::HALVES * 8; i += 32)
+          *reinterpret_cast<uint4*>(v + (i / 8 % C::HALVES) * C::HALF_BYTES + i / (C::HALVES * 8) * 128 +
+                                    i % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.full[blank]);
+        blank = -1;
       };
-      auto pv = [&](const Step& s) {  // O (+)= P V
-        use(s.mine, [&](int off) {
-          const int buf = pi & 1;
-          wait(&sm.p_full[h][buf], (pi >> 1) & 1);
-          ++pi;
-          const uint64_t vd = v_desc + off;
-#pragma unroll
-          for (int k = 0; k < kBlock / 16; ++k)
-            tc_mma_ts(t_o, t_s + buf * 64 + k * 8, vd + (k * 2048 >> 4), idesc_o, !s.first || k > 0);
-          tc_commit(&sm.pv_done[h]);
-          if (s.last) tc_commit(&sm.o_full[h]);
-        });
-      };
-      Step cur = advance();
-      if (cur.valid) qk(cur);
-      Step nx1 = advance();
-      if (nx1.valid) qk(nx1);
-      while (ok && cur.valid) {
-        pv(cur);
-        // (a piece's rows may have to wait for the softmax of the piece two
-        // before, which needs this PV)
-        const Step nx2 = advance();
-        if (nx2.valid) qk(nx2);
-        cur = nx1;
-        nx1 = nx2;
-      }
-      // every MMA has retired before TMEM is freed
-      tc_commit(&sm.drain[h]);
-      const unsigned long long start = globaltimer_ns();
-      while (!mbar_try_wait(&sm.drain[h], 0)) {
-        if (globaltimer_ns() - start > kWaitLimitNs) {
-          atomicOr(a.status, DEV_TIMEOUT_DRAIN);
-          break;
+      PagedPiece p;
+      while (ok && walk.next(a, p)) {
+        for (int i = p.begin; ok && i < p.end; ++i) {
+          const int block0 = p.r.at(i) * kBlock, key = block0 + row;
+          int page = a.b.num_pages, slot = 0;  // out of range: zeros
+          if (lane < boxes && key < p.s.keys) {
+            const int at = paged_page(a.b, p.seq, key);
+            if (at >= 0) page = at;
+            slot = key % a.b.page_size;
+          }
+          load(&maps.k, p.head, page, slot, kBlock);
+          finish();
+          load(&maps.v, p.head, page, slot, p.s.keys - block0);
         }
       }
+      finish();
+      if (!ok) {  // let the copies in flight land before the CTA ends
+        for (int i = 0; i < STAGES && i < issued; ++i) {
+          if (--stage < 0) stage = STAGES - 1, phase ^= 1;
+          const unsigned long long start = globaltimer_ns();
+          while (!(stage == blank ? mbar_try_wait(&sm.landed, ph_landed)
+                                  : mbar_try_wait(&sm.full[stage], phase)) &&
+                 globaltimer_ns() - start < kWaitLimitNs) {
+          }
+        }
+      }
+    } else if (warp == kRowWarp) {  // ---- pieces and their rows
+      constexpr int CH = D / 8;  // 16-byte chunks of a row
+      const int chunk = lane % CH;
+      bool ok = true, any = false;
+      PagedPiece p;
+      for (int n = 0; ok; ++n) {
+        const int buf = n & 1;
+        const bool more = walk.next(a, p);
+        any |= more;
+        ok = mbar_wait_relaxed(&sm.q_empty[buf], (n >> 1 & 1) ^ 1, &sm.abort_flag, a.status,
+                               DEV_TIMEOUT_PRODUCER, 100);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        const int rows = p.s.n * group, first = p.rt * kRows;
+        if (more) {
+          const int here = min(rows - first, kRows), all = here > 128 ? kRows : 128;
+          int r = lane / CH, tok = (first + r) / group, g = (first + r) % group;
+          for (; r < all; r += 32 / CH) {
+            const bool in = r < here;
+            const T* src = static_cast<const T*>(a.q) + int64_t(p.s.row0 + (in ? tok : 0)) * a.q_token +
+                           (p.head * group + g) * a.q_head + chunk * 8;
+            cp_async16(smem_u32(q_smem + buf * 2 * C::Q_BYTES + (r / 128) * C::Q_BYTES +
+                                (chunk / 8) * C::Q_HALF + (r % 128) * 128 +
+                                (((chunk % 8) ^ (r & 7)) << 4)), src, in);
+            for (g += 32 / CH; g >= group; g -= group) ++tok;
+          }
+        }
+        if (lane == 0) {
+          Piece d{};
+          if (more) {
+            d.begin = p.begin;
+            d.end = p.end;
+            d.pre = p.r.pre;
+            d.from = p.r.from;
+            d.keys = p.s.keys;
+            d.prefix = p.s.prefix;
+            d.pos0 = p.s.pos0;
+            d.rows = rows;
+            d.first = first;
+            d.row0 = p.s.row0;
+            d.head = p.head;
+            d.whole = p.whole();
+            d.slot = 2 * blockIdx.x + (p.begin == 0 ? 1 : 0);
+          }
+          sm.piece[buf] = d;
+        }
+        cp_async_wait_all();
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_full[buf]);
+        if (!more) break;
+      }
+      if (lane == 0)  // (p is the last piece)
+        paged_write_split(&PagedPartials<kRows, D>(a.workspace, gridDim.x).split[blockIdx.x],
+                          any ? &p : nullptr, walk.share, kRows, group);
+    } else {  // ---- QK or PV of both halves, by one thread
+      const bool is_pv = warp != kMmaWarp;
+      if (elect_one()) {
+        constexpr int kind = DTypeOf<T>::value == DT_BF16 ? KIND_BF16 : KIND_F16;
+        constexpr uint32_t idesc_s = make_idesc(kind, 128, kBlock);
+        constexpr uint32_t idesc_o = make_idesc(kind, 128, D) | (1u << 16);  // B is MN-major
+        const uint64_t q_desc = smem_desc_k128(smem_u32(q_smem));
+        const uint64_t k_desc = smem_desc_k128(smem_u32(ring));
+        const uint64_t v_desc = smem_desc_mn128(smem_u32(ring), C::HALF_BYTES);
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, int parity) {
+          if (ok) ok = mbar_wait_bounded(bar, parity, &sm.abort_flag, a.status, DEV_TIMEOUT_MMA);
+          tc_fence_after();
+        };
+        // K blocks are in the ring's even stages, V blocks in the odd ones
+        int stage = is_pv ? 1 : 0, phase = 0;
+        int done[2] = {0, 0};  // steps of the halves
+        for (int piece = 0; ok; ++piece) {
+          wait(&sm.q_full[piece & 1], piece >> 1 & 1);
+          if (!ok) break;
+          const Piece& d = sm.piece[piece & 1];
+          const int steps = d.end - d.begin, halves = d.rows - d.first > 128 ? 2 : 1;
+          mbar_arrive(&sm.q_empty[piece & 1]);
+          if (steps == 0) break;
+          const uint64_t qd = q_desc + ((piece & 1) * 2 * C::Q_BYTES >> 4);
+          for (int i = 0; ok && i < steps; ++i) {
+            wait(&sm.full[stage], phase);
+            const int at = stage * C::TILE_BYTES >> 4;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h >= halves) break;
+              if (!is_pv) {  // S = Q K^T
+                if (done[h] > 0) wait(&sm.s_free[h], (done[h] - 1) & 1);
+                if (!ok) break;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                  tc_mma<KIND_F16>(tmem + kColS + h * 64,
+                                   qd + ((h * C::Q_BYTES + (k / 4) * C::Q_HALF + (k % 4) * 32) >> 4),
+                                   k_desc + at + (((k / 4) * C::HALF_BYTES + (k % 4) * 32) >> 4),
+                                   idesc_s, k > 0);
+                tc_commit(&sm.s_full[h]);
+              } else {  // O (+)= P V
+                const int buf = done[h] & 1;
+                wait(&sm.p_full[h][buf], (done[h] >> 1) & 1);
+                if (!ok) break;
+#pragma unroll
+                for (int k = 0; k < kBlock / 16; ++k)
+                  tc_mma_ts(tmem + kColO + h * 128, tmem + kColP + h * 64 + buf * 32 + k * 8,
+                            v_desc + at + (k * 2048 >> 4), idesc_o, i > 0 || k > 0);
+                tc_commit(&sm.pv_done[h][buf]);
+                if (i + 1 == steps) tc_commit(&sm.o_full[h]);
+              }
+              ++done[h];
+            }
+            if (ok) tc_commit(&sm.empty[stage]);
+            stage += 2;
+            if (stage >= STAGES) stage -= STAGES, phase ^= 1;
+          }
+        }
+        // every MMA has retired before TMEM is freed
+        uint64_t* drain = &sm.drain[warp - kMmaWarp];
+        tc_commit(drain);
+        const unsigned long long start = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0)) {
+          if (globaltimer_ns() - start > kWaitLimitNs) {
+            atomicOr(a.status, DEV_TIMEOUT_DRAIN);
+            break;
+          }
+        }
+      }
+      __syncwarp();
     }
-    __syncwarp();
   } else {  // ---- softmax: thread `row` of half h
+    regs_inc<208>();
     const int h = warp / 4;
     const int row = threadIdx.x % 128;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
-    const uint32_t t_s = lanes + kColS + h * 128, t_o = lanes + kColO + h * 128;
+    const uint32_t t_s = lanes + kColS + h * 64, t_p = lanes + kColP + h * 64;
+    const uint32_t t_o = lanes + kColO + h * 128;
     const float c = MOD ? 1.0f : a.scale * kLog2e;
     int step = 0, outs = 0;  // steps and pieces of this half
     bool ok = true;
@@ -464,77 +496,65 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int all_lo = pos_hi >= a.window ? pos_hi - a.window + 1 : 0, all_hi = min(pos_lo, d.keys - 1);
       const int begin = d.begin;
       float m = -INFINITY, l = 0.0f;
-      for (int i = begin; i < end; ++i, ++step) {
-        const int block0 = (i < pre ? i : from + i - pre) * kBlock, buf = step & 1;
-        if (!wait(&sm.s_full[h][buf], (step >> 1) & 1)) break;
+      auto softmax = [&](auto masked, int i, int block0, bool open) {
+        const int buf = step & 1;
         uint32_t s[2][32];
-        tmem_ld32(t_s + buf * 64, s[0]);
-        tmem_ld32(t_s + buf * 64 + 32, s[1]);
+        tmem_ld32(t_s, s[0]);
+        tmem_ld32(t_s + 32, s[1]);
         tmem_wait_ld();
-        if (MOD) {
-#pragma unroll
-          for (int e = 0; e < kBlock; ++e)
-            s[e / 32][e % 32] = __float_as_uint(modify(__uint_as_float(s[e / 32][e % 32]) * a.scale,
-                                                       a.softcap, slope, pos, block0 + e));
-        }
-        if (!(block0 + kBlock <= prefix || (block0 >= all_lo && block0 + kBlock - 1 <= all_hi))) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.s_free[h]);
+        if (MOD) modify(s, a.scale, a.softcap, a.slopes != nullptr, slope, pos - block0);
+        if (decltype(masked)::value && !(MOD && open)) {
           const int hi = row_hi - block0, lo = row_lo - block0, pr = prefix - block0;
 #pragma unroll
           for (int e = 0; e < kBlock; ++e)
             if (!(e < pr || (e <= hi && e >= lo))) s[e / 32][e % 32] = 0xff800000u;
         }
+        float top[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t* x = &s[q / 2][(q % 2) * 16];
+          top[q] = __uint_as_float(x[0]);
+#pragma unroll
+          for (int e = 1; e < 15; e += 2)
+            top[q] = fmaxf(top[q], fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+          top[q] = fmaxf(top[q], __uint_as_float(x[15]));
+        }
+        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+        const bool grow = high > m + kGrow;  // (m = -inf: any key)
+        const bool any = __any_sync(~0u, grow);
+        const float m2 = grow ? high : m, f = m == -INFINITY ? 0.0f : ex2(m - m2);
+        m = m2;
         uint32_t pk[32];
-        float2 sum[2];
-        float over;  // the largest t - m
-        auto exponentials = [&]() {
-          const float base = m == -INFINITY ? 0.0f : -m;
-          const float2 c2 = make_float2(c, c), b2 = make_float2(base, base);
-          float top[2] = {-INFINITY, -INFINITY};
-          sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+        const float base = m == -INFINITY ? 0.0f : -m;
+        const float2 c2 = make_float2(c, c), b2 = make_float2(base, base);
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {  // (16 at a time, to have them in flight)
-            float2 x[8];
+        for (int e = 0; e < 32; e += 8) {  // (16 at a time, to have them in flight)
+          float2 x[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int at = 2 * (e + k);
-              x[k] = __ffma2_rn(make_float2(__uint_as_float(s[at / 32][at % 32]),
-                                            __uint_as_float(s[at / 32][at % 32 + 1])), c2, b2);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) top[k & 1] = fmaxf(top[k & 1], fmaxf(x[k].x, x[k].y));
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              x[k] = k % 8 < kFmaPairs ? ex2_fma<T>(x[k]) : make_float2(ex2(x[k].x), ex2(x[k].y));
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              sum[k & 1] = __fadd2_rn(sum[k & 1], x[k]);
-              pk[e + k] = pack2<T>(x[k].x, x[k].y);
-            }
+          for (int k = 0; k < 8; ++k) {
+            const int at = 2 * (e + k);
+            x[k] = __ffma2_rn(make_float2(__uint_as_float(s[at / 32][at % 32]),
+                                          __uint_as_float(s[at / 32][at % 32 + 1])), c2, b2);
           }
-          over = fmaxf(top[0], top[1]);
-        };
-        auto maximum = [&]() {
-          float top[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            top[q] = __uint_as_float(s[q / 2][(q % 2) * 16]);
+          for (int k = 0; k < 8; ++k)
+            x[k] = k % 8 < (MOD ? 0 : kFmaPairs) ? ex2_fma<T>(x[k]) : make_float2(ex2(x[k].x), ex2(x[k].y));
 #pragma unroll
-            for (int e = 1; e < 16; ++e)
-              top[q] = fmaxf(top[q], __uint_as_float(s[q / 2][(q % 2) * 16 + e]));
+          for (int k = 0; k < 8; ++k) {
+            sum[k & 1] = __fadd2_rn(sum[k & 1], x[k]);
+            pk[e + k] = pack2<T>(x[k].x, x[k].y);
           }
-          return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-        };
-        if (i == begin) m = maximum();
-        exponentials();
-        // (a row without any key so far has no m yet)
-        if (__any_sync(~0u, over > (m == -INFINITY ? -INFINITY : kGrow))) {
-          // O holds the steps before this one, once they are done.  (S of this
-          // step says so of all but the last, so that the parity is not two
-          // phases off.)
-          if (!wait(&sm.pv_done[h], (step - 1) & 1)) break;
-          const float m2 = fmaxf(m, maximum()), f = m == -INFINITY ? 0.0f : ex2(m - m2);
-          m = m2;
-          l *= f;
+        }
+        l = l * f + (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        // (PV of two steps before has long been done with this buffer)
+        if (step > 1 && !wait(&sm.pv_done[h][buf], ((step >> 1) - 1) & 1)) return;
+        tmem_st32(t_p + buf * 32, pk);
+        if (any && i > begin) {  // O holds the steps before this one, once they are done
+          if (!wait(&sm.pv_done[h][buf ^ 1], ((step - 1) >> 1) & 1)) return;
           uint32_t o[32];
 #pragma unroll
           for (int q = 0; q < D / 32; ++q) {
@@ -544,14 +564,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
             tmem_st32(t_o + q * 32, o);
           }
-          exponentials();
         }
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        tmem_st32(t_s + buf * 64, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.p_full[h][buf]);
+      };
+      for (int i = begin; i < end; ++i, ++step) {
+        const int block0 = (i < pre ? i : from + i - pre) * kBlock;
+        if (!wait(&sm.s_full[h], step & 1)) break;
+        // (two bodies, where they are short: scores that a branch may change
+        // cost the other way too, but a body may outgrow the instruction cache)
+        const bool open =
+            block0 + kBlock <= prefix || (block0 >= all_lo && block0 + kBlock - 1 <= all_hi);
+        if (!MOD && open)
+          softmax(Flag<false>(), i, block0, true);
+        else
+          softmax(Flag<true>(), i, block0, open);
+        if (!ok) break;
       }
       if (!ok) break;
 
