@@ -344,16 +344,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const int rows = p.s.n * group, first = p.rt * kRows;
         if (more) {
+          // a row after every 32 / CH; the pointer follows head and token
+          constexpr int STEP = 32 / CH;
           const int here = min(rows - first, kRows), all = here > 128 ? kRows : 128;
-          int r = lane / CH, tok = (first + r) / group, g = (first + r) % group;
-          for (; r < all; r += 32 / CH) {
-            const bool in = r < here;
-            const T* src = static_cast<const T*>(a.q) + int64_t(p.s.row0 + (in ? tok : 0)) * a.q_token +
-                           (p.head * group + g) * a.q_head + chunk * 8;
-            cp_async16(smem_u32(q_smem + buf * 2 * C::Q_BYTES + (r / 128) * C::Q_BYTES +
-                                (chunk / 8) * C::Q_HALF + (r % 128) * 128 +
-                                (((chunk % 8) ^ (r & 7)) << 4)), src, in);
-            for (g += 32 / CH; g >= group; g -= group) ++tok;
+          const int r0 = lane / CH;
+          int g = (first + r0) % group;
+          const T* src = static_cast<const T*>(a.q) +
+                         int64_t(p.s.row0 + (first + r0) / group) * a.q_token +
+                         (p.head * group + g) * a.q_head + chunk * 8;
+          const int64_t next = (STEP / group) * a.q_token + (STEP % group) * a.q_head;
+          const int64_t wrap = a.q_token - group * a.q_head;
+          uint32_t dst = smem_u32(q_smem + buf * 2 * C::Q_BYTES + (chunk / 8) * C::Q_HALF);
+#pragma unroll 4
+          for (int r = r0; r < all; r += STEP) {
+            cp_async16(dst + (r / 128) * C::Q_BYTES + (r % 128) * 128 + (((chunk % 8) ^ (r & 7)) << 4),
+                       r < here ? src : static_cast<const T*>(a.q), r < here);
+            src += next;
+            g += STEP % group;
+            if (g >= group) g -= group, src += wrap;
           }
         }
         if (lane == 0) {
