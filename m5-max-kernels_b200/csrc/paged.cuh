@@ -62,6 +62,10 @@ constexpr int kPagedBlock = 64;  // keys of a block of the tiled kernels
 struct PagedMaps {
   CUtensorMap k, v;
   int box_rows;
+  // The prompt kernel's rows, {channel, head, token}, boxes of 64 channels x a
+  // group of heads x as many tokens as make 128 rows; where the group divides 128.
+  CUtensorMap q;
+  int has_q;
 };
 
 cudaError_t launch_paged_append(const PagedAppendArgs& a, int x_dtype, int cache_dtype,

@@ -106,6 +106,16 @@ bool cache_map(CUtensorMap* map, const void* ptr, const PagedBatch& b, bool f16,
   return make_swizzled_map16(map, f16, 4, ptr, dims, strides, box);
 }
 
+void row_map(PagedMaps& m, const PagedAttnArgs& a, int64_t dtype) {
+  const PagedBatch& b = a.b;
+  m.has_q = 0;
+  if (128 % b.group || a.q_head == 0 || a.q_token == 0) return;
+  const uint64_t dims[3] = {uint64_t(b.head_dim), uint64_t(b.q_heads), uint64_t(b.tokens)};
+  const uint64_t strides[2] = {uint64_t(a.q_head) * 2, uint64_t(a.q_token) * 2};
+  const uint32_t box[3] = {64, uint32_t(b.group), uint32_t(128 / b.group)};
+  m.has_q = make_swizzled_map16(&m.q, dtype == M5B_F16, 3, a.q, dims, strides, box) ? 1 : 0;
+}
+
 bool cache_maps(PagedMaps& m, const PagedAttnArgs& a, int64_t dtype) {
   const PagedBatch& b = a.b;
   m.box_rows = b.page_size < kPagedBlock ? b.page_size : kPagedBlock;
@@ -203,7 +213,8 @@ int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
         s->workspace_bytes < m5b_paged_attention_workspace_bytes(a.b.head_dim))
       return einval("workspace of m5b_paged_attention_workspace_bytes(head_dim) bytes required");
     const bool few = int64_t(a.max_query_len) * a.b.group <= kDecodeRows;
-    PagedMaps m;
+    PagedMaps m{};
+    if (!few) row_map(m, a, dtype);
     if (cache_maps(m, a, dtype))
       return launched(few ? launch_paged_decode(a, m, dtype, sms, st)
                           : launch_paged_prompt(a, m, dtype, sms, st),

@@ -194,12 +194,28 @@ __device__ __forceinline__ void modify(uint32_t (&s)[2][32], float scale, float 
       }
     }
   } else {
+    const float2 k2 = make_float2(k, k);
 #pragma unroll
-    for (int e = 0; e < 64; ++e)
-      s[e / 32][e % 32] = __float_as_uint(__uint_as_float(s[e / 32][e % 32]) * k);
+    for (int e = 0; e < 64; e += 2) {
+      const float2 y = __fmul2_rn(make_float2(__uint_as_float(s[e / 32][e % 32]),
+                                              __uint_as_float(s[e / 32][e % 32 + 1])), k2);
+      s[e / 32][e % 32] = __float_as_uint(y.x);
+      s[e / 32][e % 32 + 1] = __float_as_uint(y.y);
+    }
   }
-  if (biased) {
-    const float down = -slope * kLog2e, first = static_cast<float>(ahead);
+  if (!biased) return;
+  const float down = -slope * kLog2e, first = static_cast<float>(ahead);
+  if (__all_sync(~0u, ahead >= 63)) {  // no key is ahead of its row: the distance is linear
+    const float2 d2 = make_float2(down, down), f2 = make_float2(first, first);
+#pragma unroll
+    for (int e = 0; e < 64; e += 2) {
+      const float2 y = __ffma2_rn(
+          __fadd2_rn(f2, make_float2(-static_cast<float>(e), -static_cast<float>(e + 1))), d2,
+          make_float2(__uint_as_float(s[e / 32][e % 32]), __uint_as_float(s[e / 32][e % 32 + 1])));
+      s[e / 32][e % 32] = __float_as_uint(y.x);
+      s[e / 32][e % 32 + 1] = __float_as_uint(y.y);
+    }
+  } else {
 #pragma unroll
     for (int e = 0; e < 64; ++e)
       s[e / 32][e % 32] = __float_as_uint(
@@ -333,8 +349,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr int CH = D / 8;  // 16-byte chunks of a row
       const int chunk = lane % CH;
       bool ok = true, any = false;
+      int n = 0;
       PagedPiece p;
-      for (int n = 0; ok; ++n) {
+      for (;; ++n) {
         const int buf = n & 1;
         const bool more = walk.next(a, p);
         any |= more;
@@ -343,7 +360,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         const int rows = p.s.n * group, first = p.rt * kRows;
-        if (more) {
+        const bool by_tma = more && maps.has_q;
+        if (more && !by_tma) {
           // a row after every 32 / CH; the pointer follows head and token
           constexpr int STEP = 32 / CH;
           const int here = min(rows - first, kRows), all = here > 128 ? kRows : 128;
@@ -383,11 +401,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           sm.piece[buf] = d;
         }
-        cp_async_wait_all();
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.q_full[buf]);
+        if (by_tma) {
+          // (rows behind the sequence's are another's: computed, not stored)
+          __syncwarp();
+          if (lane == 0) {
+            const int halves = rows - first > 128 ? 2 : 1;
+            mbar_arrive_expect_tx(&sm.q_full[buf], halves * C::Q_BYTES);
+            for (int i = 0; i < halves * C::HALVES; ++i)
+              tma_load_3d(q_smem + (buf * 2 + i / C::HALVES) * C::Q_BYTES + i % C::HALVES * C::Q_HALF,
+                          &maps.q, &sm.q_full[buf], i % C::HALVES * 64, p.head * group,
+                          p.s.row0 + (first + i / C::HALVES * 128) / group);
+          }
+        } else {
+          cp_async_wait_all();
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.q_full[buf]);
+        }
         if (!more) break;
+      }
+      // let the rows in flight land before the CTA ends
+      for (int i = n - 1; !ok && maps.has_q && i >= 0 && i >= n - 2; --i) {
+        const unsigned long long start = globaltimer_ns();
+        while (!mbar_try_wait(&sm.q_full[i & 1], i >> 1 & 1) &&
+               globaltimer_ns() - start < kWaitLimitNs) {
+        }
       }
       if (lane == 0)  // (p is the last piece)
         paged_write_split(&PagedPartials<kRows, D>(a.workspace, gridDim.x).split[blockIdx.x],
@@ -648,6 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (in) parts.ml[int64_t(d.slot) * kRows + h * 128 + row] = make_float2(m, l);
       }
       tc_fence_before();
+      fence_proxy_async_shared();  // before the buffer's next rows come by TMA
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.q_empty[qb]);
     }

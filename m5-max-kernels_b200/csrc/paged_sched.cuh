@@ -107,6 +107,11 @@ struct PagedPiece {
 
 // The stretch of this CTA, piece by piece.  Every thread that walks it sees
 // the same pieces.
+// a / b, by the short division where that does (a long one is a call).
+__device__ __forceinline__ long long paged_div(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
+}
+
 template <int ROWS, int BK>
 struct PagedWalk {
   int seq, head, rt, tiles, blk;
@@ -177,7 +182,7 @@ __device__ __forceinline__ PagedWalk<ROWS, BK> paged_walk(const PagedAttnArgs& a
     total += scratch[w];
   }
   PagedWalk<ROWS, BK> walk;
-  walk.share = (total + gridDim.x - 1) / gridDim.x;
+  walk.share = paged_div(total + gridDim.x - 1, gridDim.x);
   const long long at = walk.share * blockIdx.x;
   walk.left = max(0ll, min(walk.share, total - at));
   // the thread whose sequences hold block `at` looks which one does (all lanes
@@ -193,8 +198,9 @@ __device__ __forceinline__ PagedWalk<ROWS, BK> paged_walk(const PagedAttnArgs& a
       if (here && !found && at < base + all) {
         found = true;
         scratch[kWarps] = b0 + i;
-        scratch[kWarps + 1] = (at - base) / one;
-        scratch[kWarps + 2] = (at - base) % one;
+        const long long head = paged_div(at - base, one);
+        scratch[kWarps + 1] = head;
+        scratch[kWarps + 2] = at - base - head * one;
       }
       base += all;
     }
@@ -259,7 +265,7 @@ __device__ __forceinline__ void paged_write_split(PagedSplit* at, const PagedPie
                                                   long long share, int rows_per_tile, int group) {
   PagedSplit m{};
   if (last && last->end < last->r.blocks && last->begin == 0) {
-    m.parts = 1 + static_cast<int>((last->r.blocks - last->end + share - 1) / share);
+    m.parts = 1 + static_cast<int>(paged_div(last->r.blocks - last->end + share - 1, share));
     m.row0 = last->s.row0;
     m.first = last->rt * rows_per_tile;
     m.rows = min(rows_per_tile, last->s.n * group - m.first);
