@@ -35,7 +35,7 @@ template <int D, int MT> struct Cfg {
   static constexpr int SMEM = STAGES * 2 * TILE_BYTES + JOIN_BYTES + 1024;  // + Small
   struct Small {
     uint64_t full[STAGES], empty[STAGES];
-    long long scratch[THREADS / 32 + 4];
+    PagedWalkScratch<THREADS> scratch;
     float2 join_ml[2 * MT][16];
     volatile int abort_flag;
   };

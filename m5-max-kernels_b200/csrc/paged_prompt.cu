@@ -67,7 +67,7 @@ template <int D> struct Cfg {
     uint64_t pv_done[2][2];                  // [half][buffer]
     uint64_t o_full[2], drain[2];            // after a piece's last PV; [MMA thread]
     uint64_t landed;                            // a V block to be blanked
-    long long scratch[kThreads / 32 + 4];
+    PagedWalkScratch<kThreads> scratch;
     Piece piece[2];
     uint32_t tmem;
     volatile int abort_flag;
@@ -160,15 +160,21 @@ __device__ __forceinline__ float2 tanh_ratio(float2 z) {
   return __ffma2_rn(p, z, make_float2(0x1.ffffecp-1f, 0x1.ffffecp-1f));
 }
 
+// What is done to the scores: nothing, a bias, a cap (and, by a flag, a bias).
+// Each has a kernel, for the sake of the instruction cache: one for all took 4
+// to 7 % longer.
+enum Scores : int { kPlain = 0, kBiased = 1, kCapped = 2 };
+
 // A row's 64 scores capped, biased and in log2 units; `ahead` is the row's
 // position minus that of the first key.  Special functions would take as long
 // as the exponentials do three times over, so scores within the cap, the usual
 // case, go by tanh_ratio; a warp with any beyond it takes
 // tanh(y) = 1 - 2 / (e^2y + 1) for all of its own.
+template <int SCORES>
 __device__ __forceinline__ void modify(uint32_t (&s)[2][32], float scale, float softcap,
                                        bool biased, float slope, int ahead) {
   const float k = scale * kLog2e;
-  if (softcap > 0.0f) {
+  if (SCORES == kCapped) {
     const float r = scale / softcap;
     float top[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -203,7 +209,7 @@ __device__ __forceinline__ void modify(uint32_t (&s)[2][32], float scale, float 
       s[e / 32][e % 32 + 1] = __float_as_uint(y.y);
     }
   }
-  if (!biased) return;
+  if (SCORES == kCapped && !biased) return;
   const float down = -slope * kLog2e, first = static_cast<float>(ahead);
   if (__all_sync(~0u, ahead >= 63)) {  // no key is ahead of its row: the distance is linear
     const float2 d2 = make_float2(down, down), f2 = make_float2(first, first);
@@ -227,11 +233,12 @@ template <bool B> struct Flag {
   static constexpr bool value = B;
 };
 
-template <typename T, int D, bool MOD>
+template <typename T, int D, int SCORES>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_prompt_kernel(const PagedAttnArgs a, const __grid_constant__ PagedMaps maps) {
   using C = Cfg<D>;
   constexpr int STAGES = C::STAGES;
+  constexpr bool MOD = SCORES != kPlain;
   // (no static shared memory: the tiles start on the swizzle's 1024-byte grid)
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* const q_smem = smem;  // [buffer][half]
@@ -551,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.s_free[h]);
-        if (MOD) modify(s, a.scale, a.softcap, a.slopes != nullptr, slope, pos - block0);
+        if (MOD) modify<SCORES>(s, a.scale, a.softcap, a.slopes != nullptr, slope, pos - block0);
         if (decltype(masked)::value && !(MOD && open)) {
           const int hi = row_hi - block0, lo = row_lo - block0, pr = prefix - block0;
 #pragma unroll
@@ -696,10 +703,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int D, bool MOD>
+template <typename T, int D, int SCORES>
 cudaError_t launch(const PagedAttnArgs& a, const PagedMaps& m, int sms, cudaStream_t stream) {
   using C = Cfg<D>;
-  auto kern = paged_prompt_kernel<T, D, MOD>;
+  auto kern = paged_prompt_kernel<T, D, SCORES>;
   static std::atomic<long long> shape[kMaxLaunchDevices];
   int dev = 0, n = 0, per_sm = 0;
   cudaError_t e = launch_shape(reinterpret_cast<const void*>(kern), kThreads, C::SMEM, shape, &dev,
@@ -725,8 +732,8 @@ cudaError_t launch(const PagedAttnArgs& a, const PagedMaps& m, int sms, cudaStre
 
 template <typename T, int D>
 cudaError_t by_scores(const PagedAttnArgs& a, const PagedMaps& m, int sms, cudaStream_t stream) {
-  return a.softcap > 0.0f || a.slopes ? launch<T, D, true>(a, m, sms, stream)
-                                      : launch<T, D, false>(a, m, sms, stream);
+  if (a.softcap > 0.0f) return launch<T, D, kCapped>(a, m, sms, stream);
+  return a.slopes ? launch<T, D, kBiased>(a, m, sms, stream) : launch<T, D, kPlain>(a, m, sms, stream);
 }
 
 }  // namespace

@@ -153,86 +153,99 @@ struct PagedWalk {
   }
 };
 
-// Called by all threads of the CTA (THREADS of them, whole warps); `scratch`
-// is shared memory for THREADS / 32 + 4 values.
+// Shared memory of paged_walk.
+template <int THREADS> struct PagedWalkScratch {
+  long long sums[THREADS / 32];
+  long long rest;  // blocks of the head before the stretch
+  int seq, head;
+  PagedSeq s;
+};
+
+// Called by all threads of the CTA (THREADS of them, whole warps).  A thread
+// sums the blocks of its sequences, and the one whose sequences hold the
+// stretch's first block says where; the rest of the way every warp goes alone.
 template <int ROWS, int BK, int THREADS>
 __device__ __forceinline__ PagedWalk<ROWS, BK> paged_walk(const PagedAttnArgs& a,
-                                                          long long* scratch) {
+                                                          PagedWalkScratch<THREADS>& scratch) {
   constexpr int kWarps = THREADS / 32;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int per = (a.b.batch + THREADS - 1) / THREADS;
   const int b0 = threadIdx.x * per;
-  long long mine = 0;
+  long long mine = 0, one = 0;
+  PagedSeq s{};
   for (int i = 0; i < per; ++i) {
-    PagedSeq s{};
+    s = PagedSeq{};
     if (b0 + i < a.b.batch) s = paged_seq(a, b0 + i);
-    mine += paged_seq_blocks<ROWS, BK>(a, s) * a.b.kv_heads;
+    one = paged_seq_blocks<ROWS, BK>(a, s);
+    mine += one * a.b.kv_heads;
   }
   long long upto = mine;
   for (int d = 1; d < 32; d <<= 1) {
     const long long o = __shfl_up_sync(~0u, upto, d);
     if (lane >= d) upto += o;
   }
-  if (lane == 31) scratch[warp] = upto;
-  if (threadIdx.x == 0) scratch[kWarps] = -1;
+  if (lane == 31) scratch.sums[warp] = upto;
   __syncthreads();
   long long before = upto - mine, total = 0;
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += scratch[w];
-    total += scratch[w];
+    if (w < warp) before += scratch.sums[w];
+    total += scratch.sums[w];
   }
   PagedWalk<ROWS, BK> walk;
   walk.share = paged_div(total + gridDim.x - 1, gridDim.x);
   const long long at = walk.share * blockIdx.x;
   walk.left = max(0ll, min(walk.share, total - at));
-  // the thread whose sequences hold block `at` looks which one does (all lanes
-  // of its warp take part in the sums)
+  // (all lanes of the warp take part in the sums of more sequences than threads)
   const bool here = walk.left > 0 && before <= at && at < before + mine;
   if (__any_sync(~0u, here)) {
     long long base = before;
     bool found = false;
     for (int i = 0; i < per; ++i) {
-      PagedSeq s{};
-      if (b0 + i < a.b.batch) s = paged_seq(a, b0 + i);
-      const long long one = paged_seq_blocks<ROWS, BK>(a, s), all = one * a.b.kv_heads;
+      if (per > 1) {
+        s = PagedSeq{};
+        if (b0 + i < a.b.batch) s = paged_seq(a, b0 + i);
+        one = paged_seq_blocks<ROWS, BK>(a, s);
+      }
+      const long long all = one * a.b.kv_heads;
       if (here && !found && at < base + all) {
         found = true;
-        scratch[kWarps] = b0 + i;
         const long long head = paged_div(at - base, one);
-        scratch[kWarps + 1] = head;
-        scratch[kWarps + 2] = at - base - head * one;
+        scratch.seq = b0 + i;
+        scratch.head = static_cast<int>(head);
+        scratch.rest = at - base - head * one;
+        scratch.s = s;
       }
       base += all;
     }
   }
   __syncthreads();
-  walk.seq = static_cast<int>(scratch[kWarps]);
-  walk.head = 0;
-  walk.rt = 0;
-  walk.blk = 0;
-  walk.tiles = 0;
-  if (walk.seq < 0) walk.left = 0;
+  walk.seq = walk.head = walk.rt = walk.blk = walk.tiles = 0;
   if (walk.left > 0) {
-    walk.head = static_cast<int>(scratch[kWarps + 1]);
-    long long rest = scratch[kWarps + 2];
-    walk.s = paged_seq(a, walk.seq);
+    walk.seq = scratch.seq;
+    walk.head = scratch.head;
+    walk.s = scratch.s;
+    long long rest = scratch.rest;
     walk.tiles = paged_tiles(a, walk.s.n, ROWS);
-    for (int base = 0; base < walk.tiles; base += 32) {  // 32 row tiles at a time
-      const int t = base + lane;
-      const int blocks = t < walk.tiles ? paged_blocks<ROWS, BK>(a, walk.s, t).blocks : 0;
-      long long sum = blocks;
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(~0u, sum, d);
-        if (lane >= d) sum += o;
+    if (walk.tiles == 1) {
+      walk.blk = static_cast<int>(rest);
+    } else {
+      for (int base = 0; base < walk.tiles; base += 32) {  // 32 row tiles at a time
+        const int t = base + lane;
+        const int blocks = t < walk.tiles ? paged_blocks<ROWS, BK>(a, walk.s, t).blocks : 0;
+        long long sum = blocks;
+        for (int d = 1; d < 32; d <<= 1) {
+          const long long o = __shfl_up_sync(~0u, sum, d);
+          if (lane >= d) sum += o;
+        }
+        const uint32_t past = __ballot_sync(~0u, sum > rest);
+        if (past) {
+          const int src = __ffs(past) - 1;
+          walk.rt = base + src;
+          walk.blk = static_cast<int>(rest - __shfl_sync(~0u, sum - blocks, src));
+          break;
+        }
+        rest -= __shfl_sync(~0u, sum, 31);
       }
-      const uint32_t past = __ballot_sync(~0u, sum > rest);
-      if (past) {
-        const int src = __ffs(past) - 1;
-        walk.rt = base + src;
-        walk.blk = static_cast<int>(rest - __shfl_sync(~0u, sum - blocks, src));
-        break;
-      }
-      rest -= __shfl_sync(~0u, sum, 31);
     }
   }
   return walk;
