@@ -435,8 +435,10 @@ M5B_API int m5b_paged_append(const m5b_paged_append_args* args, void* stream);
  * largest n_b and chooses the kernel; the result does not depend on it.
  * Slots behind a sequence's end may hold anything; keys and values of the
  * sequences themselves are finite.  The workspace
- * (m5b_paged_attention_workspace_bytes) is scratch, overwritten by every call;
- * calls that overlap on the GPU need separate ones. */
+ * (m5b_paged_attention_workspace_bytes) must be all zero before its first use
+ * (cudaMemset once after allocating it) and is left in a state that later calls
+ * of any shape may find; calls that overlap on the GPU need separate ones.
+ * After a nonzero m5b_device_status (a timed-out wait) zero it again. */
 typedef struct m5b_paged_attention_args {
   m5b_paged_batch b;
   const void* q;

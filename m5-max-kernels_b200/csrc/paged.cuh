@@ -52,6 +52,7 @@ struct PagedAttnArgs {
   const float* slopes;
   int window;  // INT_MAX: none
   const int32_t* prefix_lens;
+  int* tickets;          // [kPagedTickets], zero between launches (decode kernel)
   void* workspace;       // the tiled kernels' PagedPartials
   unsigned int* status;  // device status word (bounded-wait errors)
 };
@@ -73,6 +74,7 @@ cudaError_t launch_paged_append(const PagedAppendArgs& a, int x_dtype, int cache
 cudaError_t launch_paged_attention_rows(const PagedAttnArgs& a, int dtype, cudaStream_t stream);
 // The tiled kernels: 16-bit types, 64 or 128 channels, pages of 2^k >= 8
 // slots, everything on the 16-byte grid.
+constexpr int kPagedTickets = 1024;  // CTAs of a decode launch, at most
 constexpr int kDecodeRows = 32;  // rows per kv head and sequence that the decode kernel is for
 cudaError_t launch_paged_decode(const PagedAttnArgs& a, const PagedMaps& m, int dtype, int sms,
                                 cudaStream_t stream);

@@ -64,6 +64,8 @@ int take_batch(const m5b_paged_batch& s, PagedBatch& d) {
   return M5B_OK;
 }
 
+constexpr int64_t kTicketBytes = kPagedTickets * sizeof(int);  // first in the workspace
+
 bool pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
 bool grid16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -172,7 +174,7 @@ int64_t m5b_paged_attention_workspace_bytes(int64_t head_dim) {
   if ((head_dim != 64 && head_dim != 128) || current_device_state(nullptr, &sms)) return 0;
   const int64_t few = paged_decode_workspace(static_cast<int>(head_dim), sms);
   const int64_t many = paged_prompt_workspace(static_cast<int>(head_dim), sms);
-  return few > many ? few : many;
+  return kTicketBytes + (few > many ? few : many);
 }
 
 int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
@@ -208,8 +210,9 @@ int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
     int sms = 0;
     rc = current_device_state(&a.status, &sms);
     if (rc) return rc;
-    a.workspace = s->workspace;
-    if (!a.workspace || !grid16(a.workspace) ||
+    a.tickets = static_cast<int*>(s->workspace);
+    a.workspace = static_cast<uint8_t*>(s->workspace) + kTicketBytes;
+    if (!s->workspace || !grid16(s->workspace) || 2 * sms > kPagedTickets ||
         s->workspace_bytes < m5b_paged_attention_workspace_bytes(a.b.head_dim))
       return einval("workspace of m5b_paged_attention_workspace_bytes(head_dim) bytes required");
     const bool few = int64_t(a.max_query_len) * a.b.group <= kDecodeRows;

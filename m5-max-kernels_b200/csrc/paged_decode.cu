@@ -13,7 +13,9 @@
 // rounding).  m only follows the row's maximum when that has grown by more
 // than 2^8, so that o is rarely rescaled; p stays below 2^8.  At a tile's end
 // the warps' parts are added through shared memory.  paged_sched.cuh deals
-// the blocks out evenly whatever the lengths are.
+// the blocks out evenly whatever the lengths are; the parts of a split tile
+// are joined by whichever CTA finishes its part last (a ticket per tile tells),
+// always in the same order.
 #include "paged_sched.cuh"
 
 namespace m5b {
@@ -37,6 +39,7 @@ template <int D, int MT> struct Cfg {
     uint64_t full[STAGES], empty[STAGES];
     PagedWalkScratch<THREADS> scratch;
     float2 join_ml[2 * MT][16];
+    int last;
     volatile int abort_flag;
   };
   static_assert(sizeof(Small) <= 1024, "shared memory layout");
@@ -175,10 +178,9 @@ __global__ void __launch_bounds__(Cfg<D, MT>::THREADS, Cfg<D, MT>::PER_SM)
   const int lrow = slice * 16 + (lane & 7);
   const int k_row = lrow + ((lane >> 4) & 1) * 8, k_chunk = (lane >> 3) & 1;  // keys 0-7 | 8-15 last
   const int v_row = lrow + ((lane >> 3) & 1) * 8, v_chunk = (lane >> 4) & 1;  // channels last
-  bool any = false, ok = true;
+  bool ok = true;
   // (a warp whose wait gave up still walks along, for the barriers' sake)
   while (walk.next(a, p)) {
-    any = true;
     const int first = p.rt * ROWS + mt * 16;  // this warp's packed rows
     const int rows = p.s.n * group;
     uint32_t q[D / 16][4];
@@ -349,8 +351,8 @@ __global__ void __launch_bounds__(Cfg<D, MT>::THREADS, Cfg<D, MT>::PER_SM)
         }
       }
     }
+    const bool whole = p.whole();
     if (slice == 0) {
-      const bool whole = p.whole();
       const int64_t slot = 2 * int64_t(blockIdx.x) + (p.begin == 0 ? 1 : 0);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -377,9 +379,24 @@ __global__ void __launch_bounds__(Cfg<D, MT>::THREADS, Cfg<D, MT>::PER_SM)
         }
       }
     }
+    if (!whole) {  // the last CTA to get here joins the tile's parts
+      __threadfence();
+      consumers_sync<C::WARPS * 32>();
+      const int from = static_cast<int>(paged_div(p.tile_at, walk.share));
+      const int to = static_cast<int>(paged_div(p.tile_at + p.r.blocks - 1, walk.share));
+      if (threadIdx.x == 0) small.last = atomicAdd(&a.tickets[from], 1) == to - from;
+      consumers_sync<C::WARPS * 32>();
+      if (small.last) {
+        __threadfence();
+        for (int r = warp; r < ROWS && p.rt * ROWS + r < rows; r += C::WARPS) {
+          const int packed = p.rt * ROWS + r;
+          paged_join_row<T, ROWS, D>(a, parts, from, to - from + 1, r, p.s.row0 + packed / group,
+                                     p.head * group + packed % group);
+        }
+        if (threadIdx.x == 0) a.tickets[from] = 0;
+      }
+    }
   }
-  if (threadIdx.x == 0)
-    paged_write_split(&parts.split[blockIdx.x], any ? &p : nullptr, walk.share, ROWS, group);
   paged_zero_outside<T, D>(a, int64_t(blockIdx.x) * (C::WARPS * 32) + threadIdx.x,
                            int64_t(gridDim.x) * (C::WARPS * 32));
 }
@@ -404,12 +421,7 @@ cudaError_t launch(const PagedAttnArgs& a, const PagedMaps& m, int sms, cudaStre
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, a, m);
-  if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), C::ROWS / 4);
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<T, C::ROWS, D>, a, ctas);
+  return cudaLaunchKernelEx(&cfg, kern, a, m);
 }
 
 template <typename T, int D>

@@ -100,6 +100,7 @@ __device__ __forceinline__ long long paged_seq_blocks(const PagedAttnArgs& a, co
 // One stretch of a tile: blocks [begin, end) of its `r.blocks`.
 struct PagedPiece {
   int seq, head, rt, begin, end;
+  long long tile_at;  // place of the tile's first block in the line
   PagedSeq s;
   PagedBlocks r;
   __device__ __forceinline__ bool whole() const { return begin == 0 && end == r.blocks; }
@@ -115,7 +116,7 @@ __device__ __forceinline__ long long paged_div(long long a, long long b) {
 template <int ROWS, int BK>
 struct PagedWalk {
   int seq, head, rt, tiles, blk;
-  long long left, share;
+  long long left, share, at;  // blocks left, of an equal stretch; the next block's place in the line
   PagedSeq s;
 
   __device__ __forceinline__ void enter(const PagedAttnArgs& a) {  // first tile of a sequence >= seq
@@ -138,6 +139,8 @@ struct PagedWalk {
     p.begin = blk;
     p.end = static_cast<int>(min(static_cast<long long>(p.r.blocks), blk + left));
     left -= p.end - p.begin;
+    p.tile_at = at - p.begin;
+    at += p.end - p.begin;
     if (p.end == p.r.blocks) {
       blk = 0;
       if (++rt == tiles) {
@@ -194,6 +197,7 @@ __device__ __forceinline__ PagedWalk<ROWS, BK> paged_walk(const PagedAttnArgs& a
   PagedWalk<ROWS, BK> walk;
   walk.share = paged_div(total + gridDim.x - 1, gridDim.x);
   const long long at = walk.share * blockIdx.x;
+  walk.at = at;
   walk.left = max(0ll, min(walk.share, total - at));
   // (all lanes of the warp take part in the sums of more sequences than threads)
   const bool here = walk.left > 0 && before <= at && at < before + mine;
@@ -287,54 +291,46 @@ __device__ __forceinline__ void paged_write_split(PagedSplit* at, const PagedPie
   *at = m;
 }
 
-// Joins the parts of the tiles that were split: CTA (c, i) takes every
-// gridDim.y-th four rows of the tile that CTA c left to others, one warp a
-// row, the lanes across the channels.
+// Joins the `parts` of a tile that CTA c began, stored by rows: the calling
+// warp takes row `row` of the workspace's, the lanes across the channels.
 template <typename T, int ROWS, int D>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnArgs a, int ctas) {
+__device__ __forceinline__ void paged_join_row(const PagedAttnArgs& a, const PagedPartials<ROWS, D>& w,
+                                               int c, int parts, int row, int token, int head) {
   constexpr int V = D / 32;
-  grid_dependency_wait();
-  const PagedPartials<ROWS, D> w(a.workspace, ctas);
-  const int c = blockIdx.x;
-  const PagedSplit m = w.split[c];
-  if (m.parts == 0) return;
   const int lane = threadIdx.x % 32;
-  for (int row = blockIdx.y * 4 + threadIdx.x / 32; row < m.rows; row += gridDim.y * 4) {
-    float top = -INFINITY;
-    for (int i = lane; i < m.parts; i += 32) {
-      const int slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
-      top = fmaxf(top, w.ml[int64_t(slot) * ROWS + row].x);
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    float sum = 0.0f, o[V] = {};
-#pragma unroll 4
-    for (int i = 0; i < m.parts; ++i) {
-      const int slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
-      const float2 ml = w.ml[int64_t(slot) * ROWS + row];
-      const float* po = w.o + (int64_t(slot) * ROWS + row) * D + lane * V;
-      const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
-      sum = fmaf(ml.y, f, sum);
-#pragma unroll
-      for (int v = 0; v < V; v += 2) {
-        const float2 x = *reinterpret_cast<const float2*>(po + v);
-        o[v] = fmaf(x.x, f, o[v]);
-        o[v + 1] = fmaf(x.y, f, o[v + 1]);
-      }
-    }
-    const int packed = m.first + row, t = m.row0 + packed / a.b.group;
-    const int h = m.head * a.b.group + packed % a.b.group;
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    T* out = static_cast<T*>(a.out) + t * a.o_token + h * a.o_head + lane * V;
-#pragma unroll
-    for (int v = 0; v < V; ++v) out[v] = from_f32<T>(o[v] * inv);
-    if (a.lse && lane == 0)
-      a.lse[int64_t(t) * a.b.q_heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) {
+    const int64_t slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
+    top = fmaxf(top, __ldcg(&w.ml[slot * ROWS + row]).x);
   }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+  float sum = 0.0f, o[V] = {};
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) {
+    const int64_t slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
+    const float2 ml = __ldcg(&w.ml[slot * ROWS + row]);
+    const float2* po = reinterpret_cast<const float2*>(w.o + (slot * ROWS + row) * D + lane * V);
+    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+#pragma unroll
+    for (int v = 0; v < V; v += 2) {
+      const float2 x = __ldcg(po + v / 2);
+      o[v] = fmaf(x.x, f, o[v]);
+      o[v + 1] = fmaf(x.y, f, o[v + 1]);
+    }
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  T* out = static_cast<T*>(a.out) + int64_t(token) * a.o_token + head * a.o_head + lane * V;
+#pragma unroll
+  for (int v = 0; v < V; ++v) out[v] = from_f32<T>(o[v] * inv);
+  if (a.lse && lane == 0)
+    a.lse[int64_t(token) * a.b.q_heads + head] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
-// The same for parts stored by columns, [D / 4][ROWS][4]: CTA (c, i) takes
-// channels 16 i .. 16 i + 15, a thread a row.
+// Joins the parts, stored by columns, [D / 4][ROWS][4], of the tiles that were
+// split: CTA (c, i) takes channels 16 i .. 16 i + 15 of the one that CTA c left
+// to others, a thread a row.
 template <typename T, int ROWS, int D>
 __global__ void __launch_bounds__(ROWS) paged_join_columns_kernel(const PagedAttnArgs a, int ctas) {
   grid_dependency_wait();

@@ -112,7 +112,7 @@ _scratch_bytes: dict = {}
 
 
 def _scratch(index, dim):
-    """Cached scratch of the attention kernels, one per device and stream."""
+    """Cached workspace of the attention kernels, one per device and stream, zeroed once."""
     need = _scratch_bytes.get((index, dim))
     if need is None:
         with torch.cuda.device(index):
@@ -124,7 +124,7 @@ def _scratch(index, dim):
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < need:
         with _ws_lock:
-            buf = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index))
+            buf = torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", index))
             _workspaces[key] = buf
     return buf.data_ptr(), need
 
