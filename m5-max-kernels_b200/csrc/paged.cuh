@@ -75,7 +75,7 @@ cudaError_t launch_paged_attention_rows(const PagedAttnArgs& a, int dtype, cudaS
 // The tiled kernels: 16-bit types, 64 or 128 channels, pages of 2^k >= 8
 // slots, everything on the 16-byte grid.
 constexpr int kPagedTickets = 1024;  // CTAs of a decode launch, at most
-constexpr int kDecodeRows = 32;  // rows per kv head and sequence that the decode kernel is for
+constexpr int kDecodeRows = 16;  // rows per kv head and sequence that the decode kernel is for
 cudaError_t launch_paged_decode(const PagedAttnArgs& a, const PagedMaps& m, int dtype, int sms,
                                 cudaStream_t stream);
 int64_t paged_decode_workspace(int head_dim, int sms);

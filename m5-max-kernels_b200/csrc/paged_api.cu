@@ -215,6 +215,10 @@ int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
     if (!s->workspace || !grid16(s->workspace) || 2 * sms > kPagedTickets ||
         s->workspace_bytes < m5b_paged_attention_workspace_bytes(a.b.head_dim))
       return einval("workspace of m5b_paged_attention_workspace_bytes(head_dim) bytes required");
+    // Up to 16 rows a kv head the decode kernel, beyond that the prompt kernel,
+    // for 4 (16) rows: 158 (165) against 179 us for 4 sequences of 60000 keys,
+    // 54 (55) against 58 for 16 of 4000, 9.4 (12.9) against 13.7 for one of 517;
+    // for 24 rows, two tiles of 16: 305 against 184 and 69 against 59.
     const bool few = int64_t(a.max_query_len) * a.b.group <= kDecodeRows;
     PagedMaps m{};
     if (!few) row_map(m, a, dtype);

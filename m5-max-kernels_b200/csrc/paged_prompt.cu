@@ -18,27 +18,34 @@
 //
 // TMEM's 512 columns hold O (2 x 128), S (2 x 64) and P (2 x 2 x 32): QK of
 // the next step starts when the softmax has read S, and PV of this one when P
-// is there, and neither waits for the other.  (One S buffer of 128 keys a
-// half, with P over it, fits as well and needs fewer bytes of shared memory a
-// flop, but chains softmax, PV, QK, softmax: 4250 cycles for 128 keys.)  m
-// only follows the row's maximum when that has grown by more than 2^8; then O
-// is rescaled in place.  (Taking the exponentials with the old m while looking
-// for the maximum, and again in the rare case, keeps the scores in registers
-// for longer: 2200 cycles a step for TIME.)
+// is there.  (Measured and not kept: two S buffers with P over them, whose
+// reuse chains softmax, PV and QK, 1830 cycles; one S buffer of 128 keys, which
+// needs fewer bytes of shared memory a flop but chains them all the more, 4250
+// for 128 keys.)  m only follows the row's maximum when that has grown by more
+// than 2^8; then O is rescaled in place.  (Taking the exponentials with the
+// old m first, and again in the rare case: 2200 cycles.)  P is rounded to the
+// cache's type for the product, once, at the size of the output's own rounding;
+// sums, m and O are fp32.
 //
-// Bound by shared memory's bandwidth in the products: an MMA of 128 x 64 x 16
-// reads 6 KB where its 32 cycles have 4, so that a step takes 8 * 48 + 4 * 64
-// cycles a half at D = 128, 80 % of the tensor cores' rate; the exponentials,
-// 128 * 64 / 16 = 512 cycles a half, fit beside them.
+// What bounds it: an MMA of 128 x 64 x 16 reads 6 KB of shared memory where its
+// 32 cycles have room for 4, so the products take 8 * 48 + 4 * 64 cycles a half
+// and step at D = 128, 1290 for both halves with the softmax beside them (a
+// test of the two alone), 1460 here without the exponentials (TMA writes, the
+// issuing threads' waits) and 1730 with them: two prompts of 8192 tokens, 32 +
+// 8 heads, 1.15 ms, 958 TFLOP/s.
 #include "paged_sched.cuh"
 
 namespace m5b {
 namespace {
 
 constexpr int kBlock = kPagedBlock;  // keys per step
-constexpr int kRows = 256;     // packed rows per tile, two halves
-constexpr float kGrow = 8.0f;           // log2 of the growth that m may lag behind
-constexpr int kFmaPairs = 3;             // of 8 pairs of exponentials, those by ex2_fma
+constexpr int kRows = 256;           // packed rows per tile, two halves
+constexpr float kGrow = 8.0f;        // log2 of the growth that m may lag behind
+// Of 8 pairs of exponentials, those by ex2_fma: 1730 cycles a step (1800 with
+// none, 1760 with 2, 1790 with 4).  None where the scores are modified, whose
+// arithmetic keeps the FMA pipes busy (162 us, 187 with 3, in the distance bias
+// of 56 heads).
+constexpr int kFmaPairs = 3;
 constexpr int kThreads = 384;  // warps 0-3, 4-7: halves; 8: QK; 9: PV; 10: K, V; 11: rows
 constexpr int kMmaWarp = 8, kTmaWarp = 10, kRowWarp = 11;
 
@@ -66,7 +73,7 @@ template <int D> struct Cfg {
     uint64_t p_full[2][2];                   // [half][buffer]
     uint64_t pv_done[2][2];                  // [half][buffer]
     uint64_t o_full[2], drain[2];            // after a piece's last PV; [MMA thread]
-    uint64_t landed;                            // a V block to be blanked
+    uint64_t landed;                         // a V block to be blanked
     PagedWalkScratch<kThreads> scratch;
     Piece piece[2];
     uint32_t tmem;
@@ -161,8 +168,8 @@ __device__ __forceinline__ float2 tanh_ratio(float2 z) {
 }
 
 // What is done to the scores: nothing, a bias, a cap (and, by a flag, a bias).
-// Each has a kernel, for the sake of the instruction cache: one for all took 4
-// to 7 % longer.
+// Each has a kernel, for the sake of the instruction cache: one for both of the
+// latter took 4 to 7 % longer.
 enum Scores : int { kPlain = 0, kBiased = 1, kCapped = 2 };
 
 // A row's 64 scores capped, biased and in log2 units; `ahead` is the row's

@@ -292,40 +292,66 @@ __device__ __forceinline__ void paged_write_split(PagedSplit* at, const PagedPie
 }
 
 // Joins the `parts` of a tile that CTA c began, stored by rows: the calling
-// warp takes row `row` of the workspace's, the lanes across the channels.
-template <typename T, int ROWS, int D>
-__device__ __forceinline__ void paged_join_row(const PagedAttnArgs& a, const PagedPartials<ROWS, D>& w,
-                                               int c, int parts, int row, int token, int head) {
-  constexpr int V = D / 32;
+// warp takes rows row, row + STEP, ... (R of them) of the tile's packed rows
+// from `first` on, the lanes across the channels, four parts at a time.  (Short
+// code on purpose: a launch runs it once, from a cold instruction cache.)
+template <typename T, int ROWS, int D, int R, int STEP>
+__device__ __forceinline__ void paged_join_rows(const PagedAttnArgs& a, const PagedPartials<ROWS, D>& w,
+                                                int c, int parts, int row, int row0, int head, int first) {
+  constexpr int V = D / 32, U = 4;
   const int lane = threadIdx.x % 32;
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) {
-    const int64_t slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
-    top = fmaxf(top, __ldcg(&w.ml[slot * ROWS + row]).x);
-  }
+  float top[R], sum[R], o[R][V] = {};
 #pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-  float sum = 0.0f, o[V] = {};
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const int64_t slot = i == 0 ? 2 * c + 1 : 2 * (c + i);
-    const float2 ml = __ldcg(&w.ml[slot * ROWS + row]);
-    const float2* po = reinterpret_cast<const float2*>(w.o + (slot * ROWS + row) * D + lane * V);
-    const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
+  for (int r = 0; r < R; ++r) top[r] = -INFINITY, sum[r] = 0.0f;
+#pragma unroll 1
+  for (int i = 0; i < parts; i += U) {
+    float2 ml[R][U], x[R][U][V / 2];
 #pragma unroll
-    for (int v = 0; v < V; v += 2) {
-      const float2 x = __ldcg(po + v / 2);
-      o[v] = fmaf(x.x, f, o[v]);
-      o[v + 1] = fmaf(x.y, f, o[v + 1]);
+    for (int u = 0; u < U; ++u) {
+      const int k = min(i + u, parts - 1);
+      const int64_t at = int64_t(k == 0 ? 2 * c + 1 : 2 * (c + k)) * ROWS + row;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        ml[r][u] = __ldcg(&w.ml[at + r * STEP]);
+        const float2* po = reinterpret_cast<const float2*>(w.o + (at + r * STEP) * D + lane * V);
+#pragma unroll
+        for (int v = 0; v < V / 2; ++v) x[r][u][v] = __ldcg(po + v);
+        if (i + u >= parts) ml[r][u].x = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float m2 = top[r];
+#pragma unroll
+      for (int u = 0; u < U; ++u) m2 = fmaxf(m2, ml[r][u].x);
+      const float base = m2 == -INFINITY ? 0.0f : m2, keep = ex2(top[r] - base);
+      top[r] = m2;
+      sum[r] *= keep;
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[r][v] *= keep;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float f = ex2(ml[r][u].x - base);
+        sum[r] = fmaf(ml[r][u].y, f, sum[r]);
+#pragma unroll
+        for (int v = 0; v < V / 2; ++v) {
+          o[r][2 * v] = fmaf(x[r][u][v].x, f, o[r][2 * v]);
+          o[r][2 * v + 1] = fmaf(x[r][u][v].y, f, o[r][2 * v + 1]);
+        }
+      }
     }
   }
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  T* out = static_cast<T*>(a.out) + int64_t(token) * a.o_token + head * a.o_head + lane * V;
 #pragma unroll
-  for (int v = 0; v < V; ++v) out[v] = from_f32<T>(o[v] * inv);
-  if (a.lse && lane == 0)
-    a.lse[int64_t(token) * a.b.q_heads + head] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  for (int r = 0; r < R; ++r) {
+    const int packed = first + row + r * STEP, h = head * a.b.group + packed % a.b.group;
+    const int64_t t = row0 + packed / a.b.group;
+    const float inv = sum[r] > 0.0f ? 1.0f / sum[r] : 0.0f;
+    T* out = static_cast<T*>(a.out) + t * a.o_token + h * a.o_head + lane * V;
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = from_f32<T>(o[r][v] * inv);
+    if (a.lse && lane == 0)
+      a.lse[t * a.b.q_heads + h] = sum[r] > 0.0f ? (top[r] + log2f(sum[r])) * kLn2 : -INFINITY;
+  }
 }
 
 // Joins the parts, stored by columns, [D / 4][ROWS][4], of the tiles that were

@@ -367,3 +367,46 @@ def test_append_skips_what_has_no_place(ops):
     assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
     # tokens at 0..3 and 30 have a table row, the one at 31 and the padding have not
     assert (out[:5] == 1).all() and (out[5:] == 0).all()
+
+
+# ---------------------------------------------------------------- together
+
+def test_generation_example():
+    """The quantized layer around the two operators: chunks and single tokens, mixed, against
+    whole prompts.  Codes of the output projection (1/127 of a row's peak apart) may differ by one
+    where two attention kernels round differently: far below 2 % of the layer's contribution."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "m5-max-kernels_b200/examples/paged_generation.py"
+    spec = importlib.util.spec_from_file_location("paged_generation", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    assert example.main(width=1024, q_heads=8, kv_heads=2, lengths=(150, 1, 40, 97), chunk=33) < 2e-2
+
+
+def test_after_the_grouped_projection(ops):
+    """The head-major Q, K, V of projection_qkv_rope go into the cache without a copy."""
+    g = torch.Generator().manual_seed(12)
+    n, width, heads = 70, 512, 3
+    x = torch.randn(n, width, generator=g).to(BF16).to(DEV)
+    w = (torch.randn(heads * 384, width, generator=g) * width**-0.5).to(BF16).to(DEV)
+    aq, sa = ops.quantize(x, "int8")
+    bq, sb = ops.quantize(w, "int8")
+    gamma = torch.ones(128, dtype=BF16, device=DEV)
+    cos, sin = ops.rope_tables(n, 64, device=DEV)
+    q, k, v = ops.projection_qkv_rope(aq, bq, gamma, gamma, cos, sin, "int8", a_scales=sa,
+                                      b_scales=sb)
+    page = 32
+    kc = torch.full((4, heads, page, 128), math.nan, dtype=BF16, device=DEV)
+    vc = kc.clone()
+    table = torch.tensor([[2, 0, 3]], dtype=torch.int32, device=DEV)
+    starts = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    assert ops.paged_append(k.transpose(0, 1), v.transpose(0, 1), kc, vc, table, starts, lens) is None
+    out = ops.paged_attention(q.transpose(0, 1), kc, vc, table, starts, lens, max_query_len=n)
+    scores = (q.double() @ k.double().transpose(1, 2)) * 128**-0.5
+    hidden = torch.ones(n, n, device=DEV).triu(1).bool()
+    p = torch.softmax(scores.masked_fill(hidden, -math.inf), -1)
+    want, spread = (p @ v.double()).transpose(0, 1), (p @ v.double().abs()).transpose(0, 1)
+    check_attention(out, None, want.cpu(), None, spread.cpu(), BF16)
