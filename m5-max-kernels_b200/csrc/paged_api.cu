@@ -64,7 +64,8 @@ int take_batch(const m5b_paged_batch& s, PagedBatch& d) {
   return M5B_OK;
 }
 
-constexpr int64_t kTicketBytes = kPagedTickets * sizeof(int);  // first in the workspace
+constexpr int64_t kTicketBytes = M5B_PAGED_COUNTER_BYTES;  // first in the workspace
+static_assert(kTicketBytes == kPagedTickets * sizeof(int), "a counter for each ticket");
 
 bool pow2(int64_t v) { return v > 0 && (v & (v - 1)) == 0; }
 bool grid16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }

@@ -109,10 +109,17 @@ def _device(tensors):
 
 
 _scratch_bytes: dict = {}
+_COUNTER_BYTES = 4096  # M5B_PAGED_COUNTER_BYTES
 
 
 def _scratch(index, dim):
-    """Cached workspace of the attention kernels, one per device and stream, zeroed once."""
+    """(pointer, bytes) of the attention kernels' workspace, its counters zero.
+
+    One is kept for each device and stream.  A stream that has none when a
+    graph is captured on it gives the captured call its own, from the graph's
+    memory and with a memset in the graph: nothing outside the graph may rely
+    on a memset that runs when it is replayed.
+    """
     need = _scratch_bytes.get((index, dim))
     if need is None:
         with torch.cuda.device(index):
@@ -123,9 +130,12 @@ def _scratch(index, dim):
     key = ("paged", "cuda", index, torch._C._cuda_getCurrentRawStream(index))
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < need:
-        with _ws_lock:
-            buf = torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", index))
-            _workspaces[key] = buf
+        buf = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index))
+        with torch.cuda.device(index):
+            buf[:_COUNTER_BYTES].zero_()
+            if not torch.cuda.is_current_stream_capturing():
+                with _ws_lock:
+                    _workspaces[key] = buf
     return buf.data_ptr(), need
 
 

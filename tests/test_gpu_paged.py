@@ -244,6 +244,42 @@ def test_graph_replay_follows_new_lengths(ops):
         check_attention(out, None, want, want_lse, spread, BF16)
 
 
+def test_graphs_captured_without_a_first_call(ops):
+    """Two captures on a stream that has no workspace yet: what one of them clears must not be
+    needed by the other, nor by calls beside them."""
+    from m5kernels_b200.linear import _workspaces
+
+    batch = Batch([1, 1], [9000, 40], q_heads=8, kv_heads=1, dim=128, page=16, dtype=BF16)
+    want, want_lse, spread = attend_oracle(batch)
+    q = batch.q.to(DEV)
+    args = batch.on(DEV)
+    outs, graphs = [], []
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    kept = {k for k in _workspaces if k[0] == "paged"}
+    if any(k[-1] == side.cuda_stream for k in kept):
+        pytest.skip("the stream pool handed out a used stream")
+    for _ in range(2):
+        out = torch.empty_like(q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            ops.paged_attention(q, *args, max_query_len=1, out=out)
+        outs.append(out)
+        graphs.append(graph)
+    assert {k for k in _workspaces if k[0] == "paged"} == kept
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    check_attention(outs[1], None, want, want_lse, spread, BF16)
+    with torch.cuda.stream(side):
+        again = ops.paged_attention(q, *args, max_query_len=1)
+    side.synchronize()
+    check_attention(again, None, want, want_lse, spread, BF16)
+    graphs[0].replay()
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], again)
+
+
 def test_offsets_beyond_32_bits(ops):
     """Pages that start more than 2^31 elements into the cache."""
     page, dim = 256, 128
