@@ -434,7 +434,8 @@ M5B_API int m5b_paged_append(const m5b_paged_append_args* args, void* stream);
  * row that sees no key gets out = 0 and lse = -inf.  max_query_len is the
  * largest n_b and chooses the kernel; the result does not depend on it.
  * Slots behind a sequence's end may hold anything; keys and values of the
- * sequences themselves are finite.  The first M5B_PAGED_COUNTER_BYTES of the
+ * sequences themselves are finite.  A NaN among a row's own queries makes that
+ * row's out and lse NaN, and no other's.  The first M5B_PAGED_COUNTER_BYTES of the
  * workspace (m5b_paged_attention_workspace_bytes) must be zero before its first
  * use (cudaMemset once after allocating it); calls of any shape leave them
  * zero.  Calls that overlap on the GPU need separate workspaces.  After a

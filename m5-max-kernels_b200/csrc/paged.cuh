@@ -1,4 +1,5 @@
-// Arguments of the paged-cache kernels (paged_append.cu, paged_attention.cu)
+// Arguments of the paged-cache kernels (paged_append.cu, paged_rows.cu,
+// paged_decode.cu, paged_prompt.cu)
 // and the device helpers that they share: where a row stands, which keys it
 // sees, where a key lives.
 #pragma once

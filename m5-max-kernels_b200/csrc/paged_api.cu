@@ -1,6 +1,7 @@
 // C-ABI entry points of the paged key/value cache (declared in
 // include/m5b200.h): contract checks, kernel choice, launches.  Nothing here
 // allocates or synchronizes, and nothing throws.
+#include <cfloat>
 #include <cmath>
 #include <cstdio>
 
@@ -86,8 +87,7 @@ bool tiled(const PagedAttnArgs& a, int64_t dtype) {
 
 // Whether appending can go by 16-channel units: heads and their rotated part
 // are whole units, and all rows (8 table entries too) are on the 16-byte grid.
-//  9914 rows of 32 + 8 + 8 heads of 128: 127 us by
-// channel pairs.
+// 9914 rows of 32 + 8 + 8 heads of 128 take 47 us so, 127 by channel pairs.
 bool whole_units(const PagedAppendArgs& a) {
   const PagedBatch& b = a.b;
   if (b.head_dim % 16 || b.head_dim > 1024 || a.rope_half % 8) return false;
@@ -186,7 +186,8 @@ int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
   if (s->b.head_dim > 256) return eunsupported("head_dim above 256 is unsupported");
   if (!(s->scale > 0.0) || !std::isfinite(static_cast<float>(s->scale)))
     return einval("scale must be a positive finite real scalar");
-  if (!(s->softcap >= 0.0) || !std::isfinite(static_cast<float>(s->softcap)))
+  if (!(s->softcap >= 0.0) || !std::isfinite(static_cast<float>(s->softcap)) ||
+      (s->softcap > 0.0 && s->softcap < FLT_MIN))
     return einval("softcap must be a positive finite real scalar");
   if (s->window < 0) return einval("window must be positive");
   if (s->max_query_len < 0) return einval("max_query_len must not be negative");

@@ -366,14 +366,15 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::PER_SM)
         if (whole) {
           const int64_t tok = p.s.row0 + packed / group;
           const int h = p.head * group + packed % group;
-          const float inv = l[r] > 0.0f ? 1.0f / l[r] : 0.0f;
+          const bool none = l[r] == 0.0f;  // (NaN is something)
+          const float inv = none ? 0.0f : 1.0f / l[r];
           T* out = static_cast<T*>(a.out) + tok * a.o_token + h * a.o_head + t4 * 2;
 #pragma unroll
           for (int c = 0; c < D / 8; ++c)
             *reinterpret_cast<uint32_t*>(out + c * 8) =
                 pack2<T>(o[c][2 * r] * inv, o[c][2 * r + 1] * inv);
           if (a.lse && t4 == 0)
-            a.lse[tok * a.b.q_heads + h] = l[r] > 0.0f ? (m[r] + log2f(l[r])) * kLn2 : -INFINITY;
+            a.lse[tok * a.b.q_heads + h] = none ? -INFINITY : (m[r] + log2f(l[r])) * kLn2;
         } else {
           const int64_t at = slot * ROWS + g + r * 8;
 #pragma unroll

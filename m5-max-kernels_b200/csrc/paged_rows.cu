@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedAttn
     float top = x;
 #pragma unroll
     for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, s));
-    if (top == -INFINITY) continue;
+    if (__all_sync(~0u, x == -INFINITY)) continue;  // (a NaN score goes on into the sums)
     const float m2 = fmaxf(m, top), keep = expf(m - m2), p = expf(x - m2);
     m = m2;
     l = l * keep + p;  // of this lane's keys; summed over the lanes at the end
@@ -102,17 +102,17 @@ __global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedAttn
   for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w]);
   float share[kWarps];
   for (int w = 0; w < kWarps; ++w) {
-    share[w] = s_m[w] == -INFINITY ? 0.0f : expf(s_m[w] - top);
+    share[w] = s_l[w] == 0.0f ? 0.0f : expf(s_m[w] - top);
     sum += s_l[w] * share[w];
   }
   T* out = static_cast<T*>(a.out) + int64_t(t) * a.o_token + h * a.o_head;
   for (int i = threadIdx.x; i < d; i += kWarps * 32) {
     float y = 0.0f;
     for (int w = 0; w < kWarps; ++w) y += s_o[w][i] * share[w];
-    out[i] = from_f32<T>(sum > 0.0f ? y / sum : 0.0f);
+    out[i] = from_f32<T>(sum == 0.0f ? 0.0f : y / sum);
   }
   if (a.lse && threadIdx.x == 0)
-    a.lse[int64_t(t) * b.q_heads + h] = sum > 0.0f ? top + logf(sum) : -INFINITY;
+    a.lse[int64_t(t) * b.q_heads + h] = sum == 0.0f ? -INFINITY : top + logf(sum);
 }
 
 template <typename T>

@@ -106,13 +106,13 @@ struct PagedPiece {
   __device__ __forceinline__ bool whole() const { return begin == 0 && end == r.blocks; }
 };
 
-// The stretch of this CTA, piece by piece.  Every thread that walks it sees
-// the same pieces.
 // a / b, by the short division where that does (a long one is a call).
 __device__ __forceinline__ long long paged_div(long long a, long long b) {
   return ((a | b) >> 32) == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
 }
 
+// The stretch of this CTA, piece by piece.  Every thread that walks it sees
+// the same pieces.
 template <int ROWS, int BK>
 struct PagedWalk {
   int seq, head, rt, tiles, blk;
@@ -345,12 +345,13 @@ __device__ __forceinline__ void paged_join_rows(const PagedAttnArgs& a, const Pa
   for (int r = 0; r < R; ++r) {
     const int packed = first + row + r * STEP, h = head * a.b.group + packed % a.b.group;
     const int64_t t = row0 + packed / a.b.group;
-    const float inv = sum[r] > 0.0f ? 1.0f / sum[r] : 0.0f;
+    const bool none = sum[r] == 0.0f;  // (NaN is something)
+    const float inv = none ? 0.0f : 1.0f / sum[r];
     T* out = static_cast<T*>(a.out) + t * a.o_token + h * a.o_head + lane * V;
 #pragma unroll
     for (int v = 0; v < V; ++v) out[v] = from_f32<T>(o[r][v] * inv);
     if (a.lse && lane == 0)
-      a.lse[t * a.b.q_heads + h] = sum[r] > 0.0f ? (top[r] + log2f(sum[r])) * kLn2 : -INFINITY;
+      a.lse[t * a.b.q_heads + h] = none ? -INFINITY : (top[r] + log2f(sum[r])) * kLn2;
   }
 }
 
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(ROWS) paged_join_columns_kernel(const PagedAtt
   }
   const int packed = m.first + row, t = m.row0 + packed / a.b.group;
   const int h = m.head * a.b.group + packed % a.b.group;
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   __align__(16) T y[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) y[k] = from_f32<T>(o[k] * inv);
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(ROWS) paged_join_columns_kernel(const PagedAtt
   out[0] = *reinterpret_cast<const uint4*>(y);
   out[1] = *reinterpret_cast<const uint4*>(y + 8);
   if (a.lse && blockIdx.y == 0)
-    a.lse[int64_t(t) * a.b.q_heads + h] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+    a.lse[int64_t(t) * a.b.q_heads + h] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 // Rows outside every sequence leave as zeros; `id` of `count` threads.

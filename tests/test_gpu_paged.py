@@ -280,6 +280,19 @@ def test_graphs_captured_without_a_first_call(ops):
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], again)
 
 
+@pytest.mark.parametrize("dtype,hint", [(BF16, 1), (BF16, 64), (torch.float32, 1)])
+@pytest.mark.parametrize("lens", [[40, 9000, 200], [7, 64, 3]])
+def test_a_nan_query_stays_in_its_row(ops, dtype, hint, lens):
+    """Its own output and lse are NaN, every other row's are as without it."""
+    batch = Batch([1, 1, 2], lens, q_heads=8, kv_heads=2, dim=64, page=16, dtype=dtype)
+    out, lse = attend(ops, batch, hint=hint)
+    batch.q[1, 5, 3] = math.nan
+    got, got_lse = attend(ops, batch, hint=hint)
+    assert got[1, 5].isnan().all() and got_lse[1, 5].isnan()
+    got[1, 5], got_lse[1, 5] = out[1, 5], lse[1, 5]
+    assert torch.equal(got, out) and torch.equal(got_lse, lse)
+
+
 def test_offsets_beyond_32_bits(ops):
     """Pages that start more than 2^31 elements into the cache."""
     page, dim = 256, 128
