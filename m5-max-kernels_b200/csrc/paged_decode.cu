@@ -10,12 +10,11 @@
 //   t = x log2 e,  p = 2^(t - m),  l += sum p,  o += p V,
 // fp32 but for p, which is rounded to the cache's type for the product (its
 // relative error enters the output once, at the size of the output's own
-// rounding).  m only follows the row's maximum when that has grown by more
-// than 2^8, so that o is rarely rescaled; p stays below 2^8.  At a tile's end
-// the warps' parts are added through shared memory.  paged_sched.cuh deals
-// the blocks out evenly whatever the lengths are; the parts of a split tile
-// are joined by whichever CTA finishes its part last (a ticket per tile tells),
-// always in the same order.
+// rounding).  m is near the row's maximum (kGrow).  At a tile's end the warps'
+// parts are added through shared memory.  paged_sched.cuh deals the blocks out
+// evenly whatever the lengths are; the parts of a split tile are joined by
+// whichever CTA finishes its part last (a ticket per tile tells), always in the
+// same order.
 //
 // 64 sequences of up to 8191 keys, 32 + 8 heads of 128: 183 us, 5.7 TB/s; all
 // of 8000 and more 6.5 TB/s, the rate of a copy.  What short calls pay is the
@@ -26,7 +25,6 @@ namespace m5b {
 namespace {
 
 constexpr int kBlock = kPagedBlock;  // keys per ring stage
-constexpr float kGrow = 8.0f;  // log2 of the growth that m may lag behind
 
 template <int D> struct Cfg {
   static constexpr int ROWS = kDecodeRows;
@@ -270,11 +268,12 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::PER_SM)
         top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], 1));
         top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], 2));
       }
-      if (__any_sync(~0u, top[0] > m[0] + kGrow || top[1] > m[1] + kGrow)) {
+      constexpr float below = kBelow<T>, lag = kGrow + below;
+      if (__any_sync(~0u, top[0] > m[0] + lag || top[1] > m[1] + lag)) {
         float f[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float m2 = fmaxf(m[r], top[r]);
+          const float m2 = fmaxf(m[r], top[r] - below);
           f[r] = m[r] == -INFINITY ? 0.0f : ex2(m[r] - m2);
           m[r] = m2;
           l[r] *= f[r];

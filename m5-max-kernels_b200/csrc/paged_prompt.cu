@@ -21,8 +21,8 @@
 // is there.  (Measured and not kept: two S buffers with P over them, whose
 // reuse chains softmax, PV and QK, 1830 cycles; one S buffer of 128 keys, which
 // needs fewer bytes of shared memory a flop but chains them all the more, 4250
-// for 128 keys.)  m only follows the row's maximum when that has grown by more
-// than 2^8; then O is rescaled in place.  (Taking the exponentials with the
+// for 128 keys.)  m is near the row's maximum (kGrow); where it changes, O is
+// rescaled in place.  (Taking the exponentials with the
 // old m first, and again in the rare case: 2200 cycles.)  P is rounded to the
 // cache's type for the product, once, at the size of the output's own rounding;
 // sums, m and O are fp32.
@@ -40,7 +40,6 @@ namespace {
 
 constexpr int kBlock = kPagedBlock;  // keys per step
 constexpr int kRows = 256;           // packed rows per tile, two halves
-constexpr float kGrow = 8.0f;        // log2 of the growth that m may lag behind
 // Of 8 pairs of exponentials, those by ex2_fma: 1730 cycles a step (1800 with
 // none, 1760 with 2, 1790 with 4).  None where the scores are modified, whose
 // arithmetic keeps the FMA pipes busy (162 us, 187 with 3, in the distance bias
@@ -583,9 +582,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           top[q] = fmaxf(top[q], __uint_as_float(x[15]));
         }
         const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-        const bool grow = high > m + kGrow;  // (m = -inf: any key)
+        const bool grow = high > m + (kGrow + kBelow<T>);  // (m = -inf: any key)
         const bool any = __any_sync(~0u, grow);
-        const float m2 = grow ? high : m, f = m == -INFINITY ? 0.0f : ex2(m - m2);
+        const float m2 = grow ? high - kBelow<T> : m, f = m == -INFINITY ? 0.0f : ex2(m - m2);
         m = m2;
         uint32_t pk[32];
         const float base = m == -INFINITY ? 0.0f : -m;

@@ -21,6 +21,14 @@ namespace m5b {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// The reference m of a row's probabilities 2^(t - m) follows the row's maximum
+// when that has grown by more than 2^kGrow, so that sums are rarely rescaled.
+// For fp16 it stays 2^7 below the maximum, which uses the type's range: they
+// reach 2^15, and those of the many faint keys of a long cache keep their bits
+// down to 2^-21 of the largest (and vanish below 2^-32, not 2^-25).
+constexpr float kGrow = 8.0f;
+template <typename T> constexpr float kBelow = DTypeOf<T>::value == DT_F16 ? 7.0f : 0.0f;
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -293,6 +293,27 @@ def test_a_nan_query_stays_in_its_row(ops, dtype, hint, lens):
     assert torch.equal(got, out) and torch.equal(got_lse, lse)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hint,cap", [(1, None), (64, None), (64, 900.0)])
+@pytest.mark.parametrize("faint", [18.6, 20.7])
+def test_many_faint_keys_beside_a_strong_one(ops, dtype, hint, cap, faint):
+    """Probabilities of 2^-faint of the largest, normal fp16 numbers only if scaled (to 2^-21): the
+    strong key's values are zero, so the output is what the faint ones add up to."""
+    batch = Batch([1] * 16, [1500] * 16, q_heads=8, kv_heads=8, dim=64, page=64, dtype=dtype)
+    batch.q.zero_()
+    batch.q[:, :, 0] = 8.0
+    batch.k_cache[~batch.k_cache.isnan()] = 0.0
+    batch.v_cache.abs_().add_(0.5)
+    for b in range(16):
+        batch.k[b].zero_()
+        batch.v[b].abs_().add_(0.5)
+        first = int(batch.table[b, 0])
+        batch.k[b][0, :, 0] = faint * math.log(2.0)
+        batch.v[b][0] = 0.0
+        batch.k_cache[first, :, 0], batch.v_cache[first, :, 0] = batch.k[b][0], batch.v[b][0]
+    compare(ops, batch, hint=hint, softcap=cap)
+
+
 def test_offsets_beyond_32_bits(ops):
     """Pages that start more than 2^31 elements into the cache."""
     page, dim = 256, 128
