@@ -433,8 +433,9 @@ M5B_API int m5b_paged_append(const m5b_paged_append_args* args, void* stream);
  * (optional, fp32 [tokens, q_heads]) = ln of the sum of exponentials of x.  A
  * row that sees no key gets out = 0 and lse = -inf.  max_query_len is the
  * largest n_b and chooses the kernel; the result does not depend on it.
- * Slots behind a sequence's end may hold anything; keys and values of the
- * sequences themselves are finite.  A NaN among a row's own queries makes that
+ * Slots behind a sequence's end may hold anything, and so may pages wholly
+ * between its prefix and the windows of all its new rows (given to others by
+ * now, say); its other keys and values are finite.  A NaN among a row's own queries makes that
  * row's out and lse NaN, and no other's.  The first M5B_PAGED_COUNTER_BYTES of the
  * workspace (m5b_paged_attention_workspace_bytes) must be zero before its first
  * use (cudaMemset once after allocating it); calls of any shape leave them

@@ -137,10 +137,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::PER_SM)
     int issued = 0;
     bool ok = true;
     while (ok && walk.next(a, p)) {
+      const int window = paged_window<ROWS>(a, p.s, p.rt);
       for (int i = p.begin; i < p.end; ++i) {
         const int key = p.r.at(i) * kBlock + row;
         int page = a.b.num_pages, slot = 0;  // out of range: zeros
-        if (lane < boxes && key < p.s.keys) {
+        if (lane < boxes && key < p.s.keys && (key < p.s.prefix || key + maps.box_rows > window)) {
           const int at = paged_page(a.b, p.seq, key);
           if (at >= 0) page = at;
           slot = key % a.b.page_size;

@@ -334,10 +334,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       PagedPiece p;
       while (ok && walk.next(a, p)) {
+        const int window = paged_window<kRows>(a, p.s, p.rt);
         for (int i = p.begin; ok && i < p.end; ++i) {
           const int block0 = p.r.at(i) * kBlock, key = block0 + row;
           int page = a.b.num_pages, slot = 0;  // out of range: zeros
-          if (lane < boxes && key < p.s.keys) {
+          if (lane < boxes && key < p.s.keys &&
+              (key < p.s.prefix || key + maps.box_rows > window)) {
             const int at = paged_page(a.b, p.seq, key);
             if (at >= 0) page = at;
             slot = key % a.b.page_size;

@@ -222,7 +222,9 @@ def paged_attention(q, k_cache, v_cache, page_table, query_start, seq_lens, *, m
     softcap * tanh(x / softcap), minus slopes[h] * |pos - j| (slopes: fp32
     [q_heads]).  A token at pos sees the keys j <= pos of its sequence, of
     those the last `window` only, and the first prefix_lens[b] (int32 [B]) keys
-    in any case.  A token that sees no key returns zeros.  max_query_len: the
+    in any case.  A token that sees no key returns zeros.  Slots behind a
+    sequence's end, and pages that neither a prefix nor a new token's window
+    reaches, may hold anything.  max_query_len: the
     most new tokens of any sequence; it selects the kernel, not the result.
     With return_lse also the fp32 [T, q_heads] natural logarithm of the sum of
     exp(x), -inf for a token that sees no key.  `out` may be given, any

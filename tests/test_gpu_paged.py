@@ -314,6 +314,24 @@ def test_many_faint_keys_beside_a_strong_one(ops, dtype, hint, cap, faint):
     compare(ops, batch, hint=hint, softcap=cap)
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16), (128, BF16), (64, torch.float32)])
+@pytest.mark.parametrize("page", [8, 16, 32, 128])
+@pytest.mark.parametrize("prefix", [None, [10, 0, 130]])
+@pytest.mark.parametrize("new,hint", [([1, 1, 1], 1), ([3, 1, 2], 3), ([1, 70, 300], 300)])
+def test_pages_before_every_window_may_hold_anything(ops, dim, dtype, page, prefix, new, hint):
+    """Pages that neither a prefix nor a new row's window reaches (others may own them by now)."""
+    window = 100
+    batch = Batch(new, [500, 259, 331], q_heads=8, kv_heads=2, dim=dim, page=page, dtype=dtype)
+    for b, n in enumerate(new):
+        first = -(-prefix[b] // page) if prefix else 0
+        for i in range(first, (batch.seq[b] - n - window + 1) // page):
+            batch.k_cache[batch.table[b, i]] = math.nan
+            batch.v_cache[batch.table[b, i]] = math.inf if i % 2 else math.nan
+            if i % 3 == 0:
+                batch.table[b, i] = -7
+    compare(ops, batch, hint=hint, window=window, prefix=prefix)
+
+
 def test_offsets_beyond_32_bits(ops):
     """Pages that start more than 2^31 elements into the cache."""
     page, dim = 256, 128
