@@ -75,6 +75,11 @@ M5B_API const char* m5b_last_error(void);
  * device.  If clear != 0 the word is reset to zero afterwards. */
 M5B_API int m5b_device_status(unsigned int* status_out, int clear);
 
+/* Number of the CUDA graph capture that `stream` is part of (unique in the
+ * process), 0 when it is not being captured.  For callers that keep workspaces:
+ * a captured call's workspace has to live as long as its graph. */
+M5B_API int m5b_stream_capture_id(void* stream, unsigned long long* id_out);
+
 /* Per-token symmetric quantization of x[rows, k] (bf16 / fp16 / fp32).
  * mode INT8: q int8, scale = amax/127, q = clip(rint(x/scale), +-127).
  * mode FP8 : q = E4M3 bits (RNE, saturating), scale = amax/448.

@@ -267,6 +267,16 @@ int m5b_device_status(unsigned int* status_out, int clear) {
   return ok();
 }
 
+int m5b_stream_capture_id(void* stream, unsigned long long* id_out) {
+  if (!id_out) return fail(M5B_EINVAL, "id_out is NULL");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamGetCaptureInfo");
+  *id_out = status == cudaStreamCaptureStatusNone ? 0 : id;
+  return ok();
+}
+
 int m5b_quantize(const void* x, int x_dtype, int64_t rows, int64_t k, int mode, void* q,
                  float* scales, void* stream) {
   RowPrepArgs a;

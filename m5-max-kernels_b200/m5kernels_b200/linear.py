@@ -11,6 +11,7 @@ bound to fixed buffers, for loops and CUDA-graph capture.
 
 from __future__ import annotations
 
+import ctypes
 import threading
 
 import torch
@@ -19,11 +20,54 @@ from . import _lib
 from ._lib import check, ptr
 
 _ws_lock = threading.Lock()
-_workspaces: dict = {}
+_workspaces: dict = {}  # (tag, device type, index, stream) -> buffer of that stream's calls
+_captured: dict = {}  # the same key -> (capture, buffer) of the capture that is in progress
 
 
 def _key(device: torch.device, tag: str):
     return (tag, device.type, device.index, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _capture_id(stream: int) -> int:
+    """The graph capture that the raw stream is part of; 0: none."""
+    value = ctypes.c_ulonglong(0)
+    check(_lib.lib().m5b_stream_capture_id(stream, ctypes.byref(value)))
+    return value.value
+
+
+def stream_buffer(tag: str, index: int, nbytes: int, make) -> torch.Tensor:
+    """Workspace of at least nbytes for a call on device `index` and its current stream.
+
+    One is kept for each stream and grown on demand.  A call that a CUDA graph
+    captures never gets that one: the graph keeps the address while the stream's
+    buffer may be replaced and its memory handed on, and it may be replayed
+    beside the stream's own calls.  It gets one from the graph's memory, which
+    the calls captured on the stream share; `make(nbytes)` runs in the capture,
+    so that what it clears is cleared at every replay.  Hold the tensor until
+    the call has been launched: another thread may replace it.
+    """
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return stream_buffer(tag, index, nbytes, make)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    key = (tag, "cuda", index, stream)
+    if torch.cuda.is_current_stream_capturing():
+        capture = _capture_id(stream)
+        with _ws_lock:
+            held = _captured.get(key)
+            if held is None or held[0] != capture or held[1].numel() < nbytes:
+                held = _captured[key] = (capture, make(nbytes))
+            return held[1]
+    buf = _workspaces.get(key)
+    if buf is None or buf.numel() < nbytes or _captured:
+        with _ws_lock:
+            # (captures that are over need not be held; one still in progress
+            # elsewhere makes another)
+            _captured.clear()
+            buf = _workspaces.get(key)
+            if buf is None or buf.numel() < nbytes:
+                buf = _workspaces[key] = make(nbytes)
+    return buf
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:

@@ -29,7 +29,7 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .linear import _workspaces, _ws_lock
+from .linear import stream_buffer
 
 _CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 # m5b_paged_batch, m5b_paged_append_args and m5b_paged_attention_args (include/m5b200.h):
@@ -113,30 +113,22 @@ _COUNTER_BYTES = 4096  # M5B_PAGED_COUNTER_BYTES
 
 
 def _scratch(index, dim):
-    """(pointer, bytes) of the attention kernels' workspace, its counters zero.
-
-    One is kept for each device and stream.  A stream that has none when a
-    graph is captured on it gives the captured call its own, from the graph's
-    memory and with a memset in the graph: nothing outside the graph may rely
-    on a memset that runs when it is replayed.
-    """
+    """(pointer, bytes, tensor) of the attention kernels' workspace, its counters zero."""
     need = _scratch_bytes.get((index, dim))
     if need is None:
         with torch.cuda.device(index):
             need = int(_lib.lib().m5b_paged_attention_workspace_bytes(dim))
         _scratch_bytes[index, dim] = need
     if need <= 0:
-        return 0, 0
-    key = ("paged", "cuda", index, torch._C._cuda_getCurrentRawStream(index))
-    buf = _workspaces.get(key)
-    if buf is None or buf.numel() < need:
-        buf = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", index))
-        with torch.cuda.device(index):
-            buf[:_COUNTER_BYTES].zero_()
-            if not torch.cuda.is_current_stream_capturing():
-                with _ws_lock:
-                    _workspaces[key] = buf
-    return buf.data_ptr(), need
+        return 0, 0, None
+
+    def make(nbytes):
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        buf[:_COUNTER_BYTES].zero_()
+        return buf
+
+    buf = stream_buffer("paged", index, need, make)
+    return buf.data_ptr(), need, buf
 
 
 def paged_append(k, v, k_cache, v_cache, page_table, query_start, seq_lens, *, cos=None, sin=None,
@@ -279,7 +271,8 @@ def paged_attention(q, k_cache, v_cache, page_table, query_start, seq_lens, *, m
         lse_ptr = lse.data_ptr()
     if tokens > 0:
         ot, oh, _ = out.stride()
+        ws_ptr, ws_bytes, _held = _scratch(index, dim)
         _call(_lib.lib().m5b_paged_attention, _PACK_ATTEND.pack(
             *fields, q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, lse_ptr, max_query_len, scale,
-            softcap, slopes_ptr, window, prefix_ptr, *_scratch(index, dim)), index)
+            softcap, slopes_ptr, window, prefix_ptr, ws_ptr, ws_bytes), index)
     return (out, lse) if return_lse else out
