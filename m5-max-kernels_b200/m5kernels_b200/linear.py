@@ -4,7 +4,7 @@ The reference composes its online stage from two operators
 (src/m5kernels/engine.py:180-182: quantize then gemm; hadamard_gemm.py:65-69
 with a rotation first).  `linear` does the same through one C-ABI call
 (m5b_linear_ex), with the per-token codes and scales in a device workspace
-that is allocated once per device and stream and grown on demand, and the
+that is kept for each device and stream and grown on demand, and the
 GEMM's split-K workspace beside it.  `OnlineProjection` is the same step
 bound to fixed buffers, for loops and CUDA-graph capture.
 """
@@ -22,10 +22,6 @@ from ._lib import check, ptr
 _ws_lock = threading.Lock()
 _workspaces: dict = {}  # (tag, device type, index, stream) -> buffer of that stream's calls
 _captured: dict = {}  # the same key -> (capture, buffer) of the capture that is in progress
-
-
-def _key(device: torch.device, tag: str):
-    return (tag, device.type, device.index, torch.cuda.current_stream(device).cuda_stream)
 
 
 def _capture_id(stream: int) -> int:
@@ -71,43 +67,28 @@ def stream_buffer(tag: str, index: int, nbytes: int, make) -> torch.Tensor:
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Cached uint8 device buffer of at least nbytes for the codes and scales
-    (256-byte aligned by torch), one per device and stream."""
-    key = _key(device, "codes")
-    with _ws_lock:
-        buf = _workspaces.get(key)
-        if buf is None or buf.numel() < nbytes:
-            buf = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
-            _workspaces[key] = buf
-        return buf
+    """Uint8 device buffer of at least nbytes for the codes and scales
+    (256-byte aligned by torch; `stream_buffer`)."""
+    return stream_buffer("codes", device.index, max(nbytes, 1),
+                         lambda n: torch.empty(n, dtype=torch.uint8, device=device))
 
 
 def gemm_workspace(device: torch.device, nbytes: int):
-    """Cached zero-filled split-K workspace of the GEMM (m5b_gemm_ex), one per
-    device and stream, or None when nbytes is 0.  It is zeroed once when
-    allocated; every GEMM call leaves it zeroed again."""
+    """Zero-filled split-K workspace of the GEMM (m5b_gemm_ex; `stream_buffer`),
+    or None when nbytes is 0.  It is zeroed once when allocated; every GEMM
+    call leaves it zeroed again."""
     if nbytes <= 0:
         return None
-    key = _key(device, "gemm")
-    with _ws_lock:
-        buf = _workspaces.get(key)
-        if buf is None or buf.numel() < nbytes:
-            buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-            _workspaces[key] = buf
-        return buf
+    return stream_buffer("gemm", device.index, nbytes,
+                         lambda n: torch.zeros(n, dtype=torch.uint8, device=device))
 
 
 def fp32_workspace(device: torch.device, nbytes: int):
-    """Cached scratch of the FP32 GEMM mode (its split operands), one per device
-    and stream.  Kept apart from the split-K workspace, which must stay zeroed
-    between calls; this one is overwritten by every FP32 GEMM."""
-    key = _key(device, "fp32")
-    with _ws_lock:
-        buf = _workspaces.get(key)
-        if buf is None or buf.numel() < nbytes:
-            buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-            _workspaces[key] = buf
-        return buf
+    """Scratch of the FP32 GEMM mode (its split operands; `stream_buffer`).
+    Kept apart from the split-K workspace, which must stay zeroed between
+    calls; this one is overwritten by every FP32 GEMM."""
+    return stream_buffer("fp32", device.index, nbytes,
+                         lambda n: torch.empty(n, dtype=torch.uint8, device=device))
 
 
 def linear(x, wq, w_scales, mode="int8", *, block_size=0, signs=None,

@@ -80,6 +80,23 @@ def test_a_captured_attention_call_has_its_graphs_workspace(cuda):
     assert _scratch(0, 64)[0] == eager[0]
 
 
+@pytest.mark.parametrize("name", ["workspace", "gemm_workspace", "fp32_workspace"])
+def test_a_captured_product_has_its_graphs_workspaces(cuda, name):
+    """Also without a first call: what a capture clears is not clear for calls beside the graph."""
+    get = getattr(importlib.import_module("m5kernels_b200.linear"), name)
+    dev = torch.device("cuda", 0)
+    cuda.capture = 7
+    owners = [owner(cuda, get(dev, 1000).data_ptr())]
+    cuda.capture = 0
+    first = get(dev, 1000)
+    owners.append(owner(cuda, first.data_ptr()))
+    cuda.capture = 8
+    owners.append(owner(cuda, get(dev, 900).data_ptr()))
+    assert [o[0] for o in owners] == [7, 0, 8]
+    cuda.capture = 0
+    assert get(dev, 1000) is first and get(dev, 2000) is not first
+
+
 def test_a_workspace_lives_until_its_call_is_launched(cuda):
     """Another thread may replace the stream's buffer in between."""
     from m5kernels_b200.paged import _scratch
