@@ -135,8 +135,18 @@ def stream_handle(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+after_timeout: list = []  # called with the device whose status word is nonzero
+
+
 def device_status(clear: bool = False) -> int:
-    """Device status word (bounded-wait failures); synchronizes the device."""
+    """Device status word (bounded-wait failures); synchronizes the device.
+
+    After a failure the workspaces that the package keeps are made anew, since
+    their counters may have been left anywhere.
+    """
     value = ctypes.c_uint(0)
     check(lib().m5b_device_status(ctypes.byref(value), 1 if clear else 0))
+    if value.value:
+        for renew in after_timeout:
+            renew(torch._C._cuda_getDevice())
     return int(value.value)

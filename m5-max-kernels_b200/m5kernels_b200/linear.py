@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+import weakref
 
 import torch
 
@@ -64,6 +65,24 @@ def stream_buffer(tag: str, index: int, nbytes: int, make) -> torch.Tensor:
             if buf is None or buf.numel() < nbytes:
                 buf = _workspaces[key] = make(nbytes)
     return buf
+
+
+_bound: weakref.WeakSet = weakref.WeakSet()  # objects with a `gemm_ws` of their own
+
+
+def _renew_counters(index: int) -> None:
+    """After a wait on device `index` gave up (and the device was waited for): workspaces with
+    counters that calls expect to be zero.  A graph clears its own when it is replayed."""
+    with _ws_lock:
+        for buffers in (_workspaces, _captured):
+            for key in [k for k in buffers if k[0] in ("gemm", "paged") and k[2] == index]:
+                del buffers[key]
+    for step in list(_bound):
+        if step.gemm_ws is not None and step.device.index == index:
+            step.gemm_ws.zero_()
+
+
+_lib.after_timeout.append(_renew_counters)
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
@@ -174,6 +193,7 @@ class OnlineProjection:
         self._lib = _lib.lib()
         need = int(self._lib.m5b_gemm_workspace_bytes(m, n, k, _lib.MODE[mode]))
         self.gemm_ws = torch.zeros(need, dtype=torch.uint8, device=self.device) if need else None
+        _bound.add(self)
         xd, md = _lib.DTYPE_CODE[x.dtype], _lib.MODE[mode]
         if block_size:
             self._qfn = self._lib.m5b_hadamard_quantize

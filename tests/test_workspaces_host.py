@@ -117,6 +117,43 @@ def test_workspaces_of_finished_captures_are_let_go(cuda):
     assert cuda.made[0][1]() is None
 
 
+def test_counters_are_renewed_after_a_timeout(cuda, monkeypatch):
+    """A wait that gave up may leave counters that later calls expect to be zero."""
+    from m5kernels_b200 import _lib
+    from m5kernels_b200.paged import _scratch
+
+    linear = importlib.import_module("m5kernels_b200.linear")
+    status = types.SimpleNamespace(value=0, cleared=0)
+
+    class Lib(type(_lib.lib())):
+        def m5b_device_status(self, out, clear):
+            out._obj.value = status.value
+            status.cleared += clear
+            return 0
+
+    monkeypatch.setattr(_lib, "lib", lambda: Lib())
+
+    class Step:
+        gemm_ws, device = torch.ones(4, dtype=torch.uint8), torch.device("cuda", 0)
+
+    class Elsewhere(Step):
+        gemm_ws, device = torch.ones(4, dtype=torch.uint8), torch.device("cuda", 1)
+
+    bound = [Step(), Elsewhere()]
+    monkeypatch.setattr(linear, "_bound", set(bound), raising=False)
+    dev = torch.device("cuda", 0)
+    get = lambda: (linear.gemm_workspace(dev, 100), _scratch(0, 64)[-1], linear.workspace(dev, 100))
+    before = get()
+    assert _lib.device_status() == 0
+    assert all(a is b for a, b in zip(get(), before)) and bound[0].gemm_ws.all()
+    status.value = 2
+    assert _lib.device_status(clear=True) == 2 and status.cleared == 1
+    after = get()
+    assert after[0] is not before[0] and after[1] is not before[1] and after[2] is before[2]
+    assert not after[0].any() and not after[1][:4096].any()
+    assert not bound[0].gemm_ws.any() and bound[1].gemm_ws.all()
+
+
 def test_streams_have_their_own(cuda):
     from m5kernels_b200.paged import _scratch
 
