@@ -126,6 +126,12 @@ template <int N> __device__ __forceinline__ void regs_dec() {
 __device__ __forceinline__ void cp_async_wait_all() {
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
 // 2^x of a pair on the FMA pipes, for x < 100: x = n + f with n the nearest
 // integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a polynomial,
 // n added to its exponent.  The coefficients are the minimax fit of the
@@ -580,13 +586,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           top[q] = __uint_as_float(x[0]);
 #pragma unroll
           for (int e = 1; e < 15; e += 2)
-            top[q] = fmaxf(top[q], fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
-          top[q] = fmaxf(top[q], __uint_as_float(x[15]));
+            top[q] = max_nan(top[q], max_nan(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+          top[q] = max_nan(top[q], __uint_as_float(x[15]));
         }
-        const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-        const bool grow = high > m + (kGrow + kBelow<T>);  // (m = -inf: any key)
+        // A row with a NaN or +inf among its scores gets m = NaN, which stays
+        // and makes l and O NaN: ex2_fma would lose a single NaN score.
+        const float high = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3])) * c;
+        const bool grow = !(high <= m + (kGrow + kBelow<T>)) && m == m;  // (m = -inf: any key)
         const bool any = __any_sync(~0u, grow);
-        const float m2 = grow ? high - kBelow<T> : m, f = m == -INFINITY ? 0.0f : ex2(m - m2);
+        const float m2 = !grow ? m : high < INFINITY ? high - kBelow<T> : NAN;
+        const float f = m == -INFINITY ? 0.0f : ex2(m - m2);
         m = m2;
         uint32_t pk[32];
         const float base = m == -INFINITY ? 0.0f : -m;
@@ -652,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (d.whole) {
         // by way of the rows' buffer, which is done with: a thread has a row,
         // a row's stores shall be whole lines
-        const float inv = m > -INFINITY ? 1.0f / l : 0.0f;
+        const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
         uint8_t* const stage = q_smem + (qb * 2 + h) * C::Q_BYTES;
 #pragma unroll
         for (int q = 0; q < D / 32; ++q) {

@@ -73,3 +73,51 @@ def test_graphs_replayed_beside_each_other(ops):
             got = ops.paged_attention(q, *args, max_query_len=1)
     torch.cuda.synchronize()
     assert torch.equal(got, want) and all(torch.equal(out, want) for out in outs)
+
+
+# ---------------------------------------------------------------- NaN and infinities
+
+KINDS = [(64, BF16, 64), (128, F16, 64), (128, BF16, 1), (64, F32, 1)]  # prompt, decode, row kernel
+
+
+def attend(ops, batch, hint, **kw):
+    return ops.paged_attention(batch.q.to(DEV), *batch.on(DEV), max_query_len=hint, return_lse=True,
+                               **kw)
+
+
+def check_nan_rows(got, clean, rows, heads):
+    """The named rows and heads are NaN, all others as they were."""
+    for x, y in zip(got, clean):
+        assert x[rows][:, heads].isnan().all()
+        x[rows, heads] = y[rows, heads]
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dim,dtype,hint", KINDS)
+@pytest.mark.parametrize("window", [None, 3])
+def test_a_nan_query_at_any_position(ops, dim, dtype, hint, window):
+    """Whichever keys the row sees, however few: its out and lse are NaN, no other's."""
+    batch = Batch([21, 2], [0, 40], q_heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype)
+    clean = attend(ops, batch, hint, window=window)
+    for at in range(21):
+        batch.q[at, 1, 5], kept = float("nan"), batch.q[at, 1, 5].clone()
+        check_nan_rows(attend(ops, batch, hint, window=window), clean, slice(at, at + 1), slice(1, 2))
+        batch.q[at, 1, 5] = kept
+
+
+@pytest.mark.parametrize("dim,dtype,hint", KINDS)
+@pytest.mark.parametrize("value", ["nan", "overflow"])
+def test_a_nan_or_infinite_score_reaches_its_rows(ops, dim, dtype, hint, value):
+    """A key at each slot of a block, NaN or so large that the score overflows to +inf: the rows
+    that see it are NaN, as the softmax of such scores is."""
+    if value == "overflow" and dtype is F16:
+        pytest.skip("fp16 products do not overflow fp32")
+    batch = Batch([70, 2], [0, 40], q_heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype)
+    batch.q[:, :, 0] = 1.0 if value == "nan" else 1e30
+    batch.k_cache[..., 0] = 0.0
+    clean = attend(ops, batch, hint)
+    for slot in range(64):
+        home = int(batch.table[0, slot // 16]), 1, slot % 16, 0
+        batch.k_cache[home] = float("nan") if value == "nan" else 1e30
+        check_nan_rows(attend(ops, batch, hint), clean, slice(slot, 70), slice(2, 4))
+        batch.k_cache[home] = 0.0
