@@ -32,39 +32,50 @@ def _capture_id(stream: int) -> int:
     return value.value
 
 
-def stream_buffer(tag: str, index: int, nbytes: int, make) -> torch.Tensor:
-    """Workspace of at least nbytes for a call on device `index` and its current stream.
+def stream_buffer(tag: str, index: int, stream: int, nbytes: int, make) -> torch.Tensor:
+    """Workspace of at least nbytes for a call on the current device `index` and its current stream.
 
     One is kept for each stream and grown on demand.  A call that a CUDA graph
     captures never gets that one: the graph keeps the address while the stream's
     buffer may be replaced and its memory handed on, and it may be replayed
     beside the stream's own calls.  It gets one from the graph's memory, which
-    the calls captured on the stream share; `make(nbytes)` runs in the capture,
+    the calls captured on the stream share; `make(nbytes, index)` runs in the capture,
     so that what it clears is cleared at every replay.  Hold the tensor until
     the call has been launched: another thread may replace it.
     """
-    if index != torch._C._cuda_getDevice():
-        with torch.cuda.device(index):
-            return stream_buffer(tag, index, nbytes, make)
-    stream = torch._C._cuda_getCurrentRawStream(index)
     key = (tag, "cuda", index, stream)
-    if torch.cuda.is_current_stream_capturing():
-        capture = _capture_id(stream)
-        with _ws_lock:
-            held = _captured.get(key)
-            if held is None or held[0] != capture or held[1].numel() < nbytes:
-                held = _captured[key] = (capture, make(nbytes))
-            return held[1]
-    buf = _workspaces.get(key)
-    if buf is None or buf.numel() < nbytes or _captured:
+    if not torch._C._cuda_isCurrentStreamCapturing():
+        buf = _workspaces.get(key)
+        if buf is not None and buf.numel() >= nbytes and not _captured:
+            return buf
         with _ws_lock:
             # (captures that are over need not be held; one still in progress
             # elsewhere makes another)
             _captured.clear()
             buf = _workspaces.get(key)
             if buf is None or buf.numel() < nbytes:
-                buf = _workspaces[key] = make(nbytes)
-    return buf
+                buf = _workspaces[key] = make(nbytes, index)
+            return buf
+    capture = _capture_id(stream)
+    with _ws_lock:
+        held = _captured.get(key)
+        if held is None or held[0] != capture or held[1].numel() < nbytes:
+            held = _captured[key] = (capture, make(nbytes, index))
+        return held[1]
+
+
+def _buffer(tag: str, device: torch.device, nbytes: int, make) -> torch.Tensor:
+    with torch.cuda.device(device.index):
+        stream = torch._C._cuda_getCurrentRawStream(device.index)
+        return stream_buffer(tag, device.index, stream, nbytes, make)
+
+
+def _bytes(nbytes: int, index: int) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+
+
+def _zeros(nbytes: int, index: int) -> torch.Tensor:
+    return torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
 
 
 _bound: weakref.WeakSet = weakref.WeakSet()  # objects with a `gemm_ws` of their own
@@ -88,8 +99,7 @@ _lib.after_timeout.append(_renew_counters)
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Uint8 device buffer of at least nbytes for the codes and scales
     (256-byte aligned by torch; `stream_buffer`)."""
-    return stream_buffer("codes", device.index, max(nbytes, 1),
-                         lambda n: torch.empty(n, dtype=torch.uint8, device=device))
+    return _buffer("codes", device, max(nbytes, 1), _bytes)
 
 
 def gemm_workspace(device: torch.device, nbytes: int):
@@ -98,16 +108,14 @@ def gemm_workspace(device: torch.device, nbytes: int):
     call leaves it zeroed again."""
     if nbytes <= 0:
         return None
-    return stream_buffer("gemm", device.index, nbytes,
-                         lambda n: torch.zeros(n, dtype=torch.uint8, device=device))
+    return _buffer("gemm", device, nbytes, _zeros)
 
 
 def fp32_workspace(device: torch.device, nbytes: int):
     """Scratch of the FP32 GEMM mode (its split operands; `stream_buffer`).
     Kept apart from the split-K workspace, which must stay zeroed between
     calls; this one is overwritten by every FP32 GEMM."""
-    return stream_buffer("fp32", device.index, nbytes,
-                         lambda n: torch.empty(n, dtype=torch.uint8, device=device))
+    return _buffer("fp32", device, nbytes, _bytes)
 
 
 def linear(x, wq, w_scales, mode="int8", *, block_size=0, signs=None,

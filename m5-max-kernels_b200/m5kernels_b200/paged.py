@@ -112,23 +112,31 @@ _scratch_bytes: dict = {}
 _COUNTER_BYTES = 4096  # M5B_PAGED_COUNTER_BYTES
 
 
+def _counted(nbytes, index):
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+    buf[:_COUNTER_BYTES].zero_()
+    return buf
+
+
 def _scratch(index, dim):
-    """(pointer, bytes, tensor) of the attention kernels' workspace, its counters zero."""
+    """The attention kernels' workspace on the current device, its counters zero:
+    (pointer, bytes, the current stream, tensor to hold until the launch)."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
     need = _scratch_bytes.get((index, dim))
     if need is None:
-        with torch.cuda.device(index):
-            need = int(_lib.lib().m5b_paged_attention_workspace_bytes(dim))
-        _scratch_bytes[index, dim] = need
+        need = _scratch_bytes[index, dim] = int(_lib.lib().m5b_paged_attention_workspace_bytes(dim))
     if need <= 0:
-        return 0, 0, None
+        return 0, 0, stream, None
+    buf = stream_buffer("paged", index, stream, need, _counted)
+    return buf.data_ptr(), need, stream, buf
 
-    def make(nbytes):
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-        buf[:_COUNTER_BYTES].zero_()
-        return buf
 
-    buf = stream_buffer("paged", index, need, make)
-    return buf.data_ptr(), need, buf
+def _attend(index, dim, fields):
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _attend(index, dim, fields)
+    pointer, size, stream, _held = _scratch(index, dim)
+    check(_lib.lib().m5b_paged_attention(_PACK_ATTEND.pack(*fields, pointer, size), stream))
 
 
 def paged_append(k, v, k_cache, v_cache, page_table, query_start, seq_lens, *, cos=None, sin=None,
@@ -271,8 +279,7 @@ def paged_attention(q, k_cache, v_cache, page_table, query_start, seq_lens, *, m
         lse_ptr = lse.data_ptr()
     if tokens > 0:
         ot, oh, _ = out.stride()
-        ws_ptr, ws_bytes, _held = _scratch(index, dim)
-        _call(_lib.lib().m5b_paged_attention, _PACK_ATTEND.pack(
-            *fields, q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, lse_ptr, max_query_len, scale,
-            softcap, slopes_ptr, window, prefix_ptr, ws_ptr, ws_bytes), index)
+        _attend(index, dim, fields + (
+            q.data_ptr(), qt, qh, out.data_ptr(), ot, oh, lse_ptr, max_query_len, scale, softcap,
+            slopes_ptr, window, prefix_ptr))
     return (out, lse) if return_lse else out

@@ -39,7 +39,8 @@ def cuda(monkeypatch):
         monkeypatch.setattr(torch, f, recorded(f))
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: state.stream, raising=False)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state.capture != 0)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: state.capture != 0,
+                        raising=False)
     monkeypatch.setattr(torch.cuda, "current_stream",
                         lambda d=None: types.SimpleNamespace(cuda_stream=state.stream))
     monkeypatch.setattr(torch.cuda, "device", lambda i: contextlib.nullcontext())
