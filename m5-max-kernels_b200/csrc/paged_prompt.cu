@@ -133,30 +133,26 @@ __device__ __forceinline__ float max_nan(float x, float y) {
   return r;
 }
 // 2^x of a pair on the FMA pipes, for x < 100: x = n + f with n the nearest
-// integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a polynomial,
-// n added to its exponent.  The coefficients are the minimax fit of the
-// relative error on [-1/2, 1/2] (Remez exchange): 7.5e-5 with four, for bf16
-// probabilities (their rounding: up to 3.9e-3), 2.6e-6 with five, for fp16
-// (4.9e-4).  Below -126 the result stays near 2^-126, not zero: a row that saw
-// no key is known by its m.
-template <typename T> __device__ __forceinline__ float2 ex2_fma(float2 x) {
+// integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a polynomial
+// 1 + f (c1 + ...), n added to its exponent.  The coefficients are the minimax
+// fit of the relative error on [-1/2, 1/2] (Remez exchange), 2.9e-6 in fp32.
+// The sum of these is an output, lse, so bf16 takes as many terms as fp16:
+// with one less (1e-4, below its rounding of P all the same) two prompts of
+// 8192 tokens took 1150 us instead of 1168; with one more (1.6e-7) 1183.
+// Below -126 the result stays near 2^-126, not zero: a row that saw no key is
+// known by its m.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
   x.x = fmaxf(x.x, -126.0f);
   x.y = fmaxf(x.y, -126.0f);
-  const float2 big = make_float2(12582912.0f, 12582912.0f);
-  const float2 neg = make_float2(-12582912.0f, -12582912.0f), one = make_float2(-1.0f, -1.0f);
+  const float2 big = make_float2(12582912.0f, 12582912.0f), one = make_float2(1.0f, 1.0f);
   const float2 r = __fadd2_rn(x, big);
-  const float2 f = __ffma2_rn(__fadd2_rn(r, neg), one, x);
-  float2 p;
-  if (DTypeOf<T>::value == DT_BF16) {
-    p = __ffma2_rn(make_float2(0x1.c3f76p-5f, 0x1.c3f76p-5f), f, make_float2(0x1.f0de1ap-3f, 0x1.f0de1ap-3f));
-    p = __ffma2_rn(p, f, make_float2(0x1.62f31ap-1f, 0x1.62f31ap-1f));
-    p = __ffma2_rn(p, f, make_float2(0x1.fff692p-1f, 0x1.fff692p-1f));
-  } else {
-    p = __ffma2_rn(make_float2(0x1.3997d6p-7f, 0x1.3997d6p-7f), f, make_float2(0x1.ca144p-5f, 0x1.ca144p-5f));
-    p = __ffma2_rn(p, f, make_float2(0x1.ec06dap-3f, 0x1.ec06dap-3f));
-    p = __ffma2_rn(p, f, make_float2(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
-    p = __ffma2_rn(p, f, make_float2(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
-  }
+  const float2 f = __ffma2_rn(__fadd2_rn(r, make_float2(-12582912.0f, -12582912.0f)),
+                              make_float2(-1.0f, -1.0f), x);
+  float2 p = make_float2(0x1.3a02ccp-7f, 0x1.3a02ccp-7f);
+  p = __ffma2_rn(p, f, make_float2(0x1.c9fc46p-5f, 0x1.c9fc46p-5f));
+  p = __ffma2_rn(p, f, make_float2(0x1.ec0378p-3f, 0x1.ec0378p-3f));
+  p = __ffma2_rn(p, f, make_float2(0x1.62e12cp-1f, 0x1.62e12cp-1f));
+  p = __ffma2_rn(p, f, one);
   return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)),
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
 }
@@ -612,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            x[k] = k % 8 < (MOD ? 0 : kFmaPairs) ? ex2_fma<T>(x[k]) : make_float2(ex2(x[k].x), ex2(x[k].y));
+            x[k] = k % 8 < (MOD ? 0 : kFmaPairs) ? ex2_fma(x[k]) : make_float2(ex2(x[k].x), ex2(x[k].y));
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             sum[k & 1] = __fadd2_rn(sum[k & 1], x[k]);

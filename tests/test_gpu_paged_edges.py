@@ -121,3 +121,19 @@ def test_a_nan_or_infinite_score_reaches_its_rows(ops, dim, dtype, hint, value):
         batch.k_cache[home] = float("nan") if value == "nan" else 1e30
         check_nan_rows(attend(ops, batch, hint), clean, slice(slot, 70), slice(2, 4))
         batch.k_cache[home] = 0.0
+
+
+# ---------------------------------------------------------------- precision
+
+@pytest.mark.parametrize("dim,dtype,hint", [(64, BF16, 300), (128, BF16, 300), (128, F16, 300),
+                                            (64, BF16, 1), (128, F16, 1), (128, F32, 300)])
+@pytest.mark.parametrize("kw", [{}, dict(window=1), dict(window=5), dict(scale=0.01)],
+                         ids=lambda kw: "-".join(f"{k}{v}" for k, v in kw.items()) or "plain")
+def test_lse_has_the_precision_of_its_type(ops, dim, dtype, hint, kw):
+    """The products of 16-bit inputs are exact in fp32, in which scores, exponentials and sums are
+    held whatever the cache's type: 2^-16 for those and 2^-20 of the logarithm itself, as for an
+    fp32 cache."""
+    batch = Batch([300, 3], [0, 200], q_heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype)
+    want = attend_oracle(batch, **kw)[1]
+    lse = attend(ops, batch, hint, **kw)[1].double().cpu()
+    assert ((lse - want).abs() - (2.0**-16 + 2.0**-20 * want.abs())).max().item() <= 0
