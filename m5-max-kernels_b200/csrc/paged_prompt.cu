@@ -139,11 +139,12 @@ __device__ __forceinline__ float max_nan(float x, float y) {
 // The sum of these is an output, lse, so bf16 takes as many terms as fp16:
 // with one less (1e-4, below its rounding of P all the same) two prompts of
 // 8192 tokens took 1150 us instead of 1168; with one more (1.6e-7) 1183.
-// Below -126 the result stays near 2^-126, not zero: a row that saw no key is
-// known by its m.
+// From -127 down the result is zero, as hidden keys' has to be: the polynomial
+// is 1 there, whose exponent bits n = -127 takes to none (down to -126 it leaves
+// a number below 2^-126).
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
-  x.x = fmaxf(x.x, -126.0f);
-  x.y = fmaxf(x.y, -126.0f);
+  x.x = fmaxf(x.x, -127.0f);
+  x.y = fmaxf(x.y, -127.0f);
   const float2 big = make_float2(12582912.0f, 12582912.0f), one = make_float2(1.0f, 1.0f);
   const float2 r = __fadd2_rn(x, big);
   const float2 f = __ffma2_rn(__fadd2_rn(r, make_float2(-12582912.0f, -12582912.0f)),

@@ -137,3 +137,23 @@ def test_lse_has_the_precision_of_its_type(ops, dim, dtype, hint, kw):
     want = attend_oracle(batch, **kw)[1]
     lse = attend(ops, batch, hint, **kw)[1].double().cpu()
     assert ((lse - want).abs() - (2.0**-16 + 2.0**-20 * want.abs())).max().item() <= 0
+
+
+@pytest.mark.parametrize("dim,dtype,hint", KINDS)
+@pytest.mark.parametrize("kw", [{}, dict(window=40), dict(softcap=30.0)],
+                         ids=lambda kw: "-".join(kw) or "plain")
+def test_hidden_keys_weigh_nothing(ops, dim, dtype, hint, kw):
+    """Values of hidden keys as large as the type holds do not move a row by a bit."""
+    large = 60000.0 if dtype is F16 else 3e38
+    batch = Batch([150, 1], [30, 40], q_heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype)
+    clean = attend(ops, batch, hint, **kw)
+    for key in (33, 90, 134, 179):  # positions 30 .. 179 are new rows
+        home = int(batch.table[0, key // 16]), slice(None), key % 16
+        kept = batch.v_cache[home].clone()
+        batch.v_cache[home] = large
+        got = attend(ops, batch, hint, **kw)
+        seen = torch.zeros(151, dtype=torch.bool)
+        seen[key - 30:min(150, key - 30 + kw.get("window", 1000))] = True
+        assert torch.equal(got[0].cpu()[~seen], clean[0].cpu()[~seen])
+        assert torch.equal(got[1], clean[1])
+        batch.v_cache[home] = kept
