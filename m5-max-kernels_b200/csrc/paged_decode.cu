@@ -19,6 +19,8 @@
 // 64 sequences of up to 8191 keys, 32 + 8 heads of 128: 183 us, 5.7 TB/s; all
 // of 8000 and more 6.5 TB/s, the rate of a copy.  What short calls pay is the
 // start (lengths, table, first block) and the joins, 10 us together.
+#include <cfloat>
+
 #include "paged_sched.cuh"
 
 namespace m5b {
@@ -94,11 +96,29 @@ template <int N> __device__ __forceinline__ void consumers_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
 }
 
-// x of one score: capped and biased, in log2 units.
-__device__ __forceinline__ float modify(float x, float softcap, float slope, int pos, int key) {
-  if (softcap > 0.0f)  // tanh(y) = 1 - 2 / (e^2y + 1)
-    x = softcap * (1.0f - __fdividef(2.0f, ex2(x * (2.0f * kLog2e / softcap)) + 1.0f));
-  return (x - slope * fabsf(static_cast<float>(pos - key))) * kLog2e;
+// A warp's scores q.k scaled and capped; r = scale / softcap.  Scores up to the
+// cap go by tanh_ratio, those beyond by tanh(y) = 1 - 2 / (e^2y + 1), which would
+// leave small ones off by 1e-7 of the cap, however large that is.
+__device__ __forceinline__ void cap_scores(float (&s)[2][4], float scale, float softcap, float r) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(s[i / 4][i % 4]));
+  const bool within = __all_sync(~0u, top * r <= 1.0f);
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float &x0 = s[i / 4][i % 4], &x1 = s[i / 4][i % 4 + 1];
+    const float2 x = make_float2(x0, x1), y = __fmul2_rn(x, make_float2(r, r));
+    const float2 in = __fmul2_rn(__fmul2_rn(x, make_float2(scale, scale)),
+                                 tanh_ratio(__fmul2_rn(y, y)));
+    x0 = in.x;
+    x1 = in.y;
+    if (!within) {
+      if (!(fabsf(y.x) <= 1.0f))
+        x0 = softcap * (1.0f - __fdividef(2.0f, ex2(y.x * (2.0f * kLog2e)) + 1.0f));
+      if (!(fabsf(y.y) <= 1.0f))
+        x1 = softcap * (1.0f - __fdividef(2.0f, ex2(y.y * (2.0f * kLog2e)) + 1.0f));
+    }
+  }
 }
 
 template <typename T, int D, bool MOD>
@@ -182,6 +202,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::PER_SM)
   const int lrow = slice * 16 + (lane & 7);
   const int k_row = lrow + ((lane >> 4) & 1) * 8, k_chunk = (lane >> 3) & 1;  // keys 0-7 | 8-15 last
   const int v_row = lrow + ((lane >> 3) & 1) * 8, v_chunk = (lane >> 4) & 1;  // channels last
+  const float cap_ratio = MOD && a.softcap > 0.0f ? fminf(a.scale / a.softcap, FLT_MAX) : 0.0f;
   bool ok = true;
   // (a warp whose wait gave up still walks along, for the barriers' sake)
   while (walk.next(a, p)) {
@@ -228,13 +249,18 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::PER_SM)
         mma16816<T>(s[1], q[k], b[2], b[3]);
       }
       const int key0 = block0 + slice * 16 + t4 * 2;
+      if (MOD && a.softcap > 0.0f) {
+        cap_scores(s, a.scale, a.softcap, cap_ratio);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e / 4][e % 4] *= a.scale;
+      }
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = s[n][e] * a.scale;
-          s[n][e] = MOD ? modify(x, a.softcap, slope[e / 2], pos[e / 2], key0 + n * 8 + (e & 1))
-                        : x * kLog2e;
+          if (MOD) s[n][e] -= slope[e / 2] * fabsf(static_cast<float>(pos[e / 2] - key0 - n * 8 - (e & 1)));
+          s[n][e] *= kLog2e;
         }
       const bool open = block0 + kBlock <= p.s.keys &&
                         (block0 + kBlock <= p.s.prefix ||

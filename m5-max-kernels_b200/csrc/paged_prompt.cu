@@ -158,17 +158,6 @@ __device__ __forceinline__ float2 ex2_fma(float2 x) {
                      __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
 }
 
-// tanh(y) / y for a pair of y^2 in [0, 1]: the minimax fit of the relative
-// error (Remez exchange), 6e-7.
-__device__ __forceinline__ float2 tanh_ratio(float2 z) {
-  float2 p = make_float2(-0x1.920178p-9f, -0x1.920178p-9f);
-  p = __ffma2_rn(p, z, make_float2(0x1.1251b6p-6f, 0x1.1251b6p-6f));
-  p = __ffma2_rn(p, z, make_float2(-0x1.a6c0f2p-5f, -0x1.a6c0f2p-5f));
-  p = __ffma2_rn(p, z, make_float2(0x1.1000f6p-3f, 0x1.1000f6p-3f));
-  p = __ffma2_rn(p, z, make_float2(-0x1.554a16p-2f, -0x1.554a16p-2f));
-  return __ffma2_rn(p, z, make_float2(0x1.ffffecp-1f, 0x1.ffffecp-1f));
-}
-
 // What is done to the scores: nothing, a bias, a cap (and, by a flag, a bias).
 // Each has a kernel, for the sake of the instruction cache: one for both of the
 // latter took 4 to 7 % longer.

@@ -157,3 +157,17 @@ def test_hidden_keys_weigh_nothing(ops, dim, dtype, hint, kw):
         assert torch.equal(got[0].cpu()[~seen], clean[0].cpu()[~seen])
         assert torch.equal(got[1], clean[1])
         batch.v_cache[home] = kept
+
+
+@pytest.mark.parametrize("dim,dtype,hint", [(64, BF16, 64), (128, F16, 64), (128, BF16, 1),
+                                            (64, F16, 1), (64, F32, 1)])
+@pytest.mark.parametrize("cap", [3.0, 900.0, 1e3, 1e4, 1e5, 1e6, 1e8, 1e30])
+def test_large_caps(ops, dim, dtype, hint, cap):
+    """A cap far above the scores changes next to nothing, in every kernel: scores are off by
+    2^-16 at most (check_attention's e for fp32), not by a share of the cap."""
+    batch = Batch([1, 70, 2], [200, 30, 500], q_heads=8, kv_heads=2, dim=dim, page=16, dtype=dtype)
+    want, want_lse, spread = attend_oracle(batch, softcap=cap)
+    out, lse = attend(ops, batch, hint, softcap=cap)
+    check_attention(out, lse, want, want_lse, spread, dtype)
+    off = (lse.double().cpu() - want_lse).abs()
+    assert (off - (2.0**-16 + 2.0**-20 * want_lse.abs())).max().item() <= 0
