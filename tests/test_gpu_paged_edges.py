@@ -171,3 +171,24 @@ def test_large_caps(ops, dim, dtype, hint, cap):
     check_attention(out, lse, want, want_lse, spread, dtype)
     off = (lse.double().cpu() - want_lse).abs()
     assert (off - (2.0**-16 + 2.0**-20 * want_lse.abs())).max().item() <= 0
+
+
+@pytest.mark.parametrize("dim,dtype,hint", [(64, BF16, 64), (128, F16, 64), (128, BF16, 1)])
+@pytest.mark.parametrize("cap", [1e3, 1e5])
+def test_scores_on_both_sides_of_a_large_cap(ops, dim, dtype, hint, cap):
+    """Ordinary rows beside ones whose scores exceed the cap: 2^-16 for the scores of the former
+    as without those; the others' scores are of the cap's size and off by the 2^-20 of it that tanh
+    has and a few fp32 roundings, 2^-19 together."""
+    batch = Batch([70, 2], [60, 500], q_heads=8, kv_heads=2, dim=dim, page=16, dtype=dtype)
+    batch.q[::3] *= 60000.0 / batch.q.abs().max()  # (within fp16)
+    scale = 2 * cap / 60000.0 if cap > 1e4 else dim ** -0.5
+    batch.q[1::3] *= dim ** -0.5 / scale if cap > 1e4 else 1.0
+    batch.q[2::3] *= dim ** -0.5 / scale if cap > 1e4 else 1.0
+    want, want_lse, _ = attend_oracle(batch, softcap=cap, scale=scale)
+    lse = attend(ops, batch, hint, softcap=cap, scale=scale)[1].double().cpu()
+    large = torch.zeros(72, dtype=torch.bool)
+    large[::3] = True
+    assert want_lse[large].max().item() > 0.7 * cap
+    off = (lse - want_lse).abs() - (2.0**-16 + 2.0**-20 * want_lse.abs())
+    assert off[~large].max().item() <= 0 and want_lse[~large].abs().max().item() < 100
+    assert (lse - want_lse)[large].abs().max().item() <= 2.0**-19 * cap
