@@ -177,7 +177,8 @@ __device__ __forceinline__ void modify(uint32_t (&s)[2][32], float scale, float 
                                        bool biased, float slope, int ahead) {
   const float k = scale * kLog2e;
   if (SCORES >= kCapped) {
-    const float r = scale / softcap;
+    // ((x r^2) x, not x^2 r^2: x^2 may be beyond the range; r^2 is not)
+    const float r = fminf(scale / softcap, 0x1p63f);
     float top[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int e = 0; e < 64; e += 2)
@@ -189,7 +190,7 @@ __device__ __forceinline__ void modify(uint32_t (&s)[2][32], float scale, float 
       for (int e = 0; e < 64; e += 2) {
         const float2 x = make_float2(__uint_as_float(s[e / 32][e % 32]),
                                      __uint_as_float(s[e / 32][e % 32 + 1]));
-        const float2 y = __fmul2_rn(__fmul2_rn(x, k2), tanh_ratio(__fmul2_rn(__fmul2_rn(x, x), r2)));
+        const float2 y = __fmul2_rn(__fmul2_rn(x, k2), tanh_ratio(__fmul2_rn(__fmul2_rn(x, r2), x)));
         s[e / 32][e % 32] = __float_as_uint(y.x);
         s[e / 32][e % 32 + 1] = __float_as_uint(y.y);
       }
@@ -200,7 +201,7 @@ __device__ __forceinline__ void modify(uint32_t (&s)[2][32], float scale, float 
         const float x = __uint_as_float(s[e / 32][e % 32]);
         float y = cap * (1.0f - __fdividef(2.0f, ex2(x * two) + 1.0f));
         if (SCORES == kCappedFar) {
-          const float z = x * x * (r * r);
+          const float z = x * (r * r) * x;
           if (z <= 1.0f) y = x * k * tanh_ratio(make_float2(z, z)).x;
         }
         s[e / 32][e % 32] = __float_as_uint(y);

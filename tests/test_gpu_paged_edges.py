@@ -192,3 +192,23 @@ def test_scores_on_both_sides_of_a_large_cap(ops, dim, dtype, hint, cap):
     off = (lse - want_lse).abs() - (2.0**-16 + 2.0**-20 * want_lse.abs())
     assert off[~large].max().item() <= 0 and want_lse[~large].abs().max().item() < 100
     assert (lse - want_lse)[large].abs().max().item() <= 2.0**-19 * cap
+
+
+@pytest.mark.parametrize("dim,hint", [(64, 64), (128, 64), (128, 1)])
+@pytest.mark.parametrize("cap,scale,size", [(1e30, 1.0, 1e12), (1e37, 0.125, 1e12),
+                                            (1.5e-38, 8.0, 1.0), (1e-30, 1e20, 1e-3)])
+def test_caps_and_scores_at_the_ends_of_the_range(ops, dim, hint, cap, scale, size):
+    """Squares and ratios of them that fp32 does not hold: no NaN, and the softmax is right."""
+    batch = Batch([70, 2], [60, 300], q_heads=4, kv_heads=2, dim=dim, page=16, dtype=BF16)
+    batch.q *= size
+    batch.q[3] = 0.0  # scores of zero
+    for b in range(2):
+        batch.k[b] *= size if size > 1.0 else 1.0
+    batch.k_cache *= size if size > 1.0 else 1.0
+    want, want_lse, spread = attend_oracle(batch, softcap=cap, scale=scale)
+    out, lse = attend(ops, batch, hint, softcap=cap, scale=scale)
+    if cap < 1.0:  # scores next to zero: every key weighs the same
+        check_attention(out, lse, want, want_lse, spread, BF16)
+    else:  # one key takes all, unless two are within fp32's rounding of one another
+        assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+        assert ((lse.double().cpu() - want_lse).abs() <= 2.0**-18 * want_lse.abs() + 2.0**-16).all()
