@@ -184,7 +184,10 @@ int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
   int rc = take_batch(s->b, a.b);
   if (rc) return rc;
   if (s->b.head_dim > 256) return eunsupported("head_dim above 256 is unsupported");
-  if (!(s->scale > 0.0) || !std::isfinite(static_cast<float>(s->scale)))
+  // (as fp32, in which the kernels scale, times log2 e too: -inf * 0 would make
+  // hidden scores NaN)
+  const float scale = static_cast<float>(s->scale);
+  if (!(scale > 0.0f) || !std::isfinite(scale * 1.4426950408889634f))
     return einval("scale must be a positive finite real scalar");
   if (!(s->softcap >= 0.0) || !std::isfinite(static_cast<float>(s->softcap)) ||
       (s->softcap > 0.0 && s->softcap < FLT_MIN))
@@ -201,7 +204,7 @@ int m5b_paged_attention(const m5b_paged_attention_args* s, void* stream) {
   a.o_head = s->out_head_stride;
   a.lse = s->lse;
   a.max_query_len = s->max_query_len > INT_MAX ? INT_MAX : static_cast<int>(s->max_query_len);
-  a.scale = static_cast<float>(s->scale);
+  a.scale = scale;
   a.softcap = static_cast<float>(s->softcap);
   a.slopes = s->slopes;
   a.window = s->window == 0 || s->window > INT_MAX ? INT_MAX : static_cast<int>(s->window);
