@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::PER_SM)
       for (int i = p.begin; i < p.end; ++i) {
         const int key = p.r.at(i) * kBlock + row;
         int page = a.b.num_pages, slot = 0;  // out of range: zeros
-        if (lane < boxes && key < p.s.keys && (key < p.s.prefix || key + maps.box_rows > window)) {
+        if (lane < boxes && key < p.s.keys && (key < p.s.prefix || key > window - maps.box_rows)) {
           const int at = paged_page(a.b, p.seq, key);
           if (at >= 0) page = at;
           slot = key % a.b.page_size;
@@ -262,9 +262,10 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::PER_SM)
           if (MOD) s[n][e] -= slope[e / 2] * fabsf(static_cast<float>(pos[e / 2] - key0 - n * 8 - (e & 1)));
           s[n][e] *= kLog2e;
         }
-      const bool open = block0 + kBlock <= p.s.keys &&
-                        (block0 + kBlock <= p.s.prefix ||
-                         (block0 + kBlock - 1 <= pos_lo && pos_hi - block0 < a.window));
+      // (differences: positions reach the last 32-bit one)
+      const bool open = p.s.keys - block0 >= kBlock &&
+                        (p.s.prefix - block0 >= kBlock ||
+                         (pos_lo - block0 >= kBlock - 1 && pos_hi - block0 < a.window));
       if (!open) {
 #pragma unroll
         for (int n = 0; n < 2; ++n)

@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int block0 = p.r.at(i) * kBlock, key = block0 + row;
           int page = a.b.num_pages, slot = 0;  // out of range: zeros
           if (lane < boxes && key < p.s.keys &&
-              (key < p.s.prefix || key + maps.box_rows > window)) {
+              (key < p.s.prefix || key > window - maps.box_rows)) {
             const int at = paged_page(a.b, p.seq, key);
             if (at >= 0) page = at;
             slot = key % a.b.page_size;
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // (two bodies, where they are short: scores that a branch may change
         // cost the other way too, but a body may outgrow the instruction cache)
         const bool open =
-            block0 + kBlock <= prefix || (block0 >= all_lo && block0 + kBlock - 1 <= all_hi);
+            prefix - block0 >= kBlock || (block0 >= all_lo && all_hi - block0 >= kBlock - 1);
         if (!MOD && open)
           softmax(Flag<false>(), i, block0, true);
         else

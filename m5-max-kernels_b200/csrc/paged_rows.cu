@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const PagedAttn
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) o[i] = 0.0f;
   // chunks [0, pre) hold the prefix, [from, end) the row's own window
-  const int pre = (prefix + 31) / 32;
+  const int pre = prefix / 32 + (prefix % 32 != 0);
   const int last = min(pos, len - 1);
   const int first = (pos >= a.window) ? pos - a.window + 1 : 0;
   const int from = max(pre, first / 32), end = last >= 0 ? last / 32 + 1 : 0;

@@ -81,7 +81,7 @@ __device__ __forceinline__ PagedBlocks paged_blocks(const PagedAttnArgs& a, cons
   const int hi = s.pos0 + min(rt * ROWS + ROWS - 1, s.n * g - 1) / g;
   const int last = min(hi, s.keys - 1);
   PagedBlocks r;
-  r.pre = (s.prefix + BK - 1) / BK;
+  r.pre = s.prefix / BK + (s.prefix % BK != 0);
   r.from = max(r.pre, lo >= a.window ? (lo - a.window + 1) / BK : 0);
   r.blocks = max(1, r.pre + (last >= 0 ? max(0, last / BK + 1 - r.from) : 0));
   return r;

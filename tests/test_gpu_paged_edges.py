@@ -212,3 +212,27 @@ def test_caps_and_scores_at_the_ends_of_the_range(ops, dim, hint, cap, scale, si
     else:  # one key takes all, unless two are within fp32's rounding of one another
         assert torch.isfinite(out).all() and torch.isfinite(lse).all()
         assert ((lse.double().cpu() - want_lse).abs() <= 2.0**-18 * want_lse.abs() + 2.0**-16).all()
+
+
+# ---------------------------------------------------------------- positions
+
+@pytest.mark.parametrize("dim,dtype,hint", KINDS)
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("page", [16, 256])
+def test_the_last_positions_of_32_bits(ops, dim, dtype, hint, new, page):
+    """A sequence of 2^31 - 1 tokens, of which a window sees the last ones."""
+    length = 2 * page - 1 + (512 if page == 16 else 0)
+    batch = Batch([new], [length - new], q_heads=4, kv_heads=2, dim=dim, page=page, dtype=dtype)
+    want, want_lse, spread = attend_oracle(batch, window=100)
+    kc, vc, table, starts, lens = batch.on(DEV)
+    far = torch.full((1, 2**31 // page), -1, dtype=torch.int32, device=DEV)
+    far[:, -table.shape[1]:] = table
+    lens.fill_(2**31 - 1)
+    out, lse = ops.paged_attention(batch.q.to(DEV), kc, vc, far, starts, lens, max_query_len=hint,
+                                   window=100, return_lse=True)
+    check_attention(out, lse, want, want_lse, spread, dtype)
+    rows = torch.randn(new, 2, dim, device=DEV).to(dtype)
+    ops.paged_append(rows, rows, kc, vc, far, starts, lens)
+    at = torch.arange(length - new, length, device=DEV)
+    where = table[0, at // page].long()
+    assert torch.equal(kc[where, :, at % page], rows) and torch.equal(vc[where, :, at % page], rows)
