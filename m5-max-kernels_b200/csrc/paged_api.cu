@@ -35,7 +35,9 @@ int take_batch(const m5b_paged_batch& s, PagedBatch& d) {
   if (!fits_int(s.tokens) || !fits_int(s.batch) || !fits_int(s.num_pages) ||
       !fits_int(s.page_size) || !fits_int(s.max_pages) || s.q_heads > 65535 || s.head_dim > 65535)
     return eunsupported("batch or cache dimensions exceed the index range");
-  if (s.tokens * s.q_heads > INT_MAX) return eunsupported("tokens x heads exceed the launch grid limit");
+  // (the kernels round rows up to whole tiles, and count a token's channels)
+  if (s.tokens * s.q_heads > INT_MAX - 4096 || (s.q_heads + 2 * s.kv_heads) * s.head_dim > INT_MAX)
+    return eunsupported("tokens x heads or heads x head_dim exceed the index range");
   if (!s.query_start || !s.seq_lens || !s.k_cache || !s.v_cache || (!s.page_table && s.max_pages > 0))
     return einval("query_start, seq_lens, the caches and the page table are required");
   d = PagedBatch{};

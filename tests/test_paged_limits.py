@@ -28,3 +28,11 @@ def m5():
 def test_scales_that_fp32_does_not_hold(m5, scale):
     code, text = attend(m5, scale=scale)
     assert code == m5[2].EINVAL and b"scale" in text
+
+
+@pytest.mark.parametrize("change", [dict(tokens=(2**31 - 1) // 4), dict(tokens=2**31 - 1, q_heads=1, kv_heads=1),
+                                    dict(q_heads=65535, kv_heads=65535, dim=65535, tokens=1)])
+def test_rows_and_channels_beyond_the_index_range(m5, change):
+    """What the kernels count in 32 bits, rounded up to tiles of rows."""
+    code, text = attend(m5, **change)
+    assert code == m5[2].EUNSUPPORTED and b"range" in text
