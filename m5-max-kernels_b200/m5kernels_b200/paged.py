@@ -38,6 +38,7 @@ _PACK_APPEND = struct.Struct("@38q")
 _PACK_ATTEND = struct.Struct("@29q2d5q")
 _Tensor = torch.Tensor
 _CONTIGUOUS = torch.contiguous_format
+_FAR = 2**31 - 1  # no position is beyond
 
 
 def _ints(t, name):
@@ -244,12 +245,16 @@ def paged_attention(q, k_cache, v_cache, page_table, query_start, seq_lens, *, m
         raise ValueError("max_query_len must be a whole number")
     if max_query_len < 0:
         raise ValueError("max_query_len must not be negative")
+    if max_query_len > _FAR:
+        max_query_len = _FAR
     scale = dim ** -0.5 if scale is None else _positive(scale, "scale")
     softcap = 0.0 if softcap is None else _positive(softcap, "softcap")
     if window is None:
         window = 0
     elif isinstance(window, bool) or not isinstance(window, Integral) or window < 1:
         raise ValueError("window must be a positive whole number")
+    elif window > _FAR:
+        window = _FAR
     used.append(q)
     slopes_ptr = prefix_ptr = lse_ptr = 0
     if slopes is not None:

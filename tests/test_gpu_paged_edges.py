@@ -236,3 +236,11 @@ def test_the_last_positions_of_32_bits(ops, dim, dtype, hint, new, page):
     at = torch.arange(length - new, length, device=DEV)
     where = table[0, at // page].long()
     assert torch.equal(kc[where, :, at % page], rows) and torch.equal(vc[where, :, at % page], rows)
+
+
+@pytest.mark.parametrize("far", [2**31, 10**30])
+def test_windows_and_hints_of_any_size(ops, far):
+    batch = Batch([1, 70], [200, 30], q_heads=4, kv_heads=2, dim=64, page=16, dtype=BF16)
+    want, want_lse, spread = attend_oracle(batch)
+    out, lse = attend(ops, batch, far, window=far)
+    check_attention(out, lse, want, want_lse, spread, BF16)
