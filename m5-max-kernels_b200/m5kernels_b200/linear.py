@@ -60,6 +60,8 @@ def stream_buffer(tag: str, index: int, stream: int, nbytes: int, make) -> torch
     with _ws_lock:
         held = _captured.get(key)
         if held is None or held[0] != capture or held[1].numel() < nbytes:
+            held = None  # (first: where graphs share a pool, they share this memory)
+            _captured.pop(key, None)
             held = _captured[key] = (capture, make(nbytes, index))
         return held[1]
 

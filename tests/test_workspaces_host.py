@@ -155,6 +155,26 @@ def test_counters_are_renewed_after_a_timeout(cuda, monkeypatch):
     assert not bound[0].gemm_ws.any() and bound[1].gemm_ws.all()
 
 
+def test_captures_one_after_another_hold_one_workspace(cuda):
+    """Graphs of one memory pool can take it in turn."""
+    from m5kernels_b200.paged import _scratch
+
+    real = torch.empty
+    alive = []
+
+    def counted(*shape, **kw):
+        alive.append(sum(ref() is not None for _, ref in cuda.made))
+        return real(*shape, **kw)
+
+    torch.empty = counted
+    try:
+        for cuda.capture in (7, 8, 9):
+            _scratch(0, 128)
+    finally:
+        torch.empty = real
+    assert alive == [0, 0, 0]
+
+
 def test_streams_have_their_own(cuda):
     from m5kernels_b200.paged import _scratch
 
