@@ -440,12 +440,14 @@ M5B_API int m5b_paged_append(const m5b_paged_append_args* args, void* stream);
  * largest n_b and chooses the kernel; the result does not depend on it.
  * Slots behind a sequence's end may hold anything, and so may pages wholly
  * between its prefix and the windows of all its new rows (given to others by
- * now, say); its other keys and values are finite.  A NaN among a row's own queries makes that
- * row's out and lse NaN, and no other's.  The first M5B_PAGED_COUNTER_BYTES of the
+ * now, say); its other keys and values are finite.  Hidden keys weigh nothing, whatever finite
+ * values theirs are.  A NaN among a row's own queries makes that row's out and lse NaN, and no
+ * other's; so does a score that is NaN or +inf (uncapped), for the rows that see its key.  lse is
+ * held in fp32 throughout.  The first M5B_PAGED_COUNTER_BYTES of the
  * workspace (m5b_paged_attention_workspace_bytes) must be zero before its first
  * use (cudaMemset once after allocating it); calls of any shape leave them
- * zero.  Calls that overlap on the GPU need separate workspaces.  After a
- * nonzero m5b_device_status (a timed-out wait) zero them again. */
+ * zero.  Calls that overlap on the GPU need separate workspaces; so do graphs,
+ * for as long as they live (m5b_stream_capture_id).  After a nonzero m5b_device_status (a timed-out wait) zero them again. */
 #define M5B_PAGED_COUNTER_BYTES 4096
 typedef struct m5b_paged_attention_args {
   m5b_paged_batch b;

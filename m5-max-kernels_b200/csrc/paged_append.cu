@@ -4,10 +4,10 @@
 // A rotated pair of channels is
 //   (fma(a, c, -(b s)), fma(b, c, a s))
 // in FP32, rounded once more to the cache's type.
-// One CTA per new row.  Two kernels with the same arithmetic: whole 16-channel
-// units in 16-byte accesses, and a channel pair at a time for everything else
-// (head dimensions and rotated widths that units do not divide, operands off
-// the 16-byte grid).
+// Two kernels with the same arithmetic: whole 16-channel units in 16-byte
+// accesses, up to eight rows a CTA and the heads over several if need be, and a
+// channel pair at a time, one CTA per row, for everything else (head dimensions
+// and rotated widths that units do not divide, operands off the 16-byte grid).
 #include "paged.cuh"
 
 namespace m5b {

@@ -5,7 +5,7 @@
 // halves of 128 rows (an MMA's height).  Per step of 64 keys and half:
 //   S = Q K^T          A, B from shared memory, 128 x 64 fp32 in TMEM
 //   t = S scale log2 e, p = 2^(t - m), l += sum p   one thread a row
-//   O += P V           P (the cache's type) from TMEM over S, V from shared memory
+//   O += P V           P (the cache's type) from TMEM, V from shared memory
 // Roles: two warpgroups, one per half, each thread owning a row of S and O; one
 // thread issuing QK of both halves in turn and one issuing PV (a wait on an
 // mbarrier costs an issuing thread some 55 cycles even when there is nothing
@@ -18,21 +18,21 @@
 //
 // TMEM's 512 columns hold O (2 x 128), S (2 x 64) and P (2 x 2 x 32): QK of
 // the next step starts when the softmax has read S, and PV of this one when P
-// is there.  (Measured and not kept: two S buffers with P over them, whose
-// reuse chains softmax, PV and QK, 1830 cycles; one S buffer of 128 keys, which
-// needs fewer bytes of shared memory a flop but chains them all the more, 4250
-// for 128 keys.)  m is near the row's maximum (kGrow); where it changes, O is
-// rescaled in place.  (Taking the exponentials with the
-// old m first, and again in the rare case: 2200 cycles.)  P is rounded to the
-// cache's type for the product, once, at the size of the output's own rounding;
-// sums, m and O are fp32.
+// is there.  (Measured and not kept, with a thread per half issuing both of its
+// products: two S buffers with P over them, whose reuse chains softmax, PV and
+// QK, 1830 cycles; one S buffer of 128 keys, which needs fewer bytes of shared
+// memory a flop but chains them all the more, 4250 for 128 keys.)  m is near the
+// row's maximum (kGrow); where it changes, O is rescaled in place.  (Taking the
+// exponentials with the old m first, and again in the rare case: 2200 cycles.)
+// P is rounded to the cache's type for the product, once, at the size of the
+// output's own rounding; sums, m and O are fp32.
 //
 // What bounds it: an MMA of 128 x 64 x 16 reads 6 KB of shared memory where its
 // 32 cycles have room for 4, so the products take 8 * 48 + 4 * 64 cycles a half
 // and step at D = 128, 1290 for both halves with the softmax beside them (a
 // test of the two alone), 1460 here without the exponentials (TMA writes, the
-// issuing threads' waits) and 1730 with them: two prompts of 8192 tokens, 32 +
-// 8 heads, 1.15 ms, 958 TFLOP/s.
+// issuing threads' waits) and 1770 with them: two prompts of 8192 tokens, 32 +
+// 8 heads, 1.17 ms, 940 TFLOP/s.
 #include "paged_sched.cuh"
 
 namespace m5b {
@@ -40,10 +40,11 @@ namespace {
 
 constexpr int kBlock = kPagedBlock;  // keys per step
 constexpr int kRows = 256;           // packed rows per tile, two halves
-// Of 8 pairs of exponentials, those by ex2_fma: 1730 cycles a step (1800 with
-// none, 1760 with 2, 1790 with 4).  None where the scores are modified, whose
-// arithmetic keeps the FMA pipes busy (162 us, 187 with 3, in the distance bias
-// of 56 heads).
+// Of 8 pairs of exponentials, those by ex2_fma: a prompt of 4096 tokens, 32 + 8
+// heads, takes 179 us (188 with none), two of 8192, which the power limit slows,
+// 1170 (1175 with none, 1172 with 2, 1226 with 4).  None where the scores are
+// modified, whose arithmetic keeps the FMA pipes busy (162 us, 187 with 3, in the
+// distance bias of 56 heads).
 constexpr int kFmaPairs = 3;
 constexpr int kThreads = 384;  // warps 0-3, 4-7: halves; 8: QK; 9: PV; 10: K, V; 11: rows
 constexpr int kMmaWarp = 8, kTmaWarp = 10, kRowWarp = 11;
