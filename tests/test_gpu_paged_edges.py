@@ -244,3 +244,16 @@ def test_windows_and_hints_of_any_size(ops, far):
     want, want_lse, spread = attend_oracle(batch)
     out, lse = attend(ops, batch, far, window=far)
     check_attention(out, lse, want, want_lse, spread, BF16)
+
+
+@pytest.mark.parametrize("dim,dtype,hint", KINDS)
+@pytest.mark.parametrize("cap", [None, 5.0, 50.0, 500.0])
+def test_other_sequences_do_not_move_a_bit(ops, dim, dtype, hint, cap):
+    """Whatever their queries and keys are, on both sides of the cap."""
+    batch = Batch([70, 30], [60, 75], q_heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype)
+    clean = attend(ops, batch, hint, softcap=cap)
+    batch.q[70:] *= 100.0
+    batch.k_cache[batch.table[1, :4].long()] *= 100.0
+    got = attend(ops, batch, hint, softcap=cap)
+    for x, y in zip(got, clean):
+        assert torch.equal(x[:70], y[:70]) and not torch.equal(x[70:], y[70:])
