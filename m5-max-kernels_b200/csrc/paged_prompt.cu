@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<D>;
   constexpr int STAGES = C::STAGES;
   constexpr bool MOD = SCORES != kPlain;
+  constexpr int kBlankK = SCORES == kCapped;  // whether K blocks are blanked behind the end
   // (no static shared memory: the tiles start on the swizzle's 1024-byte grid)
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* const q_smem = smem;  // [buffer][half]
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sm.o_full[h], 1);
       mbar_init(&sm.drain[h], 1);
     }
-    mbar_init(&sm.landed, 1);
+    mbar_init(&sm.landed, 1 + kBlankK);
     sm.abort_flag = 0;
     fence_mbarrier_init();
     tma_prefetch_desc(&maps.k);
@@ -299,27 +300,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int boxes = kBlock / maps.box_rows * C::HALVES;
       const int row = lane / C::HALVES * maps.box_rows, half = lane % C::HALVES;
       int stage = 0, phase = 0, issued = 0;
-      int blank = -1, blank_from = 0, ph_landed = 0;  // a stage whose last keys are to be blanked
+      // Slots behind the sequence's end may hold NaN, which a zero probability
+      // would not stop: V blocks that reach there land here first and are
+      // blanked, while the K block after them is on its way.  With caps that a
+      // row takes in one form or the other their K blocks too, lest what an
+      // unused slot holds choose.
+      int blank = -1, blank_from = 0, ph_landed = 0;  // the V block's stage, its first unused key
       bool ok = true;
-      auto load = [&](const CUtensorMap* map, int head, int page, int slot, int live) {
+      auto load = [&](const CUtensorMap* map, int head, int page, int slot, bool last) {
         if (ok)
           ok = mbar_wait_relaxed(&sm.empty[stage], phase ^ 1, &sm.abort_flag, a.status,
                                  DEV_TIMEOUT_PRODUCER, 100);
         ok = __all_sync(~0u, ok);
         if (!ok) return;
-        uint64_t* bar = live < kBlock ? &sm.landed : &sm.full[stage];
+        uint64_t* bar = last ? &sm.landed : &sm.full[stage];
         if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE_BYTES);
         __syncwarp();
         if (lane < boxes)
           tma_load_4d(ring + stage * C::TILE_BYTES + half * C::HALF_BYTES + row * 128, map, bar,
                       half * 64, slot, head, page);
-        if (live < kBlock) blank = stage, blank_from = max(live, 0);
         ++issued;
         if (++stage == STAGES) stage = 0, phase ^= 1;
       };
-      // Slots behind the sequence's end may hold NaN, which a zero probability
-      // would not stop: V blocks that reach there land here first and are
-      // blanked, while the K block after them is on its way.
       auto finish = [&]() {
         if (blank < 0) return;
         if (ok)
@@ -328,13 +330,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(~0u, ok);
         if (!ok) return;
         ph_landed ^= 1;
-        uint8_t* v = ring + blank * C::TILE_BYTES;
-        for (int i = blank_from * C::HALVES * 8 + lane; i < kBlock * C::HALVES * 8; i += 32)
-          *reinterpret_cast<uint4*>(v + (i / 8 % C::HALVES) * C::HALF_BYTES + i / (C::HALVES * 8) * 128 +
-                                    i % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+        uint8_t* at = ring + (blank - kBlankK) * C::TILE_BYTES;
+        for (int b = 0; b <= kBlankK; ++b, at += C::TILE_BYTES)
+          for (int i = blank_from * C::HALVES * 8 + lane; i < kBlock * C::HALVES * 8; i += 32)
+            *reinterpret_cast<uint4*>(at + (i / 8 % C::HALVES) * C::HALF_BYTES + i / (C::HALVES * 8) * 128 +
+                                      i % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.full[blank]);
+        if (lane <= kBlankK) mbar_arrive(&sm.full[blank - lane]);
         blank = -1;
       };
       PagedPiece p;
@@ -349,18 +352,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (at >= 0) page = at;
             slot = key % a.b.page_size;
           }
-          load(&maps.k, p.head, page, slot, kBlock);
-          finish();
-          load(&maps.v, p.head, page, slot, p.s.keys - block0);
+          // (K blocks are in the even stages, V blocks in the odd ones after them)
+          const bool last = p.s.keys - block0 < kBlock;
+          if (kBlankK) finish();
+          load(&maps.k, p.head, page, slot, kBlankK && last);
+          if (!kBlankK) finish();
+          if (last) blank = stage, blank_from = max(p.s.keys - block0, 0);
+          load(&maps.v, p.head, page, slot, last);
         }
       }
       finish();
       if (!ok) {  // let the copies in flight land before the CTA ends
         for (int i = 0; i < STAGES && i < issued; ++i) {
           if (--stage < 0) stage = STAGES - 1, phase ^= 1;
+          const bool late = blank >= 0 && stage <= blank && stage >= blank - kBlankK;
           const unsigned long long start = globaltimer_ns();
-          while (!(stage == blank ? mbar_try_wait(&sm.landed, ph_landed)
-                                  : mbar_try_wait(&sm.full[stage], phase)) &&
+          while (!(late ? mbar_try_wait(&sm.landed, ph_landed)
+                        : mbar_try_wait(&sm.full[stage], phase)) &&
                  globaltimer_ns() - start < kWaitLimitNs) {
           }
         }

@@ -257,3 +257,18 @@ def test_other_sequences_do_not_move_a_bit(ops, dim, dtype, hint, cap):
     got = attend(ops, batch, hint, softcap=cap)
     for x, y in zip(got, clean):
         assert torch.equal(x[:70], y[:70]) and not torch.equal(x[70:], y[70:])
+
+
+@pytest.mark.parametrize("dim,dtype,hint", KINDS)
+@pytest.mark.parametrize("cap", [None, 5.0, 50.0, 500.0])
+@pytest.mark.parametrize("new,ctx", [([70, 30], [60, 75]), ([1, 64, 65, 200], [3, 0, 0, 7])])
+def test_unused_slots_do_not_move_a_bit(ops, dim, dtype, hint, cap, new, ctx):
+    """Whatever the slots behind the sequences' ends hold."""
+    batch = Batch(new, ctx, q_heads=4, kv_heads=2, dim=dim, page=16, dtype=dtype, fill=0.0)
+    clean = attend(ops, batch, hint, softcap=cap)
+    for held in (1000.0, float("inf"), float("nan")):
+        for b, end in enumerate(batch.seq):
+            if end % 16:
+                batch.k_cache[batch.table[b, end // 16], :, end % 16:] = held
+                batch.v_cache[batch.table[b, end // 16], :, end % 16:] = held
+        assert all(torch.equal(x, y) for x, y in zip(attend(ops, batch, hint, softcap=cap), clean))
