@@ -332,6 +332,10 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::PER_SM)
         mma16816<T>(o[2 * c], pa, b[0], b[1]);
         mma16816<T>(o[2 * c + 1], pa, b[2], b[3]);
       }
+      // The stage's next copy comes by the async proxy, which the arrival alone
+      // does not hold behind ldmatrix: without the fence a copy out of L2 could
+      // overtake the last ones and change V under them.
+      fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[stage]);
       if (++stage == STAGES) stage = 0, phase ^= 1;

@@ -272,3 +272,43 @@ def test_unused_slots_do_not_move_a_bit(ops, dim, dtype, hint, cap, new, ctx):
                 batch.k_cache[batch.table[b, end // 16], :, end % 16:] = held
                 batch.v_cache[batch.table[b, end // 16], :, end % 16:] = held
         assert all(torch.equal(x, y) for x, y in zip(attend(ops, batch, hint, softcap=cap), clean))
+
+
+# ---------------------------------------------------------------- the ring
+
+@pytest.mark.parametrize("dim,dtype,page,window", [(128, F16, 64, None), (128, BF16, 64, 500),
+                                                   (128, BF16, 16, None), (64, F16, 64, None)])
+def test_copies_out_of_l2_wait_for_the_last_reads(ops, dim, dtype, page, window):
+    """Many row tiles over the same keys in the decode kernel, whose copies then come out of L2 and
+    follow a stage's release at once: each of 20 calls gives the same, and the right, result."""
+    kv, group = 4, 4
+    g = torch.Generator().manual_seed(11)
+    new = [1 + int(n) for n in torch.randint(0, 300, (30,), generator=g)]
+    new[::2] = [1] * 15
+    seq = [n + int(c) for n, c in zip(new, torch.randint(0, 4000, (30,), generator=g))]
+    pages = [-(-s // page) for s in seq]
+    order = torch.randperm(sum(pages), generator=g).split(pages)
+    table = torch.nn.utils.rnn.pad_sequence([o.to(torch.int32) for o in order], True, -1).to(DEV)
+    make = lambda *shape: torch.randn(*shape, generator=g).to(dtype).to(DEV)
+    kc, vc = (make(sum(pages), kv, page, dim) for _ in range(2))
+    q = make(sum(new), kv * group, dim)
+    starts = torch.tensor([0] + new, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(DEV)
+    lens = torch.tensor(seq, dtype=torch.int32, device=DEV)
+    runs = [ops.paged_attention(q, kc, vc, table, starts, lens, max_query_len=1, window=window,
+                                return_lse=True) for _ in range(20)]
+    for out, lse in runs[1:]:
+        assert torch.equal(out, runs[0][0]) and torch.equal(lse, runs[0][1])
+    want, spread = (torch.empty(q.shape, dtype=torch.float64, device=DEV) for _ in range(2))
+    want_lse = torch.empty(q.shape[:2], dtype=torch.float64, device=DEV)
+    for b, (n, length) in enumerate(zip(new, seq)):
+        k, v = (c[order[b].to(DEV)].transpose(0, 1).flatten(1, 2)[:, :length].double()
+                .repeat_interleave(group, 0) for c in (kc, vc))
+        rows = slice(int(starts[b]), int(starts[b]) + n)
+        x = q[rows].double().transpose(0, 1) @ k.transpose(1, 2) * dim ** -0.5
+        far = (torch.arange(length - n, length, device=DEV)[:, None]
+               - torch.arange(length, device=DEV)[None, :])
+        x = x.masked_fill((far < 0) | (far >= (window or length)), float("-inf"))
+        p = torch.softmax(x, -1)
+        want[rows], spread[rows] = (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1)
+        want_lse[rows] = torch.logsumexp(x, -1).t()
+    check_attention(runs[0][0], runs[0][1], want.cpu(), want_lse.cpu(), spread.cpu(), dtype)
