@@ -16,7 +16,7 @@
 // whichever CTA finishes its part last (a ticket per tile tells), always in the
 // same order.
 //
-// 64 sequences of up to 8191 keys, 32 + 8 heads of 128: 180 us, 5.8 TB/s; all
+// 64 sequences of up to 8191 keys, 32 + 8 heads of 128: 182 us, 5.7 TB/s; all
 // of 8000 and more 6.5 TB/s, the rate of a copy.  What short calls pay is the
 // start (lengths, table, first block) and the joins, 10 us together.
 #include <cfloat>
