@@ -285,7 +285,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::PER_SM)
               *reinterpret_cast<uint4*>(ring + stage * 2 * C::TILE_BYTES + C::TILE_BYTES +
                                         (c / 8) * C::HALF_BYTES + (slice * 16 + r) * 128 +
                                         (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async_shared();  // before the next TMA write of this stage
           __syncwarp();
         }
       }
@@ -333,8 +332,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::PER_SM)
         mma16816<T>(o[2 * c + 1], pa, b[2], b[3]);
       }
       // The stage's next copy comes by the async proxy, which the arrival alone
-      // does not hold behind ldmatrix: without the fence a copy out of L2 could
-      // overtake the last ones and change V under them.
+      // does not hold behind ldmatrix (and the zeros above): without the fence a
+      // copy out of L2 could overtake the last ones and change V under them.
       fence_proxy_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[stage]);

@@ -172,9 +172,9 @@ constexpr float kFarCap = 64.0f;
 // tanh(y) = 1 - 2 / (e^2y + 1) for all of its 64, which leaves small scores off by
 // up to 4e-7 of the cap.  (Each row for itself, though a warp of both kinds then
 // takes both ways, 121 us instead of 107 for two prompts of 2048 tokens: some of
-// its rows may be another sequence's, which shall not move a bit.)  With far caps only the scores beyond take it, one by
-// one (two prompts of 2048 tokens with scores beyond a cap of 100: 142 us instead
-// of 107; none beyond: 89 both ways).
+// its rows may be another sequence's, which shall not move a bit.)  With caps above
+// kFarCap only the scores beyond take it, one by one (two prompts of 2048 tokens
+// with scores beyond a cap of 100: 142 us instead of 107; none beyond: 89 both ways).
 template <int SCORES>
 __device__ __forceinline__ void modify(uint32_t (&s)[2][32], float scale, float softcap,
                                        bool biased, float slope, int ahead) {
