@@ -470,6 +470,67 @@ M5B_API int m5b_paged_attention(const m5b_paged_attention_args* args, void* stre
  * the head dimension and the SM count only. */
 M5B_API int64_t m5b_paged_attention_workspace_bytes(int64_t head_dim);
 
+/* ---- block-scaled and grouped products ------------------------------------
+ * Operands with finer scales than m5b_quantize's one a row, and products whose
+ * rows are grouped by expert.  The reference has neither: its GEMM takes one
+ * scale a row and channel, and one weight (src/m5kernels/metal.py:158-269).
+ *
+ * m5b_block_quantize: E4M3 codes (uint8) with an fp32 scale for each block of
+ * 128 channels (the last one may be shorter) of one row (block_rows 1) or of
+ * 128 rows (block_rows 128):
+ *   v     = x, or silu(gate) * x = gate / (1 + exp(-gate)) * x in fp32
+ *   scale = max|v| / 448 over the block, 1 where that is 0
+ *   code  = E4M3(RN(v / scale)), nearest even, saturating
+ * x, gate: rows of contiguous channels.  row_index (block_rows 1): row r of the
+ * output is that of x[row_index[r]]; an index outside [0, x_rows) gives zeros
+ * (and scales of 1).  q [batch, rows, k] and scales [batch, ceil(rows /
+ * block_rows), ceil(k / 128)] are contiguous; a batch, of weights, needs
+ * block_rows 128.  A block that holds an infinity or NaN gets a scale that is
+ * not finite. */
+typedef struct m5b_block_quantize_args {
+  const void* x;
+  int64_t x_dtype, x_rows, x_row_stride, x_batch_stride;
+  const void* gate; /* NULL: none */
+  int64_t gate_row_stride;
+  const int32_t* row_index; /* [rows], NULL: row r is x's */
+  int64_t rows, k, batch, block_rows;
+  uint8_t* q;
+  float* scales;
+} m5b_block_quantize_args;
+M5B_API int m5b_block_quantize(const m5b_block_quantize_args* args, void* stream);
+
+/* m5b_grouped_gemm: out[t, n] = epilogue(sum_k a[t, k] b[e, n, k]) for the rows
+ * group_start[e] <= t < group_start[e + 1] of each group e < groups (at most
+ * 1024; group_start ascends, read on the device; NULL with groups 1: all rows).
+ * mode INT8 / FP8 / BF16 / FP16 names the operands as in m5b_gemm.
+ *   INT8, FP8:  (acc * a_scales[t]) * b_scales[e, n]; bit-identical to m5b_gemm
+ *               of the group's rows for INT8
+ *   FP8 with block_scales: the sum over the blocks kb of 128 channels of K of
+ *               their products times (a_scales[t, kb] * b_scales[e, n / 128, kb]),
+ *               each product of two scales rounded to fp32 (which has to hold it)
+ * all accumulated in FP32 (INT8: INT32).  Scale strides are in elements:
+ * a_scale_row_stride between rows, a_scale_block_stride between blocks of K;
+ * b_scale_group_stride between groups, b_scale_row_stride between channels
+ * (block_scales: blocks of 128 channels), b_scale_block_stride between blocks
+ * of K.  Rows of a and b have contiguous channels and start on 16-byte
+ * boundaries.  Rows outside every group keep what out holds, or with zero_rest
+ * become zero.  No workspace. */
+typedef struct m5b_grouped_gemm_args {
+  const void* a;
+  const void* b;
+  int64_t mode, rows, groups, n, k;
+  int64_t a_row_stride, b_group_stride, b_row_stride;
+  const int32_t* group_start;
+  int64_t block_scales;
+  const float* a_scales;
+  const float* b_scales;
+  int64_t a_scale_row_stride, a_scale_block_stride;
+  int64_t b_scale_group_stride, b_scale_row_stride, b_scale_block_stride;
+  void* out;
+  int64_t out_dtype, out_row_stride, zero_rest;
+} m5b_grouped_gemm_args;
+M5B_API int m5b_grouped_gemm(const m5b_grouped_gemm_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

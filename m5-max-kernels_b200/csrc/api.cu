@@ -231,15 +231,27 @@ int m5b::set_last_error(int code, const char* msg) { return fail(code, "%s", msg
 
 int m5b::current_device_state(unsigned int** status, int* sms) { return device_state(status, sms); }
 
-bool m5b::make_swizzled_map16(CUtensorMap* map, bool f16, int rank, const void* ptr,
-                              const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+static bool swizzled_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* ptr,
+                         const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
   if (get_encode()) return false;
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  return g_encode(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                  static_cast<cuuint32_t>(rank), const_cast<void*>(ptr), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  return g_encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(ptr), dims, strides,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool m5b::make_swizzled_map16(CUtensorMap* map, bool f16, int rank, const void* ptr,
+                              const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  return swizzled_map(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                      rank, ptr, dims, strides, box);
+}
+
+bool m5b::make_swizzled_map(CUtensorMap* map, int elem_bytes, int rank, const void* ptr,
+                            const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
+  return swizzled_map(map, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                           : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                      rank, ptr, dims, strides, box);
 }
 
 extern "C" {

@@ -1,0 +1,185 @@
+// C-ABI entry points of the block-scaled and grouped products (declared in
+// include/m5b200.h): contract checks, tile and schedule choice, launches.
+// Nothing here allocates or synchronizes, and nothing throws.
+#include <climits>
+#include <cstdio>
+
+#include "grouped.cuh"
+#include "m5b200.h"
+
+using namespace m5b;
+
+namespace {
+
+int einval(const char* msg) { return set_last_error(M5B_EINVAL, msg); }
+int eunsupported(const char* msg) { return set_last_error(M5B_EUNSUPPORTED, msg); }
+
+int launched(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return set_last_error(M5B_OK, "");
+  char msg[256];
+  snprintf(msg, sizeof(msg), "%s: %s", what, cudaGetErrorString(e));
+  return set_last_error(M5B_ECUDA, msg);
+}
+
+bool float_dtype(int64_t dt) { return dt == M5B_F32 || dt == M5B_F16 || dt == M5B_BF16; }
+int64_t dtype_bytes(int64_t dt) { return dt == M5B_F32 ? 4 : 2; }
+bool grid16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Strides of a tensor map are below 2^40 bytes.
+bool map_stride(int64_t bytes) { return bytes > 0 && bytes < (int64_t(1) << 40) && bytes % 16 == 0; }
+
+struct Plan {
+  bool pair;
+  int tile_rows, splits, grid;
+};
+
+// Tiles and schedule.  Groups of few rows are bound by their weights: 64-row
+// tiles on single CTAs, several of which share a tile's K range where the tiles
+// do not fill the GPU.  Others take 256 channels x up to 256 rows on CTA pairs.
+Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int sms) {
+  Plan p{};
+  const int64_t busy = groups < rows ? groups : rows;  // groups with rows, at most
+  const int64_t each = ceil_div(rows, groups);
+  p.pair = each > kSingleTileRows;
+  p.splits = 1;
+  p.tile_rows = p.pair ? kPairTileRows : kSingleTileRows;
+  const int64_t ch_tiles = ceil_div(n, p.pair ? 256 : 128);
+  // (every group rounds its last tile up)
+  int64_t tiles = (rows / p.tile_rows + busy) * ch_tiles;
+  if (groups == 1) tiles = ceil_div(rows, p.tile_rows) * ch_tiles;
+  const int64_t units = p.pair ? sms / 2 : sms;
+  if (!p.pair)
+    while (p.splits < 8 && tiles * p.splits * 2 <= units && nkb >= p.splits * 2 * 4) p.splits *= 2;
+  const int64_t used = tiles < units ? tiles : units;
+  p.grid = static_cast<int>(used) * (p.pair ? 2 : p.splits);
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int m5b_block_quantize(const m5b_block_quantize_args* s, void* stream) {
+  if (!s) return einval("arguments are NULL");
+  if (!float_dtype(s->x_dtype)) return einval("input dtype must be float16, bfloat16 or float32");
+  if (s->block_rows != 1 && s->block_rows != 128) return einval("block_rows must be 1 or 128");
+  if (s->rows < 0 || s->k < 1 || s->batch < 1 || s->x_rows < 0)
+    return einval("rows, k and batch must be positive");
+  if (s->block_rows == 1 && s->batch != 1) return einval("a batch needs block_rows 128");
+  if (s->block_rows != 1 && (s->gate || s->row_index))
+    return einval("gate and row_index need block_rows 1");
+  if (!s->row_index && s->rows != s->x_rows) return einval("rows must be x's without row_index");
+  // (rows of blocks are counted in 32 bits, and rounded up to whole CTAs)
+  const int64_t most = INT_MAX - (1 << 20);
+  if (s->rows > most || s->x_rows > most || s->k > most || s->batch > most ||
+      ceil_div(s->rows, s->block_rows) * ceil_div(s->k, 128) > most / s->batch)
+    return eunsupported("rows x k exceed the index range");
+  if (s->rows == 0) return set_last_error(M5B_OK, "");
+  if (!s->q || !s->scales || (!s->x && s->x_rows > 0)) return einval("x, q and scales are required");
+  BlockQuantArgs a{};
+  a.x = s->x;
+  a.gate = s->gate;
+  a.index = s->row_index;
+  a.x_row = s->x_row_stride;
+  a.gate_row = s->gate_row_stride;
+  a.x_batch = s->x_batch_stride;
+  a.rows = s->rows;
+  a.x_rows = s->x_rows;
+  a.k = s->k;
+  a.batch = s->batch;
+  a.q = s->q;
+  a.scales = s->scales;
+  const int64_t size = dtype_bytes(s->x_dtype);
+  a.vec = s->k % 8 == 0 && grid16(s->x) && grid16(s->gate) && (s->x_row_stride * size) % 16 == 0 &&
+          (s->gate_row_stride * size) % 16 == 0 && (s->x_batch_stride * size) % 16 == 0 &&
+          reinterpret_cast<uintptr_t>(s->q) % 8 == 0;
+  int rc = current_device_state(nullptr, &a.sms);
+  if (rc) return rc;
+  return launched(launch_block_quantize(a, static_cast<int>(s->x_dtype), s->block_rows == 128,
+                                        static_cast<cudaStream_t>(stream)),
+                  "block quantize launch");
+}
+
+int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
+  if (!s) return einval("arguments are NULL");
+  int kind = 0;
+  int64_t elem = 1;
+  bool quantized = true;
+  switch (s->mode) {
+    case M5B_MODE_INT8: kind = KIND_I8; break;
+    case M5B_MODE_FP8: kind = KIND_F8; break;
+    case M5B_MODE_BF16: kind = KIND_BF16, elem = 2, quantized = false; break;
+    case M5B_MODE_FP16: kind = KIND_F16, elem = 2, quantized = false; break;
+    case M5B_MODE_FP32: return eunsupported("fp32 operands are not supported by the grouped GEMM");
+    default: return einval("unknown GEMM mode");
+  }
+  if (s->rows < 0 || s->groups < 1 || s->n < 1 || s->k < 1)
+    return einval("rows, groups, n and k must be positive");
+  if (!s->group_start && s->groups != 1) return einval("group_start is required");
+  if (s->block_scales && s->mode != M5B_MODE_FP8) return einval("block scales need FP8 operands");
+  if (!float_dtype(s->out_dtype))
+    return eunsupported("output dtype must be bfloat16, float16 or float32");
+  if (s->groups > kMaxGroups) return eunsupported("more than 1024 groups are unsupported");
+  if (kind == KIND_I8 && s->k > 133144)
+    return eunsupported("INT32 worst-case overflow bound exceeded");
+  // (rows and channels are rounded up to whole tiles, and tiles counted in 32 bits)
+  const int64_t most = INT_MAX - 4096;
+  if (s->rows > most || s->n > most || s->k > most ||
+      (s->rows / 64 + s->groups) * ceil_div(s->n, 128) > most)
+    return eunsupported("rows x channels exceed the index range");
+  if (s->rows == 0) return set_last_error(M5B_OK, "");
+  if (!s->a || !s->b || !s->out) return einval("a, b and out are required");
+  if (quantized && (!s->a_scales || !s->b_scales)) return einval("scales required");
+  const int64_t row_bytes = ceil_div(s->k * elem, 16) * 16;
+  const int64_t a_row = s->rows > 1 ? s->a_row_stride * elem : row_bytes;
+  const int64_t b_row = s->n > 1 ? s->b_row_stride * elem : row_bytes;
+  const int64_t b_group = s->groups > 1 ? s->b_group_stride * elem : row_bytes;
+  if (!grid16(s->a) || !grid16(s->b) || !map_stride(a_row) || !map_stride(b_row) ||
+      !map_stride(b_group))
+    return eunsupported("operand rows must start on 16-byte boundaries for TMA");
+
+  GroupedArgs g{};
+  g.rows = static_cast<int>(s->rows);
+  g.groups = static_cast<int>(s->groups);
+  g.n = static_cast<int>(s->n);
+  g.num_k_blocks = static_cast<int>(ceil_div(s->k * elem, 128));
+  g.group_start = s->group_start;
+  g.a_scales = s->a_scales;
+  g.b_scales = s->b_scales;
+  g.as_row = s->a_scale_row_stride;
+  g.as_k = s->a_scale_block_stride;
+  g.bs_group = s->b_scale_group_stride;
+  g.bs_n = s->b_scale_row_stride;
+  g.bs_k = s->b_scale_block_stride;
+  g.out = s->out;
+  g.out_row = s->out_row_stride;
+  g.out_dtype = static_cast<int>(s->out_dtype);
+  g.out_vec = s->n % 8 == 0 && s->out_row_stride % 8 == 0 && grid16(s->out);
+  g.zero_rest = s->zero_rest ? 1 : 0;
+  int sms = 0;
+  int rc = current_device_state(&g.status, &sms);
+  if (rc) return rc;
+  const Plan p = plan_for(s->rows, s->groups, s->n, g.num_k_blocks, sms);
+  g.tile_rows = p.tile_rows;
+  g.k_splits = p.splits;
+
+  GroupedMaps m;
+  const uint64_t a_dims[2] = {uint64_t(s->k), uint64_t(s->rows)};
+  const uint64_t a_strides[1] = {uint64_t(a_row)};
+  const uint64_t b_dims[3] = {uint64_t(s->k), uint64_t(s->n), uint64_t(s->groups)};
+  const uint64_t b_strides[2] = {uint64_t(b_row), uint64_t(b_group)};
+  const uint32_t wide = static_cast<uint32_t>(128 / elem);
+  const uint32_t box128[3] = {wide, 128, 1}, box64[2] = {wide, 64}, box16[2] = {wide, 16};
+  const int bytes = static_cast<int>(elem);
+  if (!make_swizzled_map(&m.a128, bytes, 2, s->a, a_dims, a_strides, box128) ||
+      !make_swizzled_map(&m.a64, bytes, 2, s->a, a_dims, a_strides, box64) ||
+      !make_swizzled_map(&m.a16, bytes, 2, s->a, a_dims, a_strides, box16) ||
+      !make_swizzled_map(&m.b, bytes, 3, s->b, b_dims, b_strides, box128))
+    return set_last_error(M5B_ECUDA, "cuTensorMapEncodeTiled failed");
+  return launched(launch_grouped_gemm(m, g, kind, s->block_scales != 0, p.pair, p.grid,
+                                      static_cast<cudaStream_t>(stream)),
+                  "grouped GEMM launch");
+}
+
+}  // extern "C"

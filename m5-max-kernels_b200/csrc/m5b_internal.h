@@ -102,6 +102,9 @@ int current_device_state(unsigned int** status, int* sms);
 // driver refuses it (api.cu).
 bool make_swizzled_map16(CUtensorMap* map, bool f16, int rank, const void* ptr,
                          const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
+// The same of 1- or 2-byte elements that are moved as they are.
+bool make_swizzled_map(CUtensorMap* map, int elem_bytes, int rank, const void* ptr,
+                       const uint64_t* dims, const uint64_t* strides, const uint32_t* box);
 
 int row_prep_warps(int64_t K, int block);
 bool quant_rows_applicable(const RowPrepArgs& a, int x_dtype, int block, int out);

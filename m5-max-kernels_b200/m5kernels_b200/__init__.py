@@ -13,11 +13,14 @@ The `cuda-b200` backend of the m5kernels operator contracts:
     linear, OnlineProjection           (the online quantize -> gemm stage in one call / bound step)
     paged_append, paged_attention      (what follows the Q/K/V projection: a paged cache and
                                         attention of new tokens over it)
+    block_quantize, block_gemm         (E4M3 with a scale for each block of 128 channels)
+    grouped_gemm                       (products whose rows are grouped by expert)
 All of them run hand-written CUDA kernels from libm5b200.so through its C ABI
 (include/m5b200.h); there is no CPU fallback.
 """
 
 from .cuda import gemm, gemm_allgather, gemm_schedule, quantize
+from .grouped import block_gemm, block_quantize, grouped_gemm
 from .hadamard import SUPPORTED_BLOCK_SIZES, hadamard_quantize, rotate
 from .linear import OnlineProjection, linear
 from .norm_hadamard import (fused_gated_residual_norm_hadamard_quantize,
@@ -32,5 +35,6 @@ __all__ = [
     "fused_norm_hadamard_quantize", "fused_gated_residual_norm_hadamard_quantize",
     "projection_qk_rope", "rope_tables", "linear", "rms_quantize", "gated_residual_add",
     "unfused_norm", "qk_norm_rope", "projection_qkv_rope", "grouped_qkv_weights",
-    "OnlineProjection", "paged_append", "paged_attention",
+    "OnlineProjection", "paged_append", "paged_attention", "block_quantize", "block_gemm",
+    "grouped_gemm",
 ]

@@ -63,6 +63,8 @@ _SIGNATURES = {
     "m5b_paged_append": ([P, P], I),
     "m5b_paged_attention": ([P, P], I),
     "m5b_paged_attention_workspace_bytes": ([I64], I64),
+    "m5b_block_quantize": ([P, P], I),
+    "m5b_grouped_gemm": ([P, P], I),
 }
 
 

@@ -1,0 +1,235 @@
+"""Block-scaled E4M3 products, and products whose rows are grouped by expert.
+
+`block_quantize` makes E4M3 codes (uint8, as `quantize` does) with one fp32
+scale for each block of 128 channels of a row (activations) or of 128 rows
+(weights); `block_gemm` multiplies such operands.  `grouped_gemm` multiplies
+each group of rows by its own weight, for operands of either kind of scales and
+for unquantized ones.  An expert layer is
+
+    codes, scales = block_quantize(x, rows=order)           # rows in the order of their experts
+    h = grouped_gemm(codes, w_up, group_start, "fp8", a_scales=scales, b_scales=w_up_scales,
+                     output_dtype=torch.bfloat16)           # [T, up and gate]
+    codes, scales = block_quantize(h[:, :d], gate=h[:, d:])
+    y = grouped_gemm(codes, w_down, group_start, "fp8", ...)
+
+The group's bounds are read on the device: nothing here waits for the GPU, and
+a captured CUDA graph may be replayed after they changed.  The reference's GEMM
+takes one weight and one scale a row and channel
+(src/m5kernels/metal.py:158-269); these operators have no twin there.
+"""
+
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from . import _lib
+from ._lib import check
+from .paged import _call, _device, _ints
+
+_Tensor = torch.Tensor
+BLOCK = 128
+_FLOAT = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_OPERAND = {"int8": torch.int8, "fp8": torch.uint8, "bf16": torch.bfloat16,
+            "fp16": torch.float16}
+_MOST_GROUPS = 1024
+# m5b_block_quantize_args and m5b_grouped_gemm_args (include/m5b200.h): every field is 8 bytes
+_PACK_QUANTIZE = struct.Struct("@14q")
+_PACK_GEMM = struct.Struct("@23q")
+
+
+def _channels(t):
+    """t with contiguous channels."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _operand(t):
+    """t with rows that TMA can read: contiguous channels, rows on the 16-byte grid."""
+    size, strides = t.element_size(), t.stride()
+    if strides[-1] == 1 and t.data_ptr() % 16 == 0:
+        for n, s in zip(t.shape[:-1], strides[:-1]):
+            if n > 1 and (s <= 0 or s * size % 16):
+                break
+        else:
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _row_index(rows):
+    if not isinstance(rows, _Tensor) or rows.dtype is not torch.int32 or rows.dim() != 1:
+        raise ValueError("rows must be an int32 vector")
+    return rows.contiguous()
+
+
+def block_quantize(x, *, gate=None, rows=None, block_rows=1):
+    """E4M3 codes with a scale for each block of 128 channels -> (codes uint8, scales fp32).
+
+    scale = max|v| / 448 over the block (1 where that is 0), codes =
+    E4M3(v / scale), nearest even, saturating, the quotient in fp32; the last
+    block of a row may be shorter.
+
+    block_rows 1 (activations): x [T, K] -> codes [T, K], scales [T, ceil(K / 128)].
+    v = x, or with `gate` [T, K] v = silu(gate) * x in fp32 (the step between
+    the products of a gated FFN).  With `rows` int32 [R], row r is x[rows[r]]:
+    codes [R, K]; indices outside x give rows of zeros.
+    block_rows 128 (weights): x [N, K] or [E, N, K]; one scale for 128 rows x
+    128 channels, scales [..., ceil(N / 128), ceil(K / 128)].
+
+    x and gate: float16, bfloat16 or float32; views with contiguous channels
+    are read in place.  A block that holds an infinity or NaN gets a scale that
+    is not finite.
+    """
+    if not isinstance(x, _Tensor) or x.dtype not in _FLOAT:
+        raise ValueError("input dtype must be float16, bfloat16 or float32")
+    if block_rows not in (1, BLOCK) or isinstance(block_rows, bool):
+        raise ValueError("block_rows must be 1 or 128")
+    if block_rows == 1:
+        if x.dim() != 2 or x.shape[1] == 0:
+            raise ValueError("input must have shape [rows, K]")
+    else:
+        if x.dim() not in (2, 3) or 0 in x.shape:
+            raise ValueError("weights must have nonempty shape [N, K] or [E, N, K]")
+        if gate is not None or rows is not None:
+            raise ValueError("gate and rows need block_rows 1")
+    x = _channels(x)
+    used = [x]
+    gate_ptr = gate_row = index_ptr = 0
+    if gate is not None:
+        if not isinstance(gate, _Tensor) or gate.shape != x.shape or gate.dtype is not x.dtype:
+            raise ValueError("gate must have x's shape and dtype")
+        gate = _channels(gate)
+        gate_ptr, gate_row = gate.data_ptr(), gate.stride(0)
+        used.append(gate)
+    batch = x.shape[0] if x.dim() == 3 else 1
+    out_rows, k = x.shape[-2], x.shape[-1]
+    if rows is not None:
+        rows = _row_index(rows)
+        index_ptr, out_rows = rows.data_ptr(), rows.shape[0]
+        used.append(rows)
+    index = _device(used)
+    lead = (*x.shape[:-2],)
+    codes = torch.empty((*lead, out_rows, k), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*lead, -(-out_rows // block_rows), -(-k // BLOCK)), dtype=torch.float32,
+                         device=x.device)
+    if out_rows > 0:
+        _call(_lib.lib().m5b_block_quantize, _PACK_QUANTIZE.pack(
+            x.data_ptr(), _FLOAT[x.dtype], x.shape[-2], x.stride(-2),
+            x.stride(0) if batch > 1 else 0, gate_ptr, gate_row, index_ptr, out_rows, k, batch,
+            block_rows, codes.data_ptr(), scales.data_ptr()), index)
+    return codes, scales
+
+
+def _product(a, b, group_start, mode, a_scales, b_scales, output_dtype, out):
+    """Both products: b [groups, N, K]; group_start None: all rows are group 0's."""
+    groups, n, k = b.shape
+    rows = a.shape[0]
+    expected = _OPERAND[mode]
+    if a.dtype is not expected or b.dtype is not expected:
+        raise ValueError("operand dtypes must match the declared mode")
+    if k * a.element_size() % 16:
+        raise NotImplementedError(f"K*{a.element_size()} bytes per row must be a multiple of 16 "
+                                  "for TMA; padding is not implicit")
+    used = [a, b]
+    scale_fields = [0] * 7
+    blocks = False
+    if mode in ("int8", "fp8"):
+        if (not isinstance(a_scales, _Tensor) or not isinstance(b_scales, _Tensor)
+                or a_scales.dtype is not torch.float32 or b_scales.dtype is not torch.float32):
+            raise ValueError("float32 scales required")
+        kb = -(-k // BLOCK)
+        sa, sb = a_scales.stride(), b_scales.stride()
+        if a_scales.shape == (rows,) and b_scales.shape == (groups, n):
+            scale_fields = [a_scales.data_ptr(), b_scales.data_ptr(), sa[0], 0, sb[0], sb[1], 0]
+        elif (mode == "fp8" and a_scales.shape == (rows, kb)
+                and b_scales.shape == (groups, -(-n // BLOCK), kb)):
+            blocks = True
+            scale_fields = [a_scales.data_ptr(), b_scales.data_ptr(), *sa, *sb]
+        else:
+            raise ValueError("scales must be those of rows and channels, or (fp8) of blocks of "
+                             "128 channels of K")
+        used += (a_scales, b_scales)
+    elif a_scales is not None or b_scales is not None:
+        raise ValueError("scales belong to int8 and fp8 operands")
+    zero_rest = out is None
+    if out is None:
+        out_dtype = output_dtype or torch.float32
+    else:
+        if (not isinstance(out, _Tensor) or out.shape != (rows, n)
+                or (n > 1 and out.stride(1) != 1)):
+            raise ValueError("out must have shape [rows, N] and contiguous channels")
+        out_dtype = out.dtype
+        if output_dtype is not None and output_dtype is not out_dtype:
+            raise ValueError("output_dtype must be out's")
+        used.append(out)
+    if out_dtype not in _FLOAT:
+        raise NotImplementedError("output dtype must be bfloat16, float16 or float32")
+    start_ptr = 0
+    if group_start is not None:
+        start_ptr = group_start.data_ptr()
+        used.append(group_start)
+    index = _device(used)
+    if out is None:
+        out = torch.empty((rows, n), dtype=out_dtype, device=a.device)
+    if rows > 0:
+        a, b = _operand(a), _operand(b)
+        _call(_lib.lib().m5b_grouped_gemm, _PACK_GEMM.pack(
+            a.data_ptr(), b.data_ptr(), _lib.MODE[mode], rows, groups, n, k, a.stride(0),
+            b.stride(0), b.stride(1), start_ptr, blocks, *scale_fields, out.data_ptr(),
+            _FLOAT[out_dtype], out.stride(0), zero_rest), index)
+    return out
+
+
+def block_gemm(a, b, a_scales, b_scales, *, output_dtype=None, out=None):
+    """Block-scaled E4M3 product a[M, K] @ b[N, K].T -> [M, N].
+
+        out[m, n] = sum over blocks g of 128 channels of K of
+                    (a_scales[m, g] * b_scales[n // 128, g]) * sum_{k in g} a[m, k] b[n, k]
+
+    a, b: E4M3 codes (uint8), a_scales fp32 [M, ceil(K / 128)], b_scales fp32
+    [ceil(N / 128), ceil(K / 128)], as `block_quantize` makes them (block_rows
+    1 and 128); views of any strides are fine.  Sums and scales in fp32; the
+    product of two scales has to be in fp32's range.  K a multiple of 16.
+    output_dtype: float32 unless given; `out` may be given, with contiguous
+    channels.
+    """
+    if (not isinstance(a, _Tensor) or not isinstance(b, _Tensor) or a.dim() != 2 or b.dim() != 2
+            or a.shape[1] != b.shape[1] or 0 in b.shape):
+        raise ValueError("A and B must be matrices [M, K] and [N, K]")
+    if (not isinstance(a_scales, _Tensor) or not isinstance(b_scales, _Tensor)
+            or a_scales.dim() != 2 or b_scales.dim() != 2):
+        raise ValueError("scales must be those of blocks of 128 channels of K")
+    return _product(a, b[None], None, "fp8", a_scales, b_scales[None], output_dtype, out)
+
+
+def grouped_gemm(a, b, group_start, mode="bf16", *, a_scales=None, b_scales=None,
+                 output_dtype=None, out=None):
+    """Rows grouped by expert: out[t] = a[t] @ b[e].T for group_start[e] <= t < group_start[e + 1].
+
+    a [T, K], b [E, N, K] (E up to 1024), group_start int32 [E + 1], ascending,
+    read on the device; groups may be empty.  mode: "bf16", "fp16", "int8" or
+    "fp8" (uint8 E4M3 codes), operands as in `gemm`.  Scales of int8 and fp8:
+    a_scales [T] and b_scales [E, N], v = (acc * a_scales[t]) * b_scales[e, n];
+    or for fp8 those of `block_gemm`, a_scales [T, ceil(K / 128)] and b_scales
+    [E, ceil(N / 128), ceil(K / 128)].  INT32 (int8) or FP32 accumulation.
+    K times the element size a multiple of 16.
+
+    Rows outside every group are zero; where `out` is given (contiguous
+    channels, output_dtype its own) they keep what it holds.  output_dtype:
+    float32 unless given.
+    """
+    if mode not in _OPERAND:
+        if mode in ("fp32", "mxint8"):
+            raise NotImplementedError(f"{mode} operands are not supported by the grouped GEMM")
+        raise ValueError(f"unknown GEMM mode {mode!r}")
+    if (not isinstance(a, _Tensor) or not isinstance(b, _Tensor) or a.dim() != 2 or b.dim() != 3
+            or a.shape[1] != b.shape[2] or 0 in b.shape):
+        raise ValueError("A and B must have shapes [T, K] and [E, N, K]")
+    group_start = _ints(group_start, "group_start")
+    if group_start.shape != (b.shape[0] + 1,):
+        raise ValueError("group_start must be a vector [E + 1]")
+    if b.shape[0] > _MOST_GROUPS:
+        raise NotImplementedError("more than 1024 groups are unsupported")
+    if mode == "int8" and a.shape[1] > 133144:
+        raise NotImplementedError("INT32 worst-case overflow bound exceeded")
+    return _product(a, b, group_start, mode, a_scales, b_scales, output_dtype, out)
