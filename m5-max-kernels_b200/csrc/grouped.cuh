@@ -26,7 +26,7 @@ struct GroupedArgs {
   void* out;
   int64_t out_row;             // elements between the output's rows
   int out_dtype;               // DT_BF16 / DT_F16 / DT_F32
-  int out_vec;                 // 16-bit output: 8 channels go in one aligned 16-byte store
+  int out_vec;                 // the output's rows are whole aligned 16-byte pieces
   int zero_rest;               // rows outside every group are set to zero
   unsigned int* status;
 };

@@ -155,7 +155,8 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
   g.out = s->out;
   g.out_row = s->out_row_stride;
   g.out_dtype = static_cast<int>(s->out_dtype);
-  g.out_vec = s->n % 8 == 0 && s->out_row_stride % 8 == 0 && grid16(s->out);
+  const int64_t piece = 16 / dtype_bytes(s->out_dtype);
+  g.out_vec = s->n % piece == 0 && s->out_row_stride % piece == 0 && grid16(s->out);
   g.zero_rest = s->zero_rest ? 1 : 0;
   int sms = 0;
   int rc = current_device_state(&g.status, &sms);

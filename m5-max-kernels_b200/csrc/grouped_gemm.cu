@@ -17,60 +17,52 @@
 // while the MMAs of the next block fill another TMEM buffer.  Without block
 // scales a tile's whole K range stays in TMEM.
 //
-// Roles: warps 0-7 epilogue, warp 8 TMA producer, warp 9 MMA issuer, 10 and 11
-// none (registers move between whole warpgroups).  TMEM is
-// read in 16 x 256-bit fragments: a thread holds pairs of neighbouring rows
-// (columns of the accumulator) of four channels, so that one scale pair serves
-// four packed multiply-adds, and stmatrix turns a fragment into rows of 32
-// channels for 16-byte stores.
+// Roles: warps 0-7 epilogue, warp 8 TMA producer, warp 9 MMA issuer, warps 10 and
+// 11 bring the block scales (products sa * sb, in shared memory).  TMEM is
+// read by whole lanes: a thread holds one channel of 32 rows (columns of the
+// accumulator).  That goes at 840 bytes a clock and SM, where 16 x 256-bit
+// fragments, which would need fewer scales a thread, came at 253, as long as
+// the MMAs of a block take.
 //
 // K split over a cluster (single CTAs, one tile a cluster): each CTA sums its
 // part of K; the sums of eight rows go to the CTA that owns them through
 // distributed shared memory, which adds the parts in the order of the ranks.
+#include <type_traits>
+
 #include "grouped.cuh"
 
 namespace m5b {
 
 namespace {
 
-template <bool PAIR>
+template <bool BLOCKS, bool PAIR>
 struct Cfg {
-  static constexpr int TN = PAIR ? kPairTileRows : kSingleTileRows;
+  static constexpr bool ROWS_M = BLOCKS && PAIR;           // the rows are the M operand
+  static constexpr int TN = PAIR ? 256 : kSingleTileRows;  // columns of an accumulator
   static constexpr int TM = PAIR ? 256 : 128;              // channels of a tile
-  static constexpr int W_BYTES = 128 * 128;                // this CTA's weights of a stage
-  static constexpr int X_BYTES = (PAIR ? TN / 2 : TN) * 128;  // this CTA's rows of a stage
+  static constexpr int STEP = PAIR ? 32 : 16;              // columns come in these
+  static constexpr int M_BYTES = 128 * 128;                // this CTA's M operand of a stage
+  static constexpr int N_BYTES = (PAIR ? TN / 2 : TN) * 128;  // and its N operand
   static constexpr int STAGES = PAIR ? 6 : 7;
   static constexpr int BUFS = 512 / TN;                    // TMEM accumulators
-  static constexpr int CHUNKS = TN / 64;                   // 32-row chunks of an epilogue warp
+  static constexpr int CHUNKS = TN / 64;                   // 32-column chunks of an epilogue warp
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 32 * (EPI_WARPS + 4);     // three warpgroups
-  static constexpr int SCALE_SLOTS = 2;                    // of four blocks each
-  static constexpr int SCALE_BYTES = SCALE_SLOTS * 4 * TN * 4;
-  static constexpr int STORE_BYTES = EPI_WARPS * 2 * 512;
+  static constexpr int SCALE_SLOTS = 2;                    // of four blocks of K each
+  static constexpr int SCALE_BYTES = BLOCKS ? SCALE_SLOTS * 4 * TN * 4 : 0;
+  static constexpr int STORE_WARP = ROWS_M ? 2048 : 1024;  // a warp's bytes to rearrange stores
+  static constexpr int STORE_BYTES = EPI_WARPS * STORE_WARP;
   static constexpr int EXCHANGE_BYTES = PAIR ? 0 : TN * 128 * 4;
   static constexpr int TABLE_BYTES = 2 * (kMaxGroups + 4) * 4;
-  static constexpr int BAR_BYTES = (2 * STAGES + 2 * BUFS + SCALE_SLOTS + 2) * 8 + 16;
-  static constexpr int SMEM_BYTES = 1024 + STAGES * (W_BYTES + X_BYTES) + EXCHANGE_BYTES +
+  static constexpr int BAR_BYTES = (2 * STAGES + 2 * BUFS + 2 * SCALE_SLOTS + 2) * 8 + 16;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * (M_BYTES + N_BYTES) + EXCHANGE_BYTES +
                                     SCALE_BYTES + STORE_BYTES + TABLE_BYTES + BAR_BYTES;
   static_assert(SMEM_BYTES <= 232448, "shared memory per CTA exceeds 227 KB");
 };
 
-// Four 8-column groups of 16 TMEM lanes: thread t receives, for group i,
-// r[4i], r[4i + 1]: lane t / 4, columns 8i + 2 (t % 4), + 1; r[4i + 2],
-// r[4i + 3]: the same columns of lane t / 4 + 8.
-__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
-// Waits for this thread's TMEM loads; the 32 registers are named so that no use
-// of them moves above the wait.
-__device__ __forceinline__ void tmem_wait_frag(uint32_t* r) {
+// Waits for this thread's TMEM load; its registers are named so that no use of
+// them moves above the wait.
+__device__ __forceinline__ void tmem_wait32(uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
                  "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
@@ -81,11 +73,23 @@ __device__ __forceinline__ void tmem_wait_frag(uint32_t* r) {
                :
                : "memory");
 }
-__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b,
-                                                  uint32_t c, uint32_t d) {
-  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
-                   addr),
-               "r"(a), "r"(b), "r"(c), "r"(d)
+// The same in 16 columns.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
                : "memory");
 }
 // As tma_load_2d_pair, of a 3D box.
@@ -98,11 +102,49 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
       "r"(z)
       : "memory");
 }
+// Arrival on a barrier of another CTA that hands over TMEM only (the tcgen05 fence
+// before it orders that): a release over the cluster would wait for every load
+// that the thread has under way, 2.1 us a block of 128 channels instead of 0.35.
+__device__ __forceinline__ void mbar_arrive_tmem(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
                                               uint32_t d) {
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
                "r"(c), "r"(d)
                : "memory");
+}
+// mbar_wait_bounded with few registers (the epilogue has none to spare): 32 bits of
+// the clock, 4.3 s.
+__device__ __forceinline__ uint32_t globaltimer_lo() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %globaltimer_lo;" : "=r"(t));
+  return t;
+}
+__device__ __forceinline__ bool mbar_wait_lean(uint32_t bar, uint32_t parity, uint32_t abort,
+                                               unsigned int* status, unsigned int code) {
+  uint32_t start = 0;
+  bool first = true;
+  while (true) {
+    uint32_t ok, stop;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (first) start = globaltimer_lo();
+    first = false;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(stop) : "r"(abort) : "memory");
+    if (stop) return false;
+    if (globaltimer_lo() - start > static_cast<uint32_t>(kWaitLimitNs)) {
+      atomicOr(status, code);
+      asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort), "r"(1) : "memory");
+      return false;
+    }
+  }
 }
 // As mbar_wait_bounded, for data that other CTAs of the cluster stored.
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity,
@@ -141,7 +183,7 @@ struct Tile {
 // Walks the tiles unit, unit + stride, ...; every role of a CTA (and both CTAs of
 // a pair) sees the same ones.  first_row[e]: the first row of group e, clamped
 // to the rows there are; first_tile[e]: the tiles of the groups before e.
-template <bool PAIR>
+template <class C>
 struct Walk {
   const int* first_row;
   const int* first_tile;
@@ -149,7 +191,6 @@ struct Walk {
   int unit, stride, e;
 
   __device__ __forceinline__ bool next(Tile& t) {
-    using C = Cfg<PAIR>;
     if (unit >= first_tile[groups]) return false;
     while (unit >= first_tile[e + 1]) ++e;
     const int rows = first_row[e + 1] - first_row[e];  // positive: the group has tiles
@@ -163,14 +204,13 @@ struct Walk {
     const int wide = left < 16 ? left : 16;
     const int ch = in_band / wide;
     const int r = 16 * band + in_band - ch * wide;
-    constexpr int STEP = PAIR ? 32 : 16;
-    const int each = ((rows + row_tiles - 1) / row_tiles + STEP - 1) / STEP * STEP;
+    const int each = ((rows + row_tiles - 1) / row_tiles + C::STEP - 1) / C::STEP * C::STEP;
     t.group = e;
     t.row0 = first_row[e] + r * each;
     // (positive too: tile_rows is a multiple of STEP, so each <= tile_rows and
     // (row_tiles - 1) * each <= (row_tiles - 1) * tile_rows < rows)
     t.rows = rows - r * each < each ? rows - r * each : each;
-    t.cols = (t.rows + STEP - 1) / STEP * STEP;
+    t.cols = (t.rows + C::STEP - 1) / C::STEP * C::STEP;
     t.ch0 = ch * C::TM;
     unit += stride;
     return true;
@@ -178,79 +218,107 @@ struct Walk {
 };
 
 template <int KIND>
-__device__ __forceinline__ float2 frag_value(uint32_t a, uint32_t b) {
+__device__ __forceinline__ float sum_value(uint32_t a) {
   if constexpr (KIND == KIND_I8)
-    return make_float2(__int2float_rn(static_cast<int>(a)), __int2float_rn(static_cast<int>(b)));
+    return __int2float_rn(static_cast<int>(a));
   else
-    return make_float2(__uint_as_float(a), __uint_as_float(b));
+    return __uint_as_float(a);
 }
 template <int KIND>
-__device__ __forceinline__ uint32_t frag_add(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t sum_add(uint32_t a, uint32_t b) {
   if constexpr (KIND == KIND_I8)
     return a + b;
   else
     return __float_as_uint(__fadd_rn(__uint_as_float(a), __uint_as_float(b)));
 }
 
-// Eight rows (row .. row + 7, of which the first `rows` exist) of this warp's 32
-// channels from ch on.  v[0..3]: the pairs of rows 2 (lane % 4), + 1 of channels
-// lane / 4, + 8, + 16, + 24.  stage: 512 bytes of the warp's.
-__device__ __forceinline__ void store_rows8(const GroupedArgs& g, const float2 (&v)[4],
+// Eight rows (row .. row + 7, of which the first `rows` exist) of channel
+// ch + lane; ch: this warp's first of 32.  stage: 512 bytes of the warp's, in
+// which 16-bit values become rows of 32 channels for 16-byte stores.
+__device__ __forceinline__ void store_rows8(const GroupedArgs& g, const float (&v)[8],
                                             uint8_t* stage, int64_t row, int rows, int ch,
                                             int lane) {
   if (g.out_dtype == DT_F32) {
-    float* o = reinterpret_cast<float*>(g.out);
-    const int r = 2 * (lane & 3);
+    float* o = reinterpret_cast<float*>(g.out) + row * g.out_row + ch + lane;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = ch + 8 * j + (lane >> 2);
-      if (c >= g.n) continue;
-      if (r < rows) o[(row + r) * g.out_row + c] = v[j].x;
-      if (r + 1 < rows) o[(row + r + 1) * g.out_row + c] = v[j].y;
-    }
+    for (int r = 0; r < 8; ++r)
+      if (r < rows && ch + lane < g.n) o[r * g.out_row] = v[r];
     return;
   }
-  uint32_t pk[4];
+  uint16_t* mine = reinterpret_cast<uint16_t*>(stage) + lane;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (g.out_dtype == DT_F16) {
-      const __half2 h = __floats2half2_rn(v[j].x, v[j].y);
-      pk[j] = *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-      pk[j] = f2_bf16x2(v[j]);
-    }
+  for (int r = 0; r < 8; ++r) {
+    if (g.out_dtype == DT_F16)
+      mine[r * 32] = __half_as_ushort(__float2half_rn(v[r]));
+    else
+      mine[r * 32] = __bfloat16_as_ushort(__float2bfloat16_rn(v[r]));
   }
-  // row r's 64 bytes of channels, 16-byte pieces swizzled by r / 2: no bank conflicts
-  const int r = lane & 7;
-  stmatrix_x4_trans(smem_u32(stage) + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4), pk[0], pk[1],
-                    pk[2], pk[3]);
   __syncwarp();
   uint16_t* o = reinterpret_cast<uint16_t*>(g.out);
   if (g.out_vec) {
-    const int rr = lane >> 2, piece = lane & 3;
-    const uint4 w =
-        *reinterpret_cast<const uint4*>(stage + rr * 64 + ((piece ^ ((rr >> 1) & 3)) << 4));
-    if (rr < rows && ch + 8 * piece < g.n)
-      *reinterpret_cast<uint4*>(o + (row + rr) * g.out_row + ch + 8 * piece) = w;
+    const int r = lane >> 2, piece = lane & 3;
+    const uint4 w = *reinterpret_cast<const uint4*>(stage + lane * 16);
+    if (r < rows && ch + 8 * piece < g.n)
+      *reinterpret_cast<uint4*>(o + (row + r) * g.out_row + ch + 8 * piece) = w;
   } else if (ch + lane < g.n) {
-    for (int rr = 0; rr < rows && rr < 8; ++rr)
-      o[(row + rr) * g.out_row + ch + lane] = *reinterpret_cast<const uint16_t*>(
-          stage + rr * 64 + (((lane >> 3) ^ ((rr >> 1) & 3)) << 4) + (lane & 7) * 2);
+    for (int r = 0; r < rows && r < 8; ++r) o[(row + r) * g.out_row + ch + lane] = mine[r * 32];
   }
 }
 
+// 64 bytes of channels, from ch on, of 32 rows (row .. row + 31, of which the first
+// `rows` exist): 32 of a 16-bit type, 16 of fp32.  w: those of row row + lane.
+// stage: 2 KB of the warp's, in which the rows' 16-byte pieces change hands, so
+// that four lanes store a row's.
+__device__ __forceinline__ void store_rows32(const GroupedArgs& g, const uint32_t (&w)[16],
+                                             uint8_t* stage, int64_t row, int rows, int ch,
+                                             int lane) {
+  const int swizzle = (lane >> 1) & 3;  // of the pieces: no bank conflicts
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(stage + lane * 64 + ((j ^ swizzle) << 4)) =
+        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  __syncwarp();
+  const bool wide = g.out_dtype == DT_F32;
+  uint8_t* o = static_cast<uint8_t*>(g.out);
+  if (g.out_vec) {
+    const int c = ch + (lane & 3) * (wide ? 4 : 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (lane >> 2) + 8 * i;
+      const uint4 x = *reinterpret_cast<const uint4*>(
+          stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+      if (r < rows && c < g.n)
+        *reinterpret_cast<uint4*>(o + ((row + r) * g.out_row + c) * (wide ? 4 : 2)) = x;
+    }
+  } else {
+    // (one row at a time: 32 values of two bytes, or 16 of four)
+    const int at = lane * (wide ? 4 : 2);
+    if (at < 64 && ch + lane < g.n) {
+      for (int r = 0; r < rows && r < 32; ++r) {
+        const uint8_t* from = stage + r * 64 + (((at >> 4) ^ ((r >> 1) & 3)) << 4) + (at & 15);
+        const int64_t to = (row + r) * g.out_row + ch + lane;
+        if (wide)
+          reinterpret_cast<float*>(o)[to] = *reinterpret_cast<const float*>(from);
+        else
+          reinterpret_cast<uint16_t*>(o)[to] = *reinterpret_cast<const uint16_t*>(from);
+      }
+    }
+  }
+  __syncwarp();
+}
+
 template <int KIND, bool BLOCKS, bool PAIR>
-__global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
+__global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
     grouped_gemm_kernel(const __grid_constant__ GroupedMaps maps, const GroupedArgs g) {
-  using C = Cfg<PAIR>;
+  using C = Cfg<BLOCKS, PAIR>;
   constexpr int K_ELEMS = (KIND == KIND_BF16 || KIND == KIND_F16) ? 64 : 128;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* s_w = smem;
-  uint8_t* s_x = s_w + C::STAGES * C::W_BYTES;
-  uint8_t* s_exchange = s_x + C::STAGES * C::X_BYTES;
+  uint8_t* s_m = smem;
+  uint8_t* s_n = s_m + C::STAGES * C::M_BYTES;
+  uint8_t* s_exchange = s_n + C::STAGES * C::N_BYTES;
   float* s_scale = reinterpret_cast<float*>(s_exchange + C::EXCHANGE_BYTES);
   uint8_t* s_store = reinterpret_cast<uint8_t*>(s_scale) + C::SCALE_BYTES;
   int* s_row = reinterpret_cast<int*>(s_store + C::STORE_BYTES);  // [groups + 1]
@@ -260,7 +328,8 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
   uint64_t* acc_full = empty + C::STAGES;
   uint64_t* acc_empty = acc_full + C::BUFS;
   uint64_t* scale_full = acc_empty + C::BUFS;
-  uint64_t* drain = scale_full + C::SCALE_SLOTS;
+  uint64_t* scale_empty = scale_full + C::SCALE_SLOTS;
+  uint64_t* drain = scale_empty + C::SCALE_SLOTS;
   uint64_t* parts = drain + 1;  // K split: the owned rows' sums of all ranks are here
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(parts + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -281,7 +350,10 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], (PAIR ? 2 : 1) * C::EPI_WARPS);
     }
-    for (int s = 0; s < C::SCALE_SLOTS; ++s) mbar_init(&scale_full[s], C::EPI_WARPS);
+    for (int s = 0; s < C::SCALE_SLOTS; ++s) {
+      mbar_init(&scale_full[s], 2);
+      mbar_init(&scale_empty[s], C::EPI_WARPS);
+    }
     mbar_init(drain, 1);
     mbar_init(parts, 32);  // eight groups of rows / splits owners, four warps, `splits` senders
     *abort_flag = 0;
@@ -337,7 +409,7 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  Walk<PAIR> walk{s_row, s_tile, g.groups, g.tile_rows, ch_tiles,
+  Walk<C> walk{s_row, s_tile, g.groups, g.tile_rows, ch_tiles,
                   static_cast<int>(blockIdx.x) / per, static_cast<int>(gridDim.x) / per, 0};
   const int kb0 = PAIR ? 0 : static_cast<int>(int64_t(g.num_k_blocks) * rank / splits);
   const int kb1 = PAIR ? g.num_k_blocks
@@ -346,7 +418,7 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
   // The fp32 sums of a pair's tile are 128 registers a thread of the epilogue:
   // it takes over registers of the other warps.  (384 threads are launched with
   // 168 each; 2 * 216 + 64 <= 3 * 168.)
-  constexpr bool MOVE_REGS = BLOCKS && PAIR;
+  constexpr bool MOVE_REGS = C::ROWS_M;
   if (warp >= C::EPI_WARPS) {
     if constexpr (MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 8) {
@@ -356,34 +428,46 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
       uint32_t phase = 0;
       Tile t;
       while (!*abort_flag && walk.next(t)) {
-        const int x_rows = PAIR ? t.cols / 2 : t.cols;  // this CTA's
-        const int x_row = t.row0 + (PAIR ? static_cast<int>(rank) * x_rows : 0);
-        const int w_row = t.ch0 + (PAIR ? static_cast<int>(rank) * 128 : 0);
-        const uint32_t bytes = C::W_BYTES + x_rows * 128;
+        // This CTA's part of the columns (of a pair's, half), and its 128 of M.
+        const int n_rows = C::ROWS_M ? 128 : PAIR ? t.cols / 2 : t.cols;
+        const int n_row =
+            (C::ROWS_M ? t.ch0 : t.row0) + (PAIR ? static_cast<int>(rank) * n_rows : 0);
+        const int m_row =
+            (C::ROWS_M ? t.row0 : t.ch0) + (PAIR ? static_cast<int>(rank) * 128 : 0);
+        const uint32_t bytes = C::M_BYTES + n_rows * 128;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, g.status,
                                  DEV_TIMEOUT_PRODUCER))
             break;
           const int kx = kb * K_ELEMS;
-          uint8_t* w = s_w + stage * C::W_BYTES;
-          uint8_t* x = s_x + stage * C::X_BYTES;
+          uint8_t* m = s_m + stage * C::M_BYTES;
+          uint8_t* n = s_n + stage * C::N_BYTES;
           if constexpr (PAIR) {
             // The even CTA's barrier counts both CTAs' bytes.
             if (leader) mbar_arrive_expect_tx(&full[stage], 2 * bytes);
-            tma_load_3d_pair(w, &maps.b, &full[stage], kx, w_row, t.group);
           } else {
             mbar_arrive_expect_tx(&full[stage], bytes);
-            tma_load_3d(w, &maps.b, &full[stage], kx, w_row, t.group);
           }
-          for (int r = 0; r < x_rows;) {
-            const int left = x_rows - r;
-            const int take = left >= 128 ? 128 : left >= 64 ? 64 : 16;
-            const CUtensorMap* m = take == 128 ? &maps.a128 : take == 64 ? &maps.a64 : &maps.a16;
+          if constexpr (C::ROWS_M) {
+            tma_load_2d_pair(m, &maps.a128, &full[stage], kx, m_row);
+            tma_load_3d_pair(n, &maps.b, &full[stage], kx, n_row, t.group);
+          } else {
             if constexpr (PAIR)
-              tma_load_2d_pair(x + r * 128, m, &full[stage], kx, x_row + r);
+              tma_load_3d_pair(m, &maps.b, &full[stage], kx, m_row, t.group);
             else
-              tma_load_2d(x + r * 128, m, &full[stage], kx, x_row + r);
-            r += take;
+              tma_load_3d(m, &maps.b, &full[stage], kx, m_row, t.group);
+            for (int r = 0; r < n_rows;) {
+              const int left = n_rows - r;
+              const int take = left >= 128 ? 128 : left >= 64 ? 64 : 16;
+              const CUtensorMap* map = take == 128 ? &maps.a128
+                                       : take == 64 ? &maps.a64
+                                                    : &maps.a16;
+              if constexpr (PAIR)
+                tma_load_2d_pair(n + r * 128, map, &full[stage], kx, n_row + r);
+              else
+                tma_load_2d(n + r * 128, map, &full[stage], kx, n_row + r);
+              r += take;
+            }
           }
           ++issued;
           if (++stage == C::STAGES) {
@@ -433,7 +517,7 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
       };
       Tile t;
       while (ok && walk.next(t)) {
-        const uint32_t idesc = make_idesc(KIND, C::TM, t.cols);
+        const uint32_t idesc = make_idesc(KIND, PAIR ? 256 : 128, C::ROWS_M ? C::TN : t.cols);
         if (!BLOCKS && !take_buffer()) break;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (BLOCKS && !take_buffer()) break;
@@ -441,16 +525,16 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
           if (!ok) break;
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * C::TN);
-          const uint32_t w = smem_u32(s_w + stage * C::W_BYTES);
-          const uint32_t x = smem_u32(s_x + stage * C::X_BYTES);
+          const uint32_t m = smem_u32(s_m + stage * C::M_BYTES);
+          const uint32_t n = smem_u32(s_n + stage * C::N_BYTES);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t accumulate = (k != 0 || (!BLOCKS && kb != kb0)) ? 1u : 0u;
             if constexpr (PAIR)
-              tc_mma_pair<KIND>(d_tmem, smem_desc_k128(w + k * 32), smem_desc_k128(x + k * 32),
+              tc_mma_pair<KIND>(d_tmem, smem_desc_k128(m + k * 32), smem_desc_k128(n + k * 32),
                                 idesc, accumulate);
             else
-              tc_mma<KIND>(d_tmem, smem_desc_k128(w + k * 32), smem_desc_k128(x + k * 32), idesc,
+              tc_mma<KIND>(d_tmem, smem_desc_k128(m + k * 32), smem_desc_k128(n + k * 32), idesc,
                            accumulate);
           }
           if constexpr (PAIR)
@@ -481,21 +565,68 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
         }
       }
     }
+    } else if constexpr (BLOCKS) {
+      // ---------------------------------------------------------- block scales
+      // Products sa * sb of four blocks of K ("a quad") a slot: of the tile's rows,
+      // or (ROWS_M) of this CTA's 128 rows with each of the tile's channel blocks.
+      const int me = static_cast<int>(threadIdx.x) - 320;
+      uint32_t quad = 0;
+      bool ok = true;
+      Tile t;
+      while (ok && walk.next(t)) {
+        const float* sa = g.a_scales + t.row0 * g.as_row;
+        const float* sb = g.b_scales + t.group * g.bs_group + t.ch0 / 128 * g.bs_n;
+        constexpr int ROWS = C::ROWS_M ? 2 : 1, COLS = C::ROWS_M ? 2 : 1;
+        for (int kq = kb0; kq < kb1; kq += 4, ++quad) {
+          // (the loads are under way before the slot is waited for)
+          float v[ROWS][4], w[COLS][4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const bool there = kq + k < kb1;
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) {
+              const int r = (C::ROWS_M ? static_cast<int>(rank) * 128 : 0) + me + 64 * i;
+              v[i][k] = there && r < t.rows ? __ldg(sa + r * g.as_row + (kq + k) * g.as_k) : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < COLS; ++j)
+              w[j][k] = there && t.ch0 + j * 128 < g.n
+                            ? __ldg(sb + j * g.bs_n + (kq + k) * g.bs_k)
+                            : 0.0f;
+          }
+          const uint32_t slot = quad % C::SCALE_SLOTS;
+          ok = mbar_wait_bounded(&scale_empty[slot], ((quad / C::SCALE_SLOTS) & 1u) ^ 1u,
+                                 abort_flag, g.status, DEV_TIMEOUT_PRODUCER);
+          __syncwarp();
+          if (!ok) break;
+          float* s = s_scale + slot * 4 * C::TN + me;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+              for (int j = 0; j < COLS; ++j)
+                s[k * C::TN + j * 128 + i * 64] = __fmul_rn(v[i][k], w[j][k]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&scale_full[slot]);
+        }
+      }
     }
   } else {
     if constexpr (MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3;  // TMEM lanes 32 quarter ..: channels
-    const int half = warp >> 2;    // chunks half, half + 2, ... of 32 rows
+    const int half = warp >> 2;    // of the 32-column chunks: every second, or (ROWS_M) half
     const uint32_t tmem_warp = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t empty0 = PAIR ? map_to_rank(acc_empty, 0) : 0u;  // in the even CTA
-    uint8_t* stage_out = s_store + warp * 1024;
+    uint8_t* stage_out = s_store + warp * C::STORE_WARP;
     int out_buf = 0;
     int buf = 0;
     uint32_t buf_phase = 0;
     auto wait_acc = [&]() {
-      const bool ok = mbar_wait_bounded(&acc_full[buf], buf_phase, abort_flag, g.status,
-                                        DEV_TIMEOUT_EPILOGUE);
+      const bool ok = mbar_wait_lean(smem_u32(acc_full) + buf * 8, buf_phase,
+                                     smem_u32(const_cast<int*>(abort_flag)), g.status,
+                                     DEV_TIMEOUT_EPILOGUE);
       __syncwarp();
       tc_fence_after();
       return ok;
@@ -505,7 +636,7 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
       __syncwarp();
       if (lane == 0) {
         if constexpr (PAIR)
-          mbar_arrive_cluster(empty0 + buf * 8);
+          mbar_arrive_tmem(empty0 + buf * 8);
         else
           mbar_arrive(&acc_empty[buf]);
       }
@@ -514,138 +645,149 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
         buf_phase ^= 1u;
       }
     };
-    auto load_chunk = [&](int c, uint32_t* r) {
-      const uint32_t t = tmem_warp + static_cast<uint32_t>(buf * C::TN + (2 * c + half) * 32);
-      tmem_ld_frag(t, r);
-      tmem_ld_frag(t + (16u << 16), r + 16);
+    auto load_chunk = [&](int c, uint32_t (&r)[32]) {
+      const int at = C::ROWS_M ? half * 4 + c : 2 * c + half;
+      tmem_ld32(tmem_warp + static_cast<uint32_t>(buf * C::TN + at * 32), r);
+      tmem_wait32(r);
     };
     auto has_chunk = [&](const Tile& t, int c) { return (2 * c + half) * 32 < t.cols; };
 
-    // Block scales: products sa * sb of four blocks ("a quad") for the tile's rows
-    // go to a slot of shared memory together.  A warp writes its share of quad
-    // q + 1 after it has finished quad q, for which it had waited until every
-    // warp had written its share of q, having finished q - 1: two slots need no
-    // second barrier.
-    float sv[4];
-    uint32_t quad = 0;  // written so far
-    constexpr int PER_THREAD = C::TN * 4 / 256;  // values of a quad a thread brings
-    auto fetch_quad = [&](const Tile& t, int kb) {
-      const int64_t ch_block = t.ch0 / 128 + (PAIR ? static_cast<int>(rank) : 0);
-      const float* sb = g.b_scales + t.group * g.bs_group + ch_block * g.bs_n;
-      const bool ch_ok = ch_block * 128 < g.n;
+    // sum += scale * r, of neighbouring columns.
+    uint32_t acc[C::CHUNKS][32];
+    auto add_columns = [&](auto& r, uint32_t* sum, auto scale) {
 #pragma unroll
-      for (int j = 0; j < PER_THREAD; ++j) {
-        const int i = static_cast<int>(threadIdx.x) + 256 * j;
-        const int r = i % C::TN, k = kb + i / C::TN;
-        sv[j] = 0.0f;
-        if (r < t.rows && k < kb1 && ch_ok)
-          sv[j] = __fmul_rn(__ldg(g.a_scales + (t.row0 + r) * g.as_row + k * g.as_k),
-                            __ldg(sb + k * g.bs_k));
+      for (int i = 0; i < static_cast<int>(sizeof(r) / 4); i += 2) {
+        const float2 v = __ffma2_rn(
+            make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), scale(i),
+            make_float2(__uint_as_float(sum[i]), __uint_as_float(sum[i + 1])));
+        sum[i] = __float_as_uint(v.x);
+        sum[i + 1] = __float_as_uint(v.y);
       }
     };
-    auto put_quad = [&]() {
-      float* s = s_scale + (quad % C::SCALE_SLOTS) * 4 * C::TN;
-#pragma unroll
-      for (int j = 0; j < PER_THREAD; ++j) s[threadIdx.x + 256 * j] = sv[j];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&scale_full[quad % C::SCALE_SLOTS]);
-      ++quad;
-    };
-
-    Tile t, ahead;
-    bool more = walk.next(t);
-    if (BLOCKS && more) fetch_quad(t, kb0);
+    uint32_t quad = 0;
+    Tile t;
     bool ok = true;
-    while (more && ok) {
-      const bool more_ahead = walk.next(ahead);
-      uint32_t acc[C::CHUNKS][32];
+    while (ok && walk.next(t)) {
       if constexpr (BLOCKS) {
 #pragma unroll
         for (int c = 0; c < C::CHUNKS; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[c][i] = 0u;
-        put_quad();
-        uint32_t now = quad - 1;
-        for (int kq = kb0; kq < kb1 && ok; kq += 4, ++now) {
-          // (the quad after this one, of this tile or the next, is on its way meanwhile)
-          if (kq + 4 < kb1) {
-            fetch_quad(t, kq + 4);
-          } else if (more_ahead) {
-            fetch_quad(ahead, kb0);
+      }
+      if constexpr (C::ROWS_M) {
+        // A thread has one row and this warp's 128 channels have one scale: one product.
+        const float* sc = s_scale + half * 128 + quarter * 32 + lane;
+#pragma unroll 1
+        for (int kb = 0; kb < kb1; ++kb) {
+          if ((kb & 3) == 0) {
+            ok = mbar_wait_lean(smem_u32(scale_full) + quad % C::SCALE_SLOTS * 8,
+                                (quad / C::SCALE_SLOTS) & 1u,
+                                smem_u32(const_cast<int*>(abort_flag)), g.status,
+                                DEV_TIMEOUT_EPILOGUE);
+            __syncwarp();
+            if (!ok) break;
           }
-          ok = mbar_wait_bounded(&scale_full[now % C::SCALE_SLOTS],
-                                 (now / C::SCALE_SLOTS) & 1u, abort_flag, g.status,
-                                 DEV_TIMEOUT_EPILOGUE);
+          const float one = sc[((quad % C::SCALE_SLOTS) * 4 + (kb & 3)) * C::TN];
+          const float2 s = make_float2(one, one);
+          ok = wait_acc();
+          if (!ok) break;
+          // 16 columns are added while the next 16 come.
+          const uint32_t from = tmem_warp + static_cast<uint32_t>(buf * C::TN + half * 128);
+          uint32_t r[2][16];
+          tmem_ld16(from, r[0]);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            tmem_wait16(r[c & 1]);
+            if (c < 7)
+              tmem_ld16(from + 16 * (c + 1), r[(c + 1) & 1]);
+            else
+              release_acc();
+            add_columns(r[c & 1], acc[c >> 1] + 16 * (c & 1), [&](int) { return s; });
+          }
+          if ((kb & 3) == 3 || kb + 1 == kb1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&scale_empty[quad % C::SCALE_SLOTS]);
+            ++quad;
+          }
+        }
+      } else if constexpr (BLOCKS) {
+        for (int kq = kb0; kq < kb1 && ok; kq += 4, ++quad) {
+          const uint32_t slot = quad % C::SCALE_SLOTS;
+          ok = mbar_wait_bounded(&scale_full[slot], (quad / C::SCALE_SLOTS) & 1u, abort_flag,
+                                 g.status, DEV_TIMEOUT_EPILOGUE);
           __syncwarp();
-          const float* sc = s_scale + (now % C::SCALE_SLOTS) * 4 * C::TN + half * 32 +
-                            2 * (lane & 3);
+          const float* sc = s_scale + slot * 4 * C::TN + half * 32;
           for (int kb = kq; kb < kq + 4 && kb < kb1 && ok; ++kb, sc += C::TN) {
             ok = wait_acc();
             if (!ok) break;
-            uint32_t r[2][32];
-            if (has_chunk(t, 0)) load_chunk(0, r[0]);
-#pragma unroll
-            for (int c = 0; c < C::CHUNKS; ++c) {
-              if (!has_chunk(t, c)) break;
-              tmem_wait_frag(r[c & 1]);
-              if (c + 1 < C::CHUNKS && has_chunk(t, c + 1))
-                load_chunk(c + 1, r[(c + 1) & 1]);
-              else
-                release_acc();
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 s = *reinterpret_cast<const float2*>(sc + c * 64 + 8 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int at = (j >> 1) * 16 + 4 * i + 2 * (j & 1);
-                  const float2 v = __ffma2_rn(
-                      make_float2(__uint_as_float(r[c & 1][at]),
-                                  __uint_as_float(r[c & 1][at + 1])),
-                      s,
-                      make_float2(__uint_as_float(acc[c][at]), __uint_as_float(acc[c][at + 1])));
-                  acc[c][at] = __float_as_uint(v.x);
-                  acc[c][at + 1] = __float_as_uint(v.y);
-                }
-              }
+            if (has_chunk(t, 0)) {
+              uint32_t r[32];
+              load_chunk(0, r);
+              release_acc();
+              add_columns(r, acc[0],
+                          [&](int i) { return *reinterpret_cast<const float2*>(sc + i); });
+            } else {
+              release_acc();
             }
-            if (!has_chunk(t, 0)) release_acc();  // no rows for this warp
           }
-          if (ok && kq + 4 < kb1) put_quad();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&scale_empty[slot]);
         }
-        if (!ok) break;
       } else {
         ok = wait_acc();
-        if (!ok) break;
       }
+      if (!ok) break;
 
-      const int ch = t.ch0 + (PAIR ? static_cast<int>(rank) * 128 : 0) + quarter * 32;
-      float sb[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-      constexpr bool ROW_SCALES = !BLOCKS && (KIND == KIND_I8 || KIND == KIND_F8);
-      if constexpr (ROW_SCALES) {
+      if constexpr (C::ROWS_M) {
+        const int row0 = static_cast<int>(rank) * 128 + quarter * 32;
+        const int rows = t.rows - row0, ch0 = t.ch0 + half * 128;
+        const int64_t first = int64_t(t.row0) + row0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int n = ch + 8 * j + (lane >> 2);
-          if (n < g.n) sb[j] = __ldg(g.b_scales + t.group * g.bs_group + n * g.bs_n);
+        for (int c = 0; c < C::CHUNKS; ++c) {
+          uint32_t w[16];
+          if (g.out_dtype == DT_F32) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = acc[c][i];
+            store_rows32(g, w, stage_out, first, rows, ch0 + 32 * c, lane);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = acc[c][16 + i];
+            store_rows32(g, w, stage_out, first, rows, ch0 + 32 * c + 16, lane);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 two = make_float2(__uint_as_float(acc[c][2 * i]),
+                                             __uint_as_float(acc[c][2 * i + 1]));
+              if (g.out_dtype == DT_F16) {
+                const __half2 h = __float22half2_rn(two);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+              } else {
+                w[i] = f2_bf16x2(two);
+              }
+            }
+            store_rows32(g, w, stage_out, first, rows, ch0 + 32 * c, lane);
+          }
         }
+        continue;
       }
-      // Rows 8 i .. 8 i + 7 of chunk c: registers r.
-      auto finish = [&](const uint32_t* r, int c, int i) {
+      const int ch = t.ch0 + (PAIR ? static_cast<int>(rank) * 128 : 0) + quarter * 32;
+      constexpr bool ROW_SCALES = !BLOCKS && (KIND == KIND_I8 || KIND == KIND_F8);
+      float sb = 1.0f;
+      if constexpr (ROW_SCALES)
+        if (ch + lane < g.n) sb = __ldg(g.b_scales + t.group * g.bs_group + (ch + lane) * g.bs_n);
+      // Rows 8 i .. 8 i + 7 of chunk c, whose sums r holds.
+      auto finish = [&](const uint32_t (&r)[32], int c, int i) {
         const int first = (2 * c + half) * 32 + 8 * i;
         if (first >= t.rows) return;
-        float2 v[4];
+        float v[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int at = (j >> 1) * 16 + 4 * i + 2 * (j & 1);
-          v[j] = frag_value<KIND>(r[at], r[at + 1]);
-        }
-        if constexpr (ROW_SCALES) {
-          const int r0 = first + 2 * (lane & 3);
-          const float* sa = g.a_scales + int64_t(t.row0 + r0) * g.as_row;
-          const float2 s = make_float2(r0 < t.rows ? __ldg(sa) : 0.0f,
-                                       r0 + 1 < t.rows ? __ldg(sa + g.as_row) : 0.0f);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            v[j] = __fmul2_rn(__fmul2_rn(v[j], s), make_float2(sb[j], sb[j]));
+        for (int j = 0; j < 8; ++j) {
+          v[j] = sum_value<KIND>(r[8 * i + j]);
+          if constexpr (ROW_SCALES) {
+            const float sa = first + j < t.rows
+                                 ? __ldg(g.a_scales + (int64_t(t.row0) + first + j) * g.as_row)
+                                 : 0.0f;
+            v[j] = __fmul_rn(__fmul_rn(v[j], sa), sb);
+          }
         }
         store_rows8(g, v, stage_out + out_buf * 512, int64_t(t.row0) + first, t.rows - first, ch,
                     lane);
@@ -656,7 +798,6 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
           if constexpr (!BLOCKS) {
             if (has_chunk(t, 0)) {
               load_chunk(0, acc[0]);
-              tmem_wait_frag(acc[0]);
             }
             release_acc();
           }
@@ -670,10 +811,10 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
               const uint32_t to =
                   map_to_rank(s_exchange, owner) +
                   ((((n / splits) * splits + rank) * 4 + quarter) * 2 * 32 + lane) * 16;
-              st_cluster_v4(to, acc[0][4 * i], acc[0][4 * i + 1], acc[0][4 * i + 2],
-                            acc[0][4 * i + 3]);
-              st_cluster_v4(to + 512, acc[0][16 + 4 * i], acc[0][17 + 4 * i], acc[0][18 + 4 * i],
-                            acc[0][19 + 4 * i]);
+              st_cluster_v4(to, acc[0][8 * i], acc[0][8 * i + 1], acc[0][8 * i + 2],
+                            acc[0][8 * i + 3]);
+              st_cluster_v4(to + 512, acc[0][8 * i + 4], acc[0][8 * i + 5], acc[0][8 * i + 6],
+                            acc[0][8 * i + 7]);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_rank(parts, owner));
@@ -694,14 +835,13 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
                 const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                  uint32_t& a = acc[0][16 * p + 4 * i + q];
-                  a = s == 0 ? u[q] : frag_add<KIND>(a, u[q]);
+                  uint32_t& a = acc[0][8 * i + 4 * p + q];
+                  a = s == 0 ? u[q] : sum_add<KIND>(a, u[q]);
                 }
               }
             }
             finish(acc[0], 0, i);
           }
-          more = false;  // one tile a cluster
         }
       } else {
         if constexpr (BLOCKS) {
@@ -715,16 +855,13 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
           for (int c = 0; c < C::CHUNKS && has_chunk(t, c); ++c) {
             uint32_t r[32];
             load_chunk(c, r);
-            tmem_wait_frag(r);
             if (!(c + 1 < C::CHUNKS && has_chunk(t, c + 1))) release_acc();
 #pragma unroll
             for (int i = 0; i < 4; ++i) finish(r, c, i);
           }
           if (!has_chunk(t, 0)) release_acc();  // no rows for this warp
         }
-        more = more_ahead;
       }
-      t = ahead;
     }
 
     if (g.zero_rest && ok) {
@@ -761,7 +898,7 @@ __global__ void __launch_bounds__(Cfg<PAIR>::THREADS, 1)
 
 template <int KIND, bool BLOCKS, bool PAIR>
 cudaError_t launch(const GroupedMaps& maps, const GroupedArgs& g, int grid, cudaStream_t stream) {
-  using C = Cfg<PAIR>;
+  using C = Cfg<BLOCKS, PAIR>;
   auto kern = grouped_gemm_kernel<KIND, BLOCKS, PAIR>;
   static std::atomic<long long> shape[kMaxLaunchDevices];
   int dev = 0, sms = 0, per_sm = 0;
