@@ -1,14 +1,14 @@
 // E4M3 quantization with a scale for each block of 128 channels: of one row
 // (activations), or of 128 rows (weights).
 //
-//   v = x, or silu(gate) x = (gate / (1 + exp(-gate))) x, in fp32
+//   v = x, or silu(gate) x = gate / (1 + exp(-gate)) x, in fp32
 //   scale = max|v| / 448 over the block, 1 where that is 0
 //   code  = E4M3(RN32(v / scale)), nearest even, saturating
 //
-// One pass: a block of one row lives in 16 lanes, 8 channels each (one 16-byte
-// load of a 16-bit type), its peak goes through four shuffles; a block of 128
-// rows lives in the registers of one CTA.  Bound by memory: size + 1 bytes a
-// value and 4 a block.
+// One pass: a block of one row lives in eight lanes, 16 channels each (32 bytes
+// of a 16-bit type, one 16-byte store of codes), its peak goes through three
+// shuffles; a block of 128 rows lives in the registers of one CTA.  Bound by
+// memory: size + 1 bytes a value and 4 a block.
 //
 // The peak is taken on the values' bit patterns without the sign, which order
 // like the values and put NaN above infinity, so that a block with either gets
@@ -20,18 +20,21 @@ namespace m5b {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kLane = 16;                // channels a thread
+constexpr int kLanes = 128 / kLane;      // threads of a block's row
+constexpr int kRows = kThreads / kLanes;  // rows of blocks that a CTA has at a time
 
 template <typename T>
-struct Raw8 {  // eight values as they are in memory
-  uint32_t w[2 * sizeof(T)];
+struct Raw {  // kLane values as they are in memory
+  uint32_t w[kLane * sizeof(T) / 4];
 };
 
 template <typename T>
-__device__ __forceinline__ Raw8<T> load8(const T* p) {
-  Raw8<T> r;
+__device__ __forceinline__ Raw<T> load(const T* p) {
+  Raw<T> r;
 #pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
-    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  for (int i = 0; i < static_cast<int>(sizeof(r) / 16); ++i) {
+    const uint4 v = reinterpret_cast<const uint4*>(p)[i];
     r.w[4 * i] = v.x;
     r.w[4 * i + 1] = v.y;
     r.w[4 * i + 2] = v.z;
@@ -39,46 +42,78 @@ __device__ __forceinline__ Raw8<T> load8(const T* p) {
   }
   return r;
 }
-// The first `count` of eight values, zeros behind them.
+// The first `count` values, zeros behind them.
 template <typename T>
-__device__ __forceinline__ Raw8<T> load8_upto(const T* p, int count) {
-  Raw8<T> r;
+__device__ __forceinline__ Raw<T> load_upto(const T* p, int count) {
+  Raw<T> r;
 #pragma unroll
-  for (int i = 0; i < 2 * static_cast<int>(sizeof(T)); ++i) r.w[i] = 0u;
+  for (int i = 0; i < static_cast<int>(sizeof(r) / 4); ++i) r.w[i] = 0u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < kLane; ++i) {
     if (i >= count) break;
     if constexpr (sizeof(T) == 4)
       r.w[i] = __float_as_uint(p[i]);
     else
-      r.w[i >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
+      r.w[i >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i])
+                     << (16 * (i & 1));
   }
   return r;
 }
-template <typename T>
-__device__ __forceinline__ void unpack8(const Raw8<T>& r, float* v) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float2 f;
-    if constexpr (sizeof(T) == 4) {
-      f = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
-    } else if constexpr (DTypeOf<T>::value == DT_BF16) {
-      f = bf16x2_f2(r.w[i]);
-    } else {
-      f = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
-    }
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw<T> load_any(const T* p, int count) {
+  if constexpr (VEC) {  // (k is a multiple of kLane: all values or none)
+    if (count > 0) return load(p);
+    return Raw<T>{};
+  } else {
+    return load_upto(p, count);
   }
 }
 
-__device__ __forceinline__ uint32_t peak8(const float* v) {
-  uint32_t m = 0u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  return m;
+template <typename T>
+__device__ __forceinline__ float2 pair(const Raw<T>& r, int i) {  // values 2 i, 2 i + 1
+  if constexpr (sizeof(T) == 4)
+    return make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+  else if constexpr (DTypeOf<T>::value == DT_BF16)
+    return bf16x2_f2(r.w[i]);
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
 }
 
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// The largest magnitude, as the bits of an fp32 number.
+template <typename T>
+__device__ __forceinline__ uint32_t peak_of(const Raw<T>& r) {
+  uint32_t m = 0u;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) m = max(m, r.w[i] & 0x7FFFFFFFu);
+    return m;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kLane / 2; ++i) m = __vmaxu2(m, r.w[i] & 0x7FFF7FFFu);
+    const uint32_t top = max(m >> 16, m & 0xFFFFu);
+    if constexpr (DTypeOf<T>::value == DT_BF16) return top << 16;
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top))));
+  }
+}
+
+// v = silu(g) x of 2 i, 2 i + 1.  Between -80 and 80 the quotient g / d, d = 1 +
+// exp(-g), comes from a reciprocal with one Newton step and one correction step
+// (Markstein's, as in i8_pair_div: right but for the rarest ulp); elsewhere
+// divides, since d may be infinite.
+constexpr float kSiluFast = 80.0f;
+__device__ __forceinline__ float2 silu_fast(float2 g, float2 x) {
+  const float2 one = make_float2(1.0f, 1.0f);
+  const float2 d = __fadd2_rn(one, make_float2(expf(-g.x), expf(-g.y)));
+  const float2 nd = make_float2(-d.x, -d.y);
+  float2 y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(d.y));
+  y = __ffma2_rn(__ffma2_rn(nd, y, one), y, y);
+  const float2 q = __fmul2_rn(g, y);
+  return __fmul2_rn(__ffma2_rn(__ffma2_rn(nd, q, g), y, q), x);
+}
 __device__ __forceinline__ float silu(float g) {
   return __fdiv_rn(g, __fadd_rn(1.0f, expf(-g)));
 }
@@ -88,128 +123,145 @@ __device__ __forceinline__ float block_scale(uint32_t peak) {
   return s == 0.0f ? 1.0f : s;
 }
 
-// Codes of eight values.  Where neither the scale nor its reciprocal leaves the
-// normal range, quot_pair_div is the correctly rounded quotient wherever that
-// is not far below the smallest code's half (2^-10); elsewhere divides.
-__device__ __forceinline__ uint2 codes8(const float* v, float scale) {
-  uint32_t w[4];
+// Stores the codes of kLane values, of which the first `count` exist.  Where
+// neither the scale nor its reciprocal leaves the normal range, quot_pair_div is
+// the correctly rounded quotient wherever that is not far below half the
+// smallest code (2^-10); elsewhere divides.
+template <bool VEC, class Pair>
+__device__ __forceinline__ void store_codes(uint8_t* q, int count, float scale, Pair pair_at) {
+  uint32_t w[kLane / 4];
   if (scale >= kI8DivMinScale && scale <= 0x1p100f) {
     const I8Div d = i8_div(__frcp_rn(scale), scale);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = __nv_cvt_float2_to_fp8x2(quot_pair_div(make_float2(v[2 * i], v[2 * i + 1]), d),
-                                      __NV_SATFINITE, __NV_E4M3);
-    return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-  }
-  return make_uint2(e4m3_word_exact(v[0], v[1], v[2], v[3], scale),
-                    e4m3_word_exact(v[4], v[5], v[6], v[7], scale));
-}
-
-__device__ __forceinline__ void store8(uint8_t* q, uint2 codes, bool vec, int count) {
-  if (vec) {
-    *reinterpret_cast<uint2*>(q) = codes;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < count) q[i] = static_cast<uint8_t>((i < 4 ? codes.x : codes.y) >> (8 * (i & 3)));
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ Raw8<T> load_any(const T* p, int count) {
-  if constexpr (VEC) {  // (k is a multiple of 8: all eight or none)
-    if (count > 0) return load8(p);
-    return Raw8<T>{};
+    for (int i = 0; i < kLane / 4; ++i)
+      w[i] = __nv_cvt_float2_to_fp8x2(quot_pair_div(pair_at(2 * i), d), __NV_SATFINITE,
+                                      __NV_E4M3) |
+             static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(quot_pair_div(pair_at(2 * i + 1), d),
+                                                            __NV_SATFINITE, __NV_E4M3))
+                 << 16;
   } else {
-    return load8_upto(p, count);
+#pragma unroll
+    for (int i = 0; i < kLane / 4; ++i) {
+      const float2 a = pair_at(2 * i), b = pair_at(2 * i + 1);
+      w[i] = e4m3_word_exact(a.x, a.y, b.x, b.y, scale);
+    }
+  }
+  if constexpr (VEC) {
+    *reinterpret_cast<uint4*>(q) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kLane; ++i)
+      if (i < count) q[i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
   }
 }
 
-// Blocks of one row.  Half-warp h of the grid takes blocks h, h + halves, ...,
+// Blocks of one row.  A group of eight lanes takes blocks b, b + stride, ...,
 // UNROLL of them at a time, whose loads are all on their way before the first is
 // used.
 template <typename T, bool GATE, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
     block_quant_rows_kernel(const BlockQuantArgs a, unsigned blocks_per_row, unsigned total) {
-  const int sub = threadIdx.x & 15;
-  const unsigned halves = gridDim.x * (kThreads / 16);
-  const unsigned first = blockIdx.x * (kThreads / 16) + (threadIdx.x >> 4);
+  const int sub = threadIdx.x % kLanes;
+  const unsigned stride = gridDim.x * kRows;
+  const unsigned row_step = stride / blocks_per_row;
+  const unsigned col_step = stride - row_step * blocks_per_row;
   const T* x = static_cast<const T*>(a.x);
   const T* gate = static_cast<const T*>(a.gate);
+  unsigned b = blockIdx.x * kRows + threadIdx.x / kLanes;
+  unsigned row = b / blocks_per_row, block = b - row * blocks_per_row;
   // (whole warps leave the loop together: the shuffles below name all lanes)
-  for (unsigned b0 = first - (first & 1u); b0 < total; b0 += halves * UNROLL) {
-    Raw8<T> rx[UNROLL], rg[UNROLL];
+  while (b - threadIdx.x % 32 / kLanes < total) {
+    Raw<T> rx[UNROLL], rg[UNROLL];
     int64_t at[UNROLL];
     int count[UNROLL];
+    unsigned which[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const unsigned b = b0 + (first & 1u) + u * halves;
-      const unsigned row = b / blocks_per_row;
-      const unsigned col = (b - row * blocks_per_row) * 128u + sub * 8u;
-      int64_t left = b < total ? a.k - col : 0;
+      const int64_t col = int64_t(block) * 128 + sub * kLane;
+      const int64_t left = b < total ? a.k - col : 0;
+      which[u] = b;
       at[u] = int64_t(row) * a.k + col;
-      count[u] = static_cast<int>(left < 0 ? 0 : left > 8 ? 8 : left);
+      count[u] = static_cast<int>(left < 0 ? 0 : left > kLane ? kLane : left);
       int64_t src = row;
-      bool have = true;
-      if (a.index && b < total) {
+      int here = count[u];
+      if (a.index && here > 0) {
         src = a.index[row];
-        have = src >= 0 && src < a.x_rows;  // else a row of zeros
+        if (src < 0 || src >= a.x_rows) here = 0;  // a row of zeros
       }
-      rx[u] = load_any<T, VEC>(x + src * a.x_row + col, have ? count[u] : 0);
-      if constexpr (GATE)
-        rg[u] = load_any<T, VEC>(gate + src * a.gate_row + col, have ? count[u] : 0);
+      rx[u] = load_any<T, VEC>(x + src * a.x_row + col, here);
+      if constexpr (GATE) rg[u] = load_any<T, VEC>(gate + src * a.gate_row + col, here);
+      b += stride;
+      row += row_step;
+      block += col_step;
+      if (block >= blocks_per_row) {
+        block -= blocks_per_row;
+        ++row;
+      }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const unsigned b = b0 + (first & 1u) + u * halves;
-      float v[8];
-      unpack8(rx[u], v);
+      float2 v[kLane / 2];
+      uint32_t peak = 0u;
       if constexpr (GATE) {
-        float s[8];
-        unpack8(rg[u], s);
+        if (peak_of(rg[u]) <= __float_as_uint(kSiluFast)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(silu(s[i]), v[i]);
+          for (int i = 0; i < kLane / 2; ++i) v[i] = silu_fast(pair(rg[u], i), pair(rx[u], i));
+        } else {
+#pragma unroll
+          for (int i = 0; i < kLane / 2; ++i) {
+            const float2 g = pair(rg[u], i), f = pair(rx[u], i);
+            v[i] = make_float2(__fmul_rn(silu(g.x), f.x), __fmul_rn(silu(g.y), f.y));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kLane / 2; ++i)
+          peak = max(peak, max(magnitude(v[i].x), magnitude(v[i].y)));
+      } else {
+        peak = peak_of(rx[u]);
       }
-      uint32_t peak = peak8(v);
 #pragma unroll
-      for (int d = 8; d; d >>= 1) peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, d));
+      for (int d = kLanes / 2; d; d >>= 1)
+        peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, d));
       const float scale = block_scale(peak);
-      if (b < total && sub == 0) a.scales[b] = scale;
-      if (count[u] > 0) store8(a.q + at[u], codes8(v, scale), VEC, count[u]);
+      if (which[u] < total && sub == 0) a.scales[which[u]] = scale;
+      if (count[u] > 0)
+        store_codes<VEC>(a.q + at[u], count[u], scale, [&](int i) {
+          if constexpr (GATE)
+            return v[i];
+          else
+            return pair(rx[u], i);
+        });
     }
   }
 }
 
-// Blocks of 128 rows, one a CTA: thread t has channels 8 (t % 16) .. + 7 of rows
-// t / 16 + 16 i.
+// Blocks of 128 rows, one a CTA: thread t has channels 16 (t % 8) .. + 15 of rows
+// t / 8 + 32 i.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     block_quant_square_kernel(const BlockQuantArgs a, unsigned blocks_per_row,
                               unsigned row_blocks) {
+  constexpr int N = 128 / kRows;
   __shared__ uint32_t s_peak[kThreads / 32];
   const unsigned b = blockIdx.x;
   const unsigned rb = b / blocks_per_row;  // batch * row_blocks + row block
   const unsigned batch = rb / row_blocks;
-  const int64_t row0 = int64_t(rb - batch * row_blocks) * 128 + (threadIdx.x >> 4);
-  const int64_t col = int64_t(b - rb * blocks_per_row) * 128 + (threadIdx.x & 15) * 8;
+  const int64_t row0 = int64_t(rb - batch * row_blocks) * 128 + threadIdx.x / kLanes;
+  const int64_t col = int64_t(b - rb * blocks_per_row) * 128 + threadIdx.x % kLanes * kLane;
   const int64_t left = a.k - col;
-  const int count = static_cast<int>(left < 0 ? 0 : left > 8 ? 8 : left);
+  const int count = static_cast<int>(left < 0 ? 0 : left > kLane ? kLane : left);
   const T* x = static_cast<const T*>(a.x) + batch * a.x_batch + col;
-  Raw8<T> r[8];
+  Raw<T> r[N];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t row = row0 + 16 * i;
+  for (int i = 0; i < N; ++i) {
+    const int64_t row = row0 + kRows * i;
     r[i] = load_any<T, VEC>(x + row * a.x_row, row < a.rows ? count : 0);
   }
   uint32_t peak = 0u;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float v[8];
-    unpack8(r[i], v);
-    peak = max(peak, peak8(v));
-  }
+  for (int i = 0; i < N; ++i) peak = max(peak, peak_of(r[i]));
   peak = __reduce_max_sync(0xffffffffu, peak);
-  if ((threadIdx.x & 31) == 0) s_peak[threadIdx.x >> 5] = peak;
+  if (threadIdx.x % 32 == 0) s_peak[threadIdx.x / 32] = peak;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kThreads / 32; ++i) peak = max(peak, s_peak[i]);
@@ -217,12 +269,10 @@ __global__ void __launch_bounds__(kThreads)
   if (threadIdx.x == 0) a.scales[b] = scale;
   uint8_t* q = a.q + int64_t(batch) * a.rows * a.k + col;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t row = row0 + 16 * i;
-    if (row >= a.rows || count == 0) continue;
-    float v[8];
-    unpack8(r[i], v);
-    store8(q + row * a.k, codes8(v, scale), VEC, count);
+  for (int i = 0; i < N; ++i) {
+    const int64_t row = row0 + kRows * i;
+    if (row < a.rows && count > 0)
+      store_codes<VEC>(q + row * a.k, count, scale, [&](int j) { return pair(r[i], j); });
   }
 }
 
@@ -236,15 +286,15 @@ cudaError_t launch(const BlockQuantArgs& a, bool square, cudaStream_t stream) {
     return cudaGetLastError();
   }
   const unsigned total = static_cast<unsigned>(a.rows) * per_row;
-  constexpr int UNROLL = sizeof(T) == 4 ? 2 : 4;
-  const unsigned per_cta = kThreads / 16 * UNROLL;
-  unsigned grid = (total + per_cta - 1) / per_cta;
+  constexpr int UNROLL = sizeof(T) == 4 ? 1 : 2;
+  unsigned grid = (total + kRows - 1) / kRows;
   const unsigned most = static_cast<unsigned>(a.sms) * 8;
   if (grid > most) grid = most;
   if (a.gate)
-    block_quant_rows_kernel<T, true, VEC, 2><<<grid, kThreads, 0, stream>>>(a, per_row, total);
+    block_quant_rows_kernel<T, true, VEC, 1><<<grid, kThreads, 0, stream>>>(a, per_row, total);
   else
-    block_quant_rows_kernel<T, false, VEC, UNROLL><<<grid, kThreads, 0, stream>>>(a, per_row, total);
+    block_quant_rows_kernel<T, false, VEC, UNROLL>
+        <<<grid, kThreads, 0, stream>>>(a, per_row, total);
   return cudaGetLastError();
 }
 

@@ -55,7 +55,7 @@ struct BlockQuantArgs {
   int64_t batch;
   uint8_t* q;            // [batch, rows, k]
   float* scales;         // [batch, rows or row blocks, ceil(k / 128)]
-  int vec;               // rows on the 16-byte grid, k a multiple of 8
+  int vec;               // rows on the 16-byte grid, k a multiple of 16
   int sms;
 };
 

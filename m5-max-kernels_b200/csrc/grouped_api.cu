@@ -91,9 +91,9 @@ int m5b_block_quantize(const m5b_block_quantize_args* s, void* stream) {
   a.q = s->q;
   a.scales = s->scales;
   const int64_t size = dtype_bytes(s->x_dtype);
-  a.vec = s->k % 8 == 0 && grid16(s->x) && grid16(s->gate) && (s->x_row_stride * size) % 16 == 0 &&
+  a.vec = s->k % 16 == 0 && grid16(s->x) && grid16(s->gate) && (s->x_row_stride * size) % 16 == 0 &&
           (s->gate_row_stride * size) % 16 == 0 && (s->x_batch_stride * size) % 16 == 0 &&
-          reinterpret_cast<uintptr_t>(s->q) % 8 == 0;
+          grid16(s->q);
   int rc = current_device_state(nullptr, &a.sms);
   if (rc) return rc;
   return launched(launch_block_quantize(a, static_cast<int>(s->x_dtype), s->block_rows == 128,

@@ -31,29 +31,33 @@ from .paged import _call, _device, _ints
 _Tensor = torch.Tensor
 BLOCK = 128
 _FLOAT = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
-_OPERAND = {"int8": torch.int8, "fp8": torch.uint8, "bf16": torch.bfloat16,
-            "fp16": torch.float16}
+_OPERAND = {mode: (dtype, _lib.MODE[mode], dtype.itemsize) for mode, dtype in (
+    ("int8", torch.int8), ("fp8", torch.uint8), ("bf16", torch.bfloat16), ("fp16", torch.float16))}
+_NO_SCALES = (0,) * 7
 _MOST_GROUPS = 1024
 # m5b_block_quantize_args and m5b_grouped_gemm_args (include/m5b200.h): every field is 8 bytes
 _PACK_QUANTIZE = struct.Struct("@14q")
 _PACK_GEMM = struct.Struct("@23q")
 
 
-def _channels(t):
-    """t with contiguous channels."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+def _new(shape, dtype, device):
+    """A contiguous matrix or batch of them (empty_strided takes half of empty's time)."""
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _operand(t):
-    """t with rows that TMA can read: contiguous channels, rows on the 16-byte grid."""
-    size, strides = t.element_size(), t.stride()
+def _operand(t, size):
+    """(t, strides) with rows that TMA can read: contiguous channels, rows on the 16-byte grid."""
+    strides = t.stride()
     if strides[-1] == 1 and t.data_ptr() % 16 == 0:
-        for n, s in zip(t.shape[:-1], strides[:-1]):
+        for n, s in zip(t.shape, strides[:-1]):
             if n > 1 and (s <= 0 or s * size % 16):
                 break
         else:
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
+            return t, strides
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
 
 
 def _row_index(rows):
@@ -80,9 +84,10 @@ def block_quantize(x, *, gate=None, rows=None, block_rows=1):
     are read in place.  A block that holds an infinity or NaN gets a scale that
     is not finite.
     """
-    if not isinstance(x, _Tensor) or x.dtype not in _FLOAT:
+    code = _FLOAT.get(x.dtype) if isinstance(x, _Tensor) else None
+    if code is None:
         raise ValueError("input dtype must be float16, bfloat16 or float32")
-    if block_rows not in (1, BLOCK) or isinstance(block_rows, bool):
+    if type(block_rows) is not int or block_rows not in (1, BLOCK):
         raise ValueError("block_rows must be 1 or 128")
     if block_rows == 1:
         if x.dim() != 2 or x.shape[1] == 0:
@@ -92,59 +97,65 @@ def block_quantize(x, *, gate=None, rows=None, block_rows=1):
             raise ValueError("weights must have nonempty shape [N, K] or [E, N, K]")
         if gate is not None or rows is not None:
             raise ValueError("gate and rows need block_rows 1")
-    x = _channels(x)
+    shape, strides = x.shape, x.stride()
+    k, out_rows = shape[-1], shape[-2]
+    if strides[-1] != 1:
+        x = x.contiguous()
+        strides = x.stride()
     used = [x]
     gate_ptr = gate_row = index_ptr = 0
     if gate is not None:
-        if not isinstance(gate, _Tensor) or gate.shape != x.shape or gate.dtype is not x.dtype:
+        if not isinstance(gate, _Tensor) or gate.shape != shape or gate.dtype is not x.dtype:
             raise ValueError("gate must have x's shape and dtype")
-        gate = _channels(gate)
+        if gate.stride(1) != 1:
+            gate = gate.contiguous()
         gate_ptr, gate_row = gate.data_ptr(), gate.stride(0)
         used.append(gate)
-    batch = x.shape[0] if x.dim() == 3 else 1
-    out_rows, k = x.shape[-2], x.shape[-1]
     if rows is not None:
         rows = _row_index(rows)
         index_ptr, out_rows = rows.data_ptr(), rows.shape[0]
         used.append(rows)
     index = _device(used)
-    lead = (*x.shape[:-2],)
-    codes = torch.empty((*lead, out_rows, k), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*lead, -(-out_rows // block_rows), -(-k // BLOCK)), dtype=torch.float32,
-                         device=x.device)
+    batch, batch_stride = (shape[0], strides[0]) if len(shape) == 3 else (1, 0)
+    lead = tuple(shape[:-2])
+    device = x.device
+    codes = _new((*lead, out_rows, k), torch.uint8, device)
+    scales = _new((*lead, -(-out_rows // block_rows), -(-k // BLOCK)), torch.float32, device)
     if out_rows > 0:
         _call(_lib.lib().m5b_block_quantize, _PACK_QUANTIZE.pack(
-            x.data_ptr(), _FLOAT[x.dtype], x.shape[-2], x.stride(-2),
-            x.stride(0) if batch > 1 else 0, gate_ptr, gate_row, index_ptr, out_rows, k, batch,
-            block_rows, codes.data_ptr(), scales.data_ptr()), index)
+            x.data_ptr(), code, shape[-2], strides[-2], batch_stride, gate_ptr, gate_row,
+            index_ptr, out_rows, k, batch, block_rows, codes.data_ptr(), scales.data_ptr()), index)
     return codes, scales
 
 
 def _product(a, b, group_start, mode, a_scales, b_scales, output_dtype, out):
-    """Both products: b [groups, N, K]; group_start None: all rows are group 0's."""
-    groups, n, k = b.shape
-    rows = a.shape[0]
-    expected = _OPERAND[mode]
+    """Both products: b [groups, N, K], or with group_start None [N, K] for all rows."""
+    rows, k = a.shape
+    n = b.shape[-2]
+    groups = 1 if group_start is None else b.shape[0]
+    expected, code, size = _OPERAND[mode]
     if a.dtype is not expected or b.dtype is not expected:
         raise ValueError("operand dtypes must match the declared mode")
-    if k * a.element_size() % 16:
-        raise NotImplementedError(f"K*{a.element_size()} bytes per row must be a multiple of 16 "
-                                  "for TMA; padding is not implicit")
+    if k * size % 16:
+        raise NotImplementedError(f"K*{size} bytes per row must be a multiple of 16 for TMA; "
+                                  "padding is not implicit")
     used = [a, b]
-    scale_fields = [0] * 7
     blocks = False
-    if mode in ("int8", "fp8"):
+    scale_fields = _NO_SCALES
+    if size == 1:
         if (not isinstance(a_scales, _Tensor) or not isinstance(b_scales, _Tensor)
                 or a_scales.dtype is not torch.float32 or b_scales.dtype is not torch.float32):
             raise ValueError("float32 scales required")
         kb = -(-k // BLOCK)
         sa, sb = a_scales.stride(), b_scales.stride()
-        if a_scales.shape == (rows,) and b_scales.shape == (groups, n):
-            scale_fields = [a_scales.data_ptr(), b_scales.data_ptr(), sa[0], 0, sb[0], sb[1], 0]
-        elif (mode == "fp8" and a_scales.shape == (rows, kb)
-                and b_scales.shape == (groups, -(-n // BLOCK), kb)):
+        a_shape, b_shape = a_scales.shape, b_scales.shape
+        lead = () if group_start is None else (groups,)
+        if (mode == "fp8" and a_shape == (rows, kb) and b_shape == (*lead, -(-n // BLOCK), kb)):
             blocks = True
-            scale_fields = [a_scales.data_ptr(), b_scales.data_ptr(), *sa, *sb]
+            scale_fields = (a_scales.data_ptr(), b_scales.data_ptr(), *sa,
+                            *(sb if lead else (0, *sb)))
+        elif a_shape == (rows,) and b_shape == (groups, n):
+            scale_fields = (a_scales.data_ptr(), b_scales.data_ptr(), sa[0], 0, sb[0], sb[1], 0)
         else:
             raise ValueError("scales must be those of rows and channels, or (fp8) of blocks of "
                              "128 channels of K")
@@ -162,7 +173,8 @@ def _product(a, b, group_start, mode, a_scales, b_scales, output_dtype, out):
         if output_dtype is not None and output_dtype is not out_dtype:
             raise ValueError("output_dtype must be out's")
         used.append(out)
-    if out_dtype not in _FLOAT:
+    out_code = _FLOAT.get(out_dtype)
+    if out_code is None:
         raise NotImplementedError("output dtype must be bfloat16, float16 or float32")
     start_ptr = 0
     if group_start is not None:
@@ -170,13 +182,14 @@ def _product(a, b, group_start, mode, a_scales, b_scales, output_dtype, out):
         used.append(group_start)
     index = _device(used)
     if out is None:
-        out = torch.empty((rows, n), dtype=out_dtype, device=a.device)
+        out = torch.empty_strided((rows, n), (n, 1), dtype=out_dtype, device=a.device)
     if rows > 0:
-        a, b = _operand(a), _operand(b)
+        a, a_strides = _operand(a, size)
+        b, b_strides = _operand(b, size)
         _call(_lib.lib().m5b_grouped_gemm, _PACK_GEMM.pack(
-            a.data_ptr(), b.data_ptr(), _lib.MODE[mode], rows, groups, n, k, a.stride(0),
-            b.stride(0), b.stride(1), start_ptr, blocks, *scale_fields, out.data_ptr(),
-            _FLOAT[out_dtype], out.stride(0), zero_rest), index)
+            a.data_ptr(), b.data_ptr(), code, rows, groups, n, k, a_strides[0], b_strides[0],
+            b_strides[-2], start_ptr, blocks, *scale_fields, out.data_ptr(), out_code,
+            out.stride(0), zero_rest), index)
     return out
 
 
@@ -199,7 +212,7 @@ def block_gemm(a, b, a_scales, b_scales, *, output_dtype=None, out=None):
     if (not isinstance(a_scales, _Tensor) or not isinstance(b_scales, _Tensor)
             or a_scales.dim() != 2 or b_scales.dim() != 2):
         raise ValueError("scales must be those of blocks of 128 channels of K")
-    return _product(a, b[None], None, "fp8", a_scales, b_scales[None], output_dtype, out)
+    return _product(a, b, None, "fp8", a_scales, b_scales, output_dtype, out)
 
 
 def grouped_gemm(a, b, group_start, mode="bf16", *, a_scales=None, b_scales=None,
