@@ -44,6 +44,9 @@ constexpr int kSingleTileRows = 64;
 cudaError_t launch_grouped_gemm(const GroupedMaps& maps, const GroupedArgs& g, int kind,
                                 bool blocks, bool pair, int grid, cudaStream_t stream);
 
+// Clusters of `splits` single CTAs that the current device runs at a time; 0 on failure.
+int grouped_split_clusters(int kind, bool blocks, int splits);
+
 struct BlockQuantArgs {
   const void* x;
   const void* gate;      // NULL, or values silu(gate) * x

@@ -37,7 +37,8 @@ struct Plan {
 // Tiles and schedule.  Groups of few rows are bound by their weights: 64-row
 // tiles on single CTAs, several of which share a tile's K range where the tiles
 // do not fill the GPU.  Others take 256 channels x up to 256 rows on CTA pairs.
-Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int sms) {
+Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, bool blocks,
+              int sms) {
   Plan p{};
   const int64_t busy = groups < rows ? groups : rows;  // groups with rows, at most
   const int64_t each = ceil_div(rows, groups);
@@ -49,8 +50,11 @@ Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int sms) {
   int64_t tiles = (rows / p.tile_rows + busy) * ch_tiles;
   if (groups == 1) tiles = ceil_div(rows, p.tile_rows) * ch_tiles;
   const int64_t units = p.pair ? sms / 2 : sms;
+  // (a cluster has one tile, and all of them run at once)
   if (!p.pair)
-    while (p.splits < 8 && tiles * p.splits * 2 <= units && nkb >= p.splits * 2 * 4) p.splits *= 2;
+    while (p.splits < 8 && tiles * p.splits * 2 <= units && nkb >= p.splits * 2 * 4 &&
+           tiles <= grouped_split_clusters(kind, blocks, p.splits * 2))
+      p.splits *= 2;
   const int64_t used = tiles < units ? tiles : units;
   p.grid = static_cast<int>(used) * (p.pair ? 2 : p.splits);
   return p;
@@ -161,7 +165,8 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
   int sms = 0;
   int rc = current_device_state(&g.status, &sms);
   if (rc) return rc;
-  const Plan p = plan_for(s->rows, s->groups, s->n, g.num_k_blocks, sms);
+  const Plan p = plan_for(s->rows, s->groups, s->n, g.num_k_blocks, kind,
+                          s->block_scales != 0, sms);
   g.tile_rows = p.tile_rows;
   g.k_splits = p.splits;
 

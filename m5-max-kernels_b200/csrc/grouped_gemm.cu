@@ -48,7 +48,7 @@ struct Cfg {
   static constexpr int CHUNKS = TN / 64;                   // 32-column chunks of an epilogue warp
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 32 * (EPI_WARPS + 4);     // three warpgroups
-  static constexpr int SCALE_SLOTS = 2;                    // of four blocks of K each
+  static constexpr int SCALE_SLOTS = ROWS_M ? 2 : 8;       // of four blocks of K each
   static constexpr int SCALE_BYTES = BLOCKS ? SCALE_SLOTS * 4 * TN * 4 : 0;
   static constexpr int STORE_WARP = ROWS_M ? 2048 : 1024;  // a warp's bytes to rearrange stores
   static constexpr int STORE_BYTES = EPI_WARPS * STORE_WARP;
@@ -107,6 +107,21 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
 // that the thread has under way, 2.1 us a block of 128 channels instead of 0.35.
 __device__ __forceinline__ void mbar_arrive_tmem(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The two halves of a cluster barrier.
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void fence_cluster() {
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+}
+// Arrival that a fence_cluster before it makes a release.
+__device__ __forceinline__ void mbar_arrive_fenced(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+               : "memory");
 }
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
                                               uint32_t d) {
@@ -359,6 +374,12 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
     *abort_flag = 0;
     fence_mbarrier_init();
   }
+  // K split: the CTAs need one another's barriers only when they exchange their
+  // sums, and nothing of one another after that, so that they do not wait here
+  // and at the end (2.3 us of 14 for 3 x 7168 x 5376).
+  const bool exchange = !PAIR && splits > 1;
+  __syncwarp();
+  if (exchange) cluster_arrive();
   if (warp == 8 && lane == 0) {
     tma_prefetch_desc(&maps.b);
     tma_prefetch_desc(PAIR ? &maps.a128 : &maps.a64);
@@ -405,10 +426,11 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
     if (lane == 0) s_tile[g.groups] = before;
   }
   __syncthreads();
-  if (PAIR || splits > 1) cluster_sync();  // every CTA's barriers exist before any remote use
+  if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist before any remote use
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  bool exchanged = false;  // this warp has sent its sums
   Walk<C> walk{s_row, s_tile, g.groups, g.tile_rows, ch_tiles,
                   static_cast<int>(blockIdx.x) / per, static_cast<int>(gridDim.x) / per, 0};
   const int kb0 = PAIR ? 0 : static_cast<int>(int64_t(g.num_k_blocks) * rank / splits);
@@ -576,39 +598,44 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
       while (ok && walk.next(t)) {
         const float* sa = g.a_scales + t.row0 * g.as_row;
         const float* sb = g.b_scales + t.group * g.bs_group + t.ch0 / 128 * g.bs_n;
-        constexpr int ROWS = C::ROWS_M ? 2 : 1, COLS = C::ROWS_M ? 2 : 1;
-        for (int kq = kb0; kq < kb1; kq += 4, ++quad) {
-          // (the loads are under way before the slot is waited for)
-          float v[ROWS][4], w[COLS][4];
+        // All loads of QUADS of them are under way before the first is used.
+        constexpr int ROWS = C::ROWS_M ? 2 : 1, COLS = ROWS, QUADS = C::ROWS_M ? 1 : 4;
+        for (int k0 = kb0; k0 < kb1 && ok; k0 += 4 * QUADS) {
+          float v[ROWS][4 * QUADS], w[COLS][4 * QUADS];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const bool there = kq + k < kb1;
+          for (int k = 0; k < 4 * QUADS; ++k) {
+            const bool there = k0 + k < kb1;
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
               const int r = (C::ROWS_M ? static_cast<int>(rank) * 128 : 0) + me + 64 * i;
-              v[i][k] = there && r < t.rows ? __ldg(sa + r * g.as_row + (kq + k) * g.as_k) : 0.0f;
+              v[i][k] = there && r < t.rows ? __ldg(sa + r * g.as_row + (k0 + k) * g.as_k) : 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < COLS; ++j)
               w[j][k] = there && t.ch0 + j * 128 < g.n
-                            ? __ldg(sb + j * g.bs_n + (kq + k) * g.bs_k)
+                            ? __ldg(sb + j * g.bs_n + (k0 + k) * g.bs_k)
                             : 0.0f;
           }
-          const uint32_t slot = quad % C::SCALE_SLOTS;
-          ok = mbar_wait_bounded(&scale_empty[slot], ((quad / C::SCALE_SLOTS) & 1u) ^ 1u,
-                                 abort_flag, g.status, DEV_TIMEOUT_PRODUCER);
-          __syncwarp();
-          if (!ok) break;
-          float* s = s_scale + slot * 4 * C::TN + me;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+          for (int q = 0; q < QUADS; ++q) {
+            if (k0 + 4 * q >= kb1) break;
+            const uint32_t slot = quad % C::SCALE_SLOTS;
+            ok = mbar_wait_bounded(&scale_empty[slot], ((quad / C::SCALE_SLOTS) & 1u) ^ 1u,
+                                   abort_flag, g.status, DEV_TIMEOUT_PRODUCER);
+            __syncwarp();
+            if (!ok) break;
+            float* s = s_scale + slot * 4 * C::TN + me;
 #pragma unroll
-            for (int i = 0; i < ROWS; ++i)
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-              for (int j = 0; j < COLS; ++j)
-                s[k * C::TN + j * 128 + i * 64] = __fmul_rn(v[i][k], w[j][k]);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&scale_full[slot]);
+              for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+                for (int j = 0; j < COLS; ++j)
+                  s[k * C::TN + j * 128 + i * 64] = __fmul_rn(v[i][4 * q + k], w[j][4 * q + k]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&scale_full[slot]);
+            ++quad;
+          }
         }
       }
     }
@@ -793,8 +820,9 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
                     lane);
         out_buf ^= 1;
       };
-      if (!PAIR && splits > 1) {
+      if (exchange) {
         if constexpr (!PAIR) {
+          cluster_wait();  // (one tile a cluster: once)
           if constexpr (!BLOCKS) {
             if (has_chunk(t, 0)) {
               load_chunk(0, acc[0]);
@@ -816,9 +844,18 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
               st_cluster_v4(to + 512, acc[0][8 * i + 4], acc[0][8 * i + 5], acc[0][8 * i + 6],
                             acc[0][8 * i + 7]);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to_rank(parts, owner));
           }
+          // One fence for all: a release each would be four of them in a row.
+          __syncwarp();
+          fence_cluster();
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (lane == 0)
+              mbar_arrive_fenced(map_to_rank(parts, static_cast<uint32_t>((half * 4 + i) % splits)));
+          __syncwarp();
+          cluster_arrive();
+          exchanged = true;
           ok = mbar_wait_cluster(parts, 0, abort_flag, g.status, DEV_TIMEOUT_FIXUP);
           __syncwarp();
           if (!ok) break;
@@ -885,7 +922,15 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
   // ------------------------------------------------------------ teardown
   tc_fence_before();
   __syncthreads();
-  if (PAIR || splits > 1) cluster_sync();  // no CTA of the cluster touches this one any more
+  if constexpr (PAIR) cluster_sync();  // the peer no longer touches this CTA
+  if (exchange) {  // no CTA of the cluster sends to this one any more
+    __syncwarp();
+    if (!exchanged) {
+      cluster_wait();
+      cluster_arrive();
+    }
+    cluster_wait();
+  }
   if (warp == 9) {
     __syncwarp();
     tc_fence_after();
@@ -920,14 +965,59 @@ cudaError_t launch(const GroupedMaps& maps, const GroupedArgs& g, int grid, cuda
     attr[n_attr].val.clusterDim.z = 1;
     ++n_attr;
   }
-  cfg.attrs = n_attr ? attr : nullptr;
+  // (programmatic launch, see grid_dependency_wait)
+  attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
+  ++n_attr;
+  cfg.attrs = attr;
   cfg.numAttrs = n_attr;
   e = cudaLaunchKernelEx(&cfg, kern, maps, g);
   if (e != cudaSuccess) return e;
   return cudaGetLastError();
 }
 
+template <int KIND, bool BLOCKS>
+int split_clusters(int splits) {
+  using C = Cfg<BLOCKS, false>;
+  auto kern = grouped_gemm_kernel<KIND, BLOCKS, false>;
+  static std::atomic<int> known[kMaxLaunchDevices][4];  // + 1; of 1, 2, 4, 8
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxLaunchDevices) return 0;
+  std::atomic<int>& slot = known[dev][splits == 8 ? 3 : splits == 4 ? 2 : splits == 2 ? 1 : 0];
+  if (int n = slot.load(std::memory_order_relaxed)) return n - 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) !=
+      cudaSuccess)
+    return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(splits), 1, 1);
+  cfg.blockDim = dim3(C::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = splits;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) return 0;
+  slot.store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
 }  // namespace
+
+int grouped_split_clusters(int kind, bool blocks, int splits) {
+  switch (kind) {
+    case KIND_I8: return split_clusters<KIND_I8, false>(splits);
+    case KIND_F8:
+      return blocks ? split_clusters<KIND_F8, true>(splits)
+                    : split_clusters<KIND_F8, false>(splits);
+    case KIND_BF16: return split_clusters<KIND_BF16, false>(splits);
+    case KIND_F16: return split_clusters<KIND_F16, false>(splits);
+    default: return 0;
+  }
+}
 
 cudaError_t launch_grouped_gemm(const GroupedMaps& maps, const GroupedArgs& g, int kind,
                                 bool blocks, bool pair, int grid, cudaStream_t stream) {
