@@ -43,8 +43,12 @@ struct Cfg {
   static constexpr int STEP = PAIR ? 32 : 16;              // columns come in these
   static constexpr int M_BYTES = 128 * 128;                // this CTA's M operand of a stage
   static constexpr int N_BYTES = (PAIR ? TN / 2 : TN) * 128;  // and its N operand
+  static constexpr int FEW_ROWS = PAIR ? 64 : 16;          // a CTA's columns come in these, or all
   static constexpr int STAGES = PAIR ? 6 : 7;
-  static constexpr int BUFS = 512 / TN;                    // TMEM accumulators
+  // Blocks of K that change hands between MMAs and epilogue together, each with an
+  // accumulator of its own (few columns: a hand-over takes longer than a block).
+  static constexpr int BATCH = BLOCKS && !PAIR ? 4 : 1;
+  static constexpr int BUFS = 512 / (TN * BATCH);          // TMEM accumulators, or batches
   static constexpr int CHUNKS = TN / 64;                   // 32-column chunks of an epilogue warp
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 32 * (EPI_WARPS + 4);     // three warpgroups
@@ -209,17 +213,20 @@ struct Walk {
     if (unit >= first_tile[groups]) return false;
     while (unit >= first_tile[e + 1]) ++e;
     const int rows = first_row[e + 1] - first_row[e];  // positive: the group has tiles
-    const int row_tiles = (rows + tile_rows - 1) / tile_rows;
-    // Bands of at most 16 row tiles, within which the channel tiles follow one
-    // another: CTAs that run side by side share weights, and a band's rows stay in L2.
     const int u = unit - first_tile[e];
-    const int band = u / (16 * ch_tiles);
-    const int in_band = u - band * 16 * ch_tiles;
-    const int left = row_tiles - 16 * band;
-    const int wide = left < 16 ? left : 16;
-    const int ch = in_band / wide;
-    const int r = 16 * band + in_band - ch * wide;
-    const int each = ((rows + row_tiles - 1) / row_tiles + C::STEP - 1) / C::STEP * C::STEP;
+    int ch = u, r = 0, each = rows;  // one row tile
+    if (rows > tile_rows) {
+      const int row_tiles = (rows + tile_rows - 1) / tile_rows;
+      // Bands of at most 16 row tiles, within which the channel tiles follow one
+      // another: CTAs that run side by side share weights, and a band's rows stay in L2.
+      const int band = u / (16 * ch_tiles);
+      const int in_band = u - band * 16 * ch_tiles;
+      const int left = row_tiles - 16 * band;
+      const int wide = left < 16 ? left : 16;
+      ch = in_band / wide;
+      r = 16 * band + in_band - ch * wide;
+      each = ((rows + row_tiles - 1) / row_tiles + C::STEP - 1) / C::STEP * C::STEP;
+    }
     t.group = e;
     t.row0 = first_row[e] + r * each;
     // (positive too: tile_rows is a multiple of STEP, so each <= tile_rows and
@@ -383,7 +390,7 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
   if (warp == 8 && lane == 0) {
     tma_prefetch_desc(&maps.b);
     tma_prefetch_desc(PAIR ? &maps.a128 : &maps.a64);
-    tma_prefetch_desc(&maps.a16);
+    tma_prefetch_desc(PAIR ? &maps.a64 : &maps.a16);
   }
   if (warp == 9) {
     if constexpr (PAIR) {
@@ -398,14 +405,21 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
   grid_dependency_wait();
   // The groups' first rows, then the tiles before each group.
   const int ch_tiles = (g.n + C::TM - 1) / C::TM;
-  for (int e = threadIdx.x; e <= g.groups; e += C::THREADS) {
-    int r = g.group_start ? g.group_start[e] : (e == 0 ? 0 : g.rows);
-    r = r < 0 ? 0 : r;
-    s_row[e] = r < g.rows ? r : g.rows;
+  if (!g.group_start) {
+    if (threadIdx.x == 32) {
+      s_row[0] = s_tile[0] = 0;
+      s_row[1] = g.rows;
+      s_tile[1] = (g.rows + g.tile_rows - 1) / g.tile_rows * ch_tiles;
+    }
+  } else {
+    for (int e = threadIdx.x; e <= g.groups; e += C::THREADS) {
+      int r = g.group_start[e];
+      r = r < 0 ? 0 : r;
+      s_row[e] = r < g.rows ? r : g.rows;
+    }
+    __syncthreads();
   }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 0) {
+  if (g.group_start && warp == 0) {
     int before = 0;
     for (int e0 = 0; e0 < g.groups; e0 += 32) {
       const int e = e0 + lane;
@@ -425,6 +439,7 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
     }
     if (lane == 0) s_tile[g.groups] = before;
   }
+  tc_fence_before();
   __syncthreads();
   if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist before any remote use
   tc_fence_after();
@@ -456,7 +471,13 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
             (C::ROWS_M ? t.ch0 : t.row0) + (PAIR ? static_cast<int>(rank) * n_rows : 0);
         const int m_row =
             (C::ROWS_M ? t.row0 : t.ch0) + (PAIR ? static_cast<int>(rank) * 128 : 0);
-        const uint32_t bytes = C::M_BYTES + n_rows * 128;
+        // One box brings the columns' rows: of the next size, what lies behind the
+        // tile's is not used.
+        const bool few = n_rows <= C::FEW_ROWS;
+        const CUtensorMap* columns = few ? (PAIR ? &maps.a64 : &maps.a16)
+                                         : (PAIR ? &maps.a128 : &maps.a64);
+        const uint32_t bytes =
+            C::M_BYTES + (C::ROWS_M ? 128 : few ? C::FEW_ROWS : C::N_BYTES / 128) * 128;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, g.status,
                                  DEV_TIMEOUT_PRODUCER))
@@ -478,18 +499,10 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
               tma_load_3d_pair(m, &maps.b, &full[stage], kx, m_row, t.group);
             else
               tma_load_3d(m, &maps.b, &full[stage], kx, m_row, t.group);
-            for (int r = 0; r < n_rows;) {
-              const int left = n_rows - r;
-              const int take = left >= 128 ? 128 : left >= 64 ? 64 : 16;
-              const CUtensorMap* map = take == 128 ? &maps.a128
-                                       : take == 64 ? &maps.a64
-                                                    : &maps.a16;
-              if constexpr (PAIR)
-                tma_load_2d_pair(n + r * 128, map, &full[stage], kx, n_row + r);
-              else
-                tma_load_2d(n + r * 128, map, &full[stage], kx, n_row + r);
-              r += take;
-            }
+            if constexpr (PAIR)
+              tma_load_2d_pair(n, columns, &full[stage], kx, n_row);
+            else
+              tma_load_2d(n, columns, &full[stage], kx, n_row);
           }
           ++issued;
           if (++stage == C::STAGES) {
@@ -542,11 +555,13 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
         const uint32_t idesc = make_idesc(KIND, PAIR ? 256 : 128, C::ROWS_M ? C::TN : t.cols);
         if (!BLOCKS && !take_buffer()) break;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (BLOCKS && !take_buffer()) break;
+          const int in_batch = BLOCKS ? (kb - kb0) % C::BATCH : 0;
+          if (BLOCKS && in_batch == 0 && !take_buffer()) break;
           ok = mbar_wait_bounded(&full[stage], phase, abort_flag, g.status, DEV_TIMEOUT_MMA);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(buf * C::TN);
+          const uint32_t d_tmem =
+              tmem_base + static_cast<uint32_t>((buf * C::BATCH + in_batch) * C::TN);
           const uint32_t m = smem_u32(s_m + stage * C::M_BYTES);
           const uint32_t n = smem_u32(s_n + stage * C::N_BYTES);
 #pragma unroll
@@ -563,7 +578,7 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
             tc_commit_pair(&empty[stage]);
           else
             tc_commit(&empty[stage]);
-          if (BLOCKS) give_buffer();
+          if (BLOCKS && (in_batch == C::BATCH - 1 || kb + 1 == kb1)) give_buffer();
           if (++stage == C::STAGES) {
             stage = 0;
             phase ^= 1u;
@@ -743,19 +758,32 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
           ok = mbar_wait_bounded(&scale_full[slot], (quad / C::SCALE_SLOTS) & 1u, abort_flag,
                                  g.status, DEV_TIMEOUT_EPILOGUE);
           __syncwarp();
-          const float* sc = s_scale + slot * 4 * C::TN + half * 32;
-          for (int kb = kq; kb < kq + 4 && kb < kb1 && ok; ++kb, sc += C::TN) {
-            ok = wait_acc();
-            if (!ok) break;
-            if (has_chunk(t, 0)) {
-              uint32_t r[32];
-              load_chunk(0, r);
-              release_acc();
-              add_columns(r, acc[0],
-                          [&](int i) { return *reinterpret_cast<const float2*>(sc + i); });
-            } else {
-              release_acc();
+          if (!ok) break;
+          ok = wait_acc();
+          if (!ok) break;
+          if (has_chunk(t, 0)) {
+            const float* sc = s_scale + slot * 4 * C::TN + half * 32;
+            const uint32_t from =
+                tmem_warp + static_cast<uint32_t>(buf * C::BATCH * C::TN + half * 32);
+            // (two at a time: more need more registers than there are)
+#pragma unroll
+            for (int k0 = 0; k0 < 4; k0 += 2) {
+              uint32_t r[2][32];
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+                if (kq + k0 + k < kb1) tmem_ld32(from + (k0 + k) * C::TN, r[k]);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) tmem_wait32(r[k]);
+              if (k0 == 2) release_acc();
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+                if (kq + k0 + k < kb1)
+                  add_columns(r[k], acc[0], [&](int i) {
+                    return *reinterpret_cast<const float2*>(sc + (k0 + k) * C::TN + i);
+                  });
             }
+          } else {
+            release_acc();
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&scale_empty[slot]);
