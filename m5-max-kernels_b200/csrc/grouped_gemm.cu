@@ -58,7 +58,8 @@ struct Cfg {
   static constexpr int STORE_BYTES = EPI_WARPS * STORE_WARP;
   static constexpr int EXCHANGE_BYTES = PAIR ? 0 : TN * 128 * 4;
   static constexpr int TABLE_BYTES = 2 * (kMaxGroups + 4) * 4;
-  static constexpr int BAR_BYTES = (2 * STAGES + 2 * BUFS + 2 * SCALE_SLOTS + 2) * 8 + 16;
+  static constexpr int BAR_BYTES = (2 * STAGES + 2 * BUFS + 2 * SCALE_SLOTS + 2) * 8 + 16 +
+                                   SCALE_SLOTS * 16;
   static constexpr int SMEM_BYTES = 1024 + STAGES * (M_BYTES + N_BYTES) + EXCHANGE_BYTES +
                                     SCALE_BYTES + STORE_BYTES + TABLE_BYTES + BAR_BYTES;
   static_assert(SMEM_BYTES <= 232448, "shared memory per CTA exceeds 227 KB");
@@ -355,6 +356,8 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
   uint64_t* parts = drain + 1;  // K split: the owned rows' sums of all ranks are here
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(parts + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  // ROWS_M: the tile that a slot's scales begin, {first row, rows (0: no more), first channel}
+  volatile int* slot_tile = reinterpret_cast<volatile int*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -454,10 +457,10 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
 
   // The fp32 sums of a pair's tile are 128 registers a thread of the epilogue:
   // it takes over registers of the other warps.  (384 threads are launched with
-  // 168 each; 2 * 216 + 64 <= 3 * 168.)
+  // 168 each: 2 * 216 + 72 = 3 * 168.)
   constexpr bool MOVE_REGS = C::ROWS_M;
   if (warp >= C::EPI_WARPS) {
-    if constexpr (MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
@@ -556,23 +559,24 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
         if (!BLOCKS && !take_buffer()) break;
         for (int kb = kb0; kb < kb1; ++kb) {
           const int in_batch = BLOCKS ? (kb - kb0) % C::BATCH : 0;
-          if (BLOCKS && in_batch == 0 && !take_buffer()) break;
+          // (all that the MMAs need is ready before the accumulator is)
           ok = mbar_wait_bounded(&full[stage], phase, abort_flag, g.status, DEV_TIMEOUT_MMA);
           if (!ok) break;
-          tc_fence_after();
           const uint32_t d_tmem =
               tmem_base + static_cast<uint32_t>((buf * C::BATCH + in_batch) * C::TN);
-          const uint32_t m = smem_u32(s_m + stage * C::M_BYTES);
-          const uint32_t n = smem_u32(s_n + stage * C::N_BYTES);
+          const uint64_t m = smem_desc_k128(smem_u32(s_m + stage * C::M_BYTES));
+          const uint64_t n = smem_desc_k128(smem_u32(s_n + stage * C::N_BYTES));
+          if (BLOCKS && in_batch == 0) {
+            if (!take_buffer()) break;
+          }
+          tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 4; ++k) {  // 32 bytes of K further: 2 in the descriptors
             const uint32_t accumulate = (k != 0 || (!BLOCKS && kb != kb0)) ? 1u : 0u;
             if constexpr (PAIR)
-              tc_mma_pair<KIND>(d_tmem, smem_desc_k128(m + k * 32), smem_desc_k128(n + k * 32),
-                                idesc, accumulate);
+              tc_mma_pair<KIND>(d_tmem, m + 2 * k, n + 2 * k, idesc, accumulate);
             else
-              tc_mma<KIND>(d_tmem, smem_desc_k128(m + k * 32), smem_desc_k128(n + k * 32), idesc,
-                           accumulate);
+              tc_mma<KIND>(d_tmem, m + 2 * k, n + 2 * k, idesc, accumulate);
           }
           if constexpr (PAIR)
             tc_commit_pair(&empty[stage]);
@@ -647,11 +651,24 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < COLS; ++j)
                   s[k * C::TN + j * 128 + i * 64] = __fmul_rn(v[i][4 * q + k], w[j][4 * q + k]);
+            if (C::ROWS_M && me == 0 && k0 == kb0) {
+              slot_tile[slot * 4] = t.row0;
+              slot_tile[slot * 4 + 1] = t.rows;
+              slot_tile[slot * 4 + 2] = t.ch0;
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&scale_full[slot]);
             ++quad;
           }
         }
+      }
+      if (C::ROWS_M && ok) {
+        const uint32_t slot = quad % C::SCALE_SLOTS;
+        ok = mbar_wait_bounded(&scale_empty[slot], ((quad / C::SCALE_SLOTS) & 1u) ^ 1u, abort_flag,
+                               g.status, DEV_TIMEOUT_PRODUCER);
+        if (me == 0) slot_tile[slot * 4 + 1] = 0;
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(&scale_full[slot]);
       }
     }
   } else {
@@ -709,7 +726,26 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
     uint32_t quad = 0;
     Tile t;
     bool ok = true;
-    while (ok && walk.next(t)) {
+    auto wait_scales = [&]() {
+      ok = mbar_wait_lean(smem_u32(scale_full) + quad % C::SCALE_SLOTS * 8,
+                          (quad / C::SCALE_SLOTS) & 1u, smem_u32(const_cast<int*>(abort_flag)),
+                          g.status, DEV_TIMEOUT_EPILOGUE);
+      __syncwarp();
+      return ok;
+    };
+    while (ok) {
+      if constexpr (C::ROWS_M) {
+        // (the warps that bring the scales walk the tiles: there are no registers
+        // for that here)
+        if (!wait_scales()) break;
+        volatile int* info = slot_tile + quad % C::SCALE_SLOTS * 4;
+        t.row0 = info[0];
+        t.rows = info[1];
+        t.ch0 = info[2];
+        if (t.rows == 0) break;
+      } else {
+        if (!walk.next(t)) break;
+      }
       if constexpr (BLOCKS) {
 #pragma unroll
         for (int c = 0; c < C::CHUNKS; ++c)
@@ -721,14 +757,7 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
         const float* sc = s_scale + half * 128 + quarter * 32 + lane;
 #pragma unroll 1
         for (int kb = 0; kb < kb1; ++kb) {
-          if ((kb & 3) == 0) {
-            ok = mbar_wait_lean(smem_u32(scale_full) + quad % C::SCALE_SLOTS * 8,
-                                (quad / C::SCALE_SLOTS) & 1u,
-                                smem_u32(const_cast<int*>(abort_flag)), g.status,
-                                DEV_TIMEOUT_EPILOGUE);
-            __syncwarp();
-            if (!ok) break;
-          }
+          if ((kb & 3) == 0 && kb != 0 && !wait_scales()) break;
           const float one = sc[((quad % C::SCALE_SLOTS) * 4 + (kb & 3)) * C::TN];
           const float2 s = make_float2(one, one);
           ok = wait_acc();
