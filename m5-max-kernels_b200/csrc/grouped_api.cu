@@ -34,27 +34,44 @@ struct Plan {
   int tile_rows, splits, grid;
 };
 
-// Tiles and schedule.  Groups of few rows are bound by their weights: 64-row
-// tiles on single CTAs, several of which share a tile's K range where the tiles
-// do not fill the GPU.  Others take 256 channels x up to 256 rows on CTA pairs.
+// Tiles and schedule.  Single CTAs take 128 channels x 64 rows, several of them
+// (a cluster) sharing the K range where the tiles do not fill the GPU; CTA pairs
+// take 256 channels x 256 rows.  Taken is what needs less time for its waves, a
+// block of 128 bytes of K costing 0.32 us on a single CTA and 0.40 us on a pair
+// (0.56 where it is scaled by itself), as measured at 128 blocks and more: 200 x
+// 4096 x 16384 block-scaled 38 against 73 us, 517 rows 80 against 74; 65 rows 25
+// against 72.  Of several groups' sizes only the sum is known here: each is
+// taken to end in the middle of a tile.
 Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, bool blocks,
               int sms) {
-  Plan p{};
   const int64_t busy = groups < rows ? groups : rows;  // groups with rows, at most
-  const int64_t each = ceil_div(rows, groups);
-  p.pair = each > kSingleTileRows;
+  const int64_t half = groups == 1 ? 0 : busy;         // of a tile each
+  auto waves = [&](int64_t tile_rows, int64_t ch, int64_t units, double block, int64_t splits) {
+    const int64_t ch_tiles = ceil_div(n, ch);
+    const int64_t tiles = groups == 1 ? ceil_div(rows, tile_rows)
+                                      : ceil_div(2 * rows + tile_rows * half, 2 * tile_rows);
+    return ceil_div(tiles * ch_tiles * splits, units) * ceil_div(nkb, splits) * block;
+  };
+  // (every group rounds its last tile up: no more tiles than these)
+  const auto most_tiles = [&](int64_t tile_rows, int64_t ch) {
+    return (groups == 1 ? ceil_div(rows, tile_rows) : rows / tile_rows + busy) * ceil_div(n, ch);
+  };
+  Plan p{};
+  // a cluster has one tile, and all of them run at once
+  int64_t tiles = most_tiles(kSingleTileRows, 128);
   p.splits = 1;
+  while (p.splits < 8 && tiles * p.splits * 2 <= sms && nkb >= p.splits * 2 * 4 &&
+         tiles <= grouped_split_clusters(kind, blocks, p.splits * 2))
+    p.splits *= 2;
+  const double single = waves(kSingleTileRows, 128, sms, 0.32, p.splits);
+  const double pair = waves(kPairTileRows, 256, sms / 2, blocks ? 0.56 : 0.40, 1);
+  p.pair = pair < single;
+  if (p.pair) {
+    tiles = most_tiles(kPairTileRows, 256);
+    p.splits = 1;
+  }
   p.tile_rows = p.pair ? kPairTileRows : kSingleTileRows;
-  const int64_t ch_tiles = ceil_div(n, p.pair ? 256 : 128);
-  // (every group rounds its last tile up)
-  int64_t tiles = (rows / p.tile_rows + busy) * ch_tiles;
-  if (groups == 1) tiles = ceil_div(rows, p.tile_rows) * ch_tiles;
   const int64_t units = p.pair ? sms / 2 : sms;
-  // (a cluster has one tile, and all of them run at once)
-  if (!p.pair)
-    while (p.splits < 8 && tiles * p.splits * 2 <= units && nkb >= p.splits * 2 * 4 &&
-           tiles <= grouped_split_clusters(kind, blocks, p.splits * 2))
-      p.splits *= 2;
   const int64_t used = tiles < units ? tiles : units;
   p.grid = static_cast<int>(used) * (p.pair ? 2 : p.splits);
   return p;

@@ -817,9 +817,20 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&scale_empty[slot]);
         }
-      } else {
-        ok = wait_acc();
       }
+      // Scales of rows and channels: this thread's channel, and a row of each chunk.
+      const int ch = t.ch0 + (PAIR ? static_cast<int>(rank) * 128 : 0) + quarter * 32;
+      constexpr bool ROW_SCALES = !BLOCKS && (KIND == KIND_I8 || KIND == KIND_F8);
+      float sb = 1.0f, sa[C::CHUNKS];
+      if constexpr (ROW_SCALES) {
+        if (ch + lane < g.n) sb = __ldg(g.b_scales + t.group * g.bs_group + (ch + lane) * g.bs_n);
+#pragma unroll
+        for (int c = 0; c < C::CHUNKS; ++c) {
+          const int r = (2 * c + half) * 32 + lane;
+          sa[c] = r < t.rows ? __ldg(g.a_scales + (int64_t(t.row0) + r) * g.as_row) : 0.0f;
+        }
+      }
+      if constexpr (!BLOCKS) ok = wait_acc();
       if (!ok) break;
 
       if constexpr (C::ROWS_M) {
@@ -853,11 +864,6 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
         }
         continue;
       }
-      const int ch = t.ch0 + (PAIR ? static_cast<int>(rank) * 128 : 0) + quarter * 32;
-      constexpr bool ROW_SCALES = !BLOCKS && (KIND == KIND_I8 || KIND == KIND_F8);
-      float sb = 1.0f;
-      if constexpr (ROW_SCALES)
-        if (ch + lane < g.n) sb = __ldg(g.b_scales + t.group * g.bs_group + (ch + lane) * g.bs_n);
       // Rows 8 i .. 8 i + 7 of chunk c, whose sums r holds.
       auto finish = [&](const uint32_t (&r)[32], int c, int i) {
         const int first = (2 * c + half) * 32 + 8 * i;
@@ -866,12 +872,8 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           v[j] = sum_value<KIND>(r[8 * i + j]);
-          if constexpr (ROW_SCALES) {
-            const float sa = first + j < t.rows
-                                 ? __ldg(g.a_scales + (int64_t(t.row0) + first + j) * g.as_row)
-                                 : 0.0f;
-            v[j] = __fmul_rn(__fmul_rn(v[j], sa), sb);
-          }
+          if constexpr (ROW_SCALES)
+            v[j] = __fmul_rn(__fmul_rn(v[j], __shfl_sync(0xffffffffu, sa[c], 8 * i + j)), sb);
         }
         store_rows8(g, v, stage_out + out_buf * 512, int64_t(t.row0) + first, t.rows - first, ch,
                     lane);
@@ -946,7 +948,9 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
             for (int i = 0; i < 4; ++i) finish(acc[c], c, i);
           }
         } else {
-          for (int c = 0; c < C::CHUNKS && has_chunk(t, c); ++c) {
+#pragma unroll
+          for (int c = 0; c < C::CHUNKS; ++c) {
+            if (!has_chunk(t, c)) break;
             uint32_t r[32];
             load_chunk(c, r);
             if (!(c + 1 < C::CHUNKS && has_chunk(t, c + 1))) release_acc();
