@@ -53,7 +53,9 @@ struct Cfg {
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 32 * (EPI_WARPS + 4);     // three warpgroups
   static constexpr int SCALE_SLOTS = ROWS_M ? 2 : 8;       // of four blocks of K each
-  static constexpr int SCALE_BYTES = BLOCKS ? SCALE_SLOTS * 4 * TN * 4 : 0;
+  // Block scales' slots, or each epilogue warp's rows' scales.
+  static constexpr int SCALE_BYTES =
+      BLOCKS ? SCALE_SLOTS * 4 * TN * 4 : EPI_WARPS * CHUNKS * 32 * 4;
   static constexpr int STORE_WARP = ROWS_M ? 2048 : 1024;  // a warp's bytes to rearrange stores
   static constexpr int STORE_BYTES = EPI_WARPS * STORE_WARP;
   static constexpr int EXCHANGE_BYTES = PAIR ? 0 : TN * 128 * 4;
@@ -255,36 +257,44 @@ __device__ __forceinline__ uint32_t sum_add(uint32_t a, uint32_t b) {
     return __float_as_uint(__fadd_rn(__uint_as_float(a), __uint_as_float(b)));
 }
 
-// Eight rows (row .. row + 7, of which the first `rows` exist) of channel
-// ch + lane; ch: this warp's first of 32.  stage: 512 bytes of the warp's, in
-// which 16-bit values become rows of 32 channels for 16-byte stores.
-__device__ __forceinline__ void store_rows8(const GroupedArgs& g, const float (&v)[8],
-                                            uint8_t* stage, int64_t row, int rows, int ch,
+// Eight rows, of which the first `rows` exist, of this lane's channel.  at: the
+// first row's 32 channels of the warp, of which `channels` exist; stage: 512 bytes
+// of the warp's, in which 16-bit values become rows for 16-byte stores.
+__device__ __forceinline__ void store_rows8(const GroupedArgs& g, const float2 (&v)[4],
+                                            uint8_t* stage, uint8_t* at, int rows, int channels,
                                             int lane) {
   if (g.out_dtype == DT_F32) {
-    float* o = reinterpret_cast<float*>(g.out) + row * g.out_row + ch + lane;
+    float* o = reinterpret_cast<float*>(at) + lane;
+    if (lane >= channels) return;
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if (r < rows && ch + lane < g.n) o[r * g.out_row] = v[r];
+    for (int r = 0; r < 8; ++r) {
+      if (r < rows) *o = r & 1 ? v[r >> 1].y : v[r >> 1].x;
+      o += g.out_row;
+    }
     return;
   }
   uint16_t* mine = reinterpret_cast<uint16_t*>(stage) + lane;
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    if (g.out_dtype == DT_F16)
-      mine[r * 32] = __half_as_ushort(__float2half_rn(v[r]));
-    else
-      mine[r * 32] = __bfloat16_as_ushort(__float2bfloat16_rn(v[r]));
+  for (int r = 0; r < 8; r += 2) {
+    uint32_t two;
+    if (g.out_dtype == DT_F16) {
+      const __half2 h = __float22half2_rn(v[r >> 1]);
+      two = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      two = f2_bf16x2(v[r >> 1]);
+    }
+    mine[r * 32] = static_cast<uint16_t>(two);
+    mine[r * 32 + 32] = static_cast<uint16_t>(two >> 16);
   }
   __syncwarp();
-  uint16_t* o = reinterpret_cast<uint16_t*>(g.out);
+  uint16_t* o = reinterpret_cast<uint16_t*>(at);
   if (g.out_vec) {
     const int r = lane >> 2, piece = lane & 3;
     const uint4 w = *reinterpret_cast<const uint4*>(stage + lane * 16);
-    if (r < rows && ch + 8 * piece < g.n)
-      *reinterpret_cast<uint4*>(o + (row + r) * g.out_row + ch + 8 * piece) = w;
-  } else if (ch + lane < g.n) {
-    for (int r = 0; r < rows && r < 8; ++r) o[(row + r) * g.out_row + ch + lane] = mine[r * 32];
+    if (r < rows && 8 * piece < channels)
+      *reinterpret_cast<uint4*>(o + r * g.out_row + 8 * piece) = w;
+  } else if (lane < channels) {
+    for (int r = 0; r < rows && r < 8; ++r) o[r * g.out_row + lane] = mine[r * 32];
   }
 }
 
@@ -679,6 +689,7 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
     const uint32_t tmem_warp = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t empty0 = PAIR ? map_to_rank(acc_empty, 0) : 0u;  // in the even CTA
     uint8_t* stage_out = s_store + warp * C::STORE_WARP;
+    float* row_scales = s_scale + warp * C::CHUNKS * 32;
     int out_buf = 0;
     int buf = 0;
     uint32_t buf_phase = 0;
@@ -821,15 +832,22 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
       // Scales of rows and channels: this thread's channel, and a row of each chunk.
       const int ch = t.ch0 + (PAIR ? static_cast<int>(rank) * 128 : 0) + quarter * 32;
       constexpr bool ROW_SCALES = !BLOCKS && (KIND == KIND_I8 || KIND == KIND_F8);
-      float sb = 1.0f, sa[C::CHUNKS];
+      float sb = 1.0f;
       if constexpr (ROW_SCALES) {
         if (ch + lane < g.n) sb = __ldg(g.b_scales + t.group * g.bs_group + (ch + lane) * g.bs_n);
+        __syncwarp();  // (all lanes are done with the last tile's)
 #pragma unroll
         for (int c = 0; c < C::CHUNKS; ++c) {
           const int r = (2 * c + half) * 32 + lane;
-          sa[c] = r < t.rows ? __ldg(g.a_scales + (int64_t(t.row0) + r) * g.as_row) : 0.0f;
+          row_scales[c * 32 + lane] =
+              r < t.rows ? __ldg(g.a_scales + (int64_t(t.row0) + r) * g.as_row) : 0.0f;
         }
+        __syncwarp();
       }
+      const int channels = g.n - ch;  // from this warp's first on
+      uint8_t* out = static_cast<uint8_t*>(g.out) +
+                     (t.row0 * g.out_row + ch) * (g.out_dtype == DT_F32 ? 4 : 2);
+      const int64_t out_step = 8 * g.out_row * (g.out_dtype == DT_F32 ? 4 : 2);
       if constexpr (!BLOCKS) ok = wait_acc();
       if (!ok) break;
 
@@ -866,17 +884,23 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
       }
       // Rows 8 i .. 8 i + 7 of chunk c, whose sums r holds.
       auto finish = [&](const uint32_t (&r)[32], int c, int i) {
-        const int first = (2 * c + half) * 32 + 8 * i;
-        if (first >= t.rows) return;
-        float v[8];
+        const int eight = (2 * c + half) * 4 + i;
+        if (8 * eight >= t.rows) return;
+        float2 v[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[j] = sum_value<KIND>(r[8 * i + j]);
-          if constexpr (ROW_SCALES)
-            v[j] = __fmul_rn(__fmul_rn(v[j], __shfl_sync(0xffffffffu, sa[c], 8 * i + j)), sb);
+        for (int j = 0; j < 4; ++j)
+          v[j] = make_float2(sum_value<KIND>(r[8 * i + 2 * j]), sum_value<KIND>(r[8 * i + 2 * j + 1]));
+        if constexpr (ROW_SCALES) {
+          const float4* sa = reinterpret_cast<const float4*>(row_scales + c * 32 + 8 * i);
+          const float4 lo = sa[0], hi = sa[1];
+          const float2 by = make_float2(sb, sb);
+          v[0] = __fmul2_rn(__fmul2_rn(v[0], make_float2(lo.x, lo.y)), by);
+          v[1] = __fmul2_rn(__fmul2_rn(v[1], make_float2(lo.z, lo.w)), by);
+          v[2] = __fmul2_rn(__fmul2_rn(v[2], make_float2(hi.x, hi.y)), by);
+          v[3] = __fmul2_rn(__fmul2_rn(v[3], make_float2(hi.z, hi.w)), by);
         }
-        store_rows8(g, v, stage_out + out_buf * 512, int64_t(t.row0) + first, t.rows - first, ch,
-                    lane);
+        store_rows8(g, v, stage_out + out_buf * 512, out + eight * out_step, t.rows - 8 * eight,
+                    channels, lane);
         out_buf ^= 1;
       };
       if (exchange) {
