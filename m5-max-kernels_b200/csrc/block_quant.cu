@@ -98,19 +98,36 @@ __device__ __forceinline__ uint32_t peak_of(const Raw<T>& r) {
   }
 }
 
-// v = silu(g) x of 2 i, 2 i + 1.  Between -80 and 80 the quotient g / d, d = 1 +
-// exp(-g), comes from a reciprocal with one Newton step and one correction step
-// (Markstein's, as in i8_pair_div: right but for the rarest ulp); elsewhere
-// divides, since d may be infinite.
-constexpr float kSiluFast = 80.0f;
-__device__ __forceinline__ float2 silu_fast(float2 g, float2 x) {
-  const float2 one = make_float2(1.0f, 1.0f);
-  const float2 d = __fadd2_rn(one, make_float2(expf(-g.x), expf(-g.y)));
-  const float2 nd = make_float2(-d.x, -d.y);
+// 1 / d of a packed pair of normal numbers whose reciprocals are normal: a Newton
+// step after the approximation, right but for the rarest ulp.
+__device__ __forceinline__ float2 reciprocal(float2 d, float2 nd) {
   float2 y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(d.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(d.y));
-  y = __ffma2_rn(__ffma2_rn(nd, y, one), y, y);
+  return __ffma2_rn(__ffma2_rn(nd, y, make_float2(1.0f, 1.0f)), y, y);
+}
+
+// silu(g) x for |g| <= kSiluFast: exp(-g) = 2^t, t = -g log2 e in two parts (the
+// constant in two, the product's rounding error from one multiply-add), of which
+// the second, below 2^-17, is multiplied on: 2^(hi + lo) = 2^hi (1 + lo ln 2).
+// The quotient is Markstein's, as in i8_pair_div.  Elsewhere exp may be infinite:
+// silu() divides.
+constexpr float kSiluFast = 80.0f;
+__device__ __forceinline__ float2 silu_fast(float2 g, float2 x) {
+  const float2 one = make_float2(1.0f, 1.0f);
+  const float2 l_hi = make_float2(-0x1.715476p+0f, -0x1.715476p+0f);    // -log2 e
+  const float2 l_lo = make_float2(-0x1.4ae0c0p-26f, -0x1.4ae0c0p-26f);  // what that lacks
+  const float2 ln2 = make_float2(0x1.62e430p-1f, 0x1.62e430p-1f);
+  const float2 hi = __fmul2_rn(g, l_hi);
+  const float2 lo =
+      __ffma2_rn(g, l_lo, __ffma2_rn(g, l_hi, make_float2(-hi.x, -hi.y)));
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(hi.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(hi.y));
+  e = __ffma2_rn(e, __fmul2_rn(lo, ln2), e);
+  const float2 d = __fadd2_rn(one, e);
+  const float2 nd = make_float2(-d.x, -d.y);
+  const float2 y = reciprocal(d, nd);
   const float2 q = __fmul2_rn(g, y);
   return __fmul2_rn(__ffma2_rn(__ffma2_rn(nd, q, g), y, q), x);
 }
@@ -118,20 +135,36 @@ __device__ __forceinline__ float silu(float g) {
   return __fdiv_rn(g, __fadd_rn(1.0f, expf(-g)));
 }
 
-__device__ __forceinline__ float block_scale(uint32_t peak) {
-  const float s = __fdiv_rn(__uint_as_float(peak), 448.0f);
-  return s == 0.0f ? 1.0f : s;
+// A block's scale, and whether quotients by it may go by multiplications: where
+// peak / 448, its reciprocal and the residuals below stay normal.
+struct Scale {
+  float s;
+  bool fast;
+};
+__device__ __forceinline__ Scale block_scale(uint32_t peak) {
+  const float p = __uint_as_float(peak);
+  Scale r;
+  r.fast = p >= 0x1p-80f && p <= 0x1p100f;
+  if (r.fast) {  // RN(p / 448): Markstein's step with RN(1 / 448)
+    const float q = __fmul_rn(p, 1.0f / 448.0f);
+    r.s = __fmaf_rn(__fmaf_rn(-448.0f, q, p), 1.0f / 448.0f, q);
+  } else {
+    r.s = __fdiv_rn(p, 448.0f);
+    if (r.s == 0.0f) r.s = 1.0f;
+  }
+  return r;
 }
 
-// Stores the codes of kLane values, of which the first `count` exist.  Where
-// neither the scale nor its reciprocal leaves the normal range, quot_pair_div is
-// the correctly rounded quotient wherever that is not far below half the
-// smallest code (2^-10); elsewhere divides.
+// Stores the codes of kLane values, of which the first `count` exist.  The
+// quotient RN(v / s) decides at ties, wherever it is not far below half the
+// smallest code (2^-10): quot_pair_div.
 template <bool VEC, class Pair>
-__device__ __forceinline__ void store_codes(uint8_t* q, int count, float scale, Pair pair_at) {
+__device__ __forceinline__ void store_codes(uint8_t* q, int count, Scale scale, Pair pair_at) {
   uint32_t w[kLane / 4];
-  if (scale >= kI8DivMinScale && scale <= 0x1p100f) {
-    const I8Div d = i8_div(__frcp_rn(scale), scale);
+  if (scale.fast) {
+    I8Div d;
+    d.ns = make_float2(-scale.s, -scale.s);
+    d.y = reciprocal(make_float2(scale.s, scale.s), d.ns);
 #pragma unroll
     for (int i = 0; i < kLane / 4; ++i)
       w[i] = __nv_cvt_float2_to_fp8x2(quot_pair_div(pair_at(2 * i), d), __NV_SATFINITE,
@@ -143,7 +176,7 @@ __device__ __forceinline__ void store_codes(uint8_t* q, int count, float scale, 
 #pragma unroll
     for (int i = 0; i < kLane / 4; ++i) {
       const float2 a = pair_at(2 * i), b = pair_at(2 * i + 1);
-      w[i] = e4m3_word_exact(a.x, a.y, b.x, b.y, scale);
+      w[i] = e4m3_word_exact(a.x, a.y, b.x, b.y, scale.s);
     }
   }
   if constexpr (VEC) {
@@ -167,6 +200,7 @@ __global__ void __launch_bounds__(kThreads)
   const unsigned col_step = stride - row_step * blocks_per_row;
   const T* x = static_cast<const T*>(a.x);
   const T* gate = static_cast<const T*>(a.gate);
+  const int k = static_cast<int>(a.k), x_rows = static_cast<int>(a.x_rows);
   unsigned b = blockIdx.x * kRows + threadIdx.x / kLanes;
   unsigned row = b / blocks_per_row, block = b - row * blocks_per_row;
   // (whole warps leave the loop together: the shuffles below name all lanes)
@@ -177,16 +211,16 @@ __global__ void __launch_bounds__(kThreads)
     unsigned which[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int64_t col = int64_t(block) * 128 + sub * kLane;
-      const int64_t left = b < total ? a.k - col : 0;
+      const int col = static_cast<int>(block * 128) + sub * kLane;
+      const int left = b < total ? k - col : 0;
       which[u] = b;
-      at[u] = int64_t(row) * a.k + col;
-      count[u] = static_cast<int>(left < 0 ? 0 : left > kLane ? kLane : left);
-      int64_t src = row;
+      at[u] = int64_t(row) * k + col;
+      count[u] = left < 0 ? 0 : left > kLane ? kLane : left;
+      int src = static_cast<int>(row);
       int here = count[u];
       if (a.index && here > 0) {
         src = a.index[row];
-        if (src < 0 || src >= a.x_rows) here = 0;  // a row of zeros
+        if (src < 0 || src >= x_rows) here = 0;  // a row of zeros
       }
       rx[u] = load_any<T, VEC>(x + src * a.x_row + col, here);
       if constexpr (GATE) rg[u] = load_any<T, VEC>(gate + src * a.gate_row + col, here);
@@ -222,8 +256,8 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int d = kLanes / 2; d; d >>= 1)
         peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, d));
-      const float scale = block_scale(peak);
-      if (which[u] < total && sub == 0) a.scales[which[u]] = scale;
+      const Scale scale = block_scale(peak);
+      if (which[u] < total && sub == 0) a.scales[which[u]] = scale.s;
       if (count[u] > 0)
         store_codes<VEC>(a.q + at[u], count[u], scale, [&](int i) {
           if constexpr (GATE)
@@ -265,8 +299,8 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kThreads / 32; ++i) peak = max(peak, s_peak[i]);
-  const float scale = block_scale(peak);
-  if (threadIdx.x == 0) a.scales[b] = scale;
+  const Scale scale = block_scale(peak);
+  if (threadIdx.x == 0) a.scales[b] = scale.s;
   uint8_t* q = a.q + int64_t(batch) * a.rows * a.k + col;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
