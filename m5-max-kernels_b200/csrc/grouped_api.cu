@@ -42,8 +42,7 @@ struct Plan {
 // 4096 x 16384 block-scaled 38 against 73 us, 517 rows 80 against 74; 65 rows 25
 // against 72.  Of several groups' sizes only the sum is known here: each is
 // taken to end in the middle of a tile.
-Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, bool blocks,
-              int sms) {
+Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, int add, int sms) {
   const int64_t busy = groups < rows ? groups : rows;  // groups with rows, at most
   const int64_t half = groups == 1 ? 0 : busy;         // of a tile each
   auto waves = [&](int64_t tile_rows, int64_t ch, int64_t units, double block, int64_t splits) {
@@ -61,10 +60,10 @@ Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, bo
   int64_t tiles = most_tiles(kSingleTileRows, 128);
   p.splits = 1;
   while (p.splits < 8 && tiles * p.splits * 2 <= sms && nkb >= p.splits * 2 * 4 &&
-         tiles <= grouped_split_clusters(kind, blocks, p.splits * 2))
+         tiles <= grouped_split_clusters(kind, add, p.splits * 2))
     p.splits *= 2;
   const double single = waves(kSingleTileRows, 128, sms, 0.32, p.splits);
-  const double pair = waves(kPairTileRows, 256, sms / 2, blocks ? 0.56 : 0.40, 1);
+  const double pair = waves(kPairTileRows, 256, sms / 2, add == GROUPED_ADD_SCALED ? 0.56 : 0.40, 1);
   p.pair = pair < single;
   if (p.pair) {
     tiles = most_tiles(kPairTileRows, 256);
@@ -182,8 +181,10 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
   int sms = 0;
   int rc = current_device_state(&g.status, &sms);
   if (rc) return rc;
-  const Plan p = plan_for(s->rows, s->groups, s->n, g.num_k_blocks, kind,
-                          s->block_scales != 0, sms);
+  const int add = s->block_scales                         ? GROUPED_ADD_SCALED
+                  : elem == 2 && s->out_dtype == M5B_F32 ? GROUPED_ADD_PARTS
+                                                         : GROUPED_ADD_NONE;
+  const Plan p = plan_for(s->rows, s->groups, s->n, g.num_k_blocks, kind, add, sms);
   g.tile_rows = p.tile_rows;
   g.k_splits = p.splits;
 
@@ -200,7 +201,7 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
       !make_swizzled_map(&m.a16, bytes, 2, s->a, a_dims, a_strides, box16) ||
       !make_swizzled_map(&m.b, bytes, 3, s->b, b_dims, b_strides, box128))
     return set_last_error(M5B_ECUDA, "cuTensorMapEncodeTiled failed");
-  return launched(launch_grouped_gemm(m, g, kind, s->block_scales != 0, p.pair, p.grid,
+  return launched(launch_grouped_gemm(m, g, kind, add, p.pair, p.grid,
                                       static_cast<cudaStream_t>(stream)),
                   "grouped GEMM launch");
 }

@@ -35,8 +35,10 @@ namespace m5b {
 
 namespace {
 
-template <bool BLOCKS, bool PAIR>
+template <int ADD, bool PAIR>
 struct Cfg {
+  static constexpr bool BLOCKS = ADD == GROUPED_ADD_SCALED;
+  static constexpr bool PARTS = ADD == GROUPED_ADD_PARTS;  // blocks of an accumulator: four
   static constexpr bool ROWS_M = BLOCKS && PAIR;           // the rows are the M operand
   static constexpr int TN = PAIR ? 256 : kSingleTileRows;  // columns of an accumulator
   static constexpr int TM = PAIR ? 256 : 128;              // channels of a tile
@@ -340,10 +342,11 @@ __device__ __forceinline__ void store_rows32(const GroupedArgs& g, const uint32_
   __syncwarp();
 }
 
-template <int KIND, bool BLOCKS, bool PAIR>
-__global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
+template <int KIND, int ADD, bool PAIR>
+__global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
     grouped_gemm_kernel(const __grid_constant__ GroupedMaps maps, const GroupedArgs g) {
-  using C = Cfg<BLOCKS, PAIR>;
+  using C = Cfg<ADD, PAIR>;
+  constexpr bool BLOCKS = C::BLOCKS, PARTS = C::PARTS;
   constexpr int K_ELEMS = (KIND == KIND_BF16 || KIND == KIND_F16) ? 64 : 128;
 
   extern __shared__ uint8_t smem_raw[];
@@ -468,7 +471,7 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
   // The fp32 sums of a pair's tile are 128 registers a thread of the epilogue:
   // it takes over registers of the other warps.  (384 threads are launched with
   // 168 each: 2 * 216 + 72 = 3 * 168.)
-  constexpr bool MOVE_REGS = C::ROWS_M;
+  constexpr bool MOVE_REGS = PAIR && ADD != GROUPED_ADD_NONE;
   if (warp >= C::EPI_WARPS) {
     if constexpr (MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
@@ -566,9 +569,12 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
       Tile t;
       while (ok && walk.next(t)) {
         const uint32_t idesc = make_idesc(KIND, PAIR ? 256 : 128, C::ROWS_M ? C::TN : t.cols);
-        if (!BLOCKS && !take_buffer()) break;
         for (int kb = kb0; kb < kb1; ++kb) {
           const int in_batch = BLOCKS ? (kb - kb0) % C::BATCH : 0;
+          // the accumulator's first and last block
+          const bool first = BLOCKS ? in_batch == 0 : PARTS ? (kb - kb0) % 4 == 0 : kb == kb0;
+          const bool last = (BLOCKS ? in_batch == C::BATCH - 1 : PARTS && (kb - kb0) % 4 == 3) ||
+                            kb + 1 == kb1;
           // (all that the MMAs need is ready before the accumulator is)
           ok = mbar_wait_bounded(&full[stage], phase, abort_flag, g.status, DEV_TIMEOUT_MMA);
           if (!ok) break;
@@ -576,13 +582,11 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
               tmem_base + static_cast<uint32_t>((buf * C::BATCH + in_batch) * C::TN);
           const uint64_t m = smem_desc_k128(smem_u32(s_m + stage * C::M_BYTES));
           const uint64_t n = smem_desc_k128(smem_u32(s_n + stage * C::N_BYTES));
-          if (BLOCKS && in_batch == 0) {
-            if (!take_buffer()) break;
-          }
+          if (first && !take_buffer()) break;
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // 32 bytes of K further: 2 in the descriptors
-            const uint32_t accumulate = (k != 0 || (!BLOCKS && kb != kb0)) ? 1u : 0u;
+            const uint32_t accumulate = (k != 0 || (!BLOCKS && !first)) ? 1u : 0u;
             if constexpr (PAIR)
               tc_mma_pair<KIND>(d_tmem, m + 2 * k, n + 2 * k, idesc, accumulate);
             else
@@ -592,14 +596,13 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
             tc_commit_pair(&empty[stage]);
           else
             tc_commit(&empty[stage]);
-          if (BLOCKS && (in_batch == C::BATCH - 1 || kb + 1 == kb1)) give_buffer();
+          if (last) give_buffer();
           if (++stage == C::STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        if (!BLOCKS) give_buffer();
       }
       if (!ok) {
         // Aborted: let every MMA already issued retire before TMEM is freed.
@@ -757,11 +760,26 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
       } else {
         if (!walk.next(t)) break;
       }
-      if constexpr (BLOCKS) {
+      if constexpr (ADD != GROUPED_ADD_NONE) {
 #pragma unroll
         for (int c = 0; c < C::CHUNKS; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[c][i] = 0u;
+      }
+      if constexpr (PARTS) {
+        for (int kb = kb0; kb < kb1; kb += 4) {
+          ok = wait_acc();
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < C::CHUNKS; ++c) {
+            if (!has_chunk(t, c)) break;
+            uint32_t r[32];
+            load_chunk(c, r);
+            if (!(c + 1 < C::CHUNKS && has_chunk(t, c + 1))) release_acc();
+            add_columns(r, acc[c], [](int) { return make_float2(1.0f, 1.0f); });
+          }
+          if (!has_chunk(t, 0)) release_acc();  // no rows for this warp
+        }
       }
       if constexpr (C::ROWS_M) {
         // A thread has one row and this warp's 128 channels have one scale: one product.
@@ -831,7 +849,7 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
       }
       // Scales of rows and channels: this thread's channel, and a row of each chunk.
       const int ch = t.ch0 + (PAIR ? static_cast<int>(rank) * 128 : 0) + quarter * 32;
-      constexpr bool ROW_SCALES = !BLOCKS && (KIND == KIND_I8 || KIND == KIND_F8);
+      constexpr bool ROW_SCALES = ADD == GROUPED_ADD_NONE && (KIND == KIND_I8 || KIND == KIND_F8);
       float sb = 1.0f;
       if constexpr (ROW_SCALES) {
         if (ch + lane < g.n) sb = __ldg(g.b_scales + t.group * g.bs_group + (ch + lane) * g.bs_n);
@@ -848,7 +866,7 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
       uint8_t* out = static_cast<uint8_t*>(g.out) +
                      (t.row0 * g.out_row + ch) * (g.out_dtype == DT_F32 ? 4 : 2);
       const int64_t out_step = 8 * g.out_row * (g.out_dtype == DT_F32 ? 4 : 2);
-      if constexpr (!BLOCKS) ok = wait_acc();
+      if constexpr (ADD == GROUPED_ADD_NONE) ok = wait_acc();
       if (!ok) break;
 
       if constexpr (C::ROWS_M) {
@@ -906,7 +924,7 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
       if (exchange) {
         if constexpr (!PAIR) {
           cluster_wait();  // (one tile a cluster: once)
-          if constexpr (!BLOCKS) {
+          if constexpr (ADD == GROUPED_ADD_NONE) {
             if (has_chunk(t, 0)) {
               load_chunk(0, acc[0]);
             }
@@ -964,7 +982,7 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
           }
         }
       } else {
-        if constexpr (BLOCKS) {
+        if constexpr (ADD != GROUPED_ADD_NONE) {
 #pragma unroll
           for (int c = 0; c < C::CHUNKS; ++c) {
             if (!has_chunk(t, c)) break;
@@ -1026,10 +1044,10 @@ __global__ void __launch_bounds__(Cfg<BLOCKS, PAIR>::THREADS, 1)
   }
 }
 
-template <int KIND, bool BLOCKS, bool PAIR>
+template <int KIND, int ADD, bool PAIR>
 cudaError_t launch(const GroupedMaps& maps, const GroupedArgs& g, int grid, cudaStream_t stream) {
-  using C = Cfg<BLOCKS, PAIR>;
-  auto kern = grouped_gemm_kernel<KIND, BLOCKS, PAIR>;
+  using C = Cfg<ADD, PAIR>;
+  auto kern = grouped_gemm_kernel<KIND, ADD, PAIR>;
   static std::atomic<long long> shape[kMaxLaunchDevices];
   int dev = 0, sms = 0, per_sm = 0;
   cudaError_t e = launch_shape(reinterpret_cast<const void*>(kern), C::THREADS, C::SMEM_BYTES,
@@ -1061,10 +1079,10 @@ cudaError_t launch(const GroupedMaps& maps, const GroupedArgs& g, int grid, cuda
   return cudaGetLastError();
 }
 
-template <int KIND, bool BLOCKS>
+template <int KIND, int ADD>
 int split_clusters(int splits) {
-  using C = Cfg<BLOCKS, false>;
-  auto kern = grouped_gemm_kernel<KIND, BLOCKS, false>;
+  using C = Cfg<ADD, false>;
+  auto kern = grouped_gemm_kernel<KIND, ADD, false>;
   static std::atomic<int> known[kMaxLaunchDevices][4];  // + 1; of 1, 2, 4, 8
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxLaunchDevices) return 0;
@@ -1092,33 +1110,38 @@ int split_clusters(int splits) {
 
 }  // namespace
 
-int grouped_split_clusters(int kind, bool blocks, int splits) {
+// The kinds with their ways to add; `what` is called with both as constants.
+template <class What>
+auto with_kind(int kind, int add, What what) {
+  constexpr std::integral_constant<int, GROUPED_ADD_NONE> none{};
+  constexpr std::integral_constant<int, GROUPED_ADD_SCALED> scaled{};
+  constexpr std::integral_constant<int, GROUPED_ADD_PARTS> parts{};
   switch (kind) {
-    case KIND_I8: return split_clusters<KIND_I8, false>(splits);
+    case KIND_I8: return what(std::integral_constant<int, KIND_I8>{}, none);
     case KIND_F8:
-      return blocks ? split_clusters<KIND_F8, true>(splits)
-                    : split_clusters<KIND_F8, false>(splits);
-    case KIND_BF16: return split_clusters<KIND_BF16, false>(splits);
-    case KIND_F16: return split_clusters<KIND_F16, false>(splits);
-    default: return 0;
+      return add == GROUPED_ADD_SCALED ? what(std::integral_constant<int, KIND_F8>{}, scaled)
+                                       : what(std::integral_constant<int, KIND_F8>{}, none);
+    case KIND_BF16:
+      return add == GROUPED_ADD_PARTS ? what(std::integral_constant<int, KIND_BF16>{}, parts)
+                                      : what(std::integral_constant<int, KIND_BF16>{}, none);
+    default:
+      return add == GROUPED_ADD_PARTS ? what(std::integral_constant<int, KIND_F16>{}, parts)
+                                      : what(std::integral_constant<int, KIND_F16>{}, none);
   }
 }
 
-cudaError_t launch_grouped_gemm(const GroupedMaps& maps, const GroupedArgs& g, int kind,
-                                bool blocks, bool pair, int grid, cudaStream_t stream) {
-#define M5B_GROUPED(KIND_, BLOCKS_)                                             \
-  return pair ? launch<KIND_, BLOCKS_, true>(maps, g, grid, stream)             \
-              : launch<KIND_, BLOCKS_, false>(maps, g, grid, stream)
-  switch (kind) {
-    case KIND_I8: M5B_GROUPED(KIND_I8, false);
-    case KIND_F8:
-      if (blocks) M5B_GROUPED(KIND_F8, true);
-      M5B_GROUPED(KIND_F8, false);
-    case KIND_BF16: M5B_GROUPED(KIND_BF16, false);
-    case KIND_F16: M5B_GROUPED(KIND_F16, false);
-    default: return cudaErrorInvalidValue;
-  }
-#undef M5B_GROUPED
+int grouped_split_clusters(int kind, int add, int splits) {
+  return with_kind(kind, add, [&](auto k, auto a) {
+    return split_clusters<decltype(k)::value, decltype(a)::value>(splits);
+  });
+}
+
+cudaError_t launch_grouped_gemm(const GroupedMaps& maps, const GroupedArgs& g, int kind, int add,
+                                bool pair, int grid, cudaStream_t stream) {
+  return with_kind(kind, add, [&](auto k, auto a) {
+    return pair ? launch<decltype(k)::value, decltype(a)::value, true>(maps, g, grid, stream)
+                : launch<decltype(k)::value, decltype(a)::value, false>(maps, g, grid, stream);
+  });
 }
 
 }  // namespace m5b
