@@ -501,7 +501,9 @@ M5B_API int m5b_block_quantize(const m5b_block_quantize_args* args, void* stream
 
 /* m5b_grouped_gemm: out[t, n] = epilogue(sum_k a[t, k] b[e, n, k]) for the rows
  * group_start[e] <= t < group_start[e + 1] of each group e < groups (at most
- * 1024; group_start ascends, read on the device; NULL with groups 1: all rows).
+ * 1024; group_start ascends, read on the device; NULL with groups 1: all rows;
+ * a bound outside [0, rows] counts as the nearer end, one below its predecessor
+ * as that).
  * mode INT8 / FP8 / BF16 / FP16 names the operands as in m5b_gemm.
  *   INT8, FP8:  (acc * a_scales[t]) * b_scales[e, n]; bit-identical to m5b_gemm
  *               of the group's rows for INT8

@@ -436,6 +436,22 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
     __syncthreads();
   }
   if (g.group_start && warp == 0) {
+    // Bounds that do not ascend (which is the caller's to see to) are taken as the
+    // largest before them: no two groups share a row, and there are no more tiles
+    // than the host allows for.
+    int most = 0;
+    for (int e0 = 0; e0 <= g.groups; e0 += 32) {
+      int r = e0 + lane <= g.groups ? s_row[e0 + lane] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, r, d);
+        if (lane >= d) r = max(r, v);
+      }
+      r = max(r, most);
+      if (e0 + lane <= g.groups) s_row[e0 + lane] = r;
+      most = __shfl_sync(0xffffffffu, r, 31);
+    }
+    __syncwarp();
     int before = 0;
     for (int e0 = 0; e0 < g.groups; e0 += 32) {
       const int e = e0 + lane;
