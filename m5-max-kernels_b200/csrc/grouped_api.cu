@@ -196,10 +196,14 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
   const uint32_t wide = static_cast<uint32_t>(128 / elem);
   const uint32_t box128[3] = {wide, 128, 1}, box64[2] = {wide, 64}, box16[2] = {wide, 16};
   const int bytes = static_cast<int>(elem);
-  if (!make_swizzled_map(&m.a128, bytes, 2, s->a, a_dims, a_strides, box128) ||
-      !make_swizzled_map(&m.a64, bytes, 2, s->a, a_dims, a_strides, box64) ||
-      !make_swizzled_map(&m.a16, bytes, 2, s->a, a_dims, a_strides, box16) ||
-      !make_swizzled_map(&m.b, bytes, 3, s->b, b_dims, b_strides, box128))
+  // (only those that the tiles use)
+  const auto rows_map = [&](CUtensorMap* map, const uint32_t* box) {
+    return make_swizzled_map(map, bytes, 2, s->a, a_dims, a_strides, box);
+  };
+  const bool rows_m = p.pair && add == GROUPED_ADD_SCALED;
+  if (!make_swizzled_map(&m.b, bytes, 3, s->b, b_dims, b_strides, box128) ||
+      (p.pair && !rows_map(&m.a128, box128)) || (!rows_m && !rows_map(&m.a64, box64)) ||
+      (!p.pair && !rows_map(&m.a16, box16)))
     return set_last_error(M5B_ECUDA, "cuTensorMapEncodeTiled failed");
   return launched(launch_grouped_gemm(m, g, kind, add, p.pair, p.grid,
                                       static_cast<cudaStream_t>(stream)),

@@ -34,23 +34,11 @@ _FLOAT = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib
 _OPERAND = {mode: (dtype, _lib.MODE[mode], dtype.itemsize) for mode, dtype in (
     ("int8", torch.int8), ("fp8", torch.uint8), ("bf16", torch.bfloat16), ("fp16", torch.float16))}
 _NO_SCALES = (0,) * 7
+_F32 = torch.float32
 _MOST_GROUPS = 1024
 # m5b_block_quantize_args and m5b_grouped_gemm_args (include/m5b200.h): every field is 8 bytes
 _PACK_QUANTIZE = struct.Struct("@14q")
 _PACK_GEMM = struct.Struct("@23q")
-
-
-def _operand(t, size):
-    """(t, strides) with rows that TMA can read: contiguous channels, rows on the 16-byte grid."""
-    strides = t.stride()
-    if strides[-1] == 1 and t.data_ptr() % 16 == 0:
-        for n, s in zip(t.shape, strides[:-1]):
-            if n > 1 and (s <= 0 or s * size % 16):
-                break
-        else:
-            return t, strides
-    t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride()
 
 
 def _row_index(rows):
@@ -95,7 +83,7 @@ def block_quantize(x, *, gate=None, rows=None, block_rows=1):
     if strides[-1] != 1:
         x = x.contiguous()
         strides = x.stride()
-    used = [x]
+    used = None
     gate_ptr = gate_row = index_ptr = 0
     if gate is not None:
         if not isinstance(gate, _Tensor) or gate.shape != shape or gate.dtype is not x.dtype:
@@ -103,12 +91,14 @@ def block_quantize(x, *, gate=None, rows=None, block_rows=1):
         if gate.stride(1) != 1:
             gate = gate.contiguous()
         gate_ptr, gate_row = gate.data_ptr(), gate.stride(0)
-        used.append(gate)
+        used = [x, gate]
     if rows is not None:
         rows = _row_index(rows)
         index_ptr, out_rows = rows.data_ptr(), rows.shape[0]
-        used.append(rows)
-    index = _device(used)
+        used = [x, rows] if used is None else [*used, rows]
+    index = x.get_device() if used is None else _device(used)
+    if index < 0:
+        _lib.require_cuda(x)
     batch, batch_stride = (shape[0], strides[0]) if len(shape) == 3 else (1, 0)
     lead, device = shape[:-2], x.device
     # (sizes as arguments of their own take torch.empty two thirds of a tuple's time)
@@ -124,41 +114,46 @@ def block_quantize(x, *, gate=None, rows=None, block_rows=1):
 
 def _product(a, b, group_start, mode, a_scales, b_scales, output_dtype, out):
     """Both products: b [groups, N, K], or with group_start None [N, K] for all rows."""
-    rows, k = a.shape
-    n = b.shape[-2]
-    groups = 1 if group_start is None else b.shape[0]
     expected, code, size = _OPERAND[mode]
     if a.dtype is not expected or b.dtype is not expected:
         raise ValueError("operand dtypes must match the declared mode")
-    if k * size % 16:
+    rows, k = a.shape
+    if group_start is None:
+        groups, (n, _) = 1, b.shape
+    else:
+        groups, n, _ = b.shape
+    if k * size & 15:
         raise NotImplementedError(f"K*{size} bytes per row must be a multiple of 16 for TMA; "
                                   "padding is not implicit")
-    used = [a, b]
-    blocks = False
-    scale_fields = _NO_SCALES
+    index = a.get_device()
+    same = index >= 0 and b.get_device() == index
+    blocks, scale_fields = False, _NO_SCALES
     if size == 1:
         if (not isinstance(a_scales, _Tensor) or not isinstance(b_scales, _Tensor)
-                or a_scales.dtype is not torch.float32 or b_scales.dtype is not torch.float32):
+                or a_scales.dtype is not _F32 or b_scales.dtype is not _F32):
             raise ValueError("float32 scales required")
-        kb = -(-k // BLOCK)
-        sa, sb = a_scales.stride(), b_scales.stride()
         a_shape, b_shape = a_scales.shape, b_scales.shape
-        lead = () if group_start is None else (groups,)
-        if (mode == "fp8" and a_shape == (rows, kb) and b_shape == (*lead, -(-n // BLOCK), kb)):
-            blocks = True
-            scale_fields = (a_scales.data_ptr(), b_scales.data_ptr(), *sa,
-                            *(sb if lead else (0, *sb)))
-        elif a_shape == (rows,) and b_shape == (groups, n):
-            scale_fields = (a_scales.data_ptr(), b_scales.data_ptr(), sa[0], 0, sb[0], sb[1], 0)
-        else:
+        if len(a_shape) == 2 and mode == "fp8":
+            kb, nb = -(-k // BLOCK), -(-n // BLOCK)
+            blocks = a_shape == (rows, kb) and b_shape == (
+                (nb, kb) if group_start is None else (groups, nb, kb))
+        if not blocks and (a_shape != (rows,) or b_shape != (groups, n)):
             raise ValueError("scales must be those of rows and channels, or (fp8) of blocks of "
                              "128 channels of K")
-        used += (a_scales, b_scales)
+        # between rows and blocks of a, groups, channels (or blocks of them) and blocks of b
+        if not blocks:
+            strides = (*a_scales.stride(), 0, *b_scales.stride(), 0)
+        elif group_start is None:
+            strides = (*a_scales.stride(), 0, *b_scales.stride())
+        else:
+            strides = (*a_scales.stride(), *b_scales.stride())
+        scale_fields = (a_scales.data_ptr(), b_scales.data_ptr(), *strides)
+        same = same and a_scales.get_device() == index and b_scales.get_device() == index
     elif a_scales is not None or b_scales is not None:
         raise ValueError("scales belong to int8 and fp8 operands")
     zero_rest = out is None
     if out is None:
-        out_dtype = output_dtype or torch.float32
+        out_dtype = output_dtype or _F32
     else:
         if (not isinstance(out, _Tensor) or out.shape != (rows, n)
                 or (n > 1 and out.stride(1) != 1)):
@@ -166,24 +161,35 @@ def _product(a, b, group_start, mode, a_scales, b_scales, output_dtype, out):
         out_dtype = out.dtype
         if output_dtype is not None and output_dtype is not out_dtype:
             raise ValueError("output_dtype must be out's")
-        used.append(out)
+        same = same and out.get_device() == index
     out_code = _FLOAT.get(out_dtype)
     if out_code is None:
         raise NotImplementedError("output dtype must be bfloat16, float16 or float32")
     start_ptr = 0
     if group_start is not None:
         start_ptr = group_start.data_ptr()
-        used.append(group_start)
-    index = _device(used)
+        same = same and group_start.get_device() == index
+    if not same:
+        _lib.require_cuda(a, b, a_scales, b_scales, out, group_start)
     if out is None:
         out = torch.empty(rows, n, dtype=out_dtype, device=a.device)
     if rows > 0:
-        a, a_strides = _operand(a, size)
-        b, b_strides = _operand(b, size)
+        # rows that TMA can read: contiguous channels, on the 16-byte grid
+        off = 16 // size - 1
+        a_ptr, (a_row, a_step) = a.data_ptr(), a.stride()
+        if a_ptr & 15 or a_step != 1 or a_row & off or a_row <= 0:
+            a = a.clone(memory_format=torch.contiguous_format)
+            a_ptr, (a_row, _) = a.data_ptr(), a.stride()
+        b_ptr, strides = b.data_ptr(), b.stride()
+        b_group, b_row = strides[0], strides[-2]
+        if (b_ptr & 15 or strides[-1] != 1 or (b_row | b_group) & off or b_row <= 0
+                or b_group <= 0):
+            b = b.clone(memory_format=torch.contiguous_format)
+            b_ptr, strides = b.data_ptr(), b.stride()
+            b_group, b_row = strides[0], strides[-2]
         _call(_lib.lib().m5b_grouped_gemm, _PACK_GEMM.pack(
-            a.data_ptr(), b.data_ptr(), code, rows, groups, n, k, a_strides[0], b_strides[0],
-            b_strides[-2], start_ptr, blocks, *scale_fields, out.data_ptr(), out_code,
-            out.stride(0), zero_rest), index)
+            a_ptr, b_ptr, code, rows, groups, n, k, a_row, b_group, b_row, start_ptr, blocks,
+            *scale_fields, out.data_ptr(), out_code, out.stride(0), zero_rest), index)
     return out
 
 
