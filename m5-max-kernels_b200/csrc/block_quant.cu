@@ -201,6 +201,7 @@ __device__ __forceinline__ void store_codes(uint8_t* q, int count, Scale scale, 
 template <typename T, bool GATE, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
     block_quant_rows_kernel(const BlockQuantArgs a, unsigned blocks_per_row, unsigned total) {
+  grid_dependents_launch();  // (a product that follows sets itself up meanwhile)
   const int sub = threadIdx.x % kLanes;
   const unsigned stride = gridDim.x * kRows;
   const unsigned row_step = stride / blocks_per_row;
@@ -282,6 +283,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     block_quant_square_kernel(const BlockQuantArgs a, unsigned blocks_per_row,
                               unsigned row_blocks) {
+  grid_dependents_launch();
   constexpr int N = 128 / kRows;
   __shared__ uint32_t s_peak[kThreads / 32];
   const unsigned b = blockIdx.x;

@@ -419,6 +419,7 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
   }
   // With programmatic launch all that stands above overlaps the previous kernel's end.
   grid_dependency_wait();
+  grid_dependents_launch();  // (whose start waits for this kernel's end in its turn)
   // The groups' first rows, then the tiles before each group.
   const int ch_tiles = (g.n + C::TM - 1) / C::TM;
   if (!g.group_start) {
