@@ -113,7 +113,8 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorM
 }
 // Arrival on a barrier of another CTA that hands over TMEM only (the tcgen05 fence
 // before it orders that): a release over the cluster would wait for every load
-// that the thread has under way, 2.1 us a block of 128 channels instead of 0.35.
+// that the thread has under way (1.9 us a block of 128 channels instead of 1.45
+// where it had both).
 __device__ __forceinline__ void mbar_arrive_tmem(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -398,8 +399,7 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
     fence_mbarrier_init();
   }
   // K split: the CTAs need one another's barriers only when they exchange their
-  // sums, and nothing of one another after that, so that they do not wait here
-  // and at the end (2.3 us of 14 for 3 x 7168 x 5376).
+  // sums, and nothing of one another after that: they arrive here and wait there.
   const bool exchange = !PAIR && splits > 1;
   __syncwarp();
   if (exchange) cluster_arrive();
@@ -492,67 +492,143 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
   if (warp >= C::EPI_WARPS) {
     if constexpr (MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
-    // ------------------------------------------------------------ producer
-    if (elect_one()) {
-      int stage = 0, issued = 0;
-      uint32_t phase = 0;
-      Tile t;
-      while (!*abort_flag && walk.next(t)) {
-        // This CTA's part of the columns (of a pair's, half), and its 128 of M.
-        const int n_rows = C::ROWS_M ? 128 : PAIR ? t.cols / 2 : t.cols;
-        const int n_row =
-            (C::ROWS_M ? t.ch0 : t.row0) + (PAIR ? static_cast<int>(rank) * n_rows : 0);
-        const int m_row =
-            (C::ROWS_M ? t.row0 : t.ch0) + (PAIR ? static_cast<int>(rank) * 128 : 0);
-        // One box brings the columns' rows: of the next size, what lies behind the
-        // tile's is not used.
-        const bool few = n_rows <= C::FEW_ROWS;
-        const CUtensorMap* columns = few ? (PAIR ? &maps.a64 : &maps.a16)
-                                         : (PAIR ? &maps.a128 : &maps.a64);
-        const uint32_t bytes =
-            C::M_BYTES + (C::ROWS_M ? 128 : few ? C::FEW_ROWS : C::N_BYTES / 128) * 128;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, g.status,
-                                 DEV_TIMEOUT_PRODUCER))
-            break;
-          const int kx = kb * K_ELEMS;
-          uint8_t* m = s_m + stage * C::M_BYTES;
-          uint8_t* n = s_n + stage * C::N_BYTES;
-          if constexpr (PAIR) {
-            // The even CTA's barrier counts both CTAs' bytes.
-            if (leader) mbar_arrive_expect_tx(&full[stage], 2 * bytes);
-          } else {
-            mbar_arrive_expect_tx(&full[stage], bytes);
+      // ------------------------------------------------------------ producer
+      if (elect_one()) {
+        int stage = 0, issued = 0;
+        uint32_t phase = 0;
+        Tile t;
+        while (!*abort_flag && walk.next(t)) {
+          // This CTA's part of the columns (of a pair's, half), and its 128 of M.
+          const int n_rows = C::ROWS_M ? 128 : PAIR ? t.cols / 2 : t.cols;
+          const int n_row =
+              (C::ROWS_M ? t.ch0 : t.row0) + (PAIR ? static_cast<int>(rank) * n_rows : 0);
+          const int m_row =
+              (C::ROWS_M ? t.row0 : t.ch0) + (PAIR ? static_cast<int>(rank) * 128 : 0);
+          // One box brings the columns' rows: of the next size, what lies behind the
+          // tile's is not used.
+          const bool few = n_rows <= C::FEW_ROWS;
+          const CUtensorMap* columns = few ? (PAIR ? &maps.a64 : &maps.a16)
+                                           : (PAIR ? &maps.a128 : &maps.a64);
+          const uint32_t bytes =
+              C::M_BYTES + (C::ROWS_M ? 128 : few ? C::FEW_ROWS : C::N_BYTES / 128) * 128;
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, abort_flag, g.status,
+                                   DEV_TIMEOUT_PRODUCER))
+              break;
+            const int kx = kb * K_ELEMS;
+            uint8_t* m = s_m + stage * C::M_BYTES;
+            uint8_t* n = s_n + stage * C::N_BYTES;
+            if constexpr (PAIR) {
+              // The even CTA's barrier counts both CTAs' bytes.
+              if (leader) mbar_arrive_expect_tx(&full[stage], 2 * bytes);
+            } else {
+              mbar_arrive_expect_tx(&full[stage], bytes);
+            }
+            if constexpr (C::ROWS_M) {
+              tma_load_2d_pair(m, &maps.a128, &full[stage], kx, m_row);
+              tma_load_3d_pair(n, &maps.b, &full[stage], kx, n_row, t.group);
+            } else {
+              if constexpr (PAIR)
+                tma_load_3d_pair(m, &maps.b, &full[stage], kx, m_row, t.group);
+              else
+                tma_load_3d(m, &maps.b, &full[stage], kx, m_row, t.group);
+              if constexpr (PAIR)
+                tma_load_2d_pair(n, columns, &full[stage], kx, n_row);
+              else
+                tma_load_2d(n, columns, &full[stage], kx, n_row);
+            }
+            ++issued;
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
-          if constexpr (C::ROWS_M) {
-            tma_load_2d_pair(m, &maps.a128, &full[stage], kx, m_row);
-            tma_load_3d_pair(n, &maps.b, &full[stage], kx, n_row, t.group);
-          } else {
-            if constexpr (PAIR)
-              tma_load_3d_pair(m, &maps.b, &full[stage], kx, m_row, t.group);
-            else
-              tma_load_3d(m, &maps.b, &full[stage], kx, m_row, t.group);
-            if constexpr (PAIR)
-              tma_load_2d_pair(n, columns, &full[stage], kx, n_row);
-            else
-              tma_load_2d(n, columns, &full[stage], kx, n_row);
-          }
-          ++issued;
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1u;
+        }
+        if (*abort_flag && leader) {
+          // Wait (bounded) for the copies already issued, so that none lands after
+          // this CTA has gone.  (The even CTA's barriers count both CTAs' copies.)
+          int s = stage, ph = phase;
+          for (int i = 0; i < C::STAGES && i < issued; ++i) {
+            s = (s == 0) ? C::STAGES - 1 : s - 1;
+            if (s == C::STAGES - 1) ph ^= 1;
+            const unsigned long long t0 = globaltimer_ns();
+            while (!mbar_try_wait(&full[s], ph)) {
+              if (globaltimer_ns() - t0 > kWaitLimitNs) {
+                atomicOr(g.status, DEV_TIMEOUT_DRAIN);
+                break;
+              }
+            }
           }
         }
       }
-      if (*abort_flag && leader) {
-        // Wait (bounded) for the copies already issued, so that none lands after
-        // this CTA has gone.  (The even CTA's barriers count both CTAs' copies.)
-        int s = stage, ph = phase;
-        for (int i = 0; i < C::STAGES && i < issued; ++i) {
-          s = (s == 0) ? C::STAGES - 1 : s - 1;
-          if (s == C::STAGES - 1) ph ^= 1;
+    } else if (warp == 9) {
+      // ------------------------------------------------------------ MMA issuer
+      if (leader && elect_one()) {
+        int stage = 0, buf = 0;
+        uint32_t phase = 0, buf_phase = 0;
+        bool ok = true;
+        auto take_buffer = [&]() {
+          ok = mbar_wait_bounded(&acc_empty[buf], buf_phase ^ 1u, abort_flag, g.status,
+                                 DEV_TIMEOUT_MMA);
+          tc_fence_after();
+          return ok;
+        };
+        auto give_buffer = [&]() {
+          if constexpr (PAIR)
+            tc_commit_pair(&acc_full[buf]);
+          else
+            tc_commit(&acc_full[buf]);
+          if (++buf == C::BUFS) {
+            buf = 0;
+            buf_phase ^= 1u;
+          }
+        };
+        Tile t;
+        while (ok && walk.next(t)) {
+          const uint32_t idesc = make_idesc(KIND, PAIR ? 256 : 128, C::ROWS_M ? C::TN : t.cols);
+          for (int kb = kb0; kb < kb1; ++kb) {
+            const int in_batch = BLOCKS ? (kb - kb0) % C::BATCH : 0;
+            // the accumulator's first and last block
+            const bool first = BLOCKS ? in_batch == 0 : PARTS ? (kb - kb0) % 4 == 0 : kb == kb0;
+            const bool last = (BLOCKS ? in_batch == C::BATCH - 1 : PARTS && (kb - kb0) % 4 == 3) ||
+                              kb + 1 == kb1;
+            // (all that the MMAs need is ready before the accumulator is)
+            ok = mbar_wait_bounded(&full[stage], phase, abort_flag, g.status, DEV_TIMEOUT_MMA);
+            if (!ok) break;
+            const uint32_t d_tmem =
+                tmem_base + static_cast<uint32_t>((buf * C::BATCH + in_batch) * C::TN);
+            const uint64_t m = smem_desc_k128(smem_u32(s_m + stage * C::M_BYTES));
+            const uint64_t n = smem_desc_k128(smem_u32(s_n + stage * C::N_BYTES));
+            if (first && !take_buffer()) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // 32 bytes of K further: 2 in the descriptors
+              const uint32_t accumulate = (k != 0 || (!BLOCKS && !first)) ? 1u : 0u;
+              if constexpr (PAIR)
+                tc_mma_pair<KIND>(d_tmem, m + 2 * k, n + 2 * k, idesc, accumulate);
+              else
+                tc_mma<KIND>(d_tmem, m + 2 * k, n + 2 * k, idesc, accumulate);
+            }
+            if constexpr (PAIR)
+              tc_commit_pair(&empty[stage]);
+            else
+              tc_commit(&empty[stage]);
+            if (last) give_buffer();
+            if (++stage == C::STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+          if (!ok) break;
+        }
+        if (!ok) {
+          // Aborted: let every MMA already issued retire before TMEM is freed.
+          if constexpr (PAIR)
+            tc_commit_pair(drain);
+          else
+            tc_commit(drain);
           const unsigned long long t0 = globaltimer_ns();
-          while (!mbar_try_wait(&full[s], ph)) {
+          while (!mbar_try_wait(drain, 0)) {
             if (globaltimer_ns() - t0 > kWaitLimitNs) {
               atomicOr(g.status, DEV_TIMEOUT_DRAIN);
               break;
@@ -560,82 +636,6 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
           }
         }
       }
-    }
-    } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issuer
-    if (leader && elect_one()) {
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, buf_phase = 0;
-      bool ok = true;
-      auto take_buffer = [&]() {
-        ok = mbar_wait_bounded(&acc_empty[buf], buf_phase ^ 1u, abort_flag, g.status,
-                               DEV_TIMEOUT_MMA);
-        tc_fence_after();
-        return ok;
-      };
-      auto give_buffer = [&]() {
-        if constexpr (PAIR)
-          tc_commit_pair(&acc_full[buf]);
-        else
-          tc_commit(&acc_full[buf]);
-        if (++buf == C::BUFS) {
-          buf = 0;
-          buf_phase ^= 1u;
-        }
-      };
-      Tile t;
-      while (ok && walk.next(t)) {
-        const uint32_t idesc = make_idesc(KIND, PAIR ? 256 : 128, C::ROWS_M ? C::TN : t.cols);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          const int in_batch = BLOCKS ? (kb - kb0) % C::BATCH : 0;
-          // the accumulator's first and last block
-          const bool first = BLOCKS ? in_batch == 0 : PARTS ? (kb - kb0) % 4 == 0 : kb == kb0;
-          const bool last = (BLOCKS ? in_batch == C::BATCH - 1 : PARTS && (kb - kb0) % 4 == 3) ||
-                            kb + 1 == kb1;
-          // (all that the MMAs need is ready before the accumulator is)
-          ok = mbar_wait_bounded(&full[stage], phase, abort_flag, g.status, DEV_TIMEOUT_MMA);
-          if (!ok) break;
-          const uint32_t d_tmem =
-              tmem_base + static_cast<uint32_t>((buf * C::BATCH + in_batch) * C::TN);
-          const uint64_t m = smem_desc_k128(smem_u32(s_m + stage * C::M_BYTES));
-          const uint64_t n = smem_desc_k128(smem_u32(s_n + stage * C::N_BYTES));
-          if (first && !take_buffer()) break;
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {  // 32 bytes of K further: 2 in the descriptors
-            const uint32_t accumulate = (k != 0 || (!BLOCKS && !first)) ? 1u : 0u;
-            if constexpr (PAIR)
-              tc_mma_pair<KIND>(d_tmem, m + 2 * k, n + 2 * k, idesc, accumulate);
-            else
-              tc_mma<KIND>(d_tmem, m + 2 * k, n + 2 * k, idesc, accumulate);
-          }
-          if constexpr (PAIR)
-            tc_commit_pair(&empty[stage]);
-          else
-            tc_commit(&empty[stage]);
-          if (last) give_buffer();
-          if (++stage == C::STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-        if (!ok) break;
-      }
-      if (!ok) {
-        // Aborted: let every MMA already issued retire before TMEM is freed.
-        if constexpr (PAIR)
-          tc_commit_pair(drain);
-        else
-          tc_commit(drain);
-        const unsigned long long t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain, 0)) {
-          if (globaltimer_ns() - t0 > kWaitLimitNs) {
-            atomicOr(g.status, DEV_TIMEOUT_DRAIN);
-            break;
-          }
-        }
-      }
-    }
     } else if constexpr (BLOCKS) {
       // ---------------------------------------------------------- block scales
       // Products sa * sb of four blocks of K ("a quad") a slot: of the tile's rows,
@@ -924,7 +924,8 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
         float2 v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          v[j] = make_float2(sum_value<KIND>(r[8 * i + 2 * j]), sum_value<KIND>(r[8 * i + 2 * j + 1]));
+          v[j] = make_float2(sum_value<KIND>(r[8 * i + 2 * j]),
+                             sum_value<KIND>(r[8 * i + 2 * j + 1]));
         if constexpr (ROW_SCALES) {
           const float4* sa = reinterpret_cast<const float4*>(row_scales + c * 32 + 8 * i);
           const float4 lo = sa[0], hi = sa[1];
@@ -942,9 +943,7 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
         if constexpr (!PAIR) {
           cluster_wait();  // (one tile a cluster: once)
           if constexpr (ADD == GROUPED_ADD_NONE) {
-            if (has_chunk(t, 0)) {
-              load_chunk(0, acc[0]);
-            }
+            if (has_chunk(t, 0)) load_chunk(0, acc[0]);
             release_acc();
           }
           // Rows 8 n .. 8 n + 7 of the tile belong to rank n % splits, as its
@@ -968,9 +967,10 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
           fence_cluster();
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (lane == 0)
-              mbar_arrive_fenced(map_to_rank(parts, static_cast<uint32_t>((half * 4 + i) % splits)));
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t owner = static_cast<uint32_t>((half * 4 + i) % splits);
+            if (lane == 0) mbar_arrive_fenced(map_to_rank(parts, owner));
+          }
           __syncwarp();
           cluster_arrive();
           exchanged = true;
