@@ -417,9 +417,15 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
       tmem_relinquish();
     }
   }
-  // With programmatic launch all that stands above overlaps the previous kernel's end.
-  grid_dependency_wait();
-  grid_dependents_launch();  // (whose start waits for this kernel's end in its turn)
+  // With programmatic launch all that stands before the first access to global
+  // memory overlaps the previous kernel's end, and lets the next kernel start, which
+  // waits in its turn: here where the bounds are read, else in the roles, whose code
+  // is cold too (2500 cycles from here to the first copy).
+  auto inputs_ready = []() {
+    grid_dependency_wait();
+    grid_dependents_launch();
+  };
+  if (g.group_start) inputs_ready();
   // The groups' first rows, then the tiles before each group.
   const int ch_tiles = (g.n + C::TM - 1) / C::TM;
   if (!g.group_start) {
@@ -509,6 +515,7 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
           const bool few = n_rows <= C::FEW_ROWS;
           const CUtensorMap* columns = few ? (PAIR ? &maps.a64 : &maps.a16)
                                            : (PAIR ? &maps.a128 : &maps.a64);
+          if (issued == 0 && !g.group_start) inputs_ready();
           const uint32_t bytes =
               C::M_BYTES + (C::ROWS_M ? 128 : few ? C::FEW_ROWS : C::N_BYTES / 128) * 128;
           for (int kb = kb0; kb < kb1; ++kb) {
@@ -640,6 +647,7 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
       // ---------------------------------------------------------- block scales
       // Products sa * sb of four blocks of K ("a quad") a slot: of the tile's rows,
       // or (ROWS_M) of this CTA's 128 rows with each of the tile's channel blocks.
+      if (!g.group_start) inputs_ready();
       const int me = static_cast<int>(threadIdx.x) - 320;
       uint32_t quad = 0;
       bool ok = true;
@@ -704,6 +712,7 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
   } else {
     if constexpr (MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ------------------------------------------------------------ epilogue
+    if (!g.group_start) inputs_ready();
     const int quarter = warp & 3;  // TMEM lanes 32 quarter ..: channels
     const int half = warp >> 2;    // of the 32-column chunks: every second, or (ROWS_M) half
     const uint32_t tmem_warp = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
