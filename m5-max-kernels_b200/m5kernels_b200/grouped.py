@@ -112,16 +112,11 @@ def block_quantize(x, *, gate=None, rows=None, block_rows=1):
     return codes, scales
 
 
-def _product(a, b, group_start, mode, a_scales, b_scales, output_dtype, out):
+def _product(a, b, rows, groups, n, k, group_start, mode, a_scales, b_scales, output_dtype, out):
     """Both products: b [groups, N, K], or with group_start None [N, K] for all rows."""
     expected, code, size = _OPERAND[mode]
     if a.dtype is not expected or b.dtype is not expected:
         raise ValueError("operand dtypes must match the declared mode")
-    rows, k = a.shape
-    if group_start is None:
-        groups, (n, _) = 1, b.shape
-    else:
-        groups, n, _ = b.shape
     if k * size & 15:
         raise NotImplementedError(f"K*{size} bytes per row must be a multiple of 16 for TMA; "
                                   "padding is not implicit")
@@ -131,13 +126,14 @@ def _product(a, b, group_start, mode, a_scales, b_scales, output_dtype, out):
     if size == 1:
         if (not isinstance(a_scales, _Tensor) or not isinstance(b_scales, _Tensor)
                 or a_scales.dtype is not _F32 or b_scales.dtype is not _F32):
-            raise ValueError("float32 scales required")
+            raise ValueError("float32 scales required" if group_start is not None else
+                             "float32 scales of blocks of 128 channels of K required")
         a_shape, b_shape = a_scales.shape, b_scales.shape
         if len(a_shape) == 2 and mode == "fp8":
             kb, nb = -(-k // BLOCK), -(-n // BLOCK)
             blocks = a_shape == (rows, kb) and b_shape == (
                 (nb, kb) if group_start is None else (groups, nb, kb))
-        if not blocks and (a_shape != (rows,) or b_shape != (groups, n)):
+        if not blocks and (group_start is None or a_shape != (rows,) or b_shape != (groups, n)):
             raise ValueError("scales must be those of rows and channels, or (fp8) of blocks of "
                              "128 channels of K")
         # between rows and blocks of a, groups, channels (or blocks of them) and blocks of b
@@ -206,13 +202,14 @@ def block_gemm(a, b, a_scales, b_scales, *, output_dtype=None, out=None):
     output_dtype: float32 unless given; `out` may be given, with contiguous
     channels.
     """
-    if (not isinstance(a, _Tensor) or not isinstance(b, _Tensor) or a.dim() != 2 or b.dim() != 2
-            or a.shape[1] != b.shape[1] or 0 in b.shape):
-        raise ValueError("A and B must be matrices [M, K] and [N, K]")
-    if (not isinstance(a_scales, _Tensor) or not isinstance(b_scales, _Tensor)
-            or a_scales.dim() != 2 or b_scales.dim() != 2):
-        raise ValueError("scales must be those of blocks of 128 channels of K")
-    return _product(a, b, None, "fp8", a_scales, b_scales, output_dtype, out)
+    if isinstance(a, _Tensor) and isinstance(b, _Tensor):
+        a_shape, b_shape = a.shape, b.shape
+        if len(a_shape) == 2 and len(b_shape) == 2:
+            (m, k), (n, b_k) = a_shape, b_shape
+            if k == b_k and n and k:
+                return _product(a, b, m, 1, n, k, None, "fp8", a_scales, b_scales, output_dtype,
+                                out)
+    raise ValueError("A and B must be matrices [M, K] and [N, K]")
 
 
 def grouped_gemm(a, b, group_start, mode="bf16", *, a_scales=None, b_scales=None,
@@ -235,14 +232,18 @@ def grouped_gemm(a, b, group_start, mode="bf16", *, a_scales=None, b_scales=None
         if mode in ("fp32", "mxint8"):
             raise NotImplementedError(f"{mode} operands are not supported by the grouped GEMM")
         raise ValueError(f"unknown GEMM mode {mode!r}")
-    if (not isinstance(a, _Tensor) or not isinstance(b, _Tensor) or a.dim() != 2 or b.dim() != 3
-            or a.shape[1] != b.shape[2] or 0 in b.shape):
+    a_shape = a.shape if isinstance(a, _Tensor) else ()
+    b_shape = b.shape if isinstance(b, _Tensor) else ()
+    if (len(a_shape) != 2 or len(b_shape) != 3 or a_shape[1] != b_shape[2]
+            or not (b_shape[0] and b_shape[1] and b_shape[2])):
         raise ValueError("A and B must have shapes [T, K] and [E, N, K]")
+    (rows, k), (groups, n, _) = a_shape, b_shape
     group_start = _ints(group_start, "group_start")
-    if group_start.shape != (b.shape[0] + 1,):
+    if group_start.shape != (groups + 1,):
         raise ValueError("group_start must be a vector [E + 1]")
-    if b.shape[0] > _MOST_GROUPS:
+    if groups > _MOST_GROUPS:
         raise NotImplementedError("more than 1024 groups are unsupported")
-    if mode == "int8" and a.shape[1] > 133144:
+    if k > 133144 and mode == "int8":
         raise NotImplementedError("INT32 worst-case overflow bound exceeded")
-    return _product(a, b, group_start, mode, a_scales, b_scales, output_dtype, out)
+    return _product(a, b, rows, groups, n, k, group_start, mode, a_scales, b_scales, output_dtype,
+                    out)
