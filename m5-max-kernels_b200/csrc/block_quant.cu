@@ -201,7 +201,6 @@ __device__ __forceinline__ void store_codes(uint8_t* q, int count, Scale scale, 
 template <typename T, bool GATE, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
     block_quant_rows_kernel(const BlockQuantArgs a, unsigned blocks_per_row, unsigned total) {
-  grid_dependents_launch();  // (a product that follows sets itself up meanwhile)
   const int sub = threadIdx.x % kLanes;
   const unsigned stride = gridDim.x * kRows;
   const unsigned row_step = stride / blocks_per_row;
@@ -211,6 +210,8 @@ __global__ void __launch_bounds__(kThreads)
   const int k = static_cast<int>(a.k), x_rows = static_cast<int>(a.x_rows);
   unsigned b = blockIdx.x * kRows + threadIdx.x / kLanes;
   unsigned row = b / blocks_per_row, block = b - row * blocks_per_row;
+  grid_dependency_wait();
+  grid_dependents_launch();  // (a product that follows sets itself up meanwhile)
   // (whole warps leave the loop together: the shuffles below name all lanes)
   while (b - threadIdx.x % 32 / kLanes < total) {
     Raw<T> rx[UNROLL], rg[UNROLL];
@@ -283,7 +284,6 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     block_quant_square_kernel(const BlockQuantArgs a, unsigned blocks_per_row,
                               unsigned row_blocks) {
-  grid_dependents_launch();
   constexpr int N = 128 / kRows;
   __shared__ uint32_t s_peak[kThreads / 32];
   const unsigned b = blockIdx.x;
@@ -294,6 +294,8 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t left = a.k - col;
   const int count = static_cast<int>(left < 0 ? 0 : left > kLane ? kLane : left);
   const T* x = static_cast<const T*>(a.x) + batch * a.x_batch + col;
+  grid_dependency_wait();
+  grid_dependents_launch();
   Raw<T> r[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -319,14 +321,32 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// With programmatic launch (grid_dependency_wait): the start overlaps the end of
+// the kernel before.
+template <class... Params, class... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), unsigned grid, cudaStream_t stream,
+                              Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
 template <typename T, bool VEC>
 cudaError_t launch(const BlockQuantArgs& a, bool square, cudaStream_t stream) {
   const unsigned per_row = static_cast<unsigned>((a.k + 127) / 128);
   if (square) {
     const unsigned row_blocks = static_cast<unsigned>((a.rows + 127) / 128);
-    block_quant_square_kernel<T, VEC><<<static_cast<unsigned>(a.batch) * row_blocks * per_row,
-                                        kThreads, 0, stream>>>(a, per_row, row_blocks);
-    return cudaGetLastError();
+    return launch_overlapped(block_quant_square_kernel<T, VEC>,
+                             static_cast<unsigned>(a.batch) * row_blocks * per_row, stream, a,
+                             per_row, row_blocks);
   }
   const unsigned total = static_cast<unsigned>(a.rows) * per_row;
   constexpr int UNROLL = sizeof(T) == 4 ? 1 : 2;
@@ -336,12 +356,10 @@ cudaError_t launch(const BlockQuantArgs& a, bool square, cudaStream_t stream) {
   // arithmetic of one hides the loads of another, 20: 51.6 us against 54.7 with 5.
   const unsigned most = static_cast<unsigned>(a.sms) * (a.gate ? 20 : 5);
   if (grid > most) grid = most;
-  if (a.gate)
-    block_quant_rows_kernel<T, true, VEC, 1><<<grid, kThreads, 0, stream>>>(a, per_row, total);
-  else
-    block_quant_rows_kernel<T, false, VEC, UNROLL>
-        <<<grid, kThreads, 0, stream>>>(a, per_row, total);
-  return cudaGetLastError();
+  return a.gate ? launch_overlapped(block_quant_rows_kernel<T, true, VEC, 1>, grid, stream, a,
+                                    per_row, total)
+                : launch_overlapped(block_quant_rows_kernel<T, false, VEC, UNROLL>, grid, stream, a,
+                                    per_row, total);
 }
 
 }  // namespace

@@ -188,7 +188,7 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
   g.tile_rows = p.tile_rows;
   g.k_splits = p.splits;
 
-  GroupedMaps m;
+  GroupedMaps m{};
   const uint64_t a_dims[2] = {uint64_t(s->k), uint64_t(s->rows)};
   const uint64_t a_strides[1] = {uint64_t(a_row)};
   const uint64_t b_dims[3] = {uint64_t(s->k), uint64_t(s->n), uint64_t(s->groups)};

@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
   if (warp == 8 && lane == 0) {
     tma_prefetch_desc(&maps.b);
     tma_prefetch_desc(PAIR ? &maps.a128 : &maps.a64);
-    tma_prefetch_desc(PAIR ? &maps.a64 : &maps.a16);
+    if (!C::ROWS_M) tma_prefetch_desc(PAIR ? &maps.a64 : &maps.a16);  // (else not encoded)
   }
   if (warp == 9) {
     if constexpr (PAIR) {
