@@ -656,6 +656,8 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
         const float* sa = g.a_scales + t.row0 * g.as_row;
         const float* sb = g.b_scales + t.group * g.bs_group + t.ch0 / 128 * g.bs_n;
         // All loads of QUADS of them are under way before the first is used.
+        // (Plain loads, here and below: the kernel before may have written the scales
+        // after this one had started.)
         constexpr int ROWS = C::ROWS_M ? 2 : 1, COLS = ROWS, QUADS = C::ROWS_M ? 1 : 4;
         for (int k0 = kb0; k0 < kb1 && ok; k0 += 4 * QUADS) {
           float v[ROWS][4 * QUADS], w[COLS][4 * QUADS];
@@ -665,12 +667,12 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
               const int r = (C::ROWS_M ? static_cast<int>(rank) * 128 : 0) + me + 64 * i;
-              v[i][k] = there && r < t.rows ? __ldg(sa + r * g.as_row + (k0 + k) * g.as_k) : 0.0f;
+              v[i][k] = there && r < t.rows ? sa[r * g.as_row + (k0 + k) * g.as_k] : 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < COLS; ++j)
               w[j][k] = there && t.ch0 + j * 128 < g.n
-                            ? __ldg(sb + j * g.bs_n + (k0 + k) * g.bs_k)
+                            ? sb[j * g.bs_n + (k0 + k) * g.bs_k]
                             : 0.0f;
           }
 #pragma unroll
@@ -878,13 +880,13 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
       constexpr bool ROW_SCALES = ADD == GROUPED_ADD_NONE && (KIND == KIND_I8 || KIND == KIND_F8);
       float sb = 1.0f;
       if constexpr (ROW_SCALES) {
-        if (ch + lane < g.n) sb = __ldg(g.b_scales + t.group * g.bs_group + (ch + lane) * g.bs_n);
+        if (ch + lane < g.n) sb = g.b_scales[t.group * g.bs_group + (ch + lane) * g.bs_n];
         __syncwarp();  // (all lanes are done with the last tile's)
 #pragma unroll
         for (int c = 0; c < C::CHUNKS; ++c) {
           const int r = (2 * c + half) * 32 + lane;
           row_scales[c * 32 + lane] =
-              r < t.rows ? __ldg(g.a_scales + (int64_t(t.row0) + r) * g.as_row) : 0.0f;
+              r < t.rows ? g.a_scales[(int64_t(t.row0) + r) * g.as_row] : 0.0f;
         }
         __syncwarp();
       }
