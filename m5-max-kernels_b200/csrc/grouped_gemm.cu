@@ -8,7 +8,8 @@
 // (32) rows of one group, so that a group of few rows costs few columns, and a
 // group of many is cut into equal tiles.  Rows of the next group or behind the
 // last one that a tile's loads bring along are columns of their own, which are
-// not stored.
+// not stored.  (Block-scaled products on CTA pairs are the other way round, see
+// ROWS_M: a scale for each column would cost the epilogue more than the MMAs take.)
 //
 // Block scales: a block of 128 channels of K (one 128-byte slice, four MMAs) is
 // summed in TMEM by itself, and the epilogue warps add it, times the row's and
@@ -19,8 +20,8 @@
 //
 // Roles: warps 0-7 epilogue, warp 8 TMA producer, warp 9 MMA issuer, warps 10 and
 // 11 bring the block scales (products sa * sb, in shared memory).  TMEM is
-// read by whole lanes: a thread holds one channel of 32 rows (columns of the
-// accumulator).  That goes at 840 bytes a clock and SM, where 16 x 256-bit
+// read by whole lanes: a thread holds one channel of 32 rows (ROWS_M: one row of
+// 16 channels).  That goes at 840 bytes a clock and SM, where 16 x 256-bit
 // fragments, which would need fewer scales a thread, came at 253, as long as
 // the MMAs of a block take.
 //
