@@ -27,7 +27,9 @@ bool grid16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Strides of a tensor map are below 2^40 bytes.
-bool map_stride(int64_t bytes) { return bytes > 0 && bytes < (int64_t(1) << 40) && bytes % 16 == 0; }
+bool map_stride(int64_t bytes) {
+  return bytes > 0 && bytes < (int64_t(1) << 40) && bytes % 16 == 0;
+}
 
 struct Plan {
   bool pair;
@@ -41,14 +43,16 @@ struct Plan {
 // (0.56 where it is scaled by itself), as measured at 128 blocks and more: 200 x
 // 4096 x 16384 block-scaled 38 against 73 us, 517 rows 80 against 74; 65 rows 25
 // against 72.  Of several groups' sizes only the sum is known here: each is
-// taken to end in the middle of a tile.
+// taken to end in the middle of a tile, and to have one at least.
 Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, int add, int sms) {
   const int64_t busy = groups < rows ? groups : rows;  // groups with rows, at most
-  const int64_t half = groups == 1 ? 0 : busy;         // of a tile each
   auto waves = [&](int64_t tile_rows, int64_t ch, int64_t units, double block, int64_t splits) {
     const int64_t ch_tiles = ceil_div(n, ch);
-    const int64_t tiles = groups == 1 ? ceil_div(rows, tile_rows)
-                                      : ceil_div(2 * rows + tile_rows * half, 2 * tile_rows);
+    int64_t tiles = ceil_div(rows, tile_rows);
+    if (groups > 1) {
+      tiles = ceil_div(2 * rows + tile_rows * busy, 2 * tile_rows);
+      if (tiles < busy) tiles = busy;
+    }
     return ceil_div(tiles * ch_tiles * splits, units) * ceil_div(nkb, splits) * block;
   };
   // (every group rounds its last tile up: no more tiles than these)
@@ -63,7 +67,8 @@ Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, in
          tiles <= grouped_split_clusters(kind, add, p.splits * 2))
     p.splits *= 2;
   const double single = waves(kSingleTileRows, 128, sms, 0.32, p.splits);
-  const double pair = waves(kPairTileRows, 256, sms / 2, add == GROUPED_ADD_SCALED ? 0.56 : 0.40, 1);
+  const double pair =
+      waves(kPairTileRows, 256, sms / 2, add == GROUPED_ADD_SCALED ? 0.56 : 0.40, 1);
   p.pair = pair < single;
   if (p.pair) {
     tiles = most_tiles(kPairTileRows, 256);
