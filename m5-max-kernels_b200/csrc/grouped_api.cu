@@ -39,21 +39,24 @@ struct Plan {
 // Tiles and schedule.  Single CTAs take 128 channels x 64 rows, several of them
 // (a cluster) sharing the K range where the tiles do not fill the GPU; CTA pairs
 // take 256 channels x 256 rows.  Taken is what needs less time for its waves, a
-// block of 128 bytes of K costing 0.32 us on a single CTA and 0.40 us on a pair
-// (0.56 where it is scaled by itself), as measured at 128 blocks and more: 200 x
-// 4096 x 16384 block-scaled 38 against 73 us, 517 rows 80 against 74; 65 rows 25
-// against 72.  Of several groups' sizes only the sum is known here: each is
-// taken to end in the middle of a tile, and to have one at least.
+// block of 128 bytes of K costing 0.32 us on a single CTA and 0.40 us on a pair,
+// and leaving a pair's tile 0.5 us (0.56 and 2.5 where each block is scaled): fitted
+// to, in us for single CTAs and pairs, block-scaled 65, 200 and 517 rows x 4096 x
+// 16384 25 / 72, 38 / 73, 80 / 74; 64 experts of 2048 -> 4096, 64, 96, 128 and 192
+// rows each 111 / 161, 145 / 165, 182 / 172, 246 / 191, with bf16 64 and 96 rows
+// 181 / 175, 213 / 183.  Of several groups' sizes only the sum is known here: each
+// is taken to end in the middle of a tile, and to have one at least.
 Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, int add, int sms) {
   const int64_t busy = groups < rows ? groups : rows;  // groups with rows, at most
-  auto waves = [&](int64_t tile_rows, int64_t ch, int64_t units, double block, int64_t splits) {
+  auto waves = [&](int64_t tile_rows, int64_t ch, int64_t units, int64_t splits, double block,
+                   double leave) {
     const int64_t ch_tiles = ceil_div(n, ch);
     int64_t tiles = ceil_div(rows, tile_rows);
     if (groups > 1) {
       tiles = ceil_div(2 * rows + tile_rows * busy, 2 * tile_rows);
       if (tiles < busy) tiles = busy;
     }
-    return ceil_div(tiles * ch_tiles * splits, units) * ceil_div(nkb, splits) * block;
+    return ceil_div(tiles * ch_tiles * splits, units) * (ceil_div(nkb, splits) * block + leave);
   };
   // (every group rounds its last tile up: no more tiles than these)
   const auto most_tiles = [&](int64_t tile_rows, int64_t ch) {
@@ -66,9 +69,10 @@ Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, in
   while (p.splits < 8 && tiles * p.splits * 2 <= sms && nkb >= p.splits * 2 * 4 &&
          tiles <= grouped_split_clusters(kind, add, p.splits * 2))
     p.splits *= 2;
-  const double single = waves(kSingleTileRows, 128, sms, 0.32, p.splits);
+  const double single = waves(kSingleTileRows, 128, sms, p.splits, 0.32, 0.0);
+  const bool scaled = add == GROUPED_ADD_SCALED;
   const double pair =
-      waves(kPairTileRows, 256, sms / 2, add == GROUPED_ADD_SCALED ? 0.56 : 0.40, 1);
+      waves(kPairTileRows, 256, sms / 2, 1, scaled ? 0.56 : 0.40, scaled ? 2.5 : 0.5);
   p.pair = pair < single;
   if (p.pair) {
     tiles = most_tiles(kPairTileRows, 256);
