@@ -42,11 +42,11 @@ constexpr int kPairTileRows = 256;
 constexpr int kSingleTileRows = 64;
 
 // What is added in fp32 registers, not in the accumulator: nothing; blocks of 128
-// channels of K, each by its scale (E4M3); parts of four blocks of 128 bytes (16-bit
-// operands with fp32 results).  The tensor cores truncate their sums: such results
-// were off by 4.9e-6 (relative 2-norm) at K 16384 and 1.3e-6 at 4096 without parts,
-// 3.5e-7 with them; 16-bit results do not show it, INT32 sums are exact, and
-// E4M3 ones with scales of rows, of terms of fewer bits, were off by 2.3e-7.
+// channels of K, each by its scale (E4M3); parts of four blocks of 128 bytes (fp32
+// results of other operands than INT8).  The tensor cores truncate their sums: without
+// parts fp16 operands were off by 4.9e-6 (relative 2-norm) at K 16384 and 1.3e-6 at
+// 4096, E4M3 ones by 1.2e-6 at 16384; with them fp16 by 3.5e-7 at any.  16-bit results
+// do not show it, and INT32 sums are exact.
 enum GroupedAdd : int { GROUPED_ADD_NONE = 0, GROUPED_ADD_SCALED = 1, GROUPED_ADD_PARTS = 2 };
 
 cudaError_t launch_grouped_gemm(const GroupedMaps& maps, const GroupedArgs& g, int kind, int add,

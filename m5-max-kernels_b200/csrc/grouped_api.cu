@@ -190,9 +190,10 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
   int sms = 0;
   int rc = current_device_state(&g.status, &sms);
   if (rc) return rc;
-  const int add = s->block_scales                         ? GROUPED_ADD_SCALED
-                  : elem == 2 && s->out_dtype == M5B_F32 ? GROUPED_ADD_PARTS
-                                                         : GROUPED_ADD_NONE;
+  const bool parts = kind != KIND_I8 && s->out_dtype == M5B_F32;
+  const int add = s->block_scales ? GROUPED_ADD_SCALED
+                  : parts         ? GROUPED_ADD_PARTS
+                                  : GROUPED_ADD_NONE;
   const Plan p = plan_for(s->rows, s->groups, s->n, g.num_k_blocks, kind, add, sms);
   g.tile_rows = p.tile_rows;
   g.k_splits = p.splits;

@@ -878,7 +878,7 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
       }
       // Scales of rows and channels: this thread's channel, and a row of each chunk.
       const int ch = t.ch0 + (PAIR ? static_cast<int>(rank) * 128 : 0) + quarter * 32;
-      constexpr bool ROW_SCALES = ADD == GROUPED_ADD_NONE && (KIND == KIND_I8 || KIND == KIND_F8);
+      constexpr bool ROW_SCALES = !BLOCKS && (KIND == KIND_I8 || KIND == KIND_F8);
       float sb = 1.0f;
       if constexpr (ROW_SCALES) {
         if (ch + lane < g.n) sb = g.b_scales[t.group * g.bs_group + (ch + lane) * g.bs_n];
@@ -1148,8 +1148,9 @@ auto with_kind(int kind, int add, What what) {
   switch (kind) {
     case KIND_I8: return what(std::integral_constant<int, KIND_I8>{}, none);
     case KIND_F8:
-      return add == GROUPED_ADD_SCALED ? what(std::integral_constant<int, KIND_F8>{}, scaled)
-                                       : what(std::integral_constant<int, KIND_F8>{}, none);
+      if (add == GROUPED_ADD_SCALED) return what(std::integral_constant<int, KIND_F8>{}, scaled);
+      return add == GROUPED_ADD_PARTS ? what(std::integral_constant<int, KIND_F8>{}, parts)
+                                      : what(std::integral_constant<int, KIND_F8>{}, none);
     case KIND_BF16:
       return add == GROUPED_ADD_PARTS ? what(std::integral_constant<int, KIND_BF16>{}, parts)
                                       : what(std::integral_constant<int, KIND_BF16>{}, none);

@@ -513,3 +513,15 @@ def test_offsets_beyond_32_bits(ops):
     codes, scales = ops.block_quantize(x)
     check_codes(codes[-3:], scales[-3:], x[-3:].cpu())
     assert (codes[:-2].view(torch.int64) == 0).all() and (scales[:-2] == 1).all()
+
+
+@pytest.mark.parametrize("sizes,n", [([40], 300), ([300, 200], 300), ([900], 1600)])
+def test_fp32_results_of_long_e4m3_sums(ops, sizes, n):
+    """As test_fp32_results_of_long_sums: parts of four blocks of 128 channels (16 instructions),
+    and two roundings for the scales."""
+    k = 16384
+    case = Experts(sizes, n=n, k=k, mode="fp8", scales="row", seed=17)
+    got = product(ops, case, output_dtype=F32).double().cpu()
+    out, spread = case.oracle()
+    e = (16 + k // 512 + 3) * 2.0**-22
+    assert ((got - out).abs() <= 2.0**-24 * out.abs() + e * spread).all()
