@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
   }
   // With programmatic launch all that stands before the first access to global
   // memory overlaps the previous kernel's end, and lets the next kernel start, which
-  // waits in its turn: here where the bounds are read, else in the roles, whose code
+  // waits in its turn: here where the bounds are read, else in every role, whose code
   // is cold too (2500 cycles from here to the first copy).
   auto inputs_ready = []() {
     grid_dependency_wait();
@@ -572,6 +572,9 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
     } else if (warp == 9) {
       // ------------------------------------------------------------ MMA issuer
       if (leader && elect_one()) {
+        // (the limit of its waits must not count the previous kernel's time, for as long as
+        // which the producer waits)
+        if (!g.group_start) inputs_ready();
         int stage = 0, buf = 0;
         uint32_t phase = 0, buf_phase = 0;
         bool ok = true;

@@ -1,0 +1,64 @@
+"""Block-scaled and grouped products next to other work: kernels before them, errors before them."""
+
+import pytest
+import torch
+
+from grouped_cases import Experts
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+BF16, F32, U8 = torch.bfloat16, torch.float32, torch.uint8
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import m5kernels_b200 as m
+    from m5kernels_b200 import _lib
+
+    yield m
+    assert _lib.device_status() == 0  # no bounded wait gave up
+
+
+def test_a_long_kernel_before_a_dense_product(ops):
+    """A product starts on SMs that the kernel before leaves idle, and waits there for its end.
+
+    That is no wait of its own pipeline, whose waits give up after 2 s.  The kernel before is a
+    block-scaled product of 256 x 9472 outputs, 37 tiles on 148 SMs, over a K that takes longer
+    than that: its rows lie 16 bytes apart in one buffer, and its scales are one number.
+    """
+    from m5kernels_b200 import _lib
+
+    rows, n = 256, 37 * 256
+    most = 2**31 - 2**20
+    buf = torch.zeros(most + 16 * n, dtype=U8, device=DEV)
+    one = torch.ones(1, 1, device=DEV)
+
+    def long_product(k):
+        out = torch.empty(rows, n, dtype=BF16, device=DEV)
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        ops.block_gemm(buf.as_strided((rows, k), (16, 1)), buf.as_strided((n, k), (16, 1)),
+                       one.expand(rows, k // 128), one.expand(n // 128, k // 128), out=out)
+        return start, end
+
+    def timed(k):
+        start, end = long_product(k)
+        end.record()
+        end.synchronize()
+        return start.elapsed_time(end)
+
+    timed(2**22)
+    k = min(most, int(2600 / timed(2**24) * 2**24)) // 128 * 128
+    case = Experts([3], n=200, k=2064, mode="fp8", scales="block", seed=21)
+    args = case.on(DEV)
+    want = ops.block_gemm(args["a"], args["b"][0], args["a_scales"], args["b_scales"][0])
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    start, end = long_product(k)
+    out = ops.block_gemm(args["a"], args["b"][0], args["a_scales"], args["b_scales"][0])
+    end.record()
+    end.synchronize()
+    if start.elapsed_time(end) < 2100:
+        pytest.skip("the kernel before ends too soon here")
+    assert _lib.device_status() == 0 and torch.equal(out, want)
