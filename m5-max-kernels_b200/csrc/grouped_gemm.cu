@@ -140,8 +140,12 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_
                "r"(c), "r"(d)
                : "memory");
 }
-// mbar_wait_bounded with few registers (the epilogue has none to spare): 32 bits of
-// the clock, 4.3 s.
+// A wait's answer as the warp's: after a wait that gave up, lanes may have seen the barrier or the
+// abort flag first, and the aligned instructions that follow need all of them or none.
+__device__ __forceinline__ bool whole_warp(bool ok) { return __all_sync(0xffffffffu, ok); }
+
+// mbar_wait_bounded of a whole warp, with few registers (the epilogue has none to
+// spare): 32 bits of the clock, 4.3 s.
 __device__ __forceinline__ uint32_t globaltimer_lo() {
   uint32_t t;
   asm volatile("mov.u32 %0, %globaltimer_lo;" : "=r"(t));
@@ -160,12 +164,12 @@ __device__ __forceinline__ bool mbar_wait_lean(uint32_t bar, uint32_t parity, ui
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
-    if (ok) return true;
+    if (whole_warp(ok)) return true;
     if (first) start = globaltimer_lo();
     first = false;
     asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(stop) : "r"(abort) : "memory");
-    if (stop) return false;
-    if (globaltimer_lo() - start > static_cast<uint32_t>(kWaitLimitNs)) {
+    if (!whole_warp(!stop)) return false;
+    if (!whole_warp(globaltimer_lo() - start <= static_cast<uint32_t>(kWaitLimitNs))) {
       atomicOr(status, code);
       asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort), "r"(1) : "memory");
       return false;
@@ -683,9 +687,9 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
           for (int q = 0; q < QUADS; ++q) {
             if (k0 + 4 * q >= kb1) break;
             const uint32_t slot = quad % C::SCALE_SLOTS;
-            ok = mbar_wait_bounded(&scale_empty[slot], ((quad / C::SCALE_SLOTS) & 1u) ^ 1u,
-                                   abort_flag, g.status, DEV_TIMEOUT_PRODUCER);
-            __syncwarp();
+            ok = whole_warp(mbar_wait_bounded(&scale_empty[slot],
+                                              ((quad / C::SCALE_SLOTS) & 1u) ^ 1u, abort_flag,
+                                              g.status, DEV_TIMEOUT_PRODUCER));
             if (!ok) break;
             float* s = s_scale + slot * 4 * C::TN + me;
 #pragma unroll
@@ -708,8 +712,8 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
       }
       if (C::ROWS_M && ok) {
         const uint32_t slot = quad % C::SCALE_SLOTS;
-        ok = mbar_wait_bounded(&scale_empty[slot], ((quad / C::SCALE_SLOTS) & 1u) ^ 1u, abort_flag,
-                               g.status, DEV_TIMEOUT_PRODUCER);
+        ok = whole_warp(mbar_wait_bounded(&scale_empty[slot], ((quad / C::SCALE_SLOTS) & 1u) ^ 1u,
+                                          abort_flag, g.status, DEV_TIMEOUT_PRODUCER));
         if (me == 0) slot_tile[slot * 4 + 1] = 0;
         __syncwarp();
         if (ok && lane == 0) mbar_arrive(&scale_full[slot]);
@@ -732,7 +736,6 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
       const bool ok = mbar_wait_lean(smem_u32(acc_full) + buf * 8, buf_phase,
                                      smem_u32(const_cast<int*>(abort_flag)), g.status,
                                      DEV_TIMEOUT_EPILOGUE);
-      __syncwarp();
       tc_fence_after();
       return ok;
     };
@@ -776,7 +779,6 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
       ok = mbar_wait_lean(smem_u32(scale_full) + quad % C::SCALE_SLOTS * 8,
                           (quad / C::SCALE_SLOTS) & 1u, smem_u32(const_cast<int*>(abort_flag)),
                           g.status, DEV_TIMEOUT_EPILOGUE);
-      __syncwarp();
       return ok;
     };
     while (ok) {
@@ -845,9 +847,8 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
       } else if constexpr (BLOCKS) {
         for (int kq = kb0; kq < kb1 && ok; kq += 4, ++quad) {
           const uint32_t slot = quad % C::SCALE_SLOTS;
-          ok = mbar_wait_bounded(&scale_full[slot], (quad / C::SCALE_SLOTS) & 1u, abort_flag,
-                                 g.status, DEV_TIMEOUT_EPILOGUE);
-          __syncwarp();
+          ok = whole_warp(mbar_wait_bounded(&scale_full[slot], (quad / C::SCALE_SLOTS) & 1u,
+                                            abort_flag, g.status, DEV_TIMEOUT_EPILOGUE));
           if (!ok) break;
           ok = wait_acc();
           if (!ok) break;
@@ -989,8 +990,8 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
           __syncwarp();
           cluster_arrive();
           exchanged = true;
-          ok = mbar_wait_cluster(parts, 0, abort_flag, g.status, DEV_TIMEOUT_FIXUP);
-          __syncwarp();
+          ok = whole_warp(
+              mbar_wait_cluster(parts, 0, abort_flag, g.status, DEV_TIMEOUT_FIXUP));
           if (!ok) break;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
