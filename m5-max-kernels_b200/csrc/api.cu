@@ -28,6 +28,9 @@ int fail(int code, const char* fmt, ...) {
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
   va_end(ap);
+  // Reported here: a later call that asks the runtime for its launch's error
+  // must not be told of this one.
+  if (code == M5B_ECUDA) cudaGetLastError();
   return code;
 }
 

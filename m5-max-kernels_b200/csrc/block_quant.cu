@@ -344,8 +344,7 @@ cudaError_t launch_overlapped(void (*kernel)(Params...), unsigned grid, cudaStre
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <typename T, bool VEC>

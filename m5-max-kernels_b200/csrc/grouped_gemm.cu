@@ -1107,9 +1107,7 @@ cudaError_t launch(const GroupedMaps& maps, const GroupedArgs& g, int grid, cuda
   ++n_attr;
   cfg.attrs = attr;
   cfg.numAttrs = n_attr;
-  e = cudaLaunchKernelEx(&cfg, kern, maps, g);
-  if (e != cudaSuccess) return e;
-  return cudaGetLastError();
+  return cudaLaunchKernelEx(&cfg, kern, maps, g);
 }
 
 template <int KIND, int ADD>
@@ -1121,9 +1119,6 @@ int split_clusters(int splits) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxLaunchDevices) return 0;
   std::atomic<int>& slot = known[dev][splits == 8 ? 3 : splits == 4 ? 2 : splits == 2 ? 1 : 0];
   if (int n = slot.load(std::memory_order_relaxed)) return n - 1;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) !=
-      cudaSuccess)
-    return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(splits), 1, 1);
   cfg.blockDim = dim3(C::THREADS, 1, 1);
@@ -1136,7 +1131,12 @@ int split_clusters(int splits) {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) return 0;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES) !=
+          cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();  // (dealt with: K is not split)
+    n = 0;
+  }
   slot.store(n + 1, std::memory_order_relaxed);
   return n;
 }

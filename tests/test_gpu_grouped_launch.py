@@ -62,3 +62,37 @@ def test_a_long_kernel_before_a_dense_product(ops):
     if start.elapsed_time(end) < 2100:
         pytest.skip("the kernel before ends too soon here")
     assert _lib.device_status() == 0 and torch.equal(out, want)
+
+
+def test_an_earlier_error_is_not_reported_again(ops):
+    """A call that failed has said so; the next one succeeds and says that."""
+    import ctypes
+
+    from m5kernels_b200 import _lib
+
+    lib = _lib.lib()
+    buf = torch.zeros(1 << 21, dtype=U8, device=DEV)
+    handle, offset = (ctypes.c_uint8 * 64)(), ctypes.c_int64(0)
+    case = Experts([3, 5], n=200, k=272, mode="fp8", scales="block", seed=22)
+    args = case.on(DEV)
+    x = torch.randn(4, 256, device=DEV)
+
+    def fail():  # a process cannot import what it exported itself
+        mapped = ctypes.c_void_p()
+        with pytest.raises(RuntimeError):
+            _lib.check(lib.m5b_ipc_import(handle, offset, ctypes.byref(mapped)))
+
+    def grouped():
+        return ops.grouped_gemm(args["a"], args["b"], args["group_start"], "fp8",
+                                a_scales=args["a_scales"], b_scales=args["b_scales"])
+
+    calls = (lambda: ops.block_quantize(x)[0], lambda: ops.block_quantize(x, block_rows=128)[0],
+             lambda: ops.block_gemm(args["a"], args["b"][0], args["a_scales"],
+                                    args["b_scales"][0]),
+             grouped, lambda: ops.quantize(x, "int8")[0],
+             lambda: ops.gemm(x.to(BF16), x.to(BF16)))
+    want = [call() for call in calls]
+    _lib.check(lib.m5b_ipc_export(ctypes.c_void_p(buf.data_ptr()), handle, ctypes.byref(offset)))
+    for call, expected in zip(calls, want):
+        fail()
+        assert torch.equal(call(), expected)
