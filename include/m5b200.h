@@ -515,8 +515,9 @@ M5B_API int m5b_block_quantize(const m5b_block_quantize_args* args, void* stream
  * b_scale_group_stride between groups, b_scale_row_stride between channels
  * (block_scales: blocks of 128 channels), b_scale_block_stride between blocks
  * of K.  Rows of a and b have contiguous channels and start on 16-byte
- * boundaries.  Rows outside every group keep what out holds, or with zero_rest
- * become zero.  No workspace. */
+ * boundaries; out's rows have contiguous channels and do not overlap.  Rows
+ * outside every group keep what out holds, or with zero_rest become zero.  No
+ * workspace. */
 typedef struct m5b_grouped_gemm_args {
   const void* a;
   const void* b;

@@ -160,6 +160,9 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
   if (s->rows == 0) return set_last_error(M5B_OK, "");
   if (!s->a || !s->b || !s->out) return einval("a, b and out are required");
   if (quantized && (!s->a_scales || !s->b_scales)) return einval("scales required");
+  // (every element is stored by a thread of its own)
+  if (s->rows > 1 && s->out_row_stride < s->n && s->out_row_stride > -s->n)
+    return einval("out's rows must not overlap");
   const int64_t row_bytes = ceil_div(s->k * elem, 16) * 16;
   const int64_t a_row = s->rows > 1 ? s->a_row_stride * elem : row_bytes;
   const int64_t b_row = s->n > 1 ? s->b_row_stride * elem : row_bytes;

@@ -200,7 +200,7 @@ def block_gemm(a, b, a_scales, b_scales, *, output_dtype=None, out=None):
     1 and 128); views of any strides are fine.  Sums and scales in fp32; the
     product of two scales has to be in fp32's range.  K a multiple of 16.
     output_dtype: float32 unless given; `out` may be given, with contiguous
-    channels.
+    channels and rows that do not overlap.
     """
     if isinstance(a, _Tensor) and isinstance(b, _Tensor):
         a_shape, b_shape = a.shape, b.shape
@@ -225,8 +225,8 @@ def grouped_gemm(a, b, group_start, mode="bf16", *, a_scales=None, b_scales=None
     K times the element size a multiple of 16.
 
     Rows outside every group are zero; where `out` is given (contiguous
-    channels, output_dtype its own) they keep what it holds.  output_dtype:
-    float32 unless given.
+    channels, rows that do not overlap, output_dtype its own) they keep what it
+    holds.  output_dtype: float32 unless given.
     """
     if mode not in _OPERAND:
         if mode in ("fp32", "mxint8"):

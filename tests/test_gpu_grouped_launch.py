@@ -96,3 +96,18 @@ def test_an_earlier_error_is_not_reported_again(ops):
     for call, expected in zip(calls, want):
         fail()
         assert torch.equal(call(), expected)
+
+
+def test_rows_of_out_that_overlap_are_refused(ops):
+    case = Experts([3, 5], n=200, k=272, mode="bf16", seed=23)
+    args = case.on(DEV)
+    buf = torch.zeros(9 * 200, dtype=BF16, device=DEV)
+    for step in (0, 1, 199):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.grouped_gemm(args["a"], args["b"], args["group_start"],
+                             out=buf.as_strided((8, 200), (step, 1)))
+    assert (buf == 0).all()
+    out = buf.as_strided((8, 200), (200, 1))
+    ops.grouped_gemm(args["a"], args["b"], args["group_start"], out=out)
+    assert torch.equal(out, ops.grouped_gemm(args["a"], args["b"], args["group_start"],
+                                             output_dtype=BF16))
