@@ -480,8 +480,9 @@ M5B_API int64_t m5b_paged_attention_workspace_bytes(int64_t head_dim);
  * 128 rows (block_rows 128):
  *   v     = x, or silu(gate) * x = gate / (1 + exp(-gate)) * x in fp32
  *   scale = max|v| / 448 over the block, 1 where that is 0
- *   code  = E4M3(RN(v / scale)), nearest even, saturating
- * x, gate: rows of contiguous channels.  row_index (block_rows 1): row r of the
+ *   code  = E4M3(RN(v / scale)), nearest even, saturating; which of the two
+ *           zeros a v of -0 gets is not specified
+ * (exp(-gate) is infinite, and v zero, for gates below -88.7.)  x, gate: rows of contiguous channels.  row_index (block_rows 1): row r of the
  * output is that of x[row_index[r]]; an index outside [0, x_rows) gives zeros
  * (and scales of 1).  q [batch, rows, k] and scales [batch, ceil(rows /
  * block_rows), ceil(k / 128)] are contiguous; a batch, of weights, needs

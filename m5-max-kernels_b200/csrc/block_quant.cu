@@ -3,7 +3,8 @@
 //
 //   v = x, or silu(gate) x = gate / (1 + exp(-gate)) x, in fp32
 //   scale = max|v| / 448 over the block, 1 where that is 0
-//   code  = E4M3(RN32(v / scale)), nearest even, saturating
+//   code  = E4M3(RN32(v / scale)), nearest even, saturating; -0 gives code 0 where
+//           quotients go by multiplications (x - q s is +0), 0x80 where they are divided
 //
 // One pass: a block of one row lives in eight lanes, 16 channels each (32 bytes
 // of a 16-bit type, one 16-byte store of codes), its peak goes through three
@@ -79,7 +80,8 @@ __device__ __forceinline__ float2 pair(const Raw<T>& r, int i) {  // values 2 i,
     return __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
 }
 
-// m = the larger magnitude of m and v, NaN if either is, under a sign of no meaning.
+// m = the larger magnitude of m and v, NaN if either is, under a sign of no meaning
+// (magnitude() takes it off).
 __device__ __forceinline__ void larger(float& m, float v) {
   asm("max.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(m) : "f"(v));
 }

@@ -52,7 +52,8 @@ def block_quantize(x, *, gate=None, rows=None, block_rows=1):
 
     scale = max|v| / 448 over the block (1 where that is 0), codes =
     E4M3(v / scale), nearest even, saturating, the quotient in fp32; the last
-    block of a row may be shorter.
+    block of a row may be shorter.  Which of the two zeros a v of -0 gets is
+    not specified.
 
     block_rows 1 (activations): x [T, K] -> codes [T, K], scales [T, ceil(K / 128)].
     v = x, or with `gate` [T, K] v = silu(gate) * x in fp32 (the step between
