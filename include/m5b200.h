@@ -482,12 +482,12 @@ M5B_API int64_t m5b_paged_attention_workspace_bytes(int64_t head_dim);
  *   scale = max|v| / 448 over the block, 1 where that is 0
  *   code  = E4M3(RN(v / scale)), nearest even, saturating; which of the two
  *           zeros a v of -0 gets is not specified
- * (exp(-gate) is infinite, and v zero, for gates below -88.7.)  x, gate: rows of contiguous channels.  row_index (block_rows 1): row r of the
- * output is that of x[row_index[r]]; an index outside [0, x_rows) gives zeros
- * (and scales of 1).  q [batch, rows, k] and scales [batch, ceil(rows /
- * block_rows), ceil(k / 128)] are contiguous; a batch, of weights, needs
- * block_rows 128.  A block that holds an infinity or NaN gets a scale that is
- * not finite. */
+ * (exp(-gate) is infinite, and v zero, for gates below -88.7.)  x, gate: rows
+ * of contiguous channels.  row_index (block_rows 1): row r of the output is
+ * that of x[row_index[r]]; an index outside [0, x_rows) gives zeros (and scales
+ * of 1).  q [batch, rows, k] and scales [batch, ceil(rows / block_rows), ceil(k
+ * / 128)] are contiguous; a batch, of weights, needs block_rows 128.  A block
+ * that holds an infinity or NaN gets a scale that is not finite. */
 typedef struct m5b_block_quantize_args {
   const void* x;
   int64_t x_dtype, x_rows, x_row_stride, x_batch_stride;
@@ -534,6 +534,12 @@ typedef struct m5b_grouped_gemm_args {
   int64_t out_dtype, out_row_stride, zero_rest;
 } m5b_grouped_gemm_args;
 M5B_API int m5b_grouped_gemm(const m5b_grouped_gemm_args* args, void* stream);
+
+/* How m5b_grouped_gemm goes about a call on the current device; the call's
+ * pointers are not looked at.  plan[0]: CTAs that work on a tile's channels and
+ * rows together (1, or 2: a pair), plan[1]: most rows of a tile, plan[2]: CTAs
+ * that share a tile's range of K, plan[3]: CTAs in all. */
+M5B_API int m5b_grouped_gemm_plan(const m5b_grouped_gemm_args* args, int64_t* plan);
 
 #ifdef __cplusplus
 }

@@ -85,6 +85,48 @@ Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, in
   return p;
 }
 
+// What a call's sizes and types say; M5B_OK, or the error.
+struct Product {
+  int kind, add;
+  int64_t elem, num_k_blocks;
+  bool quantized;
+};
+int check_product(const m5b_grouped_gemm_args* s, Product* p) {
+  if (!s) return einval("arguments are NULL");
+  int kind = 0;
+  int64_t elem = 1;
+  bool quantized = true;
+  switch (s->mode) {
+    case M5B_MODE_INT8: kind = KIND_I8; break;
+    case M5B_MODE_FP8: kind = KIND_F8; break;
+    case M5B_MODE_BF16: kind = KIND_BF16, elem = 2, quantized = false; break;
+    case M5B_MODE_FP16: kind = KIND_F16, elem = 2, quantized = false; break;
+    case M5B_MODE_FP32: return eunsupported("fp32 operands are not supported by the grouped GEMM");
+    default: return einval("unknown GEMM mode");
+  }
+  if (s->rows < 0 || s->groups < 1 || s->n < 1 || s->k < 1)
+    return einval("rows, groups, n and k must be positive");
+  if (s->block_scales && s->mode != M5B_MODE_FP8) return einval("block scales need FP8 operands");
+  if (!float_dtype(s->out_dtype))
+    return eunsupported("output dtype must be bfloat16, float16 or float32");
+  if (s->groups > kMaxGroups) return eunsupported("more than 1024 groups are unsupported");
+  if (kind == KIND_I8 && s->k > 133144)
+    return eunsupported("INT32 worst-case overflow bound exceeded");
+  // (rows and channels are rounded up to whole tiles, and tiles counted in 32 bits)
+  const int64_t most = INT_MAX - 4096;
+  if (s->rows > most || s->n > most || s->k > most ||
+      (s->rows / 64 + s->groups) * ceil_div(s->n, 128) > most)
+    return eunsupported("rows x channels exceed the index range");
+  p->kind = kind;
+  p->elem = elem;
+  p->quantized = quantized;
+  p->num_k_blocks = ceil_div(s->k * elem, 128);
+  p->add = s->block_scales                                 ? GROUPED_ADD_SCALED
+           : kind != KIND_I8 && s->out_dtype == M5B_F32 ? GROUPED_ADD_PARTS
+                                                        : GROUPED_ADD_NONE;
+  return M5B_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -131,35 +173,15 @@ int m5b_block_quantize(const m5b_block_quantize_args* s, void* stream) {
 }
 
 int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
-  if (!s) return einval("arguments are NULL");
-  int kind = 0;
-  int64_t elem = 1;
-  bool quantized = true;
-  switch (s->mode) {
-    case M5B_MODE_INT8: kind = KIND_I8; break;
-    case M5B_MODE_FP8: kind = KIND_F8; break;
-    case M5B_MODE_BF16: kind = KIND_BF16, elem = 2, quantized = false; break;
-    case M5B_MODE_FP16: kind = KIND_F16, elem = 2, quantized = false; break;
-    case M5B_MODE_FP32: return eunsupported("fp32 operands are not supported by the grouped GEMM");
-    default: return einval("unknown GEMM mode");
-  }
-  if (s->rows < 0 || s->groups < 1 || s->n < 1 || s->k < 1)
-    return einval("rows, groups, n and k must be positive");
+  Product product{};
+  int rc = check_product(s, &product);
+  if (rc) return rc;
   if (!s->group_start && s->groups != 1) return einval("group_start is required");
-  if (s->block_scales && s->mode != M5B_MODE_FP8) return einval("block scales need FP8 operands");
-  if (!float_dtype(s->out_dtype))
-    return eunsupported("output dtype must be bfloat16, float16 or float32");
-  if (s->groups > kMaxGroups) return eunsupported("more than 1024 groups are unsupported");
-  if (kind == KIND_I8 && s->k > 133144)
-    return eunsupported("INT32 worst-case overflow bound exceeded");
-  // (rows and channels are rounded up to whole tiles, and tiles counted in 32 bits)
-  const int64_t most = INT_MAX - 4096;
-  if (s->rows > most || s->n > most || s->k > most ||
-      (s->rows / 64 + s->groups) * ceil_div(s->n, 128) > most)
-    return eunsupported("rows x channels exceed the index range");
+  const int kind = product.kind, add = product.add;
+  const int64_t elem = product.elem;
   if (s->rows == 0) return set_last_error(M5B_OK, "");
   if (!s->a || !s->b || !s->out) return einval("a, b and out are required");
-  if (quantized && (!s->a_scales || !s->b_scales)) return einval("scales required");
+  if (product.quantized && (!s->a_scales || !s->b_scales)) return einval("scales required");
   // (every element is stored by a thread of its own)
   if (s->rows > 1 && s->out_row_stride < s->n && s->out_row_stride > -s->n)
     return einval("out's rows must not overlap");
@@ -175,7 +197,7 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
   g.rows = static_cast<int>(s->rows);
   g.groups = static_cast<int>(s->groups);
   g.n = static_cast<int>(s->n);
-  g.num_k_blocks = static_cast<int>(ceil_div(s->k * elem, 128));
+  g.num_k_blocks = static_cast<int>(product.num_k_blocks);
   g.group_start = s->group_start;
   g.a_scales = s->a_scales;
   g.b_scales = s->b_scales;
@@ -191,12 +213,8 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
   g.out_vec = s->n % piece == 0 && s->out_row_stride % piece == 0 && grid16(s->out);
   g.zero_rest = s->zero_rest ? 1 : 0;
   int sms = 0;
-  int rc = current_device_state(&g.status, &sms);
+  rc = current_device_state(&g.status, &sms);
   if (rc) return rc;
-  const bool parts = kind != KIND_I8 && s->out_dtype == M5B_F32;
-  const int add = s->block_scales ? GROUPED_ADD_SCALED
-                  : parts         ? GROUPED_ADD_PARTS
-                                  : GROUPED_ADD_NONE;
   const Plan p = plan_for(s->rows, s->groups, s->n, g.num_k_blocks, kind, add, sms);
   g.tile_rows = p.tile_rows;
   g.k_splits = p.splits;
@@ -221,6 +239,24 @@ int m5b_grouped_gemm(const m5b_grouped_gemm_args* s, void* stream) {
   return launched(launch_grouped_gemm(m, g, kind, add, p.pair, p.grid,
                                       static_cast<cudaStream_t>(stream)),
                   "grouped GEMM launch");
+}
+
+int m5b_grouped_gemm_plan(const m5b_grouped_gemm_args* s, int64_t* plan) {
+  Product product{};
+  int rc = check_product(s, &product);
+  if (rc) return rc;
+  if (!plan) return einval("plan is NULL");
+  if (s->rows == 0) return einval("rows must be positive");
+  int sms = 0;
+  rc = current_device_state(nullptr, &sms);
+  if (rc) return rc;
+  const Plan p = plan_for(s->rows, s->groups, s->n, product.num_k_blocks, product.kind,
+                          product.add, sms);
+  plan[0] = p.pair ? 2 : 1;
+  plan[1] = p.tile_rows;
+  plan[2] = p.splits;
+  plan[3] = p.grid;
+  return set_last_error(M5B_OK, "");
 }
 
 }  // extern "C"

@@ -65,6 +65,7 @@ _SIGNATURES = {
     "m5b_paged_attention_workspace_bytes": ([I64], I64),
     "m5b_block_quantize": ([P, P], I),
     "m5b_grouped_gemm": ([P, P], I),
+    "m5b_grouped_gemm_plan": ([P, ctypes.POINTER(I64)], I),
 }
 
 
