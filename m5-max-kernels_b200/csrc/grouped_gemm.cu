@@ -754,8 +754,7 @@ __global__ void __launch_bounds__(Cfg<ADD, PAIR>::THREADS, 1)
       }
     };
     auto load_chunk = [&](int c, uint32_t (&r)[32]) {
-      const int at = C::ROWS_M ? half * 4 + c : 2 * c + half;
-      tmem_ld32(tmem_warp + static_cast<uint32_t>(buf * C::TN + at * 32), r);
+      tmem_ld32(tmem_warp + static_cast<uint32_t>(buf * C::TN + (2 * c + half) * 32), r);
       tmem_wait32(r);
     };
     auto has_chunk = [&](const Tile& t, int c) { return (2 * c + half) * 32 < t.cols; };
