@@ -519,6 +519,9 @@ __global__ void __launch_bounds__(GemmCfg<BN, QK, PAIR>::THREADS, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if ((!PAIR || leader) && elect_one()) {
+      // (the limit of its waits must not count the previous kernel's time, for
+      // as long as which the producer waits)
+      grid_dependency_wait();
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
