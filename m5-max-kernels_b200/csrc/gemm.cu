@@ -626,10 +626,12 @@ __global__ void __launch_bounds__(GemmCfg<BN, QK, PAIR>::THREADS, 1)
       const bool whole = w.whole;
       const int acc = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
-      if (!mbar_wait_bounded(&acc_full[acc], acc_phase, abort_flag, g.status,
-                             DEV_TIMEOUT_EPILOGUE))
+      // (the warp's answer, here and below: after a wait that gave up, lanes may
+      // have seen the barrier or the abort flag first, and the aligned
+      // instructions that follow need all of them or none)
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], acc_phase, abort_flag,
+                                                     g.status, DEV_TIMEOUT_EPILOGUE)))
         break;
-      __syncwarp();
       tc_fence_after();
       const int64_t row = int64_t(m_blk) * Cfg::TILE_M + row_in_tile;
       const uint32_t taddr =
@@ -694,7 +696,8 @@ __global__ void __launch_bounds__(GemmCfg<BN, QK, PAIR>::THREADS, 1)
           mbar_arrive_expect_tx(fix_bar, kSlotBytes);
           mbar_arrive_cluster(map_to_rank(recv_ready, crank + 2));
         }
-        if (!mbar_wait_bounded(fix_bar, fix_phase, abort_flag, g.status, DEV_TIMEOUT_FIXUP))
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(fix_bar, fix_phase, abort_flag, g.status,
+                                                         DEV_TIMEOUT_FIXUP)))
           break;
         fix_phase ^= 1u;
 #pragma unroll 1
@@ -793,7 +796,8 @@ __global__ void __launch_bounds__(GemmCfg<BN, QK, PAIR>::THREADS, 1)
             for (uint32_t off = 0; off < kSlotBytes; off += 16384)
               bulk_load_g2s(reinterpret_cast<uint8_t*>(ring) + off, src + off, 16384, fix_bar);
           }
-          if (!mbar_wait_bounded(fix_bar, fix_phase, abort_flag, g.status, DEV_TIMEOUT_FIXUP))
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(fix_bar, fix_phase, abort_flag, g.status,
+                                                         DEV_TIMEOUT_FIXUP)))
             break;
           fix_phase ^= 1u;
 #pragma unroll 1
