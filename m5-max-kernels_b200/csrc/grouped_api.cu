@@ -44,8 +44,11 @@ struct Plan {
 // to, in us for single CTAs and pairs, block-scaled 65, 200 and 517 rows x 4096 x
 // 16384 25 / 72, 38 / 73, 80 / 74; 64 experts of 2048 -> 4096, 64, 96, 128 and 192
 // rows each 111 / 161, 145 / 165, 182 / 172, 246 / 191, with bf16 64 and 96 rows
-// 181 / 175, 213 / 183.  Of several groups' sizes only the sum is known here: each
-// is taken to end in the middle of a tile, and to have one at least.
+// 181 / 175, 213 / 183.  (Block-scaled pairs take about 5 % less since their waits vote:
+// 70 at 517 rows.)  One price for all other kinds: fp32 results that add parts take pairs
+// a quarter longer, 192 us against 154 for 9914 x 5376 x 4096 in E4M3.  Of several groups'
+// sizes only the sum is known here: each is taken to end in the middle of a tile, and to
+// have one at least.
 Plan plan_for(int64_t rows, int64_t groups, int64_t n, int64_t nkb, int kind, int add, int sms) {
   const int64_t busy = groups < rows ? groups : rows;  // groups with rows, at most
   auto waves = [&](int64_t tile_rows, int64_t ch, int64_t units, int64_t splits, double block,

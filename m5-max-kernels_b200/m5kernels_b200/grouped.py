@@ -198,8 +198,10 @@ def block_gemm(a, b, a_scales, b_scales, *, output_dtype=None, out=None):
 
     a, b: E4M3 codes (uint8), a_scales fp32 [M, ceil(K / 128)], b_scales fp32
     [ceil(N / 128), ceil(K / 128)], as `block_quantize` makes them (block_rows
-    1 and 128); views of any strides are fine.  Sums and scales in fp32; the
-    product of two scales has to be in fp32's range.  K a multiple of 16.
+    1 and 128); views of any strides are fine, but operands whose rows do not
+    start on 16-byte boundaries are copied for every call.  Sums and scales in
+    fp32; the product of two scales has to be in fp32's range.  K a multiple
+    of 16.
     output_dtype: float32 unless given; `out` may be given, with contiguous
     channels and rows that do not overlap.
     """
@@ -223,7 +225,9 @@ def grouped_gemm(a, b, group_start, mode="bf16", *, a_scales=None, b_scales=None
     a_scales [T] and b_scales [E, N], v = (acc * a_scales[t]) * b_scales[e, n];
     or for fp8 those of `block_gemm`, a_scales [T, ceil(K / 128)] and b_scales
     [E, ceil(N / 128), ceil(K / 128)].  INT32 (int8) or FP32 accumulation.
-    K times the element size a multiple of 16.
+    K times the element size a multiple of 16.  Operands whose rows do not
+    start on 16-byte boundaries, or whose groups or rows are expanded, are
+    copied whole for every call.
 
     Rows outside every group are zero; where `out` is given (contiguous
     channels, rows that do not overlap, output_dtype its own) they keep what it
